@@ -261,6 +261,83 @@ int lmps_sample_rows(const uint16_t* logits, int ld, int rows, int n, int top_k,
                      unsigned long long seed, unsigned long long offset, int32_t* ids, int32_t* ids2,
                      void* stream);
 
+/* ---- 4-bit KV cache --------------------------------------------------------
+ * No counterpart in the reference (runners/engine.py:90-91 hold one token).
+ * One layer's K (and V) pool is uint8 [n_pages, n_kv_heads, page_size * 72],
+ * 72 bytes a position and head instead of the fp16 pools' 256; block_table as
+ * for those.  A (page, head) block is page_size rows of 64 code bytes (element
+ * 2j of the 128 in the low nibble of byte j, 2j + 1 in the high nibble, code +
+ * 8: the Q4 weights' nibble order) and then page_size rows of 4 fp16 scales,
+ * one per 32 elements.  A group x[32] with a = max|x| is stored with scale s =
+ * the smallest number >= a / 7 that has 8 significant bits (a multiple of
+ * 2^-24, at most 9344; 1 for a zero group) and codes rint(x / s): code * s is
+ * exact in fp16.  A row with a NaN or infinity gets four NaN scales and gives
+ * NaN to the queries that attend to its position, and to no others.
+ *
+ * head_dim 128, page_size a multiple of 16, at most 8 query heads per KV head
+ * (else UNSUPPORTED), max_pages * page_size <= 2^29; pools, q, qkv, outputs
+ * and workspace 16-byte aligned.  error (int32, may be NULL where not said
+ * otherwise) collects LMPS_Q4_ERR_* bits: a page number outside [0, n_pages)
+ * is neither read nor written (its positions count as absent), a position
+ * outside the cache likewise.  Zero it before the first call and after
+ * reading a non-zero value. */
+#define LMPS_Q4_ERR_TIMEOUT 1  /* a bounded wait for the tensor core gave up */
+#define LMPS_Q4_ERR_PAGE 2     /* a block table entry outside the pool */
+#define LMPS_Q4_ERR_POSITION 4 /* a position or length outside the cache */
+
+/* RoPE + append to the 4-bit cache: row r of qkv [rows, (n_q_heads + 2
+ * n_kv_heads) * 128] is the token at position pos[r] whose pages are row r of
+ * block_table [rows, max_pages].  q_out receives the rotated q, the cache the
+ * rotated K row (rounded to fp16, then quantised) and the V row; k_out and
+ * v_out [rows, n_kv_heads * 128] (each may be NULL) receive the values that
+ * the cache now holds.  The angle pos * inv_freq[j] is taken exactly (fp64),
+ * unlike lmps_rope_kv_append's fp32 product.  A row with pos < 0 is skipped:
+ * its outputs and the cache stay as they were.  Rows of one call name
+ * different (page, position) places. */
+int lmps_rope_kv_append_q4(const uint16_t* qkv, const int32_t* pos, const float* inv_freq, uint16_t* q_out,
+                           uint16_t* k_out, uint16_t* v_out, uint8_t* k_pool, uint8_t* v_pool, int n_pages,
+                           const int32_t* block_table, int max_pages, int page_size, int n_q_heads,
+                           int n_kv_heads, int head_dim, int rows, int style, int32_t* error, void* stream);
+
+/* lmps_gqa_decode_attention over the 4-bit cache: softmax(0.088388 q k^T) v
+ * of one query row per sequence over its first seq_lens[b] <= max_seq_len
+ * positions (0: zeros).  Split over the sequence as there; n_splits from
+ * lmps_attention_q4_splits, workspace from lmps_attention_q4_workspace_size. */
+int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len);
+size_t lmps_attention_q4_workspace_size(int batch, int n_q_heads, int head_dim, int n_splits);
+int lmps_gqa_decode_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, int n_pages,
+                                 const int32_t* block_table, const int32_t* seq_lens, uint16_t* out,
+                                 void* workspace, size_t workspace_bytes, int max_pages, int page_size,
+                                 int n_q_heads, int n_kv_heads, int head_dim, int batch, int max_seq_len,
+                                 int n_splits, int32_t* error, void* stream);
+
+/* lmps_rope_kv_append_q4 followed by lmps_gqa_decode_attention_q4 in one call
+ * (one row per sequence, seq_lens[b] = pos[b] + 1): same cache bytes, same
+ * output bits. */
+int lmps_gqa_decode_attention_rope_q4(const uint16_t* qkv, const int32_t* pos, const float* inv_freq,
+                                      int rope_style, uint8_t* k_pool, uint8_t* v_pool, int n_pages,
+                                      const int32_t* block_table, const int32_t* seq_lens, uint16_t* out,
+                                      void* workspace, size_t workspace_bytes, int max_pages, int page_size,
+                                      int n_q_heads, int n_kv_heads, int head_dim, int batch, int max_seq_len,
+                                      int n_splits, int32_t* error, void* stream);
+
+/* Causal attention of many queries a sequence over the 4-bit cache: a prompt,
+ * or a chunk of tokens behind a cached context.  Row b * seq_len + i of q (and
+ * out) [batch * seq_len, n_q_heads * 128] is the rotated query at position
+ * starts[b] + i (starts NULL: 0) for i < q_lens[b] (NULL: seq_len); it attends
+ * to positions 0 .. starts[b] + i, whose K and V are already cached.  Rows
+ * i >= q_lens[b] of out stay as they were.  starts[b] + q_lens[b] <=
+ * max_seq_len.  n_splits from lmps_prefill_q4_splits (few rows over a long
+ * context are split over the context), workspace from
+ * lmps_prefill_q4_workspace_size.  error must not be NULL. */
+int lmps_prefill_q4_splits(int batch, int seq_len, int n_q_heads, int n_kv_heads, int max_seq_len);
+size_t lmps_prefill_q4_workspace_size(int batch, int seq_len, int n_q_heads, int head_dim, int n_splits);
+int lmps_prefill_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, int n_pages,
+                              const int32_t* block_table, const int32_t* starts, const int32_t* q_lens,
+                              uint16_t* out, void* workspace, size_t workspace_bytes, int max_pages,
+                              int page_size, int n_q_heads, int n_kv_heads, int head_dim, int batch,
+                              int seq_len, int max_seq_len, int n_splits, int32_t* error, void* stream);
+
 /* ---- two-way tensor parallelism over peer memory ------------------------
  * The all-reduce (sum) of the two ranks' partial o_proj / down_proj products
  * that follows each split projection (runners/engine.py:215-221,237-243 with

@@ -69,6 +69,17 @@ _SIGS = {
                                          c_int, c_vp, ctypes.c_ulonglong, c_vp]),
     "lmps_sample_rows": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_float, ctypes.c_ulonglong,
                                  ctypes.c_ulonglong, c_vp, c_vp, c_vp]),
+    "lmps_rope_kv_append_q4": (c_int, [c_vp] * 8 + [c_int, c_vp] + [c_int] * 7 + [c_vp, c_vp]),
+    "lmps_attention_q4_splits": (c_int, [c_int, c_int, c_int]),
+    "lmps_attention_q4_workspace_size": (c_size, [c_int, c_int, c_int, c_int]),
+    "lmps_gqa_decode_attention_q4": (c_int, [c_vp] * 3 + [c_int] + [c_vp] * 4 + [c_size] + [c_int] * 8
+                                     + [c_vp, c_vp]),
+    "lmps_gqa_decode_attention_rope_q4": (c_int, [c_vp] * 3 + [c_int, c_vp, c_vp, c_int] + [c_vp] * 4 + [c_size]
+                                          + [c_int] * 8 + [c_vp, c_vp]),
+    "lmps_prefill_q4_splits": (c_int, [c_int] * 5),
+    "lmps_prefill_q4_workspace_size": (c_size, [c_int] * 5),
+    "lmps_prefill_attention_q4": (c_int, [c_vp] * 3 + [c_int] + [c_vp] * 5 + [c_size] + [c_int] * 9
+                                  + [c_vp, c_vp]),
     "lmps_w4a16_gemm_workspace_size": (c_size, [c_int, c_int]),
     "lmps_w4a16_gemm": (c_int, [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_int,
                                 c_int, c_vp, c_vp, c_size, c_vp]),

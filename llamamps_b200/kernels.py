@@ -301,6 +301,162 @@ def prefill_attention(q, k_pool, v_pool, block_table, out, batch: int, seq_len: 
     return out
 
 
+# -- 4-bit KV cache -----------------------------------------------------------
+Q4_ROW_BYTES = 72          # a cached row of 128 elements: 64 code bytes and 4 fp16 scales
+Q4_ERR_TIMEOUT, Q4_ERR_PAGE, Q4_ERR_POSITION = 1, 2, 4
+_U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
+
+
+def _q4_arg(t: torch.Tensor, name: str, dtype, dev: int, numel: int) -> int:
+    """Address of an argument of the 4-bit cache's kernels: on device ``dev``
+    (the first argument's), of this type, contiguous, exactly ``numel``
+    elements (at least, for a negative one)."""
+    if t.get_device() != dev or dev < 0:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor (the decode path has no CPU fallback)")
+        raise ValueError(f"{name} is on another device than the call's other tensors")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    n = t.numel()
+    if n != numel if numel >= 0 else n < -numel:
+        raise ValueError(f"{name}: {n} elements, expected {abs(numel)}")
+    return t.data_ptr()
+
+
+def _q4_pools(k_pool, v_pool, dev: int, page_size: int, n_kv_heads: int):
+    """Addresses of one layer's pools and their number of pages."""
+    shape = k_pool.shape
+    if len(shape) != 3 or shape[1] != n_kv_heads or shape[2] != page_size * Q4_ROW_BYTES:
+        raise ValueError(f"k_pool: shape {tuple(shape)}, expected [n_pages, {n_kv_heads}, "
+                         f"{page_size * Q4_ROW_BYTES}]")
+    n = k_pool.numel()
+    return _q4_arg(k_pool, "k_pool", _U8, dev, n), _q4_arg(v_pool, "v_pool", _U8, dev, n), shape[0]
+
+
+def _q4_table(block_table, dev: int, rows: int):
+    if block_table.dim() != 2 or block_table.shape[0] < rows:
+        raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected [{rows}, max_pages]")
+    return _q4_arg(block_table, "block_table", _I32, dev, block_table.numel()), block_table.shape[1]
+
+
+def _q4_workspace(workspace, dev: int):
+    if workspace is None:
+        return None, 0
+    n = workspace.numel()
+    return (_q4_arg(workspace, "workspace", _U8, dev, n), n) if n else (None, 0)
+
+
+def _q4_call(name: str, dev: int, *args) -> None:
+    """The call on the current stream of the tensors' device."""
+    if dev == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def rope_kv_append_q4(qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, page_size: int,
+                      n_q_heads: int, n_kv_heads: int, head_dim: int, style: int = 0, *,
+                      k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
+                      error: Optional[torch.Tensor] = None):
+    """rope_kv_append into the 4-bit cache: rotated q to ``q_out``, rotated K
+    and V rows quantised to position ``pos[r]`` of the pages of row r of
+    ``block_table``; ``k_out`` / ``v_out`` receive the values the cache then
+    holds.  Rows with pos < 0 are skipped.  ``error`` (int32 [1]) collects
+    Q4_ERR_PAGE / Q4_ERR_POSITION bits."""
+    dev, rows = qkv.get_device(), qkv.shape[0]
+    q_n, kv_n = rows * n_q_heads * head_dim, rows * n_kv_heads * head_dim
+    a_qkv = _q4_arg(qkv, "qkv", FP16, dev, q_n + 2 * kv_n)
+    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
+    bt, max_pages = _q4_table(block_table, dev, rows)
+    _q4_call("lmps_rope_kv_append_q4", dev, a_qkv, _q4_arg(pos, "pos", _I32, dev, -rows),
+             _q4_arg(inv_freq, "inv_freq", _F32, dev, head_dim // 2), _q4_arg(q_out, "q_out", FP16, dev, q_n),
+             _q4_arg(k_out, "k_out", FP16, dev, kv_n) if k_out is not None else None,
+             _q4_arg(v_out, "v_out", FP16, dev, kv_n) if v_out is not None else None, kp, vp, n_pages, bt,
+             max_pages, page_size, n_q_heads, n_kv_heads, head_dim, rows, style,
+             _q4_arg(error, "error", _I32, dev, -1) if error is not None else None)
+    return q_out
+
+
+def attention_q4_splits(batch: int, n_kv_heads: int, max_seq_len: int) -> int:
+    return int(lib().lmps_attention_q4_splits(batch, n_kv_heads, max_seq_len))
+
+
+def attention_q4_workspace_size(batch: int, n_q_heads: int, head_dim: int, n_splits: int) -> int:
+    return int(lib().lmps_attention_q4_workspace_size(batch, n_q_heads, head_dim, n_splits))
+
+
+def gqa_decode_attention_q4(q, k_pool, v_pool, block_table, seq_lens, out, workspace, page_size: int,
+                            n_q_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, n_splits: int, *,
+                            error: Optional[torch.Tensor] = None):
+    """gqa_decode_attention over the 4-bit cache: one query row per sequence
+    over its first ``seq_lens[b]`` positions (0: zeros)."""
+    dev, B = q.get_device(), q.shape[0]
+    n = B * n_q_heads * head_dim
+    a_q = _q4_arg(q, "q", FP16, dev, n)
+    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
+    bt, max_pages = _q4_table(block_table, dev, B)
+    ws, ws_bytes = _q4_workspace(workspace, dev)
+    _q4_call("lmps_gqa_decode_attention_q4", dev, a_q, kp, vp, n_pages, bt,
+             _q4_arg(seq_lens, "seq_lens", _I32, dev, -B), _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes,
+             max_pages, page_size, n_q_heads, n_kv_heads, head_dim, B, max_seq_len, n_splits,
+             _q4_arg(error, "error", _I32, dev, -1) if error is not None else None)
+    return out
+
+
+def gqa_decode_attention_rope_q4(qkv, pos, inv_freq, k_pool, v_pool, block_table, seq_lens, out, workspace,
+                                 page_size: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
+                                 max_seq_len: int, n_splits: int, style: int = 0, *,
+                                 error: Optional[torch.Tensor] = None):
+    """rope_kv_append_q4 + gqa_decode_attention_q4 in one call (seq_lens = pos + 1)."""
+    dev, B = qkv.get_device(), qkv.shape[0]
+    n = B * n_q_heads * head_dim
+    a_qkv = _q4_arg(qkv, "qkv", FP16, dev, n + 2 * B * n_kv_heads * head_dim)
+    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
+    bt, max_pages = _q4_table(block_table, dev, B)
+    ws, ws_bytes = _q4_workspace(workspace, dev)
+    _q4_call("lmps_gqa_decode_attention_rope_q4", dev, a_qkv, _q4_arg(pos, "pos", _I32, dev, -B),
+             _q4_arg(inv_freq, "inv_freq", _F32, dev, head_dim // 2), style, kp, vp, n_pages, bt,
+             _q4_arg(seq_lens, "seq_lens", _I32, dev, -B), _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes,
+             max_pages, page_size, n_q_heads, n_kv_heads, head_dim, B, max_seq_len, n_splits,
+             _q4_arg(error, "error", _I32, dev, -1) if error is not None else None)
+    return out
+
+
+def prefill_q4_splits(batch: int, seq_len: int, n_q_heads: int, n_kv_heads: int, max_seq_len: int) -> int:
+    return int(lib().lmps_prefill_q4_splits(batch, seq_len, n_q_heads, n_kv_heads, max_seq_len))
+
+
+def prefill_q4_workspace_size(batch: int, seq_len: int, n_q_heads: int, head_dim: int, n_splits: int) -> int:
+    return int(lib().lmps_prefill_q4_workspace_size(batch, seq_len, n_q_heads, head_dim, n_splits))
+
+
+def prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch: int, seq_len: int, page_size: int,
+                         n_q_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, *,
+                         starts: Optional[torch.Tensor] = None, q_lens: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None, n_splits: int = 1,
+                         error: Optional[torch.Tensor] = None):
+    """Causal attention of many queries a sequence over the 4-bit cache: row
+    b * seq_len + i of ``q`` is the query at position ``starts[b] + i`` (0 + i
+    without ``starts``) for i < ``q_lens[b]`` (seq_len without); other rows of
+    ``out`` stay as they were.  The K and V of all these positions are already
+    in the cache; starts + q_lens <= ``max_seq_len``."""
+    dev = q.get_device()
+    n = batch * seq_len * n_q_heads * head_dim
+    a_q = _q4_arg(q, "q", FP16, dev, n)
+    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
+    bt, max_pages = _q4_table(block_table, dev, batch)
+    ws, ws_bytes = _q4_workspace(workspace, dev)
+    err = error if error is not None else torch.zeros(1, dtype=_I32, device=q.device)
+    _q4_call("lmps_prefill_attention_q4", dev, a_q, kp, vp, n_pages, bt,
+             _q4_arg(starts, "starts", _I32, dev, -batch) if starts is not None else None,
+             _q4_arg(q_lens, "q_lens", _I32, dev, -batch) if q_lens is not None else None,
+             _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes, max_pages, page_size, n_q_heads, n_kv_heads,
+             head_dim, batch, seq_len, max_seq_len, n_splits, _q4_arg(err, "error", _I32, dev, -1))
+    return out
+
 
 # -- two-way tensor parallelism over peer memory ----------------------------
 class PeerExchange:
