@@ -30,8 +30,8 @@
 // reads are then free of bank conflicts.
 #include <cmath>
 
+#include "attention_q4.cuh"
 #include "flash_decode.cuh"
-#include "kv_q4.cuh"
 
 namespace lmps {
 namespace q4 {
@@ -40,25 +40,19 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * kWarp;
 constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
-constexpr int kMaxHeads = 8;  // query heads per KV head
 constexpr int kOffV = kStep * kCodeBytes;
 constexpr int kOffKs = 2 * kOffV;
 constexpr int kOffVs = kOffKs + kStep * 8;
 constexpr int kStageBytes = kOffVs + kStep * 8;  // 4608
-constexpr float kScaleLog2 = kAttnScale * 1.4426950408889634f;
 
 struct AttnParams {
   const __half* q;  // [rows, n_q * 128]
   Cache c;
   const int32_t* seq_lens;  // [rows]
   __half* out;              // [rows, n_q * 128]
-  float* part_o;            // [rows, n_q, splits, 128]
-  float2* part_ml;          // [rows, n_q, splits]: max (base 2), sum
+  float* part_o;            // with more than one split: Partials
+  float2* part_ml;
   int n_q, n_splits, chunk, max_seq_len;
-  // prefill form: row b * seq + i is query i of sequence b (seq_lens unused)
-  const int32_t* starts;
-  const int32_t* q_lens;
-  int seq;
   // fused RoPE + append (qkv != nullptr)
   const __half* qkv;
   const int32_t* pos;
@@ -68,29 +62,6 @@ struct AttnParams {
   uint8_t* v_new;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t lop_or(uint32_t a, uint32_t mask) {  // (a & mask) | 0x64006400
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(d) : "r"(a), "r"(mask));
-  return d;
-}
-// Codes (minus 8) of nibbles 0 and 4 (lo) or 1 and 5 (hi) of w as a half2:
-// 0x6400 | n is 1024 + n, 0x6400 | n << 4 is 1024 + 16 n; both steps are exact.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-  const uint32_t x = lop_or(w, 0x000F000Fu);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-  const uint32_t x = lop_or(w, 0x00F000F0u);
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00)),
-                            __half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480)));  // / 16 - 72
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ void mma_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -236,21 +207,13 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   const int split = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const int G = P.n_q / P.c.n_kv;
-  int b = row, T;
-  if (P.seq > 0) {
-    b = row / P.seq;
-    const int i = row - b * P.seq;
-    if (P.q_lens && i >= P.q_lens[b]) return;  // (uniform) not a query: its output row stays
-    T = (P.starts ? P.starts[b] : 0) + i + 1;
-  } else {
-    T = P.seq_lens[row];
-  }
+  int T = P.seq_lens[row];
   if (T > P.max_seq_len || T < 0) {
     if (tid == 0) raise_error(P.c.error, kErrPosition);
     T = T < 0 ? 0 : P.max_seq_len;
   }
   const int start = split * P.chunk, end = min(T, start + P.chunk);
-  const int32_t* bt = P.c.bt + static_cast<size_t>(b) * P.c.max_pages;
+  const int32_t* bt = P.c.bt + static_cast<size_t>(row) * P.c.max_pages;
   int pnew = -1;
 
   if (P.qkv) {
@@ -428,30 +391,34 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
 }
 
 // Log-sum-exp merge of the splits of one (row, query head).
-__global__ void __launch_bounds__(kDim) attn_q4_combine_kernel(const AttnParams P) {
+__global__ void __launch_bounds__(kDim) attn_q4_combine_kernel(const Partials P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
-  if (P.seq > 0 && P.q_lens && row % P.seq >= P.q_lens[row / P.seq]) return;
+  const int h = blockIdx.y, row = blockIdx.x, d = threadIdx.x;
+  if (P.q_lens && row % P.seq >= P.q_lens[row / P.seq]) return;
   const size_t head = static_cast<size_t>(row) * P.n_q + h, r0 = head * P.n_splits;
   float M = -INFINITY;
-  for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.part_ml[r0 + s].x);
+  for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ml[r0 + s].x);
   float num = 0.0f, den = 0.0f;
   for (int s = 0; s < P.n_splits; ++s) {
-    const float2 ml = P.part_ml[r0 + s];
+    const float2 ml = P.ml[r0 + s];
     const float f = ml.x == -INFINITY ? 1.0f : ex2(ml.x - M);
-    num = fmaf(P.part_o[(r0 + s) * kDim + d], f, num);
+    num = fmaf(P.o[(r0 + s) * kDim + d], f, num);
     den = fmaf(ml.y, f, den);
   }
   P.out[head * kDim + d] = __float2half_rn(den == 0.0f ? 0.0f : num / den);
 }
 
-static int check_cache(int n_pages, int max_pages, int page_size, int n_q_heads, int n_kv_heads, int head_dim,
-                       int max_seq_len, int n_splits) {
+int combine_launch(const Partials& p, int rows, cudaStream_t stream) {
+  return lmps_launch_pdl(attn_q4_combine_kernel, dim3(rows, p.n_q), dim3(kDim), 0, stream, p);
+}
+
+int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, int n_kv_heads, int head_dim,
+                    int max_seq_len, int n_splits) {
   LMPS_CHECK_ARG(n_pages >= 1 && max_pages >= 1 && page_size >= 1 && max_seq_len >= 1);
   LMPS_CHECK_ARG(static_cast<long long>(max_pages) * page_size <= 1LL << 29);
   LMPS_CHECK_ARG(max_seq_len <= static_cast<long long>(max_pages) * page_size);
-  LMPS_CHECK_ARG(n_kv_heads >= 1 && n_q_heads >= 1 && n_q_heads % n_kv_heads == 0);
+  LMPS_CHECK_ARG(n_kv_heads >= 1 && n_q_heads >= 1 && n_q_heads % n_kv_heads == 0 && n_q_heads <= 65535);
   LMPS_CHECK_ARG(n_splits >= 1 && n_splits <= 1024);
   if (head_dim != kDim || page_size % kRun != 0 || n_q_heads / n_kv_heads > kMaxHeads) return LMPS_ERR_UNSUPPORTED;
   return LMPS_OK;
@@ -463,9 +430,8 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
                             int max_seq_len, int n_splits, int32_t* error, void* stream) {
   LMPS_CHECK_ARG(k_pool && v_pool && block_table && out);
   LMPS_CHECK_ARG(rows >= 1 && rows <= 65535);
-  const int st = check_cache(n_pages, max_pages, page_size, n_q_heads, n_kv_heads, head_dim, max_seq_len, n_splits);
+  const int st = check_attention(n_pages, max_pages, page_size, n_q_heads, n_kv_heads, head_dim, max_seq_len, n_splits);
   if (st != LMPS_OK) return st;
-  LMPS_CHECK_ARG(n_kv_heads <= 65535);
   LMPS_CHECK_ARG(lmps_aligned(k_pool, 16) && lmps_aligned(v_pool, 16) && lmps_aligned(out, 16));
   const size_t need = lmps_attention_q4_workspace_size(rows, n_q_heads, head_dim, n_splits);
   if (need > 0 && (!workspace || workspace_bytes < need)) return LMPS_ERR_WORKSPACE;
@@ -476,15 +442,13 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   P.n_splits = n_splits;
   P.max_seq_len = max_seq_len;
   P.chunk = ((max_seq_len + n_splits - 1) / n_splits + kStep - 1) / kStep * kStep;
-  if (n_splits > 1) {
-    const size_t n = static_cast<size_t>(rows) * n_q_heads * n_splits;
-    P.part_o = reinterpret_cast<float*>(workspace);
-    P.part_ml = reinterpret_cast<float2*>(P.part_o + n * kDim);
-  }
+  const Partials parts = make_partials(workspace, rows, n_q_heads, n_splits, out);
+  P.part_o = parts.o;
+  P.part_ml = parts.ml;
   cudaStream_t s = lmps_stream(stream);
   const int status = lmps_launch_pdl(attn_q4_kernel, dim3(n_splits, n_kv_heads, rows), dim3(kThreads), 0, s, P);
   if (status || n_splits == 1) return status;
-  return lmps_launch_pdl(attn_q4_combine_kernel, dim3(n_q_heads, rows), dim3(kDim), 0, s, P);
+  return combine_launch(parts, rows, s);
 }
 
 }  // namespace q4
@@ -540,31 +504,4 @@ extern "C" int lmps_gqa_decode_attention_rope_q4(const uint16_t* qkv, const int3
   P.v_new = v_pool;
   return q4::attention_launch(P, k_pool, v_pool, n_pages, block_table, out, workspace, workspace_bytes, max_pages,
                               page_size, n_q_heads, n_kv_heads, head_dim, batch, max_seq_len, n_splits, error, stream);
-}
-
-extern "C" int lmps_prefill_q4_splits(int batch, int seq_len, int n_q_heads, int n_kv_heads, int max_seq_len) {
-  (void)batch, (void)seq_len, (void)n_q_heads, (void)n_kv_heads, (void)max_seq_len;
-  return 1;
-}
-
-extern "C" size_t lmps_prefill_q4_workspace_size(int batch, int seq_len, int n_q_heads, int head_dim, int n_splits) {
-  return lmps_attention_q4_workspace_size(batch * seq_len, n_q_heads, head_dim, n_splits);
-}
-
-extern "C" int lmps_prefill_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool,
-                                         int n_pages, const int32_t* block_table, const int32_t* starts,
-                                         const int32_t* q_lens, uint16_t* out, void* workspace,
-                                         size_t workspace_bytes, int max_pages, int page_size, int n_q_heads,
-                                         int n_kv_heads, int head_dim, int batch, int seq_len, int max_seq_len,
-                                         int n_splits, int32_t* error, void* stream) {
-  LMPS_CHECK_ARG(q && error && lmps_aligned(q, 16));
-  LMPS_CHECK_ARG(batch >= 1 && seq_len >= 1 && static_cast<long long>(batch) * seq_len <= 65535);
-  q4::AttnParams P{};
-  P.q = reinterpret_cast<const __half*>(q);
-  P.starts = starts;
-  P.q_lens = q_lens;
-  P.seq = seq_len;
-  return q4::attention_launch(P, k_pool, v_pool, n_pages, block_table, out, workspace, workspace_bytes, max_pages,
-                              page_size, n_q_heads, n_kv_heads, head_dim, batch * seq_len, max_seq_len, n_splits,
-                              error, stream);
 }

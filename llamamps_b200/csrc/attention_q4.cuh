@@ -1,0 +1,63 @@
+// Shared by the attention kernels over the 4-bit KV cache: codes as fp16
+// integers, the merge of split partials, argument checks.
+#pragma once
+
+#include "kv_q4.cuh"
+
+namespace lmps {
+namespace q4 {
+
+constexpr int kMaxHeads = 8;  // query heads per KV head
+constexpr float kScaleLog2 = kAttnScale * 1.4426950408889634f;  // scores in base 2
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t lop_or(uint32_t a, uint32_t mask) {  // (a & mask) | 0x64006400
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(d) : "r"(a), "r"(mask));
+  return d;
+}
+// Codes (minus 8) of nibbles 0 and 4 (lo) or 1 and 5 (hi) of w as a half2:
+// 0x6400 | n is 1024 + n, 0x6400 | n << 4 is 1024 + 16 n; both steps are exact.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  const uint32_t x = lop_or(w, 0x000F000Fu);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  const uint32_t x = lop_or(w, 0x00F000F0u);
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00)),
+                            __half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480)));  // / 16 - 72
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Unnormalised split results of one call: O [rows, n_q, splits, 128], and per
+// (row, head, split) the max (base 2) and the sum.
+struct Partials {
+  float* o;
+  float2* ml;
+  __half* out;  // [rows, n_q * 128]
+  int n_q, n_splits;
+  const int32_t* q_lens;  // row b * seq + i with i >= q_lens[b] is left alone (NULL: all rows count)
+  int seq;
+};
+static inline Partials make_partials(void* workspace, int rows, int n_q, int n_splits, uint16_t* out) {
+  Partials p{};
+  p.o = reinterpret_cast<float*>(workspace);
+  p.ml = reinterpret_cast<float2*>(p.o + static_cast<size_t>(rows) * n_q * n_splits * kDim);
+  p.out = reinterpret_cast<__half*>(out);
+  p.n_q = n_q;
+  p.n_splits = n_splits;
+  return p;
+}
+// Launches the merge of `rows` rows.
+int combine_launch(const Partials& p, int rows, cudaStream_t stream);
+// LMPS_OK, or why the attention entry points refuse these sizes.
+int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, int n_kv_heads, int head_dim,
+                    int max_seq_len, int n_splits);
+
+}  // namespace q4
+}  // namespace lmps

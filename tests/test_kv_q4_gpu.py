@@ -305,3 +305,82 @@ def test_prefill_attention(cuda, starts, q_lens, seq, hq, hkv, page):
                     continue
                 R.close(got[b, i], *R.attend(q[b, i], *c.rows[b], s_np[b] + i + 1),
                         f"sequence {b}, query {i}, {n_splits} splits")
+
+
+def test_prefill_nan_rows_and_bad_pages(cuda):
+    """Whoever attends to a NaN row gets NaN, nobody before it does (the rows share tiles with it); a page
+    outside the pool counts as absent and is reported; rows without a position are zeros."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(11)
+    seq, hq, hkv, page = 150, 12, 2, 16
+    c = R.Cache(rng, [150, 150, 150], hkv, page, max_len=160)
+    nan = np.full((1, hkv, D), np.nan, np.float16)
+    c._write(c.k_np, 0, 70, nan)
+    c._write(c.v_np, 1, 131, nan)
+    c.k, c.v = _cu(c.k_np), _cu(c.v_np)
+    c.bt[2, 0] = c.k.shape[0]      # positions 0..15: query 0..15 has nothing left
+    c.bt[2, 4] = -7                # positions 64..79
+    q = rng.normal(0, 1, (3, seq, hq, D)).astype(np.float16)
+    seen = np.ones(150, bool)
+    seen[:16] = seen[64:80] = False
+    for n_splits in (1, 2):
+        e, out = _err(), torch.empty(3 * seq, hq * D, dtype=torch.float16, device="cuda")
+        K.prefill_attention_q4(_cu(q.reshape(3 * seq, -1)), c.k, c.v, c.bt, out, 3, seq, page, hq, hkv, D,
+                               c.max_seq_len, workspace=_ws(K.prefill_q4_workspace_size(3, seq, hq, D, n_splits)),
+                               n_splits=n_splits, error=e)
+        assert e.item() == K.Q4_ERR_PAGE
+        got = out.cpu().numpy().reshape(3, seq, hq, D)
+        for b, at in ((0, 70), (1, 131)):
+            assert np.isnan(got[b, at:]).all()
+            for i in (0, 1, at - 30, at - 1):
+                R.close(got[b, i], *R.attend(q[b, i], *c.rows[b], i + 1), f"sequence {b}, query {i}")
+        assert (got[2, :16] == 0).all()
+        k, v = c.rows[2]
+        for i in (16, 17, 63, 64, 79, 80, 149):
+            keep = seen[:i + 1]
+            n = int(keep.sum())
+            R.close(got[2, i], *R.attend(q[2, i], k[:i + 1][keep], v[:i + 1][keep], n), f"query {i}")
+
+
+def test_prefill_positions_outside_the_cache(cuda):
+    """Queries past max_seq_len see what there is, queries before position 0 nothing; reported, nothing else read."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(12)
+    seq, hq, hkv, page = 40, 6, 1, 16
+    c = R.Cache(rng, [96, 96, 96], hkv, page)
+    q = rng.normal(0, 1, (3, seq, hq, D)).astype(np.float16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    e = _err()
+    buf, out = _guarded(3 * seq, hq * D)
+    K.prefill_attention_q4(_cu(q.reshape(3 * seq, -1)), c.k, c.v, c.bt, out, 3, seq, page, hq, hkv, D, 96,
+                           starts=torch.tensor([80, -5, 2 ** 31 - 10], **i32),
+                           q_lens=torch.tensor([40, 1000, -3], **i32), error=e)
+    assert e.item() == K.Q4_ERR_POSITION and _guards_ok(buf)
+    got = out.cpu().numpy().reshape(3, seq, hq, D)
+    for i in (0, 15, 16, 39):
+        R.close(got[0, i], *R.attend(q[0, i], *c.rows[0], min(81 + i, 96)), f"query {i}")
+    assert (got[1, :5] == 0).all() and (got[2] == 7).all()
+    for i in (5, 39):
+        R.close(got[1, i], *R.attend(q[1, i], *c.rows[1], i - 4), f"query {i} from position -5")
+
+
+def test_prefill_long_context_rows(cuda):
+    """Chunk rows behind contexts of thousands of positions, through several tiles and rescales."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(13)
+    starts, seq, hq, hkv, page = [3000, 777], 96, 12, 2, 64
+    c = R.Cache(rng, [s + seq for s in starts], hkv, page, gain=2.0)
+    # scores that grow with the position, so that the running max moves often
+    q = rng.normal(0, 2, (2, seq, hq, D)).astype(np.float16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for n_splits in (1, 3, K.prefill_q4_splits(2, seq, hq, hkv, c.max_seq_len)):
+        e, out = _err(), torch.empty(2 * seq, hq * D, dtype=torch.float16, device="cuda")
+        K.prefill_attention_q4(_cu(q.reshape(2 * seq, -1)), c.k, c.v, c.bt, out, 2, seq, page, hq, hkv, D,
+                               c.max_seq_len, starts=torch.tensor(starts, **i32),
+                               workspace=_ws(K.prefill_q4_workspace_size(2, seq, hq, D, n_splits)),
+                               n_splits=n_splits, error=e)
+        assert e.item() == 0
+        got = out.cpu().numpy().reshape(2, seq, hq, D)
+        for b in range(2):
+            for i in range(0, seq, 19):
+                R.close(got[b, i], *R.attend(q[b, i], *c.rows[b], starts[b] + i + 1), f"{b}, {i}, {n_splits}")
