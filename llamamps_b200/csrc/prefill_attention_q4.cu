@@ -62,7 +62,13 @@ struct Params {
   int n_q, G, seq, n_blocks, n_splits, max_seq_len;
 };
 
-// O += A B with A (fp16) in tensor memory.
+// One MMA with its descriptors' low words computed by the caller: within a
+// 128-byte-swizzled tile only the address field moves (it never carries out
+// of its 14 bits), so a step costs an add, not a descriptor.
+__device__ __forceinline__ uint64_t desc(uint32_t lo, uint32_t hi) {
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+// D += A B with A (fp16) in tensor memory.
 __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -108,6 +114,31 @@ __device__ __forceinline__ __half scale_of(uint2 s, int g) {
 // Whether any of four fp16 numbers is not finite (exponent bits all ones).
 __device__ __forceinline__ bool any_not_finite(uint2 s) {
   return ((((s.x & 0x7C007C00u) + 0x04000400u) | ((s.y & 0x7C007C00u) + 0x04000400u)) & 0x80008000u) != 0u;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 numbers in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 struct Raw {  // a key's cached rows
@@ -266,22 +297,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   } else if (warp == 12) {
     if (lane == 0) {  // ---- MMA issuer
       const uint32_t id_s = idesc_f16(kRows, kKeys), id_o = idesc_f16(kRows, kDim) | kBMajorMN;
+      const uint64_t dk = sw128_desc(smem_u32(sk)), dv = sw128_mn_desc(smem_u32(sv), kSub);
+      const uint32_t hi_k = static_cast<uint32_t>(dk >> 32), hi_v = static_cast<uint32_t>(dv >> 32);
+      const uint32_t lo_q = static_cast<uint32_t>(sw128_desc(smem_u32(sq))), lo_k = static_cast<uint32_t>(dk),
+                     lo_v = static_cast<uint32_t>(dv);
+      constexpr uint32_t kHalf = kSub >> 4;  // the next 64 dims
       auto issue_s = [&](int t, int s) {  // S_t = Q_t K^T over 8 steps of 16 dims
+        const uint32_t a = lo_q + 2 * t * kHalf, k = lo_k + 2 * s * kHalf, d = tmem + kColS + kKeys * t;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint64_t a = sw128_desc(smem_u32(sq + (2 * t + (j >> 2)) * kSub)) + 2 * (j & 3);
-          const uint64_t k = sw128_desc(smem_u32(sk + (2 * s + (j >> 2)) * kSub)) + 2 * (j & 3);
-          mma_f16(tmem + kColS + kKeys * t, a, k, id_s, j > 0 ? 1u : 0u);
+          const uint32_t o = (j >> 2) * kHalf + 2 * (j & 3);
+          mma_f16(d, desc(a + o, hi_k), desc(k + o, hi_k), id_s, j > 0 ? 1u : 0u);
         }
         mma_commit(&s_full[t]);
       };
       auto issue_o = [&](int t, int s, bool acc) {  // O_t += P_t V over 8 steps of 16 keys
+        const uint32_t v = lo_v + 2 * s * kHalf, d = tmem + kColO + kDim * t, a = tmem + kColS + kKeys * t + kColP;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint64_t v = sw128_mn_desc(smem_u32(sv + 2 * s * kSub + 2048 * j), kSub);
-          mma_f16_ta(tmem + kColO + kDim * t, tmem + kColS + kKeys * t + kColP + 8 * j, v, id_o,
-                     (acc || j > 0) ? 1u : 0u);
-        }
+        for (int j = 0; j < 8; ++j)
+          mma_f16_ta(d, a + 8 * j, desc(v + 128 * j, hi_v), id_o, (acc || j > 0) ? 1u : 0u);
         mma_commit(&o_done[t]);
       };
       bool ok = nt > 0 && wait(q_full, 0, P.c.error, abort_v) && wait(&k_full[0], 0, P.c.error, abort_v);
@@ -317,18 +351,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     const int t = warp >> 2, quad = warp & 3, rl = 32 * quad + lane, r = r0 + kRows * t + rl;
     {  // stage Q: 16 lanes a row, dims of each 8 in mask order
       const int c = lane & 15;
-      for (int x = 0; x < 32; x += 2) {
-        const int row = 32 * quad + x + (lane >> 4), rr = r0 + kRows * t + row;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (rr < n_rows) {
-          const int i = rr / P.G, h = rr - i * P.G;
-          const uint4* src = reinterpret_cast<const uint4*>(
-              P.q + (static_cast<size_t>(b) * P.seq + i) * P.n_q * kDim + (kvh * P.G + h) * kDim);
-          v = __ldg(src + c);
+#pragma unroll 1
+      for (int x0 = 0; x0 < 32; x0 += 16) {
+        uint4 v[8];  // loads of 16 rows in flight
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int rr = r0 + kRows * t + 32 * quad + x0 + 2 * x + (lane >> 4);
+          v[x] = make_uint4(0u, 0u, 0u, 0u);
+          if (rr < n_rows) {
+            const int i = rr / P.G, h = rr - i * P.G;
+            v[x] = __ldg(reinterpret_cast<const uint4*>(P.q + (static_cast<size_t>(b) * P.seq + i) * P.n_q * kDim +
+                                                        (kvh * P.G + h) * kDim) + c);
+          }
         }
-        const uint4 m = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                                   __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        *reinterpret_cast<uint4*>(sq + (2 * t + (c >> 3)) * kSub + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = m;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int row = 32 * quad + x0 + 2 * x + (lane >> 4);
+          const uint4 m = make_uint4(__byte_perm(v[x].x, v[x].z, 0x5410), __byte_perm(v[x].x, v[x].z, 0x7632),
+                                     __byte_perm(v[x].y, v[x].w, 0x5410), __byte_perm(v[x].y, v[x].w, 0x7632));
+          *reinterpret_cast<uint4*>(sq + (2 * t + (c >> 3)) * kSub + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = m;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -351,21 +393,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         const uint32_t gone[4] = {av[0], av[1], av[2], av[3]};
         const bool masked = k0 + kKeys > lim_min || (gone[0] | gone[1] | gone[2] | gone[3]) != 0u;  // (uniform)
         const int nv = lim - k0;  // columns below it count
-        auto valid = [&](int c) { return c < nv && !((gone[c >> 5] >> (c & 31)) & 1u); };
+        auto mask = [&](uint32_t (&sc)[64], int c0) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c0 + c >= nv || ((gone[(c0 + c) >> 5] >> (c & 31)) & 1u)) sc[c] = 0xFF800000u;  // -inf
+        };
         // row max: columns 0..63, then 64..127 (kept in registers)
         uint32_t sc[64];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           tmem_ld64(ts + 64 * half, sc);
-          if (masked) {
+          if (masked) mask(sc, 64 * half);
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (valid(64 * half + c)) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sc[c]));
-          } else {
-#pragma unroll
-            for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sc[c]));
-          }
+          for (int c = 0; c < 64; c += 2)
+            mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(sc[c]), __uint_as_float(sc[c + 1]));
         }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kScaleLog2;
         const float mnew = fmaxf(m_used, mt);
@@ -389,28 +431,32 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
           if (grow) m_used = mnew;
         }
         const float nm = m_used == -INFINITY ? 0.0f : -m_used;
-        float sm[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t nm2 = pair(nm, nm), scale2 = pair(kScaleLog2, kScaleLog2);
+        uint64_t sm[4] = {0ull, 0ull, 0ull, 0ull};
         // P over S's upper columns: keys 64..127 from the registers first (their scores lay there),
         // then keys 0..63 read again
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
-          if (half == 0) tmem_ld64(ts, sc);
+          if (half == 0) {
+            tmem_ld64(ts, sc);
+            if (masked) mask(sc, 0);
+          }
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            float a0 = ex2(fmaf(__uint_as_float(sc[2 * e]), kScaleLog2, nm));
-            float a1 = ex2(fmaf(__uint_as_float(sc[2 * e + 1]), kScaleLog2, nm));
-            if (masked) {
-              a0 = valid(64 * half + 2 * e) ? a0 : 0.0f;
-              a1 = valid(64 * half + 2 * e + 1) ? a1 : 0.0f;
-            }
-            sm[e & 3] += a0 + a1;
+            float a0, a1;
+            unpair(fma2(pair(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), scale2, nm2), a0, a1);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            sm[e & 3] = add2(sm[e & 3], pair(a0, a1));
             const __half2 hh = __floats2half2_rn(a0, a1);
             pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
           }
           tmem_st32(ts + kColP + 32 * half, pk);
         }
-        l += (sm[0] + sm[1]) + (sm[2] + sm[3]);
+        float s0, s1;
+        unpair(add2(add2(sm[0], sm[1]), add2(sm[2], sm[3])), s0, s1);
+        l += s0 + s1;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
