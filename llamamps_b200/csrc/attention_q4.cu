@@ -14,17 +14,20 @@
 // spend 15 of 16 rows on nothing, and its operands would have to be written
 // to shared memory as fp16 first; the work here is unpacking nibbles.
 // Fragments come straight from the nibbles:
-//   K (A operand, rows = positions): word 4g + t of a row holds the dims
-//     32g + 8t + 0..7; masking gives pairs (n, n + 4), and the sum over dims
-//     does not care about their order, so q is loaded in the same order.
-//   V (A operand, rows = dims): the halfwords 4(g8) .. of two positions are
-//     joined by one byte permute, and masking then gives (position 2t,
-//     position 2t + 1) pairs of one dim: no transpose.
+//   K (A operand, rows = positions): ldmatrix gives lane (g8, t) word 4g + t
+//     of row g8, the dims 32g + 8t + 0..7; masking gives pairs (n, n + 4), and
+//     the sum over dims does not care about their order, so q is loaded in the
+//     same order.
+//   V (A operand, rows = dims): a transposing ldmatrix over halfwords (4 dims)
+//     gives halfword g8 of positions 2t and 2t + 1 in one register, and masking
+//     then gives (position 2t, position 2t + 1) pairs of one dim.
 //     m-tile 2g + m: rows r < 8 are dims 32g + 4r + 2m, rows r >= 8 the dims
 //     32g + 4(r - 8) + 2m + 1; a lane ends with 4 consecutive dims per group.
 //
-// One item (split, KV head, sequence) per CTA of 4 warps.  A warp walks its
-// own 32-position steps (every 4th of the split) through its own ring of
+// One piece of a sequence and a KV head per CTA of 4 warps.  The n_splits *
+// rows pieces that a call has room for are shared out by the sequences' lengths
+// (in the kernel: lengths are on the device), so that ragged batches finish
+// together.  A warp walks its own 32-position steps (every 4th) through its own ring of
 // cp.async stages; no CTA-wide barrier until the warps' states meet.  16-byte
 // chunk c of a staged row r is stored at c ^ ((r >> 1) & 3): both fragment
 // reads are then free of bank conflicts.
@@ -52,7 +55,8 @@ struct AttnParams {
   __half* out;              // [rows, n_q * 128]
   float* part_o;            // with more than one split: Partials
   float2* part_ml;
-  int n_q, n_splits, chunk, max_seq_len;
+  int2* pieces;             // with more than one split: first piece and their number, per row
+  int n_q, n_splits, rows, max_seq_len;
   // fused RoPE + append (qkv != nullptr)
   const __half* qkv;
   const int32_t* pos;
@@ -60,23 +64,44 @@ struct AttnParams {
   int style;
   uint8_t* k_new;
   uint8_t* v_new;
+
+  // Positions of a row that are in the cache.
+  __device__ __forceinline__ int length(int row) const { return max(0, min(seq_lens[row], max_seq_len)); }
 };
 
+// mma.sync m16n8k16 without `volatile`: the scheduler may move it among the unpacking.
 __device__ __forceinline__ void mma_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void lds_scales(uint32_t a, float (&s)[4]) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+__device__ __forceinline__ uint32_t transpose(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// Four 8 x 8 matrices of 16-bit elements, 16-byte rows at the lanes' addresses (lanes 8i .. 8i+7: matrix i).
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void load_scales(const unsigned char* p, float (&s)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
   const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
   const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
   s[0] = lo.x;
@@ -106,54 +131,52 @@ struct State {
 };
 
 // Folds the staged step (first position p0, `end` exclusive; `ok` bit x: run x
-// is loaded) into the state.
-__device__ __forceinline__ void fold_step(uint32_t st, int p0, int end, uint32_t ok, const uint32_t (&qf)[16],
-                                          State& S) {
+// is loaded) into the state.  kFull: every position counts.
+template <bool kFull>
+__device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int end, uint32_t ok,
+                                          const uint32_t (&qf)[16], State& S) {
   const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-  const bool full = ok == 3u && p0 + kStep <= end;
+  // this lane's row address for ldmatrix: row lane & 7, chunk lane >> 3, stored at chunk ^ ((row >> 1) & 3)
+  const uint32_t lm = smem_u32(st) + (lane & 7) * kCodeBytes + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
   float s[2][4];
   bool v0[2], v1[2];  // rows g8 / g8 + 8 of each run count
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const bool run = (ok >> x) & 1u;
-    v0[x] = full || (run && p0 + 16 * x + g8 < end);
-    v1[x] = full || (run && p0 + 16 * x + g8 + 8 < end);
-    const uint32_t kr = st + (16 * x + g8) * kCodeBytes + 4 * t4;
+    v0[x] = kFull || (run && p0 + 16 * x + g8 < end);
+    v1[x] = kFull || (run && p0 + 16 * x + g8 + 8 < end);
+    uint32_t w0[4], w1[4];  // word 4g + t of rows g8 and g8 + 8
+    ldmatrix4(lm + 16 * x * kCodeBytes, w0);
+    ldmatrix4(lm + (16 * x + 8) * kCodeBytes, w1);
     float ks0[4], ks1[4];
-    lds_scales(st + kOffKs + (16 * x + g8) * 8, ks0);
-    lds_scales(st + kOffKs + (16 * x + g8 + 8) * 8, ks1);
+    load_scales(st + kOffKs + (16 * x + g8) * 8, ks0);
+    load_scales(st + kOffKs + (16 * x + g8 + 8) * 8, ks1);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const uint32_t off = static_cast<uint32_t>(g ^ ((g8 >> 1) & 3)) << 4;
-      const uint32_t w0 = lds32(kr + off), w1 = lds32(kr + 8 * kCodeBytes + off);
+      const uint32_t a0 = w0[g], a1 = w1[g];
       float a[4];
-      mma_zero(a, codes_lo(w0), codes_lo(w1), codes_hi(w0), codes_hi(w1), qf[4 * g], qf[4 * g + 1]);
-      fd::mma_16816(a, codes_lo(w0 >> 8), codes_lo(w1 >> 8), codes_hi(w0 >> 8), codes_hi(w1 >> 8), qf[4 * g + 2],
-                    qf[4 * g + 3]);
-      if (g == 0) {
-        s[x][0] = ks0[0] * a[0];
-        s[x][1] = ks0[0] * a[1];
-        s[x][2] = ks1[0] * a[2];
-        s[x][3] = ks1[0] * a[3];
-      } else {
-        s[x][0] = fmaf(ks0[g], a[0], s[x][0]);
-        s[x][1] = fmaf(ks0[g], a[1], s[x][1]);
-        s[x][2] = fmaf(ks1[g], a[2], s[x][2]);
-        s[x][3] = fmaf(ks1[g], a[3], s[x][3]);
+      mma_zero(a, codes_lo(a0), codes_lo(a1), codes_hi(a0), codes_hi(a1), qf[4 * g], qf[4 * g + 1]);
+      mma(a, codes_lo(a0 >> 8), codes_lo(a1 >> 8), codes_hi(a0 >> 8), codes_hi(a1 >> 8), qf[4 * g + 2], qf[4 * g + 3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ks = i < 2 ? ks0[g] : ks1[g];
+        s[x][i] = g == 0 ? ks * a[i] : fmaf(ks, a[i], s[x][i]);
       }
     }
+    if (!kFull) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[x][i] = (i < 2 ? v0[x] : v1[x]) ? s[x][i] * kScaleLog2 : -INFINITY;
+      for (int i = 0; i < 4; ++i) s[x][i] = (i < 2 ? v0[x] : v1[x]) ? s[x][i] : -INFINITY;
+    }
   }
-  float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
-  float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+  float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * kScaleLog2;
+  float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * kScaleLog2;
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
   }
-  const float n0 = fmaxf(S.m0, mx0), n1 = fmaxf(S.m1, mx1);
-  if (__any_sync(0xffffffffu, n0 != S.m0 || n1 != S.m1)) {  // some head's max grew
+  if (__any_sync(0xffffffffu, mx0 > S.m0 || mx1 > S.m1)) {  // some head's max grew
+    const float n0 = fmaxf(S.m0, mx0), n1 = fmaxf(S.m1, mx1);
     // a head without a position yet keeps max -inf; its sums are zero
     const float a0 = n0 == -INFINITY ? 1.0f : ex2(S.m0 - n0), a1 = n1 == -INFINITY ? 1.0f : ex2(S.m1 - n1);
     S.l0 *= a0;
@@ -168,34 +191,33 @@ __device__ __forceinline__ void fold_step(uint32_t st, int p0, int end, uint32_t
     S.m0 = n0;
     S.m1 = n1;
   }
-  const float r0 = n0 == -INFINITY ? 0.0f : n0, r1 = n1 == -INFINITY ? 0.0f : n1;
-  const uint32_t sel = (g8 & 1) ? 0x7632u : 0x5410u;
+  const float r0 = S.m0 == -INFINITY ? 0.0f : -S.m0, r1 = S.m1 == -INFINITY ? 0.0f : -S.m1;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const float e0 = ex2(s[x][0] - r0), e1 = ex2(s[x][1] - r1), e2 = ex2(s[x][2] - r0), e3 = ex2(s[x][3] - r1);
+    const float e0 = ex2(fmaf(s[x][0], kScaleLog2, r0)), e1 = ex2(fmaf(s[x][1], kScaleLog2, r1));
+    const float e2 = ex2(fmaf(s[x][2], kScaleLog2, r0)), e3 = ex2(fmaf(s[x][3], kScaleLog2, r1));
     S.l0 += e0 + e2;
     S.l1 += e1 + e3;
+    uint32_t u0[4], u1[4];  // halfword g8 of chunk g: positions 2t, 2t + 1 and 2t + 8, 2t + 9
+    ldmatrix4_trans(lm + kOffV + 16 * x * kCodeBytes, u0);
+    ldmatrix4_trans(lm + kOffV + (16 * x + 8) * kCodeBytes, u1);
     float vs0[4], vs1[4];
-    lds_scales(st + kOffVs + (16 * x + g8) * 8, vs0);
-    lds_scales(st + kOffVs + (16 * x + g8 + 8) * 8, vs1);
-    // rows that do not count: whatever lies there as a scale, zero
-    if (!full) {
+    load_scales(st + kOffVs + (16 * x + g8) * 8, vs0);
+    load_scales(st + kOffVs + (16 * x + g8 + 8) * 8, vs1);
+    if (!kFull) {  // rows that do not count: whatever lies there as a scale, zero
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         vs0[g] = v0[x] ? vs0[g] : 0.0f;
         vs1[g] = v1[x] ? vs1[g] : 0.0f;
       }
     }
-    const uint32_t vr = st + kOffV + (16 * x + 2 * t4) * kCodeBytes + 4 * (g8 >> 1);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const uint32_t off = static_cast<uint32_t>(g ^ t4) << 4;
-      const uint32_t u = __byte_perm(lds32(vr + off), lds32(vr + kCodeBytes + off), sel);
-      const uint32_t w = __byte_perm(lds32(vr + 8 * kCodeBytes + off), lds32(vr + 9 * kCodeBytes + off), sel);
-      const uint32_t b0 = fd::movmatrix_t(fd::pack_half2(e0 * vs0[g], e1 * vs0[g]));
-      const uint32_t b1 = fd::movmatrix_t(fd::pack_half2(e2 * vs1[g], e3 * vs1[g]));
-      fd::mma_16816(S.o[2 * g], codes_lo(u), codes_hi(u), codes_lo(w), codes_hi(w), b0, b1);
-      fd::mma_16816(S.o[2 * g + 1], codes_lo(u >> 8), codes_hi(u >> 8), codes_lo(w >> 8), codes_hi(w >> 8), b0, b1);
+      const uint32_t u = u0[g], w = u1[g];
+      const uint32_t b0 = transpose(fd::pack_half2(e0 * vs0[g], e1 * vs0[g]));
+      const uint32_t b1 = transpose(fd::pack_half2(e2 * vs1[g], e3 * vs1[g]));
+      mma(S.o[2 * g], codes_lo(u), codes_hi(u), codes_lo(w), codes_hi(w), b0, b1);
+      mma(S.o[2 * g + 1], codes_lo(u >> 8), codes_hi(u >> 8), codes_lo(w >> 8), codes_hi(w >> 8), b0, b1);
     }
   }
 }
@@ -204,15 +226,57 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
   __shared__ Smem S;
-  const int split = blockIdx.x, kvh = blockIdx.y, row = blockIdx.z;
+  const int kvh = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const int G = P.n_q / P.c.n_kv;
-  int T = P.seq_lens[row];
-  if (T > P.max_seq_len || T < 0) {
-    if (tid == 0) raise_error(P.c.error, kErrPosition);
-    T = T < 0 ? 0 : P.max_seq_len;
+  int row = blockIdx.x, T, start = 0, end;
+  if (P.n_splits == 1) {
+    T = P.length(row);
+    end = T;
+  } else {
+    // Pieces of equal size: blockIdx.x counts them over the rows in order, every warp finds the
+    // row of its own (`cut` is at least total / ((n_splits - 1) rows), so with a last, shorter piece
+    // per row there are at most n_splits * rows).
+    unsigned long long total = 0ull;
+    for (int r = lane; r < P.rows; r += kWarp) total += P.length(r);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const unsigned long long share = static_cast<unsigned long long>(P.n_splits - 1) * P.rows;
+    constexpr int kPiece = kWarps * kStep;
+    const int cut = max(1, static_cast<int>((total + share * kPiece - 1) / (share * kPiece))) * kPiece;
+    int before = 0, n = 0;
+    bool found = false;
+    for (int r0 = 0; r0 < P.rows && !found; r0 += kWarp) {
+      const int r = r0 + lane;
+      const int len = r < P.rows ? P.length(r) : 0;
+      const int mine = r < P.rows ? max(1, (len + cut - 1) / cut) : 0;
+      int sum = mine;  // inclusive prefix
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, static_cast<int>(blockIdx.x) < before + sum);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        row = r0 + l;
+        T = __shfl_sync(0xffffffffu, len, l);
+        n = __shfl_sync(0xffffffffu, mine, l);
+        before += __shfl_sync(0xffffffffu, sum - mine, l);
+        found = true;
+      } else {
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    if (!found) return;  // (uniform) fewer pieces than the grid has room for
+    start = (static_cast<int>(blockIdx.x) - before) * cut;
+    end = min(T, start + cut);
+    if (start == 0 && kvh == 0 && tid == 0) P.pieces[row] = make_int2(before, n);
   }
-  const int start = split * P.chunk, end = min(T, start + P.chunk);
+  if (tid == 0 && kvh == 0 && start == 0) {
+    const int given = P.seq_lens[row];
+    if (given < 0 || given > P.max_seq_len) raise_error(P.c.error, kErrPosition);
+  }
   const int32_t* bt = P.c.bt + static_cast<size_t>(row) * P.c.max_pages;
   int pnew = -1;
 
@@ -275,6 +339,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
 
   const uint32_t ring = smem_u32(&S.stage[warp][0][0]);
   const size_t scale_off = static_cast<size_t>(P.c.page_size) * kCodeBytes;
+  const bool one_page = P.c.page_size % kStep == 0;  // a step's two runs lie in one page
   // Page of the run at position p (or -1: past the end or a bad page).
   auto page_of = [&](int p) {
     if (p >= end) return -1;
@@ -283,29 +348,33 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
     if (lane == 0) raise_error(P.c.error, kErrPage);
     return -1;
   };
-  // Copies the step at p0 into stage sb; returns the bits of the loaded runs.
-  auto load = [&](int p0, int sb, int page0, int page1) {
+  // Pages of the two runs of the step at p.
+  auto pages_of = [&](int p) {
+    const int a = page_of(p);
+    return make_int2(a, one_page ? (p + 16 < end ? a : -1) : page_of(p + 16));
+  };
+  // Copies the step at p0 into stage sb; returns the bits of the loaded runs.  Code chunk i of a run
+  // (row i / 4) goes to chunk (i & 3) ^ ((row >> 1) & 3) of its row; 8 rows on that is the same place.
+  const uint32_t code_dst = (lane >> 2) * kCodeBytes + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  auto load = [&](int p0, int sb, int2 pages) {
     const uint32_t st = ring + sb * kStageBytes;
     uint32_t ok = 0u;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int page = x ? page1 : page0;
+      const int page = x ? pages.y : pages.x;
       if (page < 0) continue;
       ok |= 1u << x;
       const int p = p0 + 16 * x, off = p - P.c.page_index(p) * P.c.page_size;
-      const size_t blk = P.c.block(page, kvh);
-      const uint8_t* kc = P.c.k + blk + off * kCodeBytes;
-      const uint8_t* vc = P.c.v + blk + off * kCodeBytes;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = lane + 32 * j, r = i >> 2;
-        const uint32_t d = st + (16 * x + r) * kCodeBytes + (((i & 3) ^ ((r >> 1) & 3)) << 4);
-        cp16(d, kc + 16 * i);
-        cp16(d + kOffV, vc + 16 * i);
+      const size_t at = P.c.block(page, kvh), code = at + off * kCodeBytes + 16 * lane;
+      const uint32_t d = st + 16 * x * kCodeBytes + code_dst;
+      cp16(d, P.c.k + code);
+      cp16(d + 8 * kCodeBytes, P.c.k + code + 8 * kCodeBytes);
+      cp16(d + kOffV, P.c.v + code);
+      cp16(d + kOffV + 8 * kCodeBytes, P.c.v + code + 8 * kCodeBytes);
+      if (lane < 16) {  // scales: 8 chunks of K, 8 of V
+        const uint8_t* src = (lane < 8 ? P.c.k : P.c.v) + at + scale_off + off * 8 + 16 * (lane & 7);
+        cp16(st + (lane < 8 ? kOffKs : kOffVs) + 128 * x + 16 * (lane & 7), src);
       }
-      if (lane < 8) cp16(st + kOffKs + 128 * x + 16 * lane, P.c.k + blk + scale_off + off * 8 + 16 * lane);
-      else if (lane < 16)
-        cp16(st + kOffVs + 128 * x + 16 * (lane - 8), P.c.v + blk + scale_off + off * 8 + 16 * (lane - 8));
     }
     return ok;
   };
@@ -316,16 +385,15 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   A.m0 = A.m1 = -INFINITY;
   A.l0 = A.l1 = 0.0f;
   const int first = start + warp * kStep, stride = kWarps * kStep;
-  uint32_t ok = first < end ? load(first, 0, page_of(first), page_of(first + 16)) : 0u;
+  uint32_t ok = first < end ? load(first, 0, pages_of(first)) : 0u;
   asm volatile("cp.async.commit_group;" ::: "memory");
   int sb = 0;
-  int np0 = page_of(first + stride), np1 = page_of(first + stride + 16);
+  int2 next = pages_of(first + stride);
   for (int p0 = first; p0 < end; p0 += stride) {
     uint32_t next_ok = 0u;
-    if (p0 + stride < end) next_ok = load(p0 + stride, sb ^ 1, np0, np1);
+    if (p0 + stride < end) next_ok = load(p0 + stride, sb ^ 1, next);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    np0 = page_of(p0 + 2 * stride);
-    np1 = page_of(p0 + 2 * stride + 16);
+    next = pages_of(p0 + 2 * stride);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
     const uint32_t st = ring + sb * kStageBytes;
@@ -339,7 +407,9 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(st + kOffVs + r * 8 + 4 * (lane - 2)), "r"(S.vnew[14 + lane]) : "memory");
       __syncwarp();
     }
-    if (ok) fold_step(st, p0, end, ok, qf, A);
+    const unsigned char* sp = &S.stage[warp][sb][0];
+    if (ok == 3u && p0 + kStep <= end) fold_step<true>(sp, p0, end, ok, qf, A);
+    else if (ok) fold_step<false>(sp, p0, end, ok, qf, A);
     __syncwarp();  // the stage is free
     ok = next_ok;
     sb ^= 1;
@@ -380,37 +450,78 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
       num = fmaf(S.wo[i][h][d], f, num);
       den = fmaf(S.wl[i][h], f, den);
     }
-    const size_t head = static_cast<size_t>(row) * P.n_q + kvh * G + h;
     if (P.n_splits == 1) {
-      P.out[head * kDim + d] = __float2half_rn(den == 0.0f ? 0.0f : num / den);
+      P.out[(static_cast<size_t>(row) * P.n_q + kvh * G + h) * kDim + d] =
+          __float2half_rn(den == 0.0f ? 0.0f : num / den);
     } else {
-      P.part_o[(head * P.n_splits + split) * kDim + d] = num;
-      if (d == 0) P.part_ml[head * P.n_splits + split] = make_float2(M, den);
+      const size_t at = static_cast<size_t>(blockIdx.x) * P.n_q + kvh * G + h;
+      P.part_o[at * kDim + d] = num;
+      if (d == 0) P.part_ml[at] = make_float2(M, den);
     }
   }
 }
 
-// Log-sum-exp merge of the splits of one (row, query head).
-__global__ void __launch_bounds__(kDim) attn_q4_combine_kernel(const Partials P) {
+// Log-sum-exp merge of the pieces of one (row, query head).  A warp takes every
+// 8th piece, 4 dims a lane; the partials of the first 64 pieces are on their
+// way before the weights are known.
+constexpr int kMergeWarps = 8, kMergeLoads = 8;
+__global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(const Partials P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
-  const int h = blockIdx.y, row = blockIdx.x, d = threadIdx.x;
+  __shared__ float red[2][kMergeWarps];
+  __shared__ float4 acc[kMergeWarps][kWarp];
+  const int h = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (P.q_lens && row % P.seq >= P.q_lens[row / P.seq]) return;
-  const size_t head = static_cast<size_t>(row) * P.n_q + h, r0 = head * P.n_splits;
-  float M = -INFINITY;
-  for (int s = 0; s < P.n_splits; ++s) M = fmaxf(M, P.ml[r0 + s].x);
-  float num = 0.0f, den = 0.0f;
-  for (int s = 0; s < P.n_splits; ++s) {
-    const float2 ml = P.ml[r0 + s];
-    const float f = ml.x == -INFINITY ? 1.0f : ex2(ml.x - M);
-    num = fmaf(P.o[(r0 + s) * kDim + d], f, num);
-    den = fmaf(ml.y, f, den);
+  const int2 pc = P.pieces ? P.pieces[row] : make_int2(row * P.n_splits, P.n_splits);
+  const size_t first = static_cast<size_t>(pc.x) * P.n_q + h;  // piece s at first + s * n_q
+  const float2* ml = P.ml + first;
+  const float4* o = reinterpret_cast<const float4*>(P.o + first * kDim) + lane;
+  const size_t stride = static_cast<size_t>(P.n_q) * (kDim / 4);
+  float4 v[kMergeLoads];
+#pragma unroll
+  for (int i = 0; i < kMergeLoads; ++i) {
+    const int s = warp + kMergeWarps * i;
+    v[i] = s < pc.y ? o[s * stride] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
-  P.out[head * kDim + d] = __float2half_rn(den == 0.0f ? 0.0f : num / den);
+  float M = -INFINITY;
+  for (int s = tid; s < pc.y; s += kMergeWarps * kWarp) M = fmaxf(M, ml[static_cast<size_t>(s) * P.n_q].x);
+  M = warp_max(M);
+  if (lane == 0) red[0][warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMergeWarps; ++i) M = fmaxf(M, red[0][i]);
+  float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float den = 0.0f;
+  auto add = [&](int s, const float4& x) {
+    const float2 m = ml[static_cast<size_t>(s) * P.n_q];
+    // a piece without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
+    const float f = m.x == -INFINITY ? 1.0f : ex2(m.x - M);
+    den = fmaf(m.y, f, den);
+    num.x = fmaf(x.x, f, num.x);
+    num.y = fmaf(x.y, f, num.y);
+    num.z = fmaf(x.z, f, num.z);
+    num.w = fmaf(x.w, f, num.w);
+  };
+#pragma unroll
+  for (int i = 0; i < kMergeLoads; ++i)
+    if (warp + kMergeWarps * i < pc.y) add(warp + kMergeWarps * i, v[i]);
+  for (int s = warp + kMergeWarps * kMergeLoads; s < pc.y; s += kMergeWarps) add(s, o[s * stride]);
+  acc[warp][lane] = num;
+  if (lane == 0) red[1][warp] = den;
+  __syncthreads();
+  if (tid >= kDim) return;
+  const float* a = reinterpret_cast<const float*>(&acc[0][0]) + tid;
+  float n = 0.0f, d = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMergeWarps; ++i) {
+    n += a[i * kDim];
+    d += red[1][i];
+  }
+  P.out[(static_cast<size_t>(row) * P.n_q + h) * kDim + tid] = __float2half_rn(d == 0.0f ? 0.0f : n / d);
 }
 
 int combine_launch(const Partials& p, int rows, cudaStream_t stream) {
-  return lmps_launch_pdl(attn_q4_combine_kernel, dim3(rows, p.n_q), dim3(kDim), 0, stream, p);
+  return lmps_launch_pdl(attn_q4_combine_kernel, dim3(rows, p.n_q), dim3(kMergeWarps * kWarp), 0, stream, p);
 }
 
 int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, int n_kv_heads, int head_dim,
@@ -441,12 +552,14 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   P.n_q = n_q_heads;
   P.n_splits = n_splits;
   P.max_seq_len = max_seq_len;
-  P.chunk = ((max_seq_len + n_splits - 1) / n_splits + kStep - 1) / kStep * kStep;
-  const Partials parts = make_partials(workspace, rows, n_q_heads, n_splits, out);
+  P.rows = rows;
+  Partials parts = make_partials(workspace, rows, n_q_heads, n_splits, out);
+  P.pieces = reinterpret_cast<int2*>(parts.ml + static_cast<size_t>(rows) * n_q_heads * n_splits);
+  parts.pieces = P.pieces;
   P.part_o = parts.o;
   P.part_ml = parts.ml;
   cudaStream_t s = lmps_stream(stream);
-  const int status = lmps_launch_pdl(attn_q4_kernel, dim3(n_splits, n_kv_heads, rows), dim3(kThreads), 0, s, P);
+  const int status = lmps_launch_pdl(attn_q4_kernel, dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), dim3(kThreads), 0, s, P);
   if (status || n_splits == 1) return status;
   return combine_launch(parts, rows, s);
 }
@@ -458,18 +571,20 @@ using namespace lmps;
 
 extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len) {
   if (batch <= 0 || n_kv_heads <= 0 || max_seq_len <= 0) return 1;
-  const long long items = static_cast<long long>(batch) * n_kv_heads;
-  const int tiles = (max_seq_len + q4::kWarps * q4::kStep - 1) / (q4::kWarps * q4::kStep);
-  long long cap = (4 * 148) / items;
-  cap = cap < 1 ? 1 : cap > tiles ? tiles : cap;
-  if (cap > 256) cap = 256;
-  const int per = static_cast<int>((tiles + cap - 1) / cap);
-  return (tiles + per - 1) / per;
+  // Four CTAs per SM run at once (128 registers).  Short caches and batches that fill the GPU several
+  // times over are not split; else as many pieces as run at once, but none below 128 positions.
+  const long long items = static_cast<long long>(batch) * n_kv_heads, slots = 4 * 148;
+  if (max_seq_len <= 2 * q4::kWarps * q4::kStep || items >= 4 * slots) return 1;
+  const long long most = (max_seq_len + q4::kWarps * q4::kStep - 1) / (q4::kWarps * q4::kStep);
+  long long n = slots / items;
+  n = n < 1 ? 1 : n > most ? most : n;
+  return static_cast<int>(n > 1023 ? 1024 : n + 1);
 }
 
 extern "C" size_t lmps_attention_q4_workspace_size(int batch, int n_q_heads, int head_dim, int n_splits) {
   if (n_splits <= 1 || batch <= 0 || n_q_heads <= 0 || head_dim <= 0) return 0;
-  return static_cast<size_t>(batch) * n_q_heads * n_splits * (head_dim * sizeof(float) + sizeof(float2));
+  return static_cast<size_t>(batch) * n_splits * n_q_heads * (head_dim * sizeof(float) + sizeof(float2)) +
+         static_cast<size_t>(batch) * sizeof(int2);
 }
 
 extern "C" int lmps_gqa_decode_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool,

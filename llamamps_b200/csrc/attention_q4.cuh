@@ -34,11 +34,13 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Unnormalised split results of one call: O [rows, n_q, splits, 128], and per
-// (row, head, split) the max (base 2) and the sum.
+// Unnormalised results of the pieces of a call: O [pieces, n_q, 128], and per
+// (piece, head) the max (base 2) and the sum.  Row r has pieces[r].y of them
+// from pieces[r].x on; n_splits from r * n_splits on where `pieces` is NULL.
 struct Partials {
   float* o;
   float2* ml;
+  const int2* pieces;
   __half* out;  // [rows, n_q * 128]
   int n_q, n_splits;
   const int32_t* q_lens;  // row b * seq + i with i >= q_lens[b] is left alone (NULL: all rows count)

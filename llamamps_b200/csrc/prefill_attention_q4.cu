@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int h = r - qi * P.G;
         const size_t head = (static_cast<size_t>(b) * P.seq + qi) * P.n_q + kvh * P.G + h;
-        const size_t part = head * P.n_splits + split;
+        const size_t part = ((static_cast<size_t>(b) * P.seq + qi) * P.n_splits + split) * P.n_q + kvh * P.G + h;
         if (P.n_splits > 1 && r < n_rows) P.part_ml[part] = make_float2(m_used, l);
 #pragma unroll 1
         for (int cc = 0; cc < kDim; cc += 32) {

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import call, lib
+from ._lib import call, check, lib
 
 FP16 = torch.float16
 
@@ -307,38 +307,47 @@ Q4_ERR_TIMEOUT, Q4_ERR_PAGE, Q4_ERR_POSITION = 1, 2, 4
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 
 
-def _q4_arg(t: torch.Tensor, name: str, dtype, dev: int, numel: int) -> int:
-    """Address of an argument of the 4-bit cache's kernels: on device ``dev``
-    (the first argument's), of this type, contiguous, exactly ``numel``
-    elements (at least, for a negative one)."""
-    if t.get_device() != dev or dev < 0:
+def _q4_explain(dev: int, named) -> None:
+    """Raises for the first of (name, tensor, dtype, elements) that is not on
+    device ``dev`` (the first argument's), of this type, contiguous and of
+    this many elements (at least, for a negative number)."""
+    for name, t, dtype, n in named:
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor (the decode path has no CPU fallback)")
-        raise ValueError(f"{name} is on another device than the call's other tensors")
-    if t.dtype is not dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    n = t.numel()
-    if n != numel if numel >= 0 else n < -numel:
-        raise ValueError(f"{name}: {n} elements, expected {abs(numel)}")
-    return t.data_ptr()
+        if t.get_device() != dev:
+            raise ValueError(f"{name} is on another device than the call's other tensors")
+        if t.dtype is not dtype:
+            raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.numel() != n if n >= 0 else t.numel() < -n:
+            raise ValueError(f"{name}: {t.numel()} elements, expected {abs(n)}")
 
 
-def _q4_pools(k_pool, v_pool, dev: int, page_size: int, n_kv_heads: int):
-    """Addresses of one layer's pools and their number of pages."""
-    shape = k_pool.shape
-    if len(shape) != 3 or shape[1] != n_kv_heads or shape[2] != page_size * Q4_ROW_BYTES:
-        raise ValueError(f"k_pool: shape {tuple(shape)}, expected [n_pages, {n_kv_heads}, "
+def _q4_arg(t: torch.Tensor, name: str, dtype, dev: int, n: int) -> int:
+    """Address of an argument after :func:`_q4_explain`'s checks (the attribute
+    reads are most of an eager call's host time: 0.06 us each, 5 a tensor)."""
+    m = t.numel()
+    if t.dtype is dtype and t.get_device() == dev and dev >= 0 and (m == n or m >= -n > 0) and t.is_contiguous():
+        return t.data_ptr()
+    _q4_explain(dev, ((name, t, dtype, n),))
+    raise RuntimeError(f"{name} must be a CUDA tensor")
+
+
+def _q4_cache(k_pool, v_pool, block_table, dev: int, page_size: int, n_kv_heads: int, rows: int):
+    """(k, v, n_pages, block_table, max_pages) of one layer's pools and a table of ``rows`` rows at least."""
+    shape, table = k_pool.shape, block_table.shape
+    if len(shape) != 3 or shape[1] != n_kv_heads or shape[2] != page_size * Q4_ROW_BYTES or v_pool.shape != shape:
+        raise ValueError(f"pools: shapes {tuple(shape)} and {tuple(v_pool.shape)}, expected [n_pages, {n_kv_heads}, "
                          f"{page_size * Q4_ROW_BYTES}]")
-    n = k_pool.numel()
-    return _q4_arg(k_pool, "k_pool", _U8, dev, n), _q4_arg(v_pool, "v_pool", _U8, dev, n), shape[0]
-
-
-def _q4_table(block_table, dev: int, rows: int):
-    if block_table.dim() != 2 or block_table.shape[0] < rows:
-        raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected [{rows}, max_pages]")
-    return _q4_arg(block_table, "block_table", _I32, dev, block_table.numel()), block_table.shape[1]
+    if len(table) != 2 or table[0] < rows:
+        raise ValueError(f"block_table: shape {tuple(table)}, expected [{rows}, max_pages]")
+    if not (k_pool.dtype is _U8 and v_pool.dtype is _U8 and block_table.dtype is _I32
+            and k_pool.get_device() == v_pool.get_device() == block_table.get_device() == dev and dev >= 0
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and block_table.is_contiguous()):
+        _q4_explain(dev, (("k_pool", k_pool, _U8, -1), ("v_pool", v_pool, _U8, -1),
+                          ("block_table", block_table, _I32, -1)))
+    return k_pool.data_ptr(), v_pool.data_ptr(), shape[0], block_table.data_ptr(), table[1]
 
 
 def _q4_workspace(workspace, dev: int):
@@ -350,11 +359,13 @@ def _q4_workspace(workspace, dev: int):
 
 def _q4_call(name: str, dev: int, *args) -> None:
     """The call on the current stream of the tensors' device."""
-    if dev == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch._C._cuda_getDevice():
+        status = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            status = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        check(status, name)
 
 
 def rope_kv_append_q4(qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, page_size: int,
@@ -369,13 +380,12 @@ def rope_kv_append_q4(qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, pa
     dev, rows = qkv.get_device(), qkv.shape[0]
     q_n, kv_n = rows * n_q_heads * head_dim, rows * n_kv_heads * head_dim
     a_qkv = _q4_arg(qkv, "qkv", FP16, dev, q_n + 2 * kv_n)
-    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
-    bt, max_pages = _q4_table(block_table, dev, rows)
+    cache = _q4_cache(k_pool, v_pool, block_table, dev, page_size, n_kv_heads, rows)
     _q4_call("lmps_rope_kv_append_q4", dev, a_qkv, _q4_arg(pos, "pos", _I32, dev, -rows),
              _q4_arg(inv_freq, "inv_freq", _F32, dev, head_dim // 2), _q4_arg(q_out, "q_out", FP16, dev, q_n),
              _q4_arg(k_out, "k_out", FP16, dev, kv_n) if k_out is not None else None,
-             _q4_arg(v_out, "v_out", FP16, dev, kv_n) if v_out is not None else None, kp, vp, n_pages, bt,
-             max_pages, page_size, n_q_heads, n_kv_heads, head_dim, rows, style,
+             _q4_arg(v_out, "v_out", FP16, dev, kv_n) if v_out is not None else None, *cache,
+             page_size, n_q_heads, n_kv_heads, head_dim, rows, style,
              _q4_arg(error, "error", _I32, dev, -1) if error is not None else None)
     return q_out
 
@@ -396,8 +406,7 @@ def gqa_decode_attention_q4(q, k_pool, v_pool, block_table, seq_lens, out, works
     dev, B = q.get_device(), q.shape[0]
     n = B * n_q_heads * head_dim
     a_q = _q4_arg(q, "q", FP16, dev, n)
-    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
-    bt, max_pages = _q4_table(block_table, dev, B)
+    kp, vp, n_pages, bt, max_pages = _q4_cache(k_pool, v_pool, block_table, dev, page_size, n_kv_heads, B)
     ws, ws_bytes = _q4_workspace(workspace, dev)
     _q4_call("lmps_gqa_decode_attention_q4", dev, a_q, kp, vp, n_pages, bt,
              _q4_arg(seq_lens, "seq_lens", _I32, dev, -B), _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes,
@@ -414,8 +423,7 @@ def gqa_decode_attention_rope_q4(qkv, pos, inv_freq, k_pool, v_pool, block_table
     dev, B = qkv.get_device(), qkv.shape[0]
     n = B * n_q_heads * head_dim
     a_qkv = _q4_arg(qkv, "qkv", FP16, dev, n + 2 * B * n_kv_heads * head_dim)
-    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
-    bt, max_pages = _q4_table(block_table, dev, B)
+    kp, vp, n_pages, bt, max_pages = _q4_cache(k_pool, v_pool, block_table, dev, page_size, n_kv_heads, B)
     ws, ws_bytes = _q4_workspace(workspace, dev)
     _q4_call("lmps_gqa_decode_attention_rope_q4", dev, a_qkv, _q4_arg(pos, "pos", _I32, dev, -B),
              _q4_arg(inv_freq, "inv_freq", _F32, dev, head_dim // 2), style, kp, vp, n_pages, bt,
@@ -446,8 +454,7 @@ def prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch: int, seq_le
     dev = q.get_device()
     n = batch * seq_len * n_q_heads * head_dim
     a_q = _q4_arg(q, "q", FP16, dev, n)
-    kp, vp, n_pages = _q4_pools(k_pool, v_pool, dev, page_size, n_kv_heads)
-    bt, max_pages = _q4_table(block_table, dev, batch)
+    kp, vp, n_pages, bt, max_pages = _q4_cache(k_pool, v_pool, block_table, dev, page_size, n_kv_heads, batch)
     ws, ws_bytes = _q4_workspace(workspace, dev)
     err = error if error is not None else torch.zeros(1, dtype=_I32, device=q.device)
     _q4_call("lmps_prefill_attention_q4", dev, a_q, kp, vp, n_pages, bt,

@@ -76,10 +76,10 @@ def test_refusals_of_one_form():
 
 def test_sizes():
     assert K.attention_q4_workspace_size(3, 12, 128, 1) == 0
-    assert K.attention_q4_workspace_size(3, 12, 128, 4) == 3 * 12 * 4 * (128 * 4 + 8)
+    assert K.attention_q4_workspace_size(3, 12, 128, 4) == 3 * 12 * 4 * (128 * 4 + 8) + 3 * 8
     assert K.attention_q4_splits(0, 2, 100) == K.prefill_q4_splits(0, 1, 12, 2, 100) == 1
     for b, n in ((1, 1), (1, 32768), (64, 8200), (300, 100)):
-        assert 1 <= K.attention_q4_splits(b, 2, n) <= 256
+        assert 1 <= K.attention_q4_splits(b, 2, n) <= 1024
 
 
 def test_python_layer_refuses_cpu_tensors():
