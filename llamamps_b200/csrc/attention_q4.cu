@@ -120,7 +120,8 @@ struct __align__(16) Smem {
   };
   __half q[kMaxHeads][kDim];
   uint32_t knew[kRowBytes / 4], vnew[kRowBytes / 4];  // the appended row (fused form)
-  double2 cs[kDim / 2];
+  double2 csd[kDim / 2];  // (cos, sin) of the new position: K's and q's
+  float2 csf[kDim / 2];
   float wm[kWarps][kMaxHeads], wl[kWarps][kMaxHeads];
 };
 
@@ -286,7 +287,12 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
     if (p != T - 1 && tid == 0) raise_error(P.c.error, kErrPosition);
     const int heads = P.n_q + 2 * P.c.n_kv;
     const __half* src = P.qkv + static_cast<size_t>(row) * heads * kDim;
-    if (tid < kDim / 2) rope_cos_sin(p, P.inv_freq[tid], S.cs[tid].x, S.cs[tid].y);
+    if (tid < kDim / 2) {
+      double2 d;
+      rope_cos_sin(p, P.inv_freq[tid], d.x, d.y);
+      S.csd[tid] = d;
+      S.csf[tid] = make_float2(static_cast<float>(d.x), static_cast<float>(d.y));
+    }
     __syncthreads();
     for (int h = warp; h < G + 2; h += kWarps) {  // the query heads, then K and V of the new position
       if (h >= G && !mine) continue;
@@ -296,11 +302,12 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
       } e;
       const int from = h < G ? kvh * G + h : P.n_q + (h - G) * P.c.n_kv + kvh;
       e.u = *reinterpret_cast<const uint2*>(src + from * kDim + 4 * lane);
-      if (h <= G) rotate_head(e.x, S.cs, P.style, lane);
       if (h < G) {
+        rotate_head(e.x, S.csf, P.style, lane);
         *reinterpret_cast<uint2*>(&S.q[h][4 * lane]) = e.u;
         continue;
       }
+      if (h == G) rotate_head(e.x, S.csd, P.style, lane);
       const int pi = P.c.page_index(p), off = p - pi * P.c.page_size;
       const int page = bt[pi];
       if (page < 0 || page >= P.c.n_pages) continue;  // raised where the steps are loaded

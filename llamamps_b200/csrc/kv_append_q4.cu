@@ -1,14 +1,16 @@
 // RoPE on q and k of the fused q|k|v rows, then the append of the K and V rows
 // to the paged 4-bit cache (kv_q4.cuh: format and quantiser).
 //
-// One CTA per token row: the row's 64 (cos, sin) pairs are computed once in
-// fp64, then each warp takes whole heads (128 elements, 4 per lane).
+// A CTA takes one token row, or four of a long call (so that all threads have
+// a cosine to compute): the rows' 64 (cos, sin) pairs once in fp64, q in units
+// of 16 bytes a thread, then a warp per K or V row (4 elements a lane).
 #include "kv_q4.cuh"
 
 namespace lmps {
 namespace q4 {
 
 constexpr int kAppendThreads = 256;
+constexpr int kSmallRows = 1024;  // up to here a CTA per token, then per 4
 
 struct AppendParams {
   const __half* qkv;
@@ -20,43 +22,116 @@ struct AppendParams {
   uint8_t* k_pool;
   uint8_t* v_pool;
   Cache c;
-  int n_q, style;
+  int n_q, style, rows;
 };
 
+// The pair in one word (interleaved), or two pairs with their second elements in another word (NeoX).
+__device__ __forceinline__ void rotate_word(uint32_t& w, float2 c) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  float2 y;
+  rope_rotate32(x.x, x.y, c, y.x, y.y);
+  const __half2 h = __floats2half2_rn(y.x, y.y);
+  w = *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void rotate_words(uint32_t& a, uint32_t& b, float2 c0, float2 c1) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  float2 u, v;
+  rope_rotate32(x.x, y.x, c0, u.x, v.x);
+  rope_rotate32(x.y, y.y, c1, u.y, v.y);
+  const __half2 hu = __floats2half2_rn(u.x, u.y), hv = __floats2half2_rn(v.x, v.y);
+  a = *reinterpret_cast<const uint32_t*>(&hu);
+  b = *reinterpret_cast<const uint32_t*>(&hv);
+}
+
+template <int kTokens, int kStyle>
 __global__ void __launch_bounds__(kAppendThreads) rope_kv_append_q4_kernel(const AppendParams P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
-  __shared__ double2 cs[kDim / 2];
-  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int p = P.pos[row];
-  if (p < 0) return;  // a row that is not in use
+  __shared__ double2 csd[kTokens][kDim / 2];                // K's rotation
+  __shared__ __align__(16) float2 csf[kTokens][kDim / 2];  // q's
+  constexpr int kPer = kAppendThreads / kTokens;           // threads of a token
+  constexpr int kUnit = kStyle == LMPS_ROPE_INTERLEAVED ? 8 : 16;  // elements a thread rotates at a time
+  constexpr int kAhead = kUnit == 8 ? 4 : 2;                       // units loaded before the table is ready
+  const int tid = threadIdx.x, lane = tid & 31, t = tid / kPer, l = tid % kPer;
+  const int row = blockIdx.x * kTokens + t;
+  const int n_kv = P.c.n_kv, heads = P.n_q + 2 * n_kv, units = P.n_q * (kDim / kUnit);
+  const bool used = row < P.rows;
+  const __half* src = P.qkv + static_cast<size_t>(used ? row : 0) * heads * kDim;
+  // first element of unit u (NeoX: of its first halves; the second are 64 on)
+  auto at = [](int u) { return kUnit == 8 ? 8 * u : (u >> 3) * kDim + 8 * (u & 7); };
+  // everything that does not wait for the position: q units, and the first K or V row of this warp
+  uint4 a[kAhead], b[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int u = l + k * kPer;
+    if (u < units) {
+      a[k] = *reinterpret_cast<const uint4*>(src + at(u));
+      if (kUnit == 16) b[k] = *reinterpret_cast<const uint4*>(src + at(u) + kDim / 2);
+    }
+  }
+  const int r0 = l >> 5;
+  uint2 kv = make_uint2(0u, 0u);
+  if (r0 < 2 * n_kv) kv = *reinterpret_cast<const uint2*>(src + (P.n_q + r0) * kDim + 4 * lane);
+
+  const int p = used ? P.pos[row] : -1;
+  int page = -1, off = 0;
   if (p >= P.c.max_pages * P.c.page_size) {
-    if (tid == 0) raise_error(P.c.error, kErrPosition);
-    return;
+    if (l == 0) raise_error(P.c.error, kErrPosition);
+  } else if (p >= 0) {
+    const int pi = P.c.page_index(p);
+    off = p - pi * P.c.page_size;
+    page = P.c.bt[static_cast<size_t>(row) * P.c.max_pages + pi];
+    if (page < 0 || page >= P.c.n_pages) {
+      if (l == 0) raise_error(P.c.error, kErrPage);
+      page = -1;
+    }
   }
-  const int pi = P.c.page_index(p), off = p - pi * P.c.page_size;
-  const int page = P.c.bt[static_cast<size_t>(row) * P.c.max_pages + pi];
-  if (page < 0 || page >= P.c.n_pages) {
-    if (tid == 0) raise_error(P.c.error, kErrPage);
-    return;
+  if (l < kDim / 2) {
+    double2 d;
+    rope_cos_sin(p, P.inv_freq[l], d.x, d.y);
+    csd[t][l] = d;
+    csf[t][l] = make_float2(static_cast<float>(d.x), static_cast<float>(d.y));
   }
-  if (tid < kDim / 2) rope_cos_sin(p, P.inv_freq[tid], cs[tid].x, cs[tid].y);
   __syncthreads();
-  const int n_kv = P.c.n_kv, heads = P.n_q + 2 * n_kv;
-  const __half* src = P.qkv + static_cast<size_t>(row) * heads * kDim;
-  for (int h = warp; h < heads; h += kAppendThreads / kWarp) {
+  if (page < 0) return;  // (uniform in a warp; no barrier follows) the row is left alone
+  __half* q_out = P.q_out + static_cast<size_t>(row) * P.n_q * kDim;
+  auto rotate = [&](int u, uint4 x, uint4 y) {
+    const float4* cs = reinterpret_cast<const float4*>(&csf[t][kUnit == 8 ? 4 * (u & 15) : 8 * (u & 7)]);
+    uint32_t* px = &x.x;
+    uint32_t* py = &y.x;
+#pragma unroll
+    for (int e = 0; e < 4; e += kUnit == 8 ? 2 : 1) {
+      const float4 c = cs[kUnit == 8 ? e / 2 : e];
+      if (kUnit == 8) {
+        rotate_word(px[e], make_float2(c.x, c.y));
+        rotate_word(px[e + 1], make_float2(c.z, c.w));
+      } else {
+        rotate_words(px[e], py[e], make_float2(c.x, c.y), make_float2(c.z, c.w));
+      }
+    }
+    *reinterpret_cast<uint4*>(q_out + at(u)) = x;
+    if (kUnit == 16) *reinterpret_cast<uint4*>(q_out + at(u) + kDim / 2) = y;
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (l + k * kPer < units) rotate(l + k * kPer, a[k], b[k]);
+  for (int u = l + kAhead * kPer; u < units; u += kPer) {
+    const uint4 x = *reinterpret_cast<const uint4*>(src + at(u));
+    rotate(u, x, kUnit == 16 ? *reinterpret_cast<const uint4*>(src + at(u) + kDim / 2) : x);
+  }
+  // K and V: a warp per row of 128, the next row's load ahead
+  for (int r = r0; r < 2 * n_kv; r += kPer / kWarp) {
     union {
       uint2 u;
       __half x[4];
     } e;
-    e.u = *reinterpret_cast<const uint2*>(src + h * kDim + 4 * lane);
-    const bool is_v = h >= P.n_q + n_kv;
-    if (!is_v) rotate_head(e.x, cs, P.style, lane);
-    if (h < P.n_q) {
-      *reinterpret_cast<uint2*>(P.q_out + (static_cast<size_t>(row) * P.n_q + h) * kDim + 4 * lane) = e.u;
-      continue;
-    }
-    const int kvh = h - P.n_q - (is_v ? n_kv : 0);
+    e.u = kv;
+    if (r + kPer / kWarp < 2 * n_kv)
+      kv = *reinterpret_cast<const uint2*>(src + (P.n_q + r + kPer / kWarp) * kDim + 4 * lane);
+    const bool is_v = r >= n_kv;
+    const int kvh = r - (is_v ? n_kv : 0);
+    if (!is_v) rotate_head(e.x, csd[t], kStyle, lane);
     const float x[4] = {__half2float(e.x[0]), __half2float(e.x[1]), __half2float(e.x[2]), __half2float(e.x[3])};
     float scale;
     const uint32_t w = quantise_row(x, scale);
@@ -66,9 +141,10 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv_append_q4_kernel(const
       *reinterpret_cast<__half*>(block + P.c.page_size * kCodeBytes + off * 8 + (lane >> 3) * 2) = __float2half_rn(scale);
     __half* copy = is_v ? P.v_out : P.k_out;
     if (copy) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e.x[i] = __float2half_rn(nib_code(w, i) * scale);
-      *reinterpret_cast<uint2*>(copy + (static_cast<size_t>(row) * n_kv + kvh) * kDim + 4 * lane) = e.u;
+      const __half2 lo = __floats2half2_rn(nib_code(w, 0) * scale, nib_code(w, 1) * scale);
+      const __half2 hi = __floats2half2_rn(nib_code(w, 2) * scale, nib_code(w, 3) * scale);
+      *reinterpret_cast<uint2*>(copy + (static_cast<size_t>(row) * n_kv + kvh) * kDim + 4 * lane) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
   }
 }
@@ -103,6 +179,13 @@ extern "C" int lmps_rope_kv_append_q4(const uint16_t* qkv, const int32_t* pos, c
                   q4::page_shift_of(page_size), error};
   P.n_q = n_q_heads;
   P.style = style;
-  return lmps_launch_pdl(q4::rope_kv_append_q4_kernel, dim3(rows), dim3(q4::kAppendThreads), 0, lmps_stream(stream),
+  P.rows = rows;
+  // a CTA per token while that does not fill the GPU, else four tokens a CTA
+  const bool il = style == LMPS_ROPE_INTERLEAVED, few = rows <= q4::kSmallRows;
+  const auto kernel = il ? (few ? q4::rope_kv_append_q4_kernel<1, LMPS_ROPE_INTERLEAVED>
+                                : q4::rope_kv_append_q4_kernel<4, LMPS_ROPE_INTERLEAVED>)
+                         : (few ? q4::rope_kv_append_q4_kernel<1, LMPS_ROPE_NEOX>
+                                : q4::rope_kv_append_q4_kernel<4, LMPS_ROPE_NEOX>);
+  return lmps_launch_pdl(kernel, dim3(few ? rows : (rows + 3) / 4), dim3(q4::kAppendThreads), 0, lmps_stream(stream),
                          P);
 }

@@ -58,13 +58,15 @@ static inline int page_shift_of(int page_size) {
   return (page_size & (page_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(page_size)) : -1;
 }
 
-// Scale of a group whose largest magnitude is `a` (finite).  a / 7 is rounded
-// up to 24 bits and that up to 8 (the low 16 of fp32's 24): rounding up twice
-// on nested grids is rounding up once.
+// Scale of a group whose largest magnitude is `a` (finite).  a has 11
+// significant bits, so a / 7 is either a number of 8 bits or at least 2^-14 of
+// itself away from one: the product below, a little above a / 7 by less than
+// that, truncates to the largest 8-bit number <= a / 7.
 __device__ __forceinline__ float group_scale(float a) {
   if (a == 0.0f) return 1.0f;
-  float s = __uint_as_float((__float_as_uint(__fdiv_ru(a, 7.0f)) + 0xFFFFu) & 0xFFFF0000u);
-  if (s < 1.52587890625e-05f) s = ceilf(s * 16777216.0f) * 5.9604644775390625e-08f;  // 2^-16: fp16's 2^-24 grid
+  const uint32_t low = __float_as_uint(a * (0.14285714285f * (1.0f + 3.8147e-06f))) & 0xFFFF0000u;  // (2^-18)
+  float s = __uint_as_float(__uint_as_float(low) * 7.0f >= a ? low : low + 0x10000u);  // the product is exact
+  if (s < 1.52587890625e-05f) s = ceilf(s * 16777216.0f) * 5.9604644775390625e-08f;    // 2^-16: fp16's 2^-24 grid
   return fminf(s, 9344.0f);
 }
 
@@ -86,48 +88,91 @@ __device__ __forceinline__ uint32_t quantise_row(const float (&x)[4], float& sca
     return 0x8888u;
   }
   scale = group_scale(a);
+  // x / s by a reciprocal and one residual step (Markstein): exact where the
+  // quotient is a number, and it must be where it lies on a tie, which goes to
+  // the even code; with 11 bits over 8, other quotients are 2^-12 away from ties.
+  // Adding 1.5 * 2^23 rounds to an integer, here code + 8 in the low bits.
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
   uint32_t w = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // IEEE division: x / s may lie on a tie, which rint sends to the even code
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -7.0f), 7.0f);
-    w |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
+    const float q = x[i] * r;
+    const float c = fmaf(fmaf(-q, scale, x[i]), r, q) + 12582920.0f;
+    w |= (__float_as_uint(c) & 0xFu) << (4 * i);
   }
   return w;
 }
 
-// cos and sin of pos * inv_freq: the product of a position below 2^29 and an
-// fp32 frequency is exact in fp64, where an fp32 product is off by up to
-// pos * inv_freq * 2^-24 radians (2e-3 at position 32768).  fp64 throughout,
+// cos and sin of pos * inv_freq in fp64, error below 2^-50: the product of a
+// position below 2^29 and an fp32 frequency is exact, where an fp32 product is
+// off by up to pos * inv_freq * 2^-24 radians (2e-3 at position 32768).  fp64,
 // so that K's codes are those of the exactly rotated row: an fp32 rotation
 // moves about one code in 10^6 across a rounding border.
+// x = k pi/2 + r with pi/2 in two fp64 parts, then the Taylor series of sine and
+// cosine on |r| <= pi/4 to r^15 and r^16 (the next terms are below 2^-54).
 __device__ __forceinline__ void rope_cos_sin(int pos, float inv_freq, double& c, double& s) {
-  sincos(static_cast<double>(pos) * static_cast<double>(inv_freq), &s, &c);
+  const double x = static_cast<double>(pos) * static_cast<double>(inv_freq);
+  const double k = rint(x * 0.63661977236758134308);
+  double r = fma(-k, 1.57079632679489655800, x);
+  r = fma(-k, 6.12323399573676603587e-17, r);
+  const double z = r * r;
+  double ps = -1.0 / 1307674368000.0, pc = 1.0 / 20922789888000.0;
+  ps = fma(ps, z, 1.0 / 6227020800.0);
+  pc = fma(pc, z, -1.0 / 87178291200.0);
+  ps = fma(ps, z, -1.0 / 39916800.0);
+  pc = fma(pc, z, 1.0 / 479001600.0);
+  ps = fma(ps, z, 1.0 / 362880.0);
+  pc = fma(pc, z, -1.0 / 3628800.0);
+  ps = fma(ps, z, -1.0 / 5040.0);
+  pc = fma(pc, z, 1.0 / 40320.0);
+  ps = fma(ps, z, 1.0 / 120.0);
+  pc = fma(pc, z, -1.0 / 720.0);
+  ps = fma(ps, z, -1.0 / 6.0);
+  pc = fma(pc, z, 1.0 / 24.0);
+  pc = fma(pc, z, -0.5);
+  const double sn = fma(r * z, ps, r), cn = fma(pc, z, 1.0);
+  const int q = static_cast<int>(static_cast<long long>(k)) & 3;
+  const double a = (q & 1) ? sn : cn, b = (q & 1) ? cn : sn;  // cos, sin up to their signs
+  c = (q == 1 || q == 2) ? -a : a;
+  s = (q >= 2) ? -b : b;
 }
 
 // (x1, x2) -> (x1 c - x2 s, x1 s + x2 c), fp64 rounded through fp32 to fp16.
 __device__ __forceinline__ void rope_rotate64(__half& a, __half& b, double c, double s) {
   const double x1 = static_cast<double>(__half2float(a)), x2 = static_cast<double>(__half2float(b));
-  a = __float2half_rn(static_cast<float>(x1 * c - x2 * s));
-  b = __float2half_rn(static_cast<float>(x1 * s + x2 * c));
+  a = __float2half_rn(static_cast<float>(__fma_rn(x1, c, -__dmul_rn(x2, s))));
+  b = __float2half_rn(static_cast<float>(__fma_rn(x1, s, __dmul_rn(x2, c))));
+}
+// The same in fp32, from cos and sin rounded to fp32: q, which no rounding
+// border waits for, is off by at most 3 * 2^-24 (|x1| + |x2|) before it is
+// rounded to fp16.  (Explicit operations: every kernel gets the same bits.)
+__device__ __forceinline__ void rope_rotate32(float x1, float x2, float2 cs, float& y1, float& y2) {
+  y1 = __fmaf_rn(x1, cs.x, -__fmul_rn(x2, cs.y));
+  y2 = __fmaf_rn(x1, cs.y, __fmul_rn(x2, cs.x));
 }
 
-// A warp rotates one head's row in place: lane l holds elements 4l .. 4l+3.
-__device__ __forceinline__ void rotate_head(__half (&x)[4], const double2* cs, int style, int lane) {
+__device__ __forceinline__ void rope_rotate_by(__half& a, __half& b, const double2& t) { rope_rotate64(a, b, t.x, t.y); }
+__device__ __forceinline__ void rope_rotate_by(__half& a, __half& b, const float2& t) {
+  float y1, y2;
+  rope_rotate32(__half2float(a), __half2float(b), t, y1, y2);
+  a = __float2half_rn(y1);
+  b = __float2half_rn(y2);
+}
+// A warp rotates one head's row in place: lane l holds elements 4l .. 4l+3;
+// cs: 64 (cos, sin), fp64 for K and fp32 for q.
+template <class Pair>
+__device__ __forceinline__ void rotate_head(__half (&x)[4], const Pair* cs, int style, int lane) {
   if (style == LMPS_ROPE_INTERLEAVED) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const double2 t = cs[2 * lane + i];
-      rope_rotate64(x[2 * i], x[2 * i + 1], t.x, t.y);
-    }
+    rope_rotate_by(x[0], x[1], cs[2 * lane]);
+    rope_rotate_by(x[2], x[3], cs[2 * lane + 1]);
   } else {  // element j pairs with j + 64: the partner lane is 16 away
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double2 t = cs[4 * (lane & 15) + i];
       const unsigned other = __shfl_xor_sync(0xffffffffu, static_cast<unsigned>(__half_as_ushort(x[i])), 16);
       const __half p = __ushort_as_half(static_cast<unsigned short>(other));
       __half a = lane < 16 ? x[i] : p, b = lane < 16 ? p : x[i];
-      rope_rotate64(a, b, t.x, t.y);
+      rope_rotate_by(a, b, cs[4 * (lane & 15) + i]);
       x[i] = lane < 16 ? a : b;
     }
   }

@@ -37,16 +37,22 @@ def values(codes, scales):
     return codes * np.repeat(scales, 32, axis=1)
 
 
-def rotate(x, pos, inv_freq, style):
-    """fp16 [n, heads, 128] at positions pos [n], rounded to fp16 (through fp32, as the kernels round)."""
+def rotate_exact(x, pos, inv_freq, style):
+    """fp16 [n, heads, 128] at positions pos [n]: the rotation in 64 bits, and |x1| + |x2| of each element's pair."""
     a = np.asarray(pos, np.float64)[:, None, None] * np.asarray(inv_freq, np.float32).astype(np.float64)
     c, s = np.cos(a), np.sin(a)
     x = np.asarray(x, np.float16).astype(np.float64)
-    out = np.empty_like(x)
+    out, size = np.empty_like(x), np.empty_like(x)
     i1, i2 = (np.arange(0, D, 2), np.arange(1, D, 2)) if style == 0 else (np.arange(64), np.arange(64, D))
     out[..., i1] = x[..., i1] * c - x[..., i2] * s
     out[..., i2] = x[..., i1] * s + x[..., i2] * c
-    return out.astype(np.float32).astype(np.float16)
+    size[..., i1] = size[..., i2] = np.abs(x[..., i1]) + np.abs(x[..., i2])
+    return out, size
+
+
+def rotate(x, pos, inv_freq, style):
+    """The rotation rounded to fp16 (through fp32, as K is before it is quantised)."""
+    return rotate_exact(x, pos, inv_freq, style)[0].astype(np.float32).astype(np.float16)
 
 
 class Cache:

@@ -45,7 +45,7 @@ def _ws(n):
 ])
 def test_append_bytes(cuda, style, hq, hkv, page, ends):
     """Cache bytes equal the restatement's everywhere (rows that the call does
-    not name keep theirs), values and rotated q as well."""
+    not name keep theirs), the values too; rotated q within its roundings."""
     from llamamps_b200 import kernels as K
     rng = np.random.default_rng(sum(ends) + hq + style)
     c = R.Cache(rng, [min(e - 1, 70) for e in ends], hkv, page, max_len=max(ends))
@@ -62,7 +62,10 @@ def test_append_bytes(cuda, style, hq, hkv, page, ends):
                         style, k_out=k_out, v_out=v_out, error=e)
     assert e.item() == 0 and _guards_ok(buf)
     assert np.array_equal(c.k.cpu().numpy(), c.k_np) and np.array_equal(c.v.cpu().numpy(), c.v_np)
-    assert np.array_equal(q_out.cpu().numpy().reshape(B, hq, D), rot[:, :hq])
+    # q is rotated in fp32: 3 roundings of 2^-24 of |x1| + |x2|, then half a step of fp16
+    exact, size = R.rotate_exact(qkv[:, :hq], pos, _inv(), style)
+    off = np.abs(q_out.cpu().numpy().reshape(B, hq, D).astype(np.float64) - exact)
+    assert (off <= np.abs(exact) * 2.0 ** -11 + size * 3 * 2.0 ** -24 * (1 + 2.0 ** -11) + 2.0 ** -25).all()
     assert np.array_equal(k_out.cpu().numpy().astype(np.float64).reshape(k_vals.shape), k_vals)
     assert np.array_equal(v_out.cpu().numpy().astype(np.float64).reshape(v_vals.shape), v_vals)
 
