@@ -11,13 +11,13 @@
 //   * warps 8-11 (thread = key) read the key's K and V codes, write them as
 //     fp16 code * scale -- exact, see kv_q4.cuh -- into two 128-byte-swizzled
 //     stages each (K read K-major, V MN-major), loads one tile ahead;
-//   * warp 12 (one lane) issues S_t = Q_t K^T and O_t += P_t V, tile t's S
-//     right behind its P V, so that the tensor core works on one tile while
-//     the softmax of the other runs;
-//   * warps 0-3 / 4-7 (thread = row, its TMEM lane) take the softmax of tile
-//     0 / 1: row max, P = 2^(s - m) as fp16 packed over S's own columns (A
-//     operand from tensor memory), sums in fp32, and O rescaled in place only
-//     when the max grew by more than 2^8.
+//   * warps 12, 13 (row tile 0, 1) issue S_t = Q_t K^T and O_t += P_t V in half tiles of 64 keys:
+//     S has two halves per row tile, so the softmax finds the next one ready
+//     while the products behind the last run;
+//   * warps 0-3 / 4-7 (thread = row, its TMEM lane) take the softmax of row
+//     tile 0 / 1: row max, P = 2^(s - m) as fp16 packed over S's own columns
+//     (A operand from tensor memory), sums in fp32, and O rescaled in place
+//     only when the max grew by more than 2^8.
 // The dims inside a group of 8 stay in the order in which masking the nibbles
 // yields them (0 4 1 5 2 6 3 7): Q is staged in that order, and the epilogue
 // undoes it for O by naming registers.
@@ -38,7 +38,7 @@ using namespace tc;
 constexpr int kRows = 128;  // rows per tile (TMEM lanes)
 constexpr int kTiles = 2;   // row tiles per CTA
 constexpr int kKeys = 128;  // keys per tile
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 14 * 32;
 constexpr int kStages = 2;
 constexpr int kSub = 128 * 128;  // 64 dims of 128 rows or keys: 128-byte rows
 constexpr int kOffK = kTiles * 2 * kSub;
@@ -46,9 +46,9 @@ constexpr int kOffV = kOffK + kStages * 2 * kSub;
 constexpr int kOffBar = kOffV + kStages * 2 * kSub;
 constexpr int kSmemBytes = kOffBar + 256 + 1024;  // barriers, flags; 1024-byte alignment slack
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0;    // S of tile t at columns 128 t; P over its upper half
-constexpr uint32_t kColP = 64;
-constexpr uint32_t kColO = 256;  // O of tile t at columns 256 + 128 t
+constexpr int kHalf = 64;        // keys per softmax step: half a key tile
+constexpr uint32_t kColS = 0;    // S of row tile t, half u at columns 64 (2 t + u); P over its first 32
+constexpr uint32_t kColO = 256;  // O of row tile t at columns 256 + 128 t
 constexpr float kRescaleLog2 = 8.0f;
 
 struct Params {
@@ -141,6 +141,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
 struct Raw {  // a key's cached rows
   uint4 k[4], v[4];
   uint2 ks, vs;
@@ -159,32 +163,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   uint64_t* k_empty = bars + 3;
   uint64_t* v_full = bars + 5;
   uint64_t* v_empty = bars + 7;
-  uint64_t* s_full = bars + 9;   // [kTiles]: S of the row tile ready
-  uint64_t* p_full = bars + 11;  // P written (and S read)
-  uint64_t* o_done = bars + 13;  // O += P V done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* s_full = bars + 9;   // [kTiles][2]: S of the row tile and half ready
+  uint64_t* p_full = bars + 13;  // P written (and S read)
+  uint64_t* o_done = bars + 17;  // O += P V done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
   uint32_t* absent = tmem_slot + 4;  // [4][4]: keys of a tile whose page is not in the pool, ring of 4 tiles
 
   lmps_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    mbar_init(q_full, 8);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&k_full[s], 4);
-      mbar_init(&v_full[s], 4);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
-    }
-    for (int t = 0; t < kTiles; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&o_done[t], 1);
-    }
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   lmps_pdl_wait();
   // this CTA's rows: the last (longest) row blocks first
   const int per_block = static_cast<int>(gridDim.x) / P.n_blocks;
@@ -207,7 +195,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   const int all_tiles = (kv_end + kKeys - 1) / kKeys;
   const int per_split = (all_tiles + P.n_splits - 1) / P.n_splits;
   const int tile0 = min(all_tiles, split * per_split), nt = min(all_tiles, tile0 + per_split) - tile0;
+  const int nh = min(2 * nt, (kv_end - tile0 * kKeys + kHalf - 1) / kHalf);  // softmax steps: half tiles with keys
 
+  if (tid == 0) {
+    mbar_init(q_full, 8);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&k_empty[s], n_t);
+      mbar_init(&v_empty[s], n_t);
+    }
+    for (int t = 0; t < 2 * kTiles; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemCols)
@@ -217,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
 
   if (warp >= 8 && warp < 12) {
     // ---- dequantisation: thread = key
@@ -294,57 +299,78 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[s]);
     }
-  } else if (warp == 12) {
-    if (lane == 0) {  // ---- MMA issuer
-      const uint32_t id_s = idesc_f16(kRows, kKeys), id_o = idesc_f16(kRows, kDim) | kBMajorMN;
-      const uint64_t dk = sw128_desc(smem_u32(sk)), dv = sw128_mn_desc(smem_u32(sv), kSub);
-      const uint32_t hi_k = static_cast<uint32_t>(dk >> 32), hi_v = static_cast<uint32_t>(dv >> 32);
-      const uint32_t lo_q = static_cast<uint32_t>(sw128_desc(smem_u32(sq))), lo_k = static_cast<uint32_t>(dk),
-                     lo_v = static_cast<uint32_t>(dv);
-      constexpr uint32_t kHalf = kSub >> 4;  // the next 64 dims
-      auto issue_s = [&](int t, int s) {  // S_t = Q_t K^T over 8 steps of 16 dims
-        const uint32_t a = lo_q + 2 * t * kHalf, k = lo_k + 2 * s * kHalf, d = tmem + kColS + kKeys * t;
+  } else if (warp >= 12) {
+    // ---- MMA issuers, a warp per row tile: while one waits for its softmax (some 200 cycles from
+    // the barrier to the next MMA) the other's products run.  The whole warp runs the code and one
+    // elected lane issues: uniform, with tiles and stages unrolled, it keeps the descriptors in
+    // uniform registers.  (Issued from a divergent branch an MMA costs some ten instructions, and on
+    // a scheduler shared with three busy warps they came 110 .. 130 cycles apart, not 64.)
+    uint32_t elected;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(elected));
+    const bool leader = elected != 0u;
+    const uint32_t id_s = idesc_f16(kRows, kHalf), id_o = idesc_f16(kRows, kDim) | kBMajorMN;
+    const uint64_t dk = sw128_desc(smem_u32(sk)), dv = sw128_mn_desc(smem_u32(sv), kSub);
+    const uint32_t hi_k = static_cast<uint32_t>(dk >> 32), hi_v = static_cast<uint32_t>(dv >> 32);
+    const uint32_t lo_q = static_cast<uint32_t>(sw128_desc(smem_u32(sq))), lo_k = static_cast<uint32_t>(dk),
+                   lo_v = static_cast<uint32_t>(dv);
+    constexpr uint32_t kNext = kSub >> 4;  // the next 64 dims
+    auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
+    auto run = [&](auto tile) {
+      constexpr int t = decltype(tile)::value;
+      auto issue_s = [&](int s, int u) {  // S_t,u = Q_t K_u^T over 8 steps of 16 dims
+        if (leader) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t o = (j >> 2) * kHalf + 2 * (j & 3);
-          mma_f16(d, desc(a + o, hi_k), desc(k + o, hi_k), id_s, j > 0 ? 1u : 0u);
-        }
-        mma_commit(&s_full[t]);
-      };
-      auto issue_o = [&](int t, int s, bool acc) {  // O_t += P_t V over 8 steps of 16 keys
-        const uint32_t v = lo_v + 2 * s * kHalf, d = tmem + kColO + kDim * t, a = tmem + kColS + kKeys * t + kColP;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          mma_f16_ta(d, a + 8 * j, desc(v + 128 * j, hi_v), id_o, (acc || j > 0) ? 1u : 0u);
-        mma_commit(&o_done[t]);
-      };
-      bool ok = nt > 0 && wait(q_full, 0, P.c.error, abort_v) && wait(&k_full[0], 0, P.c.error, abort_v);
-      if (ok) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int t = 0; t < n_t; ++t) issue_s(t, 0);
-        mma_commit(&k_empty[0]);
-      }
-      for (int i = 0; ok && i < nt; ++i) {
-        const int s = i & 1, s1 = s ^ 1;
-        for (int t = 0; ok && t < n_t; ++t) {
-          if (t == 0) ok = wait(&v_full[s], (i >> 1) & 1, P.c.error, abort_v);
-          ok = ok && wait(&p_full[t], i & 1, P.c.error, abort_v);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          issue_o(t, s, i > 0);
-          if (i + 1 < nt) {
-            if (t == 0) ok = wait(&k_full[s1], ((i + 1) >> 1) & 1, P.c.error, abort_v);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // P_t, under S_t's columns, is read by the P V before this in the issue order
-            issue_s(t, s1);
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t o = (j >> 2) * kNext + 2 * (j & 3);
+            mma_f16(tmem_u + kColS + kHalf * (2 * t + u), desc(lo_q + 2 * t * kNext + o, hi_k),
+                    desc(lo_k + 2 * s * kNext + u * (kHalf * 128 >> 4) + o, hi_k), id_s, j > 0 ? 1u : 0u);
           }
+          mma_commit(&s_full[2 * t + u]);
         }
-        if (ok) {
-          mma_commit(&v_empty[s]);
-          if (i + 1 < nt) mma_commit(&k_empty[s1]);
+      };
+      auto issue_o = [&](int s, int u, bool acc) {  // O_t += P_t,u V_u over 4 steps of 16 keys
+        if (leader) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_f16_ta(tmem_u + kColO + kDim * t, tmem_u + kColS + kHalf * (2 * t + u) + 8 * j,
+                       desc(lo_v + 2 * s * kNext + 128 * (4 * u + j), hi_v), id_o, (acc || j > 0) ? 1u : 0u);
+          mma_commit(&o_done[2 * t + u]);
         }
+      };
+      bool ok = wait_warp(q_full, 0, P.c.error, abort_v) && wait_warp(&k_full[0], 0, P.c.error, abort_v);
+      if (ok) {
+        after();
+        issue_s(0, 0);
+        if (nh > 1) issue_s(0, 1);
+        if (leader) mma_commit(&k_empty[0]);
       }
+      // step i, half u of key tile j in stage s: O, then S of the same half of the next tile
+      auto step = [&](int i, auto stage, auto half) {
+        constexpr int s = decltype(stage)::value, s1 = s ^ 1, u = decltype(half)::value;
+        const int j = i >> 1;
+        const bool more = i + 2 < nh;
+        if (u == 0) ok = wait_warp(&v_full[s], (j >> 1) & 1, P.c.error, abort_v);
+        if (u == 0 && more) ok = ok && wait_warp(&k_full[s1], ((j + 1) >> 1) & 1, P.c.error, abort_v);
+        ok = ok && wait_warp(&p_full[2 * t + u], j & 1, P.c.error, abort_v);
+        if (!ok) return;
+        after();
+        issue_o(s, u, i > 0);
+        if (more) issue_s(s1, u);  // (P, under S's columns, is read by the P V before it in the issue order)
+        if (u == 1 && leader) {
+          mma_commit(&v_empty[s]);
+          if (more) mma_commit(&k_empty[s1]);
+        }
+      };
+      for (int i = 0; ok && i < nh; i += 4) {
+        step(i, Int<0>{}, Int<0>{});
+        if (ok && i + 1 < nh) step(i + 1, Int<0>{}, Int<1>{});
+        if (ok && i + 2 < nh) step(i + 2, Int<1>{}, Int<0>{});
+        if (ok && i + 3 < nh) step(i + 3, Int<1>{}, Int<1>{});
+      }
+    };
+    if (nh > 0) {
+      if (warp == 12) run(Int<0>{});
+      else if (n_t > 1) run(Int<1>{});
     }
   } else {
     // ---- softmax of row tile t: thread = row (TMEM lane)
@@ -378,44 +404,39 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     }
     if (t < n_t) {
       const uint32_t tl = tmem + (static_cast<uint32_t>(32 * quad) << 16);
-      const uint32_t ts = tl + kColS + kKeys * t, to = tl + kColO + kDim * t;
+      const uint32_t to = tl + kColO + kDim * t;
       const int qi = r / P.G;
       const int lim = r < n_rows ? limit(qi) : kv_end;
       const int lim_min = limit((r0 + kRows * t) / P.G);
       float m_used = -INFINITY, l = 0.0f;  // running max (scaled, base 2) and sum
       bool ok = true;
-      for (int i = 0; ok && i < nt; ++i) {
-        const int k0 = (tile0 + i) * kKeys;
-        ok = wait_warp(&s_full[t], i & 1, P.c.error, abort_v);
+      for (int i = 0; ok && i < nh; ++i) {
+        const int u = i & 1, j = i >> 1, k0 = tile0 * kKeys + i * kHalf;
+        const uint32_t ts = tl + kColS + kHalf * (2 * t + u);
+        ok = wait_warp(&s_full[2 * t + u], j & 1, P.c.error, abort_v);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const volatile uint32_t* av = absent + 4 * (i & 3);
-        const uint32_t gone[4] = {av[0], av[1], av[2], av[3]};
-        const bool masked = k0 + kKeys > lim_min || (gone[0] | gone[1] | gone[2] | gone[3]) != 0u;  // (uniform)
-        const int nv = lim - k0;  // columns below it count
-        auto mask = [&](uint32_t (&sc)[64], int c0) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (c0 + c >= nv || ((gone[(c0 + c) >> 5] >> (c & 31)) & 1u)) sc[c] = 0xFF800000u;  // -inf
-        };
-        // row max: columns 0..63, then 64..127 (kept in registers)
         uint32_t sc[64];
+        tmem_ld64(ts, sc);
+        const volatile uint32_t* av = absent + 4 * (j & 3) + 2 * u;
+        const uint32_t gone[2] = {av[0], av[1]};
+        if (k0 + kHalf > lim_min || (gone[0] | gone[1]) != 0u) {  // (uniform)
+          const int nv = lim - k0;  // columns below it count
+#pragma unroll
+          for (int c = 0; c < kHalf; ++c)
+            if (c >= nv || ((gone[c >> 5] >> (c & 31)) & 1u)) sc[c] = 0xFF800000u;  // -inf
+        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          tmem_ld64(ts + 64 * half, sc);
-          if (masked) mask(sc, 64 * half);
-#pragma unroll
-          for (int c = 0; c < 64; c += 2)
-            mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(sc[c]), __uint_as_float(sc[c + 1]));
-        }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kScaleLog2;
+        for (int c = 0; c < kHalf; c += 2)
+          mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(sc[c]), __uint_as_float(sc[c + 1]));
+        const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * kScaleLog2;
         const float mnew = fmaxf(m_used, mt);
         const bool grow = mnew > m_used + kRescaleLog2;  // (always on a row's first positions)
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? ex2(m_used - mnew) : 1.0f;
-          if (i > 0) {  // warp-wide read-modify-write of O_t, whose P V of the previous tile is done
-            ok = wait_warp(&o_done[t], (i - 1) & 1, P.c.error, abort_v);
+          if (i > 0) {  // warp-wide read-modify-write of O_t, once the P V of the step before is done
+            ok = wait_warp(&o_done[2 * t + (u ^ 1)], ((i - 1) >> 1) & 1, P.c.error, abort_v);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -433,36 +454,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         const float nm = m_used == -INFINITY ? 0.0f : -m_used;
         const uint64_t nm2 = pair(nm, nm), scale2 = pair(kScaleLog2, kScaleLog2);
         uint64_t sm[4] = {0ull, 0ull, 0ull, 0ull};
-        // P over S's upper columns: keys 64..127 from the registers first (their scores lay there),
-        // then keys 0..63 read again
+        uint32_t pk[32];
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-          if (half == 0) {
-            tmem_ld64(ts, sc);
-            if (masked) mask(sc, 0);
-          }
-          uint32_t pk[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float a0, a1;
-            unpair(fma2(pair(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), scale2, nm2), a0, a1);
-            a0 = ex2(a0);
-            a1 = ex2(a1);
-            sm[e & 3] = add2(sm[e & 3], pair(a0, a1));
-            const __half2 hh = __floats2half2_rn(a0, a1);
-            pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
-          }
-          tmem_st32(ts + kColP + 32 * half, pk);
+        for (int e = 0; e < 32; ++e) {
+          float a0, a1;
+          const uint64_t x = fma2(pair(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), scale2, nm2);
+          unpair(x, a0, a1);
+          a0 = ex2(a0);
+          a1 = ex2(a1);
+          sm[e & 3] = add2(sm[e & 3], pair(a0, a1));
+          const __half2 hh = __floats2half2_rn(a0, a1);
+          pk[e] = *reinterpret_cast<const uint32_t*>(&hh);
         }
+        tmem_st32(ts, pk);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + u]);
         float s0, s1;
         unpair(add2(add2(sm[0], sm[1]), add2(sm[2], sm[3])), s0, s1);
         l += s0 + s1;
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
       }
       // ---- epilogue: this row of O (dims of each 8 back in order), normalised or as a partial
-      if (ok && nt > 0) ok = wait_warp(&o_done[t], (nt - 1) & 1, P.c.error, abort_v);
+      if (ok && nh > 0) ok = wait_warp(&o_done[2 * t + ((nh - 1) & 1)], ((nh - 1) >> 1) & 1, P.c.error, abort_v);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -473,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
 #pragma unroll 1
         for (int cc = 0; cc < kDim; cc += 32) {
           uint32_t o[32];
-          if (nt > 0) {
+          if (nh > 0) {
             tmem_ld32(to + cc, o);
           } else {
 #pragma unroll
