@@ -478,12 +478,23 @@ __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(co
   __shared__ float red[2][kMergeWarps];
   __shared__ float4 acc[kMergeWarps][kWarp];
   const int h = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (P.q_lens && row % P.seq >= P.q_lens[row / P.seq]) return;
-  const int2 pc = P.pieces ? P.pieces[row] : make_int2(row * P.n_splits, P.n_splits);
-  const size_t first = static_cast<size_t>(pc.x) * P.n_q + h;  // piece s at first + s * n_q
+  size_t first, step;  // piece s at first + s * step
+  int2 pc;
+  if (P.rows_item == 0) {
+    pc = P.pieces[row];
+    step = P.n_q;
+    first = pc.x * step + h;
+  } else {
+    const int b = row / P.seq, i = row - b * P.seq;
+    if (P.q_lens && i >= P.q_lens[b]) return;
+    const int G = P.n_q / P.n_kv, kvh = h / G, r = i * G + (h - kvh * G), blk = r / P.rows_item;
+    pc = P.pieces[(P.n_blocks - 1 - blk) * P.batch + b];
+    step = static_cast<size_t>(P.n_kv) * P.rows_item;
+    first = pc.x * step + static_cast<size_t>(kvh) * P.rows_item + (r - blk * P.rows_item);
+  }
   const float2* ml = P.ml + first;
   const float4* o = reinterpret_cast<const float4*>(P.o + first * kDim) + lane;
-  const size_t stride = static_cast<size_t>(P.n_q) * (kDim / 4);
+  const size_t stride = step * (kDim / 4);
   float4 v[kMergeLoads];
 #pragma unroll
   for (int i = 0; i < kMergeLoads; ++i) {
@@ -491,7 +502,7 @@ __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(co
     v[i] = s < pc.y ? o[s * stride] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   float M = -INFINITY;
-  for (int s = tid; s < pc.y; s += kMergeWarps * kWarp) M = fmaxf(M, ml[static_cast<size_t>(s) * P.n_q].x);
+  for (int s = tid; s < pc.y; s += kMergeWarps * kWarp) M = fmaxf(M, ml[s * step].x);
   M = warp_max(M);
   if (lane == 0) red[0][warp] = M;
   __syncthreads();
@@ -500,7 +511,7 @@ __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(co
   float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float den = 0.0f;
   auto add = [&](int s, const float4& x) {
-    const float2 m = ml[static_cast<size_t>(s) * P.n_q];
+    const float2 m = ml[s * step];
     // a piece without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
     const float f = m.x == -INFINITY ? 1.0f : ex2(m.x - M);
     den = fmaf(m.y, f, den);
@@ -560,11 +571,16 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   P.n_splits = n_splits;
   P.max_seq_len = max_seq_len;
   P.rows = rows;
-  Partials parts = make_partials(workspace, rows, n_q_heads, n_splits, out);
-  P.pieces = reinterpret_cast<int2*>(parts.ml + static_cast<size_t>(rows) * n_q_heads * n_splits);
+  const size_t n_part = static_cast<size_t>(rows) * n_q_heads * n_splits;
+  P.part_o = reinterpret_cast<float*>(workspace);
+  P.part_ml = reinterpret_cast<float2*>(P.part_o + n_part * kDim);
+  P.pieces = reinterpret_cast<int2*>(P.part_ml + n_part);
+  Partials parts{};
+  parts.o = P.part_o;
+  parts.ml = P.part_ml;
   parts.pieces = P.pieces;
-  P.part_o = parts.o;
-  P.part_ml = parts.ml;
+  parts.out = P.out;
+  parts.n_q = n_q_heads;
   cudaStream_t s = lmps_stream(stream);
   const int status = lmps_launch_pdl(attn_q4_kernel, dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), dim3(kThreads), 0, s, P);
   if (status || n_splits == 1) return status;

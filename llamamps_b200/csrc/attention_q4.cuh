@@ -34,27 +34,21 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Unnormalised results of the pieces of a call: O [pieces, n_q, 128], and per
-// (piece, head) the max (base 2) and the sum.  Row r has pieces[r].y of them
-// from pieces[r].x on; n_splits from r * n_splits on where `pieces` is NULL.
+// Unnormalised results of the pieces of a call and where they lie.  Decode
+// (rows_item 0): O [piece][n_q][128], row r has pieces[r].y of them from
+// pieces[r].x on.  Many queries a sequence: O [piece][n_kv][rows_item][128] of
+// blocks of rows_item (query, head) rows; entry (block from the last) * batch +
+// sequence of `pieces`, and query i >= q_lens[b] is left alone (q_lens NULL:
+// none is).  ml: per O row the max (base 2) and the sum.
 struct Partials {
   float* o;
   float2* ml;
   const int2* pieces;
   __half* out;  // [rows, n_q * 128]
-  int n_q, n_splits;
-  const int32_t* q_lens;  // row b * seq + i with i >= q_lens[b] is left alone (NULL: all rows count)
-  int seq;
+  int n_q, n_kv, rows_item;
+  const int32_t* q_lens;
+  int seq, batch, n_blocks;
 };
-static inline Partials make_partials(void* workspace, int rows, int n_q, int n_splits, uint16_t* out) {
-  Partials p{};
-  p.o = reinterpret_cast<float*>(workspace);
-  p.ml = reinterpret_cast<float2*>(p.o + static_cast<size_t>(rows) * n_q * n_splits * kDim);
-  p.out = reinterpret_cast<__half*>(out);
-  p.n_q = n_q;
-  p.n_splits = n_splits;
-  return p;
-}
 // Launches the merge of `rows` rows.
 int combine_launch(const Partials& p, int rows, cudaStream_t stream);
 // LMPS_OK, or why the attention entry points refuse these sizes.
