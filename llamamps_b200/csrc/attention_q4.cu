@@ -43,6 +43,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * kWarp;
 constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
+constexpr int kMaxCluster = 8;
+constexpr int kClusterShare = 640;  // positions of a CTA up to which a row is shared by a cluster
 constexpr int kOffV = kStep * kCodeBytes;
 constexpr int kOffKs = 2 * kOffV;
 constexpr int kOffVs = kOffKs + kStep * 8;
@@ -57,6 +59,7 @@ struct AttnParams {
   float2* part_ml;
   int2* pieces;             // with more than one split: first piece and their number, per row
   int n_q, n_splits, rows, max_seq_len;
+  int cluster;  // CTAs of a cluster that share a row (0: pieces and a merge kernel where n_splits > 1)
   // fused RoPE + append (qkv != nullptr)
   const __half* qkv;
   const int32_t* pos;
@@ -123,7 +126,20 @@ struct __align__(16) Smem {
   double2 csd[kDim / 2];  // (cos, sin) of the new position: K's and q's
   float2 csf[kDim / 2];
   float wm[kWarps][kMaxHeads], wl[kWarps][kMaxHeads];
+  float cm[kMaxHeads], cl[kMaxHeads], co[kMaxHeads][kDim];  // the CTA's, for the other CTAs of a cluster
 };
+
+// This word of shared memory in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // A warp's running state: per lane heads 2t, 2t + 1; l is the lane's own part of the sum.
 struct State {
@@ -136,7 +152,7 @@ struct State {
 template <bool kFull>
 __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int end, uint32_t ok,
                                           const uint32_t (&qf)[16], State& S) {
-  const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  const int lane = threadIdx.x & 31, g8 = lane >> 2;
   // this lane's row address for ldmatrix: row lane & 7, chunk lane >> 3, stored at chunk ^ ((row >> 1) & 3)
   const uint32_t lm = smem_u32(st) + (lane & 7) * kCodeBytes + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
   float s[2][4];
@@ -234,6 +250,12 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   if (P.n_splits == 1) {
     T = P.length(row);
     end = T;
+  } else if (P.cluster) {  // equal shares of the row
+    row = blockIdx.x / P.cluster;
+    T = P.length(row);
+    const int share = ((T + P.cluster - 1) / P.cluster + kStep - 1) / kStep * kStep;
+    start = min(T, static_cast<int>(blockIdx.x - row * P.cluster) * share);
+    end = min(T, start + share);
   } else {
     // Pieces of equal size: blockIdx.x counts them over the rows in order, every warp finds the
     // row of its own (`cut` is at least total / ((n_splits - 1) rows), so with a last, shorter piece
@@ -345,28 +367,48 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   }
 
   const uint32_t ring = smem_u32(&S.stage[warp][0][0]);
-  const size_t scale_off = static_cast<size_t>(P.c.page_size) * kCodeBytes;
+  const uint32_t scale_off = static_cast<uint32_t>(P.c.page_size) * kCodeBytes;
+  const uint32_t block_bytes = static_cast<uint32_t>(P.c.page_size) * kRowBytes;
   const bool one_page = P.c.page_size % kStep == 0;  // a step's two runs lie in one page
   // Page of the run at position p (or -1: past the end or a bad page).
   auto page_of = [&](int p) {
     if (p >= end) return -1;
     const int page = __ldg(bt + P.c.page_index(p));
-    if (page >= 0 && page < P.c.n_pages) return page;
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(P.c.n_pages)) return page;
     if (lane == 0) raise_error(P.c.error, kErrPage);
     return -1;
   };
   // Pages of the two runs of the step at p.
   auto pages_of = [&](int p) {
     const int a = page_of(p);
-    return make_int2(a, one_page ? (p + 16 < end ? a : -1) : page_of(p + 16));
+    return make_int2(a, one_page ? a : page_of(p + 16));
   };
   // Copies the step at p0 into stage sb; returns the bits of the loaded runs.  Code chunk i of a run
   // (row i / 4) goes to chunk (i & 3) ^ ((row >> 1) & 3) of its row; 8 rows on that is the same place.
+  // In one page the step is 2048 and 256 contiguous bytes of K, and of V (rows past the end are in the
+  // page too, and masked).
   const uint32_t code_dst = (lane >> 2) * kCodeBytes + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  const uint8_t* const scale_pool = lane < 16 ? P.c.k : P.c.v;
+  const uint32_t scale_dst = (lane < 16 ? kOffKs : kOffVs) + 16 * (lane & 15);
   auto load = [&](int p0, int sb, int2 pages) {
     const uint32_t st = ring + sb * kStageBytes;
-    uint32_t ok = 0u;
+    if (one_page) {
+      if (pages.x < 0) return 0u;
+      const uint32_t off = p0 - P.c.page_index(p0) * P.c.page_size;
+      const size_t blk = static_cast<size_t>(static_cast<uint32_t>(pages.x) * P.c.n_kv + kvh) * block_bytes;
+      const uint8_t* k = P.c.k + (blk + off * kCodeBytes + 16 * lane);
+      const uint8_t* v = P.c.v + (blk + off * kCodeBytes + 16 * lane);
+      const uint32_t d = st + code_dst;
 #pragma unroll
+      for (int x = 0; x < kStep / 8; ++x) {
+        cp16(d + 8 * kCodeBytes * x, k + 8 * kCodeBytes * x);
+        cp16(d + kOffV + 8 * kCodeBytes * x, v + 8 * kCodeBytes * x);
+      }
+      cp16(st + scale_dst, scale_pool + (blk + scale_off + off * 8 + 16 * (lane & 15)));
+      return 3u;
+    }
+    uint32_t ok = 0u;
+#pragma unroll 1
     for (int x = 0; x < 2; ++x) {
       const int page = x ? pages.y : pages.x;
       if (page < 0) continue;
@@ -378,10 +420,8 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
       cp16(d + 8 * kCodeBytes, P.c.k + code + 8 * kCodeBytes);
       cp16(d + kOffV, P.c.v + code);
       cp16(d + kOffV + 8 * kCodeBytes, P.c.v + code + 8 * kCodeBytes);
-      if (lane < 16) {  // scales: 8 chunks of K, 8 of V
-        const uint8_t* src = (lane < 8 ? P.c.k : P.c.v) + at + scale_off + off * 8 + 16 * (lane & 7);
-        cp16(st + (lane < 8 ? kOffKs : kOffVs) + 128 * x + 16 * (lane & 7), src);
-      }
+      if ((lane & 15) < 8)  // scales: 8 chunks of K, 8 of V
+        cp16(st + scale_dst + 128 * x, scale_pool + at + scale_off + off * 8 + 16 * (lane & 7));
     }
     return ok;
   };
@@ -460,11 +500,43 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
     if (P.n_splits == 1) {
       P.out[(static_cast<size_t>(row) * P.n_q + kvh * G + h) * kDim + d] =
           __float2half_rn(den == 0.0f ? 0.0f : num / den);
+    } else if (P.cluster) {
+      S.co[h][d] = num;
+      if (d == 0) {
+        S.cm[h] = M;
+        S.cl[h] = den;
+      }
     } else {
       const size_t at = static_cast<size_t>(blockIdx.x) * P.n_q + kvh * G + h;
       P.part_o[at * kDim + d] = num;
       if (d == 0) P.part_ml[at] = make_float2(M, den);
     }
+  }
+  if (P.cluster) {  // the CTAs' states meet: each writes its part of the row
+    cluster_sync();
+    const int rank = blockIdx.x - row * P.cluster;
+    for (int w = rank * kThreads + tid; w < G * kDim; w += P.cluster * kThreads) {
+      const int h = w / kDim, d = w - h * kDim;
+      float m[kMaxCluster], l[kMaxCluster], o[kMaxCluster], M = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i) {
+        const uint32_t from = i < P.cluster ? i : 0;
+        m[i] = ld_cluster(&S.cm[h], from);
+        l[i] = ld_cluster(&S.cl[h], from);
+        o[i] = ld_cluster(&S.co[h][d], from);
+        M = fmaxf(M, m[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i)
+        if (i < P.cluster) {
+          const float f = m[i] == -INFINITY ? 1.0f : ex2(m[i] - M);
+          num = fmaf(o[i], f, num);
+          den = fmaf(l[i], f, den);
+        }
+      P.out[(static_cast<size_t>(row) * P.n_q + kvh * G + h) * kDim + d] =
+          __float2half_rn(den == 0.0f ? 0.0f : num / den);
+    }
+    cluster_sync();  // nobody's shared memory goes while it is read
   }
 }
 
@@ -553,6 +625,23 @@ int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, in
   return LMPS_OK;
 }
 
+static int attn_launch(dim3 grid, cudaStream_t stream, const AttnParams& P) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = P.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = P.cluster ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q4_kernel, P);
+  return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
+}
+
 static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* v_pool, int n_pages,
                             const int32_t* block_table, uint16_t* out, void* workspace, size_t workspace_bytes,
                             int max_pages, int page_size, int n_q_heads, int n_kv_heads, int head_dim, int rows,
@@ -582,8 +671,11 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   parts.out = P.out;
   parts.n_q = n_q_heads;
   cudaStream_t s = lmps_stream(stream);
-  const int status = lmps_launch_pdl(attn_q4_kernel, dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), dim3(kThreads), 0, s, P);
-  if (status || n_splits == 1) return status;
+  // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one
+  // launch (1 x 2049: 8.8 -> 8.3 us, 64 x 500..2100 on 6 heads 13.9 -> 11.9).  Longer ones are cut into pieces by their lengths, merged by a kernel.
+  P.cluster = n_splits > 1 && n_splits <= kMaxCluster && max_seq_len <= n_splits * kClusterShare ? n_splits : 0;
+  const int status = attn_launch(dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), s, P);
+  if (status || n_splits == 1 || P.cluster) return status;
   return combine_launch(parts, rows, s);
 }
 
@@ -595,12 +687,17 @@ using namespace lmps;
 extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len) {
   if (batch <= 0 || n_kv_heads <= 0 || max_seq_len <= 0) return 1;
   // Four CTAs per SM run at once (128 registers).  Short caches and batches that fill the GPU several
-  // times over are not split; else as many pieces as run at once, but none below 128 positions.
+  // times over are not split; else as many pieces as run at once, but none below 128 positions, and
+  // 256 in a cluster.  Sweep, us per call (graph replay): 64 x 4100..8200 4 44.5 / 5 37.2 / 6 41.7 / 10 40.3;
+  // 4 x 32768 37 24.4 / 75 17.2 / 112 22.8.
   const long long items = static_cast<long long>(batch) * n_kv_heads, slots = 4 * 148;
   if (max_seq_len <= 2 * q4::kWarps * q4::kStep || items >= 4 * slots) return 1;
+  const long long room = slots / items < 1 ? 1 : slots / items;
+  const long long share = (max_seq_len + 255) / 256, cluster = share < room ? share : room;
+  if (cluster >= 2 && max_seq_len <= (cluster < q4::kMaxCluster ? cluster : q4::kMaxCluster) * q4::kClusterShare)
+    return static_cast<int>(cluster < q4::kMaxCluster ? cluster : q4::kMaxCluster);
   const long long most = (max_seq_len + q4::kWarps * q4::kStep - 1) / (q4::kWarps * q4::kStep);
-  long long n = slots / items;
-  n = n < 1 ? 1 : n > most ? most : n;
+  const long long n = room > most ? most : room;
   return static_cast<int>(n > 1023 ? 1024 : n + 1);
 }
 
