@@ -301,9 +301,15 @@ int lmps_rope_kv_append_q4(const uint16_t* qkv, const int32_t* pos, const float*
 
 /* lmps_gqa_decode_attention over the 4-bit cache: softmax(0.088388 q k^T) v
  * of one query row per sequence over its first seq_lens[b] <= max_seq_len
- * positions (0: zeros).  Split over the sequence as there; n_splits from
- * lmps_attention_q4_splits, workspace from lmps_attention_q4_workspace_size. */
+ * positions (0: zeros).  n_splits (any from 1 to 1024; lmps_attention_q4_splits
+ * proposes) shares the positions out: up to 8 over rows of at most 640
+ * positions a split go to a thread-block cluster per row, more are cut into at
+ * most n_splits * batch pieces by the sequences' lengths, whose partials lie in
+ * the workspace (lmps_attention_q4_workspace_size) until a second kernel
+ * merges them. */
 int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len);
+/* kernels that such a call launches: 1, or 2 where a second one merges */
+int lmps_attention_q4_launches(int n_splits, int max_seq_len);
 size_t lmps_attention_q4_workspace_size(int batch, int n_q_heads, int head_dim, int n_splits);
 int lmps_gqa_decode_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, int n_pages,
                                  const int32_t* block_table, const int32_t* seq_lens, uint16_t* out,

@@ -71,6 +71,7 @@ _SIGS = {
                                  ctypes.c_ulonglong, c_vp, c_vp, c_vp]),
     "lmps_rope_kv_append_q4": (c_int, [c_vp] * 8 + [c_int, c_vp] + [c_int] * 7 + [c_vp, c_vp]),
     "lmps_attention_q4_splits": (c_int, [c_int, c_int, c_int]),
+    "lmps_attention_q4_launches": (c_int, [c_int, c_int]),
     "lmps_attention_q4_workspace_size": (c_size, [c_int, c_int, c_int, c_int]),
     "lmps_gqa_decode_attention_q4": (c_int, [c_vp] * 3 + [c_int] + [c_vp] * 4 + [c_size] + [c_int] * 8
                                      + [c_vp, c_vp]),

@@ -56,9 +56,10 @@ class ModelConfig:
         biases = self.n_layers * self.qkv_rows * 2
         return self.n_layers * self.layer_q4_bytes() + lm + norms + biases + d * 2 + d * 2
 
-    def kv_bytes_per_position(self) -> int:
-        """K + V bytes read per attended position over all layers."""
-        return self.n_layers * 2 * self.kv_dim * 2
+    def kv_bytes_per_position(self, kv_bits: int = 16) -> int:
+        """K + V bytes read per attended position over all layers (4 bits: 64 code bytes and 4 fp16 scales
+        per row of 128)."""
+        return self.n_layers * 2 * (self.kv_dim * 2 if kv_bits == 16 else self.kv_dim // 128 * 72)
 
 
 QWEN2_5_1_5B = ModelConfig()

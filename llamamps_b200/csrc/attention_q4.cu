@@ -673,7 +673,7 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   cudaStream_t s = lmps_stream(stream);
   // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one
   // launch (1 x 2049: 8.8 -> 8.3 us, 64 x 500..2100 on 6 heads 13.9 -> 11.9).  Longer ones are cut into pieces by their lengths, merged by a kernel.
-  P.cluster = n_splits > 1 && n_splits <= kMaxCluster && max_seq_len <= n_splits * kClusterShare ? n_splits : 0;
+  P.cluster = n_splits > 1 && lmps_attention_q4_launches(n_splits, max_seq_len) == 1 ? n_splits : 0;
   const int status = attn_launch(dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), s, P);
   if (status || n_splits == 1 || P.cluster) return status;
   return combine_launch(parts, rows, s);
@@ -699,6 +699,10 @@ extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_l
   const long long most = (max_seq_len + q4::kWarps * q4::kStep - 1) / (q4::kWarps * q4::kStep);
   const long long n = room > most ? most : room;
   return static_cast<int>(n > 1023 ? 1024 : n + 1);
+}
+
+extern "C" int lmps_attention_q4_launches(int n_splits, int max_seq_len) {
+  return n_splits <= 1 || (n_splits <= q4::kMaxCluster && max_seq_len <= n_splits * q4::kClusterShare) ? 1 : 2;
 }
 
 extern "C" size_t lmps_attention_q4_workspace_size(int batch, int n_q_heads, int head_dim, int n_splits) {

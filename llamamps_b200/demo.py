@@ -71,6 +71,7 @@ def main(argv: Optional[Sequence[str]] = None, config: ModelConfig = QWEN2_5_1_5
     ap.add_argument("--seed", type=int, default=1)
     ap.add_argument("--ids", required=True, help="comma-separated prompt token ids")
     ap.add_argument("--new", type=int, default=16, help="tokens to generate")
+    ap.add_argument("--kv-bits", type=int, choices=(4, 16), default=16, help="bits of the KV cache's elements")
     a = ap.parse_args(argv)
     import torch
     from .engine import QwenEngine
@@ -78,10 +79,11 @@ def main(argv: Optional[Sequence[str]] = None, config: ModelConfig = QWEN2_5_1_5
     max_seq = len(ids) + a.new + 1
     if a.synthetic:
         from .weights import synth_model
-        engine = QwenEngine(weights=synth_model(config, seed=a.seed, device="cuda"), max_seq_len=max_seq)
+        engine = QwenEngine(weights=synth_model(config, seed=a.seed, device="cuda"), max_seq_len=max_seq,
+                            kv_bits=a.kv_bits)
         embed_row = engine.weights.embed[ids[0]].cpu().numpy()
     elif a.weights:
-        engine = QwenEngine(a.weights, config=config, max_seq_len=max_seq)
+        engine = QwenEngine(a.weights, config=config, max_seq_len=max_seq, kv_bits=a.kv_bits)
         embed_row, _ = get_input_vector(ids, os.path.join(a.weights, "global", "embed_tokens.bin"),
                                         hidden=config.hidden)
     else:

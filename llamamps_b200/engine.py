@@ -34,7 +34,7 @@ import torch
 from . import kernels as K
 from ._lib import lib
 from .config import QWEN2_5_1_5B, ModelConfig
-from .kv_cache import PagedKVCache
+from .kv_cache import PagedKVCache, PagedKVCacheQ4
 from .weights import ModelWeights, load_reference_layout
 
 
@@ -89,7 +89,13 @@ class QwenEngine:
                  weights: Optional[ModelWeights] = None, config: ModelConfig = QWEN2_5_1_5B,
                  max_batch: int = 1, max_seq_len: int = 2048, page_size: int = 64,
                  use_graphs: bool = True, page_order: Optional[List[int]] = None,
-                 decoder: Optional[str] = None, gemv_max_batch: int = GEMV_MAX_BATCH):
+                 decoder: Optional[str] = None, gemv_max_batch: int = GEMV_MAX_BATCH, kv_bits: int = 16):
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits is 16 (fp16 cache) or 4, not {kv_bits}")
+        if kv_bits == 4:  # the one-launch decoders read fp16 pools
+            if decoder not in (None, "kernels"):
+                raise ValueError(f"the {decoder!r} decoder reads an fp16 cache: kv_bits=4 runs the per-stage kernels")
+            decoder = "kernels"
         if not torch.cuda.is_available():
             raise RuntimeError("QwenEngine needs a CUDA device (B200); there is no CPU path.")
         self.device = torch.device(device if device is not None else "cuda")
@@ -108,10 +114,15 @@ class QwenEngine:
         # batches above this run the projections and LM head on the tensor-core GEMM
         self.gemv_max_batch = gemv_max_batch
         self.use_graphs = use_graphs
-        self.cache = PagedKVCache(self.cfg, self.layers, max_batch, max_seq_len, page_size,
-                                  self.device, page_order=page_order)
+        # kv_bits=4: keys and values in the 4-bit paged cache (72 bytes a row of 128 instead of 256)
+        self.kv_bits = kv_bits
+        self.cache = (PagedKVCacheQ4 if kv_bits == 4 else PagedKVCache)(
+            self.cfg, self.layers, max_batch, max_seq_len, page_size, self.device, page_order=page_order)
         self.max_seq_len = self.cache.max_seq_len
-        self.n_splits = K.attention_splits(max_batch, self.cfg.n_kv_heads, self.max_seq_len, page_size)
+        if kv_bits == 4:
+            self.n_splits = K.attention_q4_splits(max_batch, self.cfg.n_kv_heads, self.max_seq_len)
+        else:
+            self.n_splits = K.attention_splits(max_batch, self.cfg.n_kv_heads, self.max_seq_len, page_size)
         self._create_buffer_pool()
         self._graphs = {}
         # "persistent": one cooperative kernel per launch runs whole decode
@@ -156,7 +167,9 @@ class QwenEngine:
         off = (-self.gemm_ws.data_ptr()) % 256
         self.gemm_ws = self.gemm_ws[off:off + ws] if ws else None
         self.buf_logits = torch.zeros(B, c.vocab, dtype=h, device=dev)
-        ws = K.attention_workspace_size(B, c.n_q_heads, c.head_dim, self.n_splits)
+        ws = (K.attention_q4_workspace_size if self.kv_bits == 4 else K.attention_workspace_size)(
+            B, c.n_q_heads, c.head_dim, self.n_splits)
+        self.kv_err = torch.zeros(1, dtype=torch.int32, device=dev)  # Q4_ERR_* bits of the 4-bit cache's kernels
         self.attn_ws = torch.zeros(max(ws, 16), dtype=torch.uint8, device=dev)
         self.inv_freq = torch.from_numpy(rope_inv_freq(c.head_dim, c.rope_theta)).to(dev)
         i32 = torch.int32
@@ -214,10 +227,17 @@ class QwenEngine:
                                out=self.buf_qkv[:B])
             # RoPE + KV append + attention in one launch (rope_kv_append's work
             # done by the attention CTAs)
-            K.gqa_decode_attention_rope(self.buf_qkv[:B], self.pos, self.inv_freq, kp, vp,
-                                        self.cache.block_table, self.seq_lens, self.buf_attn[:B],
-                                        self.attn_ws, self.cache.page_size, c.n_q_heads, c.n_kv_heads,
-                                        c.head_dim, self.max_seq_len, self.n_splits, c.rope_style_code)
+            if self.kv_bits == 4:
+                K.gqa_decode_attention_rope_q4(self.buf_qkv[:B], self.pos, self.inv_freq, kp, vp,
+                                               self.cache.block_table, self.seq_lens, self.buf_attn[:B],
+                                               self.attn_ws, self.cache.page_size, c.n_q_heads, c.n_kv_heads,
+                                               c.head_dim, self.max_seq_len, self.n_splits, c.rope_style_code,
+                                               error=self.kv_err)
+            else:
+                K.gqa_decode_attention_rope(self.buf_qkv[:B], self.pos, self.inv_freq, kp, vp,
+                                            self.cache.block_table, self.seq_lens, self.buf_attn[:B],
+                                            self.attn_ws, self.cache.page_size, c.n_q_heads, c.n_kv_heads,
+                                            c.head_dim, self.max_seq_len, self.n_splits, c.rope_style_code)
             self._o_proj(lw, self.buf_attn[:B], x, gemm)
             K.rms_norm(x, lw.post_norm, c.eps, out=xn)
             if gemm:
@@ -316,6 +336,7 @@ class QwenEngine:
         torch.cuda.current_stream(self.device).synchronize()
         if self.pdec is not None and self._pin_err_np[0] != 0:
             self.pdec.check_error()
+        self.check_kv_error()
         self.host_pos += 1
         return self._pin_logits_np.copy()
 
@@ -397,7 +418,11 @@ class QwenEngine:
         # gate/up (+ SwiGLU on the GEMM path), down; then embed, final norm, the
         # LM head with its argmax (two launches on either path), advance
         gemm = self.batch > self.gemv_max_batch
-        per_layer = 7 + (1 if self.n_splits > 1 else 0) + (1 if gemm else 0)
+        if self.kv_bits == 4:
+            attn = K.attention_q4_launches(self.n_splits, self.max_seq_len)
+        else:
+            attn = 2 if self.n_splits > 1 else 1
+        per_layer = 6 + attn + (1 if gemm else 0)
         return 1 + self.layers * per_layer + 1 + 2 + 1
 
     def step_tokens(self, token_ids) -> np.ndarray:
@@ -416,6 +441,7 @@ class QwenEngine:
             self.pdec.check_error()
         if self.bdec is not None:
             self.bdec.check_error()
+        self.check_kv_error()
         return self._pin_next.numpy()[:B].copy()
 
     def decode_step(self, record: bool = True) -> None:
@@ -456,7 +482,7 @@ class QwenEngine:
         GEMM (:meth:`prefill_dense`); otherwise the tokens go through the
         decode path one position at a time."""
         B, P = prompts.shape
-        if P + 1 > self.max_seq_len:
+        if (self.host_pos if self.kv_bits == 4 else 0) + P + 1 > self.max_seq_len:
             raise ValueError("prompt longer than the KV cache")
         prompts = prompts.to(self.device, torch.int32)
         if dense is None:
@@ -487,15 +513,18 @@ class QwenEngine:
         are W4A16 tensor-core GEMMs over M = B*P token rows, RoPE and the KV
         append run on every (sequence, position) row, and the causal
         attention of all rows is one flash-attention launch over the paged
-        cache.  The LM head runs on each sequence's last row only."""
+        cache.  The LM head runs on each sequence's last row only.  With the
+        4-bit cache the rows may follow a cached context (``host_pos`` > 0,
+        the next turn of a conversation)."""
         c, w, dev = self.cfg, self.weights, self.device
         B, P = prompts.shape
-        if self.host_pos != 0:
+        start, q4 = self.host_pos, self.kv_bits == 4
+        if start != 0 and not q4:
             raise RuntimeError("dense prefill starts fresh sequences (call reset first)")
         Mt = B * P
         h, i32 = torch.float16, torch.int32
         ids = prompts.reshape(-1).contiguous()
-        rows_pos = torch.arange(P, dtype=i32, device=dev).repeat(B)
+        rows_pos = torch.arange(start, start + P, dtype=i32, device=dev).repeat(B)
         rows_bt = self.cache.block_table[:B].repeat_interleave(P, dim=0).contiguous()
         x = torch.empty(Mt, c.hidden, dtype=h, device=dev)
         xn = torch.empty_like(x)
@@ -505,16 +534,28 @@ class QwenEngine:
         gate = torch.empty(Mt, c.intermediate, dtype=h, device=dev)
         gu = torch.empty(Mt, 2 * c.intermediate, dtype=h, device=dev)
         err = self.gemm_err
+        if q4:  # the prompt's queries attend to what is cached before them, too
+            starts = torch.full((B,), start, dtype=i32, device=dev)
+            splits = K.prefill_q4_splits(B, P, c.n_q_heads, c.n_kv_heads, start + P)
+            size = K.prefill_q4_workspace_size(B, P, c.n_q_heads, c.head_dim, splits)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         K.embed_gather(w.embed, ids, x, self.bad_ids)
         for li, lw in enumerate(w.layers):
             kp, vp = self.cache.layer(li)
             K.rms_norm(x, lw.in_norm, c.eps, out=xn)
             K.w4a16_gemm(xn, lw.qkv_packed, lw.qkv_scales, c.qkv_rows, c.hidden, bias=lw.qkv_bias,
                          out=qkv, error=err)
-            K.rope_kv_append(qkv, rows_pos, self.inv_freq, q, kp, vp, rows_bt, self.cache.page_size,
-                             c.n_q_heads, c.n_kv_heads, c.head_dim, c.rope_style_code)
-            K.prefill_attention(q, kp, vp, self.cache.block_table[:B], att, B, P, self.cache.page_size,
-                                c.n_q_heads, c.n_kv_heads, c.head_dim, error=err)
+            if q4:
+                K.rope_kv_append_q4(qkv, rows_pos, self.inv_freq, q, kp, vp, rows_bt, self.cache.page_size,
+                                    c.n_q_heads, c.n_kv_heads, c.head_dim, c.rope_style_code, error=self.kv_err)
+                K.prefill_attention_q4(q, kp, vp, self.cache.block_table[:B], att, B, P, self.cache.page_size,
+                                       c.n_q_heads, c.n_kv_heads, c.head_dim, start + P, starts=starts,
+                                       workspace=ws, n_splits=splits, error=self.kv_err)
+            else:
+                K.rope_kv_append(qkv, rows_pos, self.inv_freq, q, kp, vp, rows_bt, self.cache.page_size,
+                                 c.n_q_heads, c.n_kv_heads, c.head_dim, c.rope_style_code)
+                K.prefill_attention(q, kp, vp, self.cache.block_table[:B], att, B, P, self.cache.page_size,
+                                    c.n_q_heads, c.n_kv_heads, c.head_dim, error=err)
             self._o_proj(lw, att, x, True, ws=False)
             K.rms_norm(x, lw.post_norm, c.eps, out=xn)
             self._gate_up(lw, xn, gu, gate, ws=False)
@@ -523,8 +564,8 @@ class QwenEngine:
         self.buf_residual[:B].copy_(x.view(B, P, c.hidden)[:, P - 1])
         self._head(B, want_logits=False)
         self.tokens[:B].copy_(self.next_ids[:B])
-        self.pos[:B].fill_(P)
-        self.seq_lens[:B].fill_(P + 1)
+        self.pos[:B].fill_(start + P)
+        self.seq_lens[:B].fill_(start + P + 1)
         self.history[0, :B].copy_(self.next_ids[:B])
         self.step_counter.fill_(1)
         self.host_pos += P
@@ -589,9 +630,22 @@ class QwenEngine:
         if int(self.bad_ids.item()) != 0:
             self.bad_ids.zero_()
             raise ValueError("token id outside the vocabulary")
+        self.check_kv_error()
         # decode_advance writes row-major [step, B] with the active batch as stride
         hist = self.history.reshape(-1)[: max_new_tokens * B].reshape(max_new_tokens, B)
         return hist.t().cpu().numpy()
+
+    def check_kv_error(self) -> None:
+        """Raises if a kernel of the 4-bit cache reported an error since the last check."""
+        if self.kv_bits != 4:
+            return
+        bits = int(self.kv_err.item())
+        if bits:
+            self.kv_err.zero_()
+            names = [n for b, n in ((K.Q4_ERR_TIMEOUT, "a wait for the tensor core timed out"),
+                                    (K.Q4_ERR_PAGE, "a block table entry outside the pool"),
+                                    (K.Q4_ERR_POSITION, "a position outside the cache")) if bits & b]
+            raise RuntimeError("4-bit KV cache: " + ", ".join(names))
 
     def generate(self, token_ids: Sequence[int], max_new_tokens: int, temperature: float = 0.0, top_k: int = 0,
                  seed: int = 0) -> List[int]:

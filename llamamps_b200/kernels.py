@@ -394,6 +394,12 @@ def attention_q4_splits(batch: int, n_kv_heads: int, max_seq_len: int) -> int:
     return int(lib().lmps_attention_q4_splits(batch, n_kv_heads, max_seq_len))
 
 
+def attention_q4_launches(n_splits: int, max_seq_len: int) -> int:
+    """Kernels of a decode attention call over the 4-bit cache: 1 unsplit or split within a thread-block
+    cluster, 2 where pieces are merged by a second one."""
+    return int(lib().lmps_attention_q4_launches(n_splits, max_seq_len))
+
+
 def attention_q4_workspace_size(batch: int, n_q_heads: int, head_dim: int, n_splits: int) -> int:
     return int(lib().lmps_attention_q4_workspace_size(batch, n_q_heads, head_dim, n_splits))
 

@@ -36,3 +36,31 @@ def pack_q4(w: torch.Tensor):
         from .kernels import q4_pack_device
         return q4_pack_device(w.detach().to(torch.float32).contiguous())
     return pack_q4_host(w)
+
+
+# -- rows of the 4-bit KV cache (include/llamamps_b200.h, "4-bit KV cache") ----
+KV_ROW_BYTES = 72     # 64 code bytes and 4 fp16 scales for 128 elements
+
+
+def quantise_kv_rows(x: torch.Tensor):
+    """fp16 rows [..., 128] as the cache holds them: (uint8 codes [..., 64],
+    fp16 scales [..., 4]).  The scale of a group of 32 is the smallest number
+    with 8 significant bits (and multiple of 2^-24, at most 9344) that is >=
+    max|x| / 7, or 1 for a zero group, so code * scale is exact in fp16; a row
+    that is not finite gets NaN scales."""
+    g = x.to(torch.float64).unflatten(-1, (-1, GROUP))
+    finite = torch.isfinite(g).all(dim=-1).all(dim=-1)[..., None]
+    g = torch.where(finite[..., None], g, torch.zeros_like(g))
+    top = g.abs().amax(dim=-1)
+    m, e = torch.frexp(top / 7.0)
+    scale = torch.ldexp(torch.ceil(m * 256.0), e - 8)
+    scale = torch.where(scale < 2.0 ** -16, torch.ceil(scale * 2.0 ** 24) * 2.0 ** -24, scale).clamp(max=9344.0)
+    scale = torch.where(top == 0, torch.ones_like(scale), scale)
+    n = (torch.round(g / scale[..., None]).clamp(-7, 7).flatten(-2) + 8).to(torch.uint8)
+    return n[..., 0::2] | (n[..., 1::2] << 4), torch.where(finite, scale, torch.nan).to(torch.float16)
+
+
+def dequantise_kv_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The fp16 values of cached rows: (codes [..., 64], scales [..., 4]) -> [..., 128] (exact)."""
+    c = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).to(torch.float32) - 8.0
+    return (c.unflatten(-1, (-1, GROUP)) * scales.to(torch.float32)[..., None]).flatten(-2).to(torch.float16)

@@ -92,3 +92,40 @@ def test_python_layer_refuses_cpu_tensors():
         K.rope_kv_append_q4(torch.zeros(1, 2048, dtype=h), one, torch.zeros(64), q, pool, pool, bt, 64, 12, 2, 128)
     with pytest.raises(RuntimeError, match="CUDA"):
         K.prefill_attention_q4(q, pool, pool, bt, q.clone(), 1, 1, 64, 12, 2, 128, 128)
+
+
+def test_cache_rows_round_trip_on_the_host():
+    """PagedKVCacheQ4 on CPU tensors: what it reads back is the restatement's quantisation of what was written."""
+    import numpy as np
+
+    from llamamps_b200.config import ModelConfig
+    from llamamps_b200.kv_cache import PagedKVCacheQ4
+    from tests import _kv_q4 as R
+    cfg = ModelConfig(n_layers=2, n_q_heads=4, n_kv_heads=2)
+    order = list(np.random.default_rng(0).permutation(2 * 4))
+    kv = PagedKVCacheQ4(cfg, 2, max_batch=2, max_seq_len=60, page_size=16, device="cpu", page_order=order)
+    rng = np.random.default_rng(1)
+    k, v = (rng.normal(0, 2, (50, 256)).astype(np.float16) for _ in range(2))
+    v[3, 5], k[7] = np.nan, 0
+    kv.write_positions(1, 1, 0, torch.from_numpy(k[:20]), torch.from_numpy(v[:20]))
+    kv.write_positions(1, 1, 20, torch.from_numpy(k[20:]), torch.from_numpy(v[20:]))
+    got = kv.read_positions(1, 1, 50)
+    for g, x in zip(got, (k, v)):
+        want = R.values(*R.quantise(x.reshape(-1, 128))).reshape(50, 256)
+        assert np.array_equal(g.numpy().astype(np.float64), want, equal_nan=True)
+    assert kv.k.shape == (2, 8, 2, 16 * 72) and kv.k.dtype == torch.uint8
+    blk = kv.k[1, kv.pages(1)[1], 1]                          # positions 16..31 of KV head 1
+    codes, scales = R.quantise(k[16:32, 128:])
+    cb, sb = R.row_bytes(codes, scales)
+    assert np.array_equal(blk[:16 * 64].numpy().reshape(16, 64), cb)
+    assert np.array_equal(blk[16 * 64:].numpy().reshape(16, 8), sb)
+    with pytest.raises(ValueError, match="page_size"):
+        PagedKVCacheQ4(cfg, 1, 1, 64, page_size=40, device="cpu")
+    with pytest.raises(ValueError, match="heads of 128"):
+        PagedKVCacheQ4(ModelConfig(head_dim=64), 1, 1, 64, device="cpu")
+    assert cfg.kv_bytes_per_position(4) * 32 == cfg.kv_bytes_per_position() * 9
+
+
+def test_launch_counts():
+    assert K.attention_q4_launches(1, 100000) == 1 and K.attention_q4_launches(8, 5120) == 1
+    assert K.attention_q4_launches(8, 5121) == 2 and K.attention_q4_launches(9, 100) == 2
