@@ -14,7 +14,7 @@ import os
 import re
 from typing import List
 
-from .build import INCLUDE, LIB_PATH
+from .build import BIND_PATH, INCLUDE, LIB_PATH
 
 c_int, c_float, c_ll, c_size = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_size_t
 c_vp = ctypes.c_void_p
@@ -111,6 +111,31 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _LIB = L
     return _LIB
+
+
+_BIND = None
+
+
+def binding():
+    """The Python extension of the 4-bit KV cache's eager calls (csrc/bind_q4.cpp), over the entry points of
+    :func:`lib`."""
+    global _BIND
+    if _BIND is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries resolve the extension's symbols)
+        if not os.path.exists(BIND_PATH):
+            raise RuntimeError(f"{BIND_PATH} is missing: build it with `python -m llamamps_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("bind_q4", BIND_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("bind_q4", loader))
+        loader.exec_module(mod)
+        L = lib()
+        mod.bind(*(ctypes.cast(getattr(L, n), c_vp).value for n in (
+            "lmps_rope_kv_append_q4", "lmps_gqa_decode_attention_q4", "lmps_gqa_decode_attention_rope_q4",
+            "lmps_prefill_attention_q4")))
+        _BIND = mod
+    return _BIND
 
 
 def status_string(status: int) -> str:

@@ -3,7 +3,9 @@
 Every ``csrc/*.cu`` file is compiled by nvcc for ``sm_100a`` only and linked
 into one C-ABI shared library (declared in ``include/llamamps_b200.h``).  The
 library is built in-tree so it ships with the source checkout; objects go to
-``llamamps_b200/_build/``.
+``llamamps_b200/_build/``.  ``csrc/bind_q4.cpp`` becomes the Python extension
+``llamamps_b200/lib/bind_q4.so`` (the 4-bit KV cache's eager calls), compiled
+by the host compiler against the installed torch.
 
     python -m llamamps_b200.build [--force] [--verbose]
 """
@@ -25,6 +27,7 @@ BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB_NAME = "libllamamps_b200.so"
 LIB_PATH = os.path.join(LIBDIR, LIB_NAME)
+BIND_PATH = os.path.join(LIBDIR, "bind_q4.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -69,8 +72,47 @@ def _compile(nvcc, src, obj, verbose):
     return r.stderr if verbose else ""
 
 
+def build_binding(force: bool = False) -> str:
+    """Compile the Python extension of csrc/bind_q4.cpp (if it, the header or torch changed)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    src = os.path.join(CSRC, "bind_q4.cpp")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    stamp = os.path.join(LIBDIR, ".bind_stamp")
+    digest = _digest([src, os.path.join(INCLUDE, "llamamps_b200.h")],
+                     " ".join(flags) + torch.__version__ + sys.version)
+    if not force and os.path.exists(BIND_PATH) and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read().strip() == digest:
+                return BIND_PATH
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
+    inc = [*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = BIND_PATH + ".tmp"
+    os.makedirs(LIBDIR, exist_ok=True)
+    r = subprocess.run([shutil.which("g++") or "g++", *flags, *[f"-I{i}" for i in inc], src, "-o", tmp, f"-L{libs}",
+                        "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on bind_q4.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BIND_PATH)
+    with open(stamp, "w") as f:
+        f.write(digest)
+    return BIND_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile (if sources changed) and return the library path."""
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        binding = ex.submit(build_binding, force)
+        path = _build_library(force, verbose)
+        binding.result()
+    return path
+
+
+def _build_library(force: bool, verbose: bool) -> str:
     srcs = _sources()
     stamp = os.path.join(LIBDIR, ".build_stamp")
     digest = _digest(srcs + _headers(), " ".join(NVCC_FLAGS))

@@ -53,6 +53,9 @@ constexpr int kHalf = 64;        // keys per softmax step: half a key tile
 constexpr uint32_t kColS = 0;    // S of row tile t, half u at columns 64 (2 t + u); P over its first 32
 constexpr uint32_t kColO = 256;  // O of row tile t at columns 256 + 128 t
 constexpr float kRescaleLog2 = 8.0f;
+// P is held times 2^7 (below 2^15 with the above): in a long flat softmax most weights lie 2^-13 and
+// less under the largest, where fp16 would lose bits to its subnormals.
+constexpr float kPBias = 7.0f;
 constexpr int kSms = 148;  // one CTA per SM
 
 struct Params {
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
           l *= alpha;
           if (grow) m_used = mnew;
         }
-        const float nm = m_used == -INFINITY ? 0.0f : -m_used;
+        const float nm = m_used == -INFINITY ? 0.0f : kPBias - m_used;
         const uint64_t nm2 = pair(nm, nm), scale2 = pair(kScaleLog2, kScaleLog2);
         uint64_t sm[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[32];

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import call, check, lib
+from ._lib import binding, call, check, lib
 
 FP16 = torch.float16
 
@@ -357,6 +357,16 @@ def _q4_workspace(workspace, dev: int):
     return (_q4_arg(workspace, "workspace", _U8, dev, n), n) if n else (None, 0)
 
 
+def _q4_done(status, name: str) -> bool:
+    """Whether the binding made the call (None: it found something to diagnose, and the call goes the checked
+    way through ctypes)."""
+    if status is None:
+        return False
+    if status:
+        check(status, name)
+    return True
+
+
 def _q4_call(name: str, dev: int, *args) -> None:
     """The call on the current stream of the tensors' device."""
     if dev == torch._C._cuda_getDevice():
@@ -377,6 +387,9 @@ def rope_kv_append_q4(qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, pa
     ``block_table``; ``k_out`` / ``v_out`` receive the values the cache then
     holds.  Rows with pos < 0 are skipped.  ``error`` (int32 [1]) collects
     Q4_ERR_PAGE / Q4_ERR_POSITION bits."""
+    if _q4_done(binding().append(qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, page_size, n_q_heads,
+                                 n_kv_heads, head_dim, style, k_out, v_out, error), "lmps_rope_kv_append_q4"):
+        return q_out
     dev, rows = qkv.get_device(), qkv.shape[0]
     q_n, kv_n = rows * n_q_heads * head_dim, rows * n_kv_heads * head_dim
     a_qkv = _q4_arg(qkv, "qkv", FP16, dev, q_n + 2 * kv_n)
@@ -409,6 +422,9 @@ def gqa_decode_attention_q4(q, k_pool, v_pool, block_table, seq_lens, out, works
                             error: Optional[torch.Tensor] = None):
     """gqa_decode_attention over the 4-bit cache: one query row per sequence
     over its first ``seq_lens[b]`` positions (0: zeros)."""
+    if _q4_done(binding().decode(q, k_pool, v_pool, block_table, seq_lens, out, workspace, page_size, n_q_heads,
+                                 n_kv_heads, head_dim, max_seq_len, n_splits, error), "lmps_gqa_decode_attention_q4"):
+        return out
     dev, B = q.get_device(), q.shape[0]
     n = B * n_q_heads * head_dim
     a_q = _q4_arg(q, "q", FP16, dev, n)
@@ -426,6 +442,10 @@ def gqa_decode_attention_rope_q4(qkv, pos, inv_freq, k_pool, v_pool, block_table
                                  max_seq_len: int, n_splits: int, style: int = 0, *,
                                  error: Optional[torch.Tensor] = None):
     """rope_kv_append_q4 + gqa_decode_attention_q4 in one call (seq_lens = pos + 1)."""
+    if _q4_done(binding().step(qkv, pos, inv_freq, k_pool, v_pool, block_table, seq_lens, out, workspace, page_size,
+                               n_q_heads, n_kv_heads, head_dim, max_seq_len, n_splits, style, error),
+                "lmps_gqa_decode_attention_rope_q4"):
+        return out
     dev, B = qkv.get_device(), qkv.shape[0]
     n = B * n_q_heads * head_dim
     a_qkv = _q4_arg(qkv, "qkv", FP16, dev, n + 2 * B * n_kv_heads * head_dim)
@@ -457,17 +477,22 @@ def prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch: int, seq_le
     without ``starts``) for i < ``q_lens[b]`` (seq_len without); other rows of
     ``out`` stay as they were.  The K and V of all these positions are already
     in the cache; starts + q_lens <= ``max_seq_len``."""
+    if error is None and q.is_cuda:
+        error = torch.zeros(1, dtype=_I32, device=q.device)
+    if _q4_done(binding().prefill(q, k_pool, v_pool, block_table, out, batch, seq_len, page_size, n_q_heads, n_kv_heads,
+                                  head_dim, max_seq_len, starts, q_lens, workspace, n_splits, error),
+                "lmps_prefill_attention_q4"):
+        return out
     dev = q.get_device()
     n = batch * seq_len * n_q_heads * head_dim
     a_q = _q4_arg(q, "q", FP16, dev, n)
     kp, vp, n_pages, bt, max_pages = _q4_cache(k_pool, v_pool, block_table, dev, page_size, n_kv_heads, batch)
     ws, ws_bytes = _q4_workspace(workspace, dev)
-    err = error if error is not None else torch.zeros(1, dtype=_I32, device=q.device)
     _q4_call("lmps_prefill_attention_q4", dev, a_q, kp, vp, n_pages, bt,
              _q4_arg(starts, "starts", _I32, dev, -batch) if starts is not None else None,
              _q4_arg(q_lens, "q_lens", _I32, dev, -batch) if q_lens is not None else None,
              _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes, max_pages, page_size, n_q_heads, n_kv_heads,
-             head_dim, batch, seq_len, max_seq_len, n_splits, _q4_arg(err, "error", _I32, dev, -1))
+             head_dim, batch, seq_len, max_seq_len, n_splits, _q4_arg(error, "error", _I32, dev, -1))
     return out
 
 

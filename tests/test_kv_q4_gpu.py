@@ -387,3 +387,176 @@ def test_prefill_long_context_rows(cuda):
         for b in range(2):
             for i in range(0, seq, 19):
                 R.close(got[b, i], *R.attend(q[b, i], *c.rows[b], starts[b] + i + 1), f"{b}, {i}, {n_splits}")
+
+
+# -- the calls around the kernels ---------------------------------------------------
+def _all_calls(rng, c, lens, hq, hkv, page, out=None):
+    """One call of each entry point on cache c, as functions of replaced arguments."""
+    from llamamps_b200 import kernels as K
+    B = len(lens)
+    seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    t = dict(qkv=_cu(rng.normal(0, 1, (B, (hq + 2 * hkv) * D)).astype(np.float16)), pos=seq - 1, inv=_cu(_inv()),
+             q=_cu(rng.normal(0, 1, (B, hq * D)).astype(np.float16)), k=c.k, v=c.v, bt=c.bt, lens=seq,
+             out=torch.full((B, hq * D), 7.0, dtype=torch.float16, device="cuda"), ws=None, err=_err(), page=page)
+
+    def append(**kw):
+        a = {**t, **kw}
+        return K.rope_kv_append_q4(a["qkv"], a["pos"], a["inv"], a["out"], a["k"], a["v"], a["bt"], a["page"], hq, hkv,
+                                   D, error=a["err"])
+
+    def decode(**kw):
+        a = {**t, **kw}
+        return K.gqa_decode_attention_q4(a["q"], a["k"], a["v"], a["bt"], a["lens"], a["out"], a["ws"], a["page"], hq,
+                                         hkv, D, c.max_seq_len, 1, error=a["err"])
+
+    def step(**kw):
+        a = {**t, **kw}
+        return K.gqa_decode_attention_rope_q4(a["qkv"], a["pos"], a["inv"], a["k"], a["v"], a["bt"], a["lens"],
+                                              a["out"], a["ws"], a["page"], hq, hkv, D, c.max_seq_len, 1,
+                                              error=a["err"])
+
+    def prefill(**kw):
+        a = {**t, **kw}
+        return K.prefill_attention_q4(a["q"], a["k"], a["v"], a["bt"], a["out"], B, 1, a["page"], hq, hkv, D,
+                                      c.max_seq_len, starts=a["pos"], workspace=a["ws"], error=a["err"])
+    return t, dict(append=append, decode=decode, step=step, prefill=prefill)
+
+
+def test_argument_mistakes_are_named_and_nothing_runs(cuda):
+    rng = np.random.default_rng(21)
+    c = R.Cache(rng, [20, 30], 2, 16, max_len=48)
+    t, calls = _all_calls(rng, c, [21, 31], 12, 2, 16)
+    before = c.k.clone(), c.v.clone()
+    used = dict(append=("qkv", "pos", "inv", "bt", "k", "v", "err"), decode=("q", "lens", "bt", "k", "v", "err"),
+                step=("qkv", "pos", "inv", "lens", "bt", "k", "v", "err"), prefill=("q", "pos", "bt", "k", "v", "err"))
+    for name, call in calls.items():
+        for arg in used[name] + ("out",):
+            good = t[arg]
+            with pytest.raises(RuntimeError, match="CUDA"):
+                call(**{arg: good.cpu()})
+            with pytest.raises(TypeError):
+                call(**{arg: good.to(torch.float64)})
+            if good.dim() == 2:
+                with pytest.raises(ValueError, match="contiguous"):
+                    call(**{arg: torch.stack([good, good], dim=2)[..., 0]})
+            if arg == "bt":
+                with pytest.raises(ValueError, match="block_table"):
+                    call(bt=good[:1])
+            elif arg in ("k", "v"):
+                with pytest.raises(ValueError, match="pools"):
+                    call(**{arg: good[:, :1].contiguous()})
+            elif arg != "err":
+                with pytest.raises(ValueError, match="elements"):
+                    call(**{arg: good.reshape(-1)[:-1].reshape(1, -1) if arg in ("q", "qkv") else good.reshape(-1)[:-1]})
+        with pytest.raises(ValueError, match="pools"):
+            call(page=32)
+        with pytest.raises(AttributeError):
+            call(out=None)
+    torch.cuda.synchronize()
+    assert torch.equal(c.k, before[0]) and torch.equal(c.v, before[1]) and bool((t["out"] == 7).all())
+    with pytest.raises(RuntimeError, match="argument"):   # misaligned: the entry point itself refuses
+        buf = torch.zeros(t["q"].numel() + 1, dtype=torch.float16, device="cuda")
+        calls["decode"](q=buf[1:].view_as(t["q"]))
+
+
+def test_side_stream_and_graph_replay(cuda):
+    """The calls run on the caller's stream; captured, they follow lengths, positions and inputs that change
+    between replays; two graphs may share a workspace."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(22)
+    hq, hkv, page, lens = 12, 2, 16, [300, 41]
+    c = R.Cache(rng, lens, hkv, page, max_len=400)
+    B, n_splits = 2, 11
+    i32 = dict(dtype=torch.int32, device="cuda")
+    seq, pos = torch.tensor(lens, **i32), torch.tensor(lens, **i32) - 1
+    qkv = _cu(rng.normal(0, 1, (B, 16 * D)).astype(np.float16))
+    q = _cu(rng.normal(0, 1, (B * 5, hq * D)).astype(np.float16))
+    inv, err = _cu(_inv()), _err()
+    ws = _ws(max(K.attention_q4_workspace_size(B, hq, D, n_splits), K.prefill_q4_workspace_size(B, 5, hq, D, 3)))
+    outs = [torch.zeros(B, hq * D, dtype=torch.float16, device="cuda"),
+            torch.zeros(B * 5, hq * D, dtype=torch.float16, device="cuda")]
+
+    def one(i):
+        if i == 0:
+            K.gqa_decode_attention_rope_q4(qkv, pos, inv, c.k, c.v, c.bt, seq, outs[0], ws, page, hq, hkv, D,
+                                           c.max_seq_len, n_splits, error=err)
+        else:
+            K.prefill_attention_q4(q, c.k, c.v, c.bt, outs[1], B, 5, page, hq, hkv, D, c.max_seq_len, starts=pos - 4,
+                                   workspace=ws, n_splits=3, error=err)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in (0, 1):
+            one(i)
+        want = [o.clone() for o in outs]
+        graphs = []
+        for i in (0, 1):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                one(i)
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(side)
+    for o in outs:
+        o.zero_()
+    for i in (0, 1, 1, 0):
+        graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    # the next position, another query
+    pos.add_(1)
+    seq.add_(1)
+    qkv.copy_(torch.randn_like(qkv))
+    q.copy_(torch.randn_like(q))
+    for g in graphs:
+        g.replay()
+    got = [o.clone() for o in outs]
+    kept = c.k.clone(), c.v.clone()
+    for i in (0, 1):
+        one(i)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, got)) and err.item() == 0
+    assert torch.equal(c.k, kept[0]) and torch.equal(c.v, kept[1])
+
+
+def test_append_decode_and_chunk_run_as_used(cuda):
+    """A prompt appended and attended, a chunk behind it, then decode steps, on one cache: every stage's
+    attention against the 64-bit restatement on what the cache holds."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(23)
+    hq, hkv, page, B, P, C = 12, 2, 16, 2, 37, 21
+    total = P + C + 3
+    c = R.Cache(rng, [0] * B, hkv, page, max_len=total)
+    inv, err = _cu(_inv()), _err()
+    held = [(np.zeros((total, hkv, D)), np.zeros((total, hkv, D))) for _ in range(B)]
+    at = 0
+    for n in (P, C):
+        qkv = rng.normal(0, 1, (B * n, (hq + 2 * hkv) * D)).astype(np.float16)
+        pos = torch.arange(at, at + n, dtype=torch.int32, device="cuda").repeat(B)
+        q, out = (torch.zeros(B * n, hq * D, dtype=torch.float16, device="cuda") for _ in range(2))
+        ko, vo = (torch.zeros(B * n, hkv * D, dtype=torch.float16, device="cuda") for _ in range(2))
+        K.rope_kv_append_q4(_cu(qkv), pos, inv, q, c.k, c.v, c.bt.repeat_interleave(n, 0).contiguous(), page, hq, hkv,
+                            D, k_out=ko, v_out=vo, error=err)
+        for b in range(B):
+            for half, x in zip(held[b], (ko, vo)):
+                half[at:at + n] = x.view(B, n, hkv, D)[b].cpu().numpy()
+        K.prefill_attention_q4(q, c.k, c.v, c.bt, out, B, n, page, hq, hkv, D, c.max_seq_len,
+                               starts=torch.full((B,), at, dtype=torch.int32, device="cuda"), error=err)
+        qn, got = q.cpu().numpy().reshape(B, n, hq, D), out.cpu().numpy().reshape(B, n, hq, D)
+        for b in range(B):
+            for i in range(0, n, 4):
+                R.close(got[b, i], *R.attend(qn[b, i], *held[b], at + i + 1), f"chunk at {at}, query {i}")
+        at += n
+    for _ in range(3):
+        qkv = rng.normal(0, 1, (B, hq + 2 * hkv, D)).astype(np.float16)
+        pos = torch.full((B,), at, dtype=torch.int32, device="cuda")
+        out = torch.zeros(B, hq * D, dtype=torch.float16, device="cuda")
+        K.gqa_decode_attention_rope_q4(_cu(qkv.reshape(B, -1)), pos, inv, c.k, c.v, c.bt, pos + 1, out, None, page, hq,
+                                       hkv, D, c.max_seq_len, 1, error=err)
+        rot = R.rotate(qkv[:, :hq + hkv], [at] * B, _inv(), 0)
+        for b in range(B):
+            for half, x in zip(held[b], (rot[b, hq:], qkv[b, hq + hkv:])):
+                half[at] = R.values(*R.quantise(x))
+            R.close(out[b].cpu().numpy().reshape(hq, D), *R.attend(rot[b, :hq], *held[b], at + 1), f"step at {at}")
+        at += 1
+    assert err.item() == 0
