@@ -125,17 +125,42 @@ struct __align__(16) Smem {
   uint32_t knew[kRowBytes / 4], vnew[kRowBytes / 4];  // the appended row (fused form)
   double2 csd[kDim / 2];  // (cos, sin) of the new position: K's and q's
   float2 csf[kDim / 2];
-  float wm[kWarps][kMaxHeads], wl[kWarps][kMaxHeads];
-  float cm[kMaxHeads], cl[kMaxHeads], co[kMaxHeads][kDim];  // the CTA's, for the other CTAs of a cluster
+  float wm[kWarps][kMaxHeads], wl[kWarps][kMaxHeads], wf[kWarps][kMaxHeads];
+  float cm[kMaxHeads], cl[kMaxHeads];
+  __align__(16) float co[kMaxHeads][kDim];  // the CTA's, for the other CTAs of a cluster
 };
 
-// This word of shared memory in CTA `rank` of the cluster.
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+// This word, or these four, of shared memory in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(const float* p, uint32_t rank) {
   uint32_t a;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return a;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(p, rank)) : "memory");
   return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr(p, rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void fma4(float4& a, const float4& x, float f) {
+  a.x = fmaf(x.x, f, a.x);
+  a.y = fmaf(x.y, f, a.y);
+  a.z = fmaf(x.z, f, a.z);
+  a.w = fmaf(x.w, f, a.w);
+}
+// o / l as fp16 (zeros where there was no position).
+__device__ __forceinline__ void store_row4(__half* dst, const float4& o, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const __half2 lo = __floats2half2_rn(o.x * inv, o.y * inv), hi = __floats2half2_rn(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -303,6 +328,73 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   const int32_t* bt = P.c.bt + static_cast<size_t>(row) * P.c.max_pages;
   int pnew = -1;
 
+  const uint32_t ring = smem_u32(&S.stage[warp][0][0]);
+  const uint32_t scale_off = static_cast<uint32_t>(P.c.page_size) * kCodeBytes;
+  const uint32_t block_bytes = static_cast<uint32_t>(P.c.page_size) * kRowBytes;
+  const bool one_page = P.c.page_size % kStep == 0;  // a step's two runs lie in one page
+  // Page of the run at position p (or -1: past the end or a bad page).
+  auto page_of = [&](int p) {
+    if (p >= end) return -1;
+    const int page = __ldg(bt + P.c.page_index(p));
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(P.c.n_pages)) return page;
+    if (lane == 0) raise_error(P.c.error, kErrPage);
+    return -1;
+  };
+  // Pages of the two runs of the step at p.
+  auto pages_of = [&](int p) {
+    const int a = page_of(p);
+    return make_int2(a, one_page ? a : page_of(p + 16));
+  };
+  // Copies the step at p0 into stage sb; returns the bits of the loaded runs.  Code chunk i of a run
+  // (row i / 4) goes to chunk (i & 3) ^ ((row >> 1) & 3) of its row; 8 rows on that is the same place.
+  // In one page the step is 2048 and 256 contiguous bytes of K, and of V (rows past the end are in the
+  // page too, and masked).
+  const uint32_t code_dst = (lane >> 2) * kCodeBytes + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+  const uint8_t* const scale_pool = lane < 16 ? P.c.k : P.c.v;
+  const uint32_t scale_dst = (lane < 16 ? kOffKs : kOffVs) + 16 * (lane & 15);
+  auto load = [&](int p0, int sb, int2 pages) {
+    const uint32_t st = ring + sb * kStageBytes;
+    if (one_page) {
+      if (pages.x < 0) return 0u;
+      const uint32_t off = p0 - P.c.page_index(p0) * P.c.page_size;
+      const size_t blk = static_cast<size_t>(static_cast<uint32_t>(pages.x) * P.c.n_kv + kvh) * block_bytes;
+      const uint8_t* k = P.c.k + (blk + off * kCodeBytes + 16 * lane);
+      const uint8_t* v = P.c.v + (blk + off * kCodeBytes + 16 * lane);
+      const uint32_t d = st + code_dst;
+#pragma unroll
+      for (int x = 0; x < kStep / 8; ++x) {
+        cp16(d + 8 * kCodeBytes * x, k + 8 * kCodeBytes * x);
+        cp16(d + kOffV + 8 * kCodeBytes * x, v + 8 * kCodeBytes * x);
+      }
+      cp16(st + scale_dst, scale_pool + (blk + scale_off + off * 8 + 16 * (lane & 15)));
+      return 3u;
+    }
+    uint32_t ok = 0u;
+#pragma unroll 1
+    for (int x = 0; x < 2; ++x) {
+      const int page = x ? pages.y : pages.x;
+      if (page < 0) continue;
+      ok |= 1u << x;
+      const int p = p0 + 16 * x, off = p - P.c.page_index(p) * P.c.page_size;
+      const size_t at = P.c.block(page, kvh), code = at + off * kCodeBytes + 16 * lane;
+      const uint32_t d = st + 16 * x * kCodeBytes + code_dst;
+      cp16(d, P.c.k + code);
+      cp16(d + 8 * kCodeBytes, P.c.k + code + 8 * kCodeBytes);
+      cp16(d + kOffV, P.c.v + code);
+      cp16(d + kOffV + 8 * kCodeBytes, P.c.v + code + 8 * kCodeBytes);
+      if ((lane & 15) < 8)  // scales: 8 chunks of K, 8 of V
+        cp16(st + scale_dst + 128 * x, scale_pool + at + scale_off + off * 8 + 16 * (lane & 7));
+    }
+    return ok;
+  };
+
+  // the first step's copies are on their way while the queries are prepared
+  const int first = start + warp * kStep, stride = kWarps * kStep;
+  uint32_t ok = first < end ? load(first, 0, pages_of(first)) : 0u;
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  int sb = 0;
+  int2 next = pages_of(first + stride);
+
   if (P.qkv) {
     const int p = P.pos[row];
     const bool mine = p >= 0 && p == T - 1 && p >= start && p < end;
@@ -366,76 +458,11 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
     }
   }
 
-  const uint32_t ring = smem_u32(&S.stage[warp][0][0]);
-  const uint32_t scale_off = static_cast<uint32_t>(P.c.page_size) * kCodeBytes;
-  const uint32_t block_bytes = static_cast<uint32_t>(P.c.page_size) * kRowBytes;
-  const bool one_page = P.c.page_size % kStep == 0;  // a step's two runs lie in one page
-  // Page of the run at position p (or -1: past the end or a bad page).
-  auto page_of = [&](int p) {
-    if (p >= end) return -1;
-    const int page = __ldg(bt + P.c.page_index(p));
-    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(P.c.n_pages)) return page;
-    if (lane == 0) raise_error(P.c.error, kErrPage);
-    return -1;
-  };
-  // Pages of the two runs of the step at p.
-  auto pages_of = [&](int p) {
-    const int a = page_of(p);
-    return make_int2(a, one_page ? a : page_of(p + 16));
-  };
-  // Copies the step at p0 into stage sb; returns the bits of the loaded runs.  Code chunk i of a run
-  // (row i / 4) goes to chunk (i & 3) ^ ((row >> 1) & 3) of its row; 8 rows on that is the same place.
-  // In one page the step is 2048 and 256 contiguous bytes of K, and of V (rows past the end are in the
-  // page too, and masked).
-  const uint32_t code_dst = (lane >> 2) * kCodeBytes + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
-  const uint8_t* const scale_pool = lane < 16 ? P.c.k : P.c.v;
-  const uint32_t scale_dst = (lane < 16 ? kOffKs : kOffVs) + 16 * (lane & 15);
-  auto load = [&](int p0, int sb, int2 pages) {
-    const uint32_t st = ring + sb * kStageBytes;
-    if (one_page) {
-      if (pages.x < 0) return 0u;
-      const uint32_t off = p0 - P.c.page_index(p0) * P.c.page_size;
-      const size_t blk = static_cast<size_t>(static_cast<uint32_t>(pages.x) * P.c.n_kv + kvh) * block_bytes;
-      const uint8_t* k = P.c.k + (blk + off * kCodeBytes + 16 * lane);
-      const uint8_t* v = P.c.v + (blk + off * kCodeBytes + 16 * lane);
-      const uint32_t d = st + code_dst;
-#pragma unroll
-      for (int x = 0; x < kStep / 8; ++x) {
-        cp16(d + 8 * kCodeBytes * x, k + 8 * kCodeBytes * x);
-        cp16(d + kOffV + 8 * kCodeBytes * x, v + 8 * kCodeBytes * x);
-      }
-      cp16(st + scale_dst, scale_pool + (blk + scale_off + off * 8 + 16 * (lane & 15)));
-      return 3u;
-    }
-    uint32_t ok = 0u;
-#pragma unroll 1
-    for (int x = 0; x < 2; ++x) {
-      const int page = x ? pages.y : pages.x;
-      if (page < 0) continue;
-      ok |= 1u << x;
-      const int p = p0 + 16 * x, off = p - P.c.page_index(p) * P.c.page_size;
-      const size_t at = P.c.block(page, kvh), code = at + off * kCodeBytes + 16 * lane;
-      const uint32_t d = st + 16 * x * kCodeBytes + code_dst;
-      cp16(d, P.c.k + code);
-      cp16(d + 8 * kCodeBytes, P.c.k + code + 8 * kCodeBytes);
-      cp16(d + kOffV, P.c.v + code);
-      cp16(d + kOffV + 8 * kCodeBytes, P.c.v + code + 8 * kCodeBytes);
-      if ((lane & 15) < 8)  // scales: 8 chunks of K, 8 of V
-        cp16(st + scale_dst + 128 * x, scale_pool + at + scale_off + off * 8 + 16 * (lane & 7));
-    }
-    return ok;
-  };
-
   State A;
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) A.o[mt][0] = A.o[mt][1] = A.o[mt][2] = A.o[mt][3] = 0.0f;
   A.m0 = A.m1 = -INFINITY;
   A.l0 = A.l1 = 0.0f;
-  const int first = start + warp * kStep, stride = kWarps * kStep;
-  uint32_t ok = first < end ? load(first, 0, pages_of(first)) : 0u;
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  int sb = 0;
-  int2 next = pages_of(first + stride);
   for (int p0 = first; p0 < end; p0 += stride) {
     uint32_t next_ok = 0u;
     if (p0 + stride < end) next_ok = load(p0 + stride, sb ^ 1, next);
@@ -484,57 +511,67 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
         make_float4(A.o[2 * g][1], A.o[2 * g][3], A.o[2 * g + 1][1], A.o[2 * g + 1][3]);
   }
   __syncthreads();
-  for (int w = tid; w < G * kDim; w += kThreads) {
-    const int h = w / kDim, d = w - h * kDim;
+  // the warps' states meet: weights once per (warp, head), then four dims a thread
+  if (tid < kWarps * kMaxHeads) {
+    const int i = tid >> 3, h = tid & 7;
     float M = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) M = fmaxf(M, S.wm[i][h]);
-    float num = 0.0f, den = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      // a warp without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
-      const float f = S.wm[i][h] == -INFINITY ? 1.0f : ex2(S.wm[i][h] - M);
-      num = fmaf(S.wo[i][h][d], f, num);
-      den = fmaf(S.wl[i][h], f, den);
+    for (int x = 0; x < kWarps; ++x) M = fmaxf(M, S.wm[x][h]);
+    // a warp without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
+    const float f = S.wm[i][h] == -INFINITY ? 1.0f : ex2(S.wm[i][h] - M);
+    float l = S.wl[i][h] * f;
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    S.wf[i][h] = f;
+    if (i == 0) {
+      S.cm[h] = M;
+      S.cl[h] = l;
     }
+  }
+  __syncthreads();
+  __half* const out = P.out + (static_cast<size_t>(row) * P.n_q + kvh * G) * kDim;
+  for (int w = tid; w < G * (kDim / 4); w += kThreads) {
+    const int h = w >> 5, d = 4 * (w & 31);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) fma4(o, *reinterpret_cast<const float4*>(&S.wo[i][h][d]), S.wf[i][h]);
     if (P.n_splits == 1) {
-      P.out[(static_cast<size_t>(row) * P.n_q + kvh * G + h) * kDim + d] =
-          __float2half_rn(den == 0.0f ? 0.0f : num / den);
+      store_row4(out + h * kDim + d, o, S.cl[h]);
     } else if (P.cluster) {
-      S.co[h][d] = num;
-      if (d == 0) {
-        S.cm[h] = M;
-        S.cl[h] = den;
-      }
+      *reinterpret_cast<float4*>(&S.co[h][d]) = o;
     } else {
       const size_t at = static_cast<size_t>(blockIdx.x) * P.n_q + kvh * G + h;
-      P.part_o[at * kDim + d] = num;
-      if (d == 0) P.part_ml[at] = make_float2(M, den);
+      *reinterpret_cast<float4*>(P.part_o + at * kDim + d) = o;
+      if (d == 0) P.part_ml[at] = make_float2(S.cm[h], S.cl[h]);
     }
   }
   if (P.cluster) {  // the CTAs' states meet: each writes its part of the row
     cluster_sync();
-    const int rank = blockIdx.x - row * P.cluster;
-    for (int w = rank * kThreads + tid; w < G * kDim; w += P.cluster * kThreads) {
-      const int h = w / kDim, d = w - h * kDim;
-      float m[kMaxCluster], l[kMaxCluster], o[kMaxCluster], M = -INFINITY, num = 0.0f, den = 0.0f;
+    const int rank = blockIdx.x - row * P.cluster, units = G * (kDim / 4), share = (units + P.cluster - 1) / P.cluster;
+    for (int x = tid; x < share; x += kThreads) {
+      const int w = rank * share + x;
+      if (w >= units) break;
+      const int h = w >> 5, d = 4 * (w & 31);
+      float m[kMaxCluster], l[kMaxCluster], M = -INFINITY, den = 0.0f;
+      float4 o[kMaxCluster], num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < kMaxCluster; ++i) {
-        const uint32_t from = i < P.cluster ? i : 0;
-        m[i] = ld_cluster(&S.cm[h], from);
-        l[i] = ld_cluster(&S.cl[h], from);
-        o[i] = ld_cluster(&S.co[h][d], from);
-        M = fmaxf(M, m[i]);
-      }
+      for (int i = 0; i < kMaxCluster; ++i)
+        if (i < P.cluster) {
+          m[i] = ld_cluster(&S.cm[h], i);
+          l[i] = ld_cluster(&S.cl[h], i);
+          o[i] = ld_cluster4(&S.co[h][d], i);
+        }
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i)
+        if (i < P.cluster) M = fmaxf(M, m[i]);
 #pragma unroll
       for (int i = 0; i < kMaxCluster; ++i)
         if (i < P.cluster) {
           const float f = m[i] == -INFINITY ? 1.0f : ex2(m[i] - M);
-          num = fmaf(o[i], f, num);
+          fma4(num, o[i], f);
           den = fmaf(l[i], f, den);
         }
-      P.out[(static_cast<size_t>(row) * P.n_q + kvh * G + h) * kDim + d] =
-          __float2half_rn(den == 0.0f ? 0.0f : num / den);
+      store_row4(out + h * kDim + d, num, den);
     }
     cluster_sync();  // nobody's shared memory goes while it is read
   }
