@@ -302,7 +302,7 @@ int lmps_rope_kv_append_q4(const uint16_t* qkv, const int32_t* pos, const float*
 /* lmps_gqa_decode_attention over the 4-bit cache: softmax(0.088388 q k^T) v
  * of one query row per sequence over its first seq_lens[b] <= max_seq_len
  * positions (0: zeros).  n_splits (any from 1 to 1024; lmps_attention_q4_splits
- * proposes) shares the positions out: up to 8 over rows of at most 640
+ * proposes) shares the positions out: up to 8 over rows of at most 1280
  * positions a split go to a thread-block cluster per row, more are cut into at
  * most n_splits * batch pieces by the sequences' lengths, whose partials lie in
  * the workspace (lmps_attention_q4_workspace_size) until a second kernel

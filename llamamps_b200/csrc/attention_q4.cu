@@ -39,12 +39,15 @@
 namespace lmps {
 namespace q4 {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * kWarp;
+// Warps per CTA.  A step takes a lone warp 1.4 us, so short rows want many warps at once (1 x 131: 8 warps
+// 4.0 us, 4 warps 4.6); long ones are cut into pieces, which fill the SMs better in units of 128 positions
+// (64 x 4100..8200: 4 warps 37 us, 8 warps 41).  16 warps run per SM either way (128 registers).
+constexpr int kShortWarps = 8, kPieceWarps = 4;
+constexpr int kWarpsPerSm = 16;
 constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
 constexpr int kMaxCluster = 8;
-constexpr int kClusterShare = 640;  // positions of a CTA up to which a row is shared by a cluster
+constexpr int kClusterShare = 1280;  // positions of a CTA up to which a row is shared by a cluster
 constexpr int kOffV = kStep * kCodeBytes;
 constexpr int kOffKs = 2 * kOffV;
 constexpr int kOffVs = kOffKs + kStep * 8;
@@ -116,6 +119,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+template <int kWarps>
 struct __align__(16) Smem {
   union {
     unsigned char stage[kWarps][kStages][kStageBytes];
@@ -264,10 +268,13 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
   }
 }
 
-__global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * kWarp, kWarpsPerSm / kWarps) attn_q4_kernel(const AttnParams P) {
+  constexpr int kThreads = kWarps * kWarp;
   lmps_pdl_trigger();
   lmps_pdl_wait();
-  __shared__ Smem S;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Smem<kWarps>& S = *reinterpret_cast<Smem<kWarps>*>(smem_raw);
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const int G = P.n_q / P.c.n_kv;
@@ -512,21 +519,19 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnParams P) {
   }
   __syncthreads();
   // the warps' states meet: weights once per (warp, head), then four dims a thread
-  if (tid < kWarps * kMaxHeads) {
-    const int i = tid >> 3, h = tid & 7;
-    float M = -INFINITY;
+  if (tid < kMaxHeads) {
+    float M = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x) M = fmaxf(M, S.wm[x][h]);
-    // a warp without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
-    const float f = S.wm[i][h] == -INFINITY ? 1.0f : ex2(S.wm[i][h] - M);
-    float l = S.wl[i][h] * f;
-    l += __shfl_xor_sync(0xffffffffu, l, 8);
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
-    S.wf[i][h] = f;
-    if (i == 0) {
-      S.cm[h] = M;
-      S.cl[h] = l;
+    for (int i = 0; i < kWarps; ++i) M = fmaxf(M, S.wm[i][tid]);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      // a warp without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
+      const float f = S.wm[i][tid] == -INFINITY ? 1.0f : ex2(S.wm[i][tid] - M);
+      l = fmaf(S.wl[i][tid], f, l);
+      S.wf[i][tid] = f;
     }
+    S.cm[tid] = M;
+    S.cl[tid] = l;
   }
   __syncthreads();
   __half* const out = P.out + (static_cast<size_t>(row) * P.n_q + kvh * G) * kDim;
@@ -662,10 +667,14 @@ int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, in
   return LMPS_OK;
 }
 
+template <int kWarps>
 static int attn_launch(dim3 grid, cudaStream_t stream, const AttnParams& P) {
+  const int st = lmps_max_dyn_smem<attn_q4_kernel<kWarps>>(static_cast<int>(sizeof(Smem<kWarps>)));
+  if (st != LMPS_OK) return st;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kWarps * kWarp);
+  cfg.dynamicSmemBytes = sizeof(Smem<kWarps>);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -675,7 +684,7 @@ static int attn_launch(dim3 grid, cudaStream_t stream, const AttnParams& P) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = P.cluster ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q4_kernel, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q4_kernel<kWarps>, P);
   return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
 }
 
@@ -711,7 +720,8 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one
   // launch (1 x 2049: 8.8 -> 8.3 us, 64 x 500..2100 on 6 heads 13.9 -> 11.9).  Longer ones are cut into pieces by their lengths, merged by a kernel.
   P.cluster = n_splits > 1 && lmps_attention_q4_launches(n_splits, max_seq_len) == 1 ? n_splits : 0;
-  const int status = attn_launch(dim3(static_cast<unsigned>(rows) * n_splits, n_kv_heads), s, P);
+  const dim3 grid(static_cast<unsigned>(rows) * n_splits, n_kv_heads);
+  const int status = n_splits == 1 || P.cluster ? attn_launch<kShortWarps>(grid, s, P) : attn_launch<kPieceWarps>(grid, s, P);
   if (status || n_splits == 1 || P.cluster) return status;
   return combine_launch(parts, rows, s);
 }
@@ -723,18 +733,23 @@ using namespace lmps;
 
 extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len) {
   if (batch <= 0 || n_kv_heads <= 0 || max_seq_len <= 0) return 1;
-  // Four CTAs per SM run at once (128 registers).  Short caches and batches that fill the GPU several
-  // times over are not split; else as many pieces as run at once, but none below 128 positions, and
-  // 256 in a cluster.  Sweep, us per call (graph replay): 64 x 4100..8200 4 44.5 / 5 37.2 / 6 41.7 / 10 40.3;
+  // Short caches and batches that fill the GPU several times over are not split.  Else a cluster per row
+  // where that leaves few positions to a CTA, and beyond as many pieces as run at once, none below 128
+  // positions.  Sweeps, us per call (graph replay): 64 x 1..1000 1 12.6 / cluster 2 10.3; 1 x 2049 with the
+  // append 1 16.0 / 4 8.8 / 8 7.7; pieces: 64 x 4100..8200 4 44.5 / 5 37.2 / 6 41.7 / 10 40.3;
   // 4 x 32768 37 24.4 / 75 17.2 / 112 22.8.
-  const long long items = static_cast<long long>(batch) * n_kv_heads, slots = 4 * 148;
-  if (max_seq_len <= 2 * q4::kWarps * q4::kStep || items >= 4 * slots) return 1;
-  const long long room = slots / items < 1 ? 1 : slots / items;
-  const long long share = (max_seq_len + 255) / 256, cluster = share < room ? share : room;
-  if (cluster >= 2 && max_seq_len <= (cluster < q4::kMaxCluster ? cluster : q4::kMaxCluster) * q4::kClusterShare)
-    return static_cast<int>(cluster < q4::kMaxCluster ? cluster : q4::kMaxCluster);
-  const long long most = (max_seq_len + q4::kWarps * q4::kStep - 1) / (q4::kWarps * q4::kStep);
-  const long long n = room > most ? most : room;
+  const long long items = static_cast<long long>(batch) * n_kv_heads;
+  constexpr long long kWarpSlots = 148 * q4::kWarpsPerSm;
+  constexpr int kShort = q4::kShortWarps * q4::kStep, kPiece = q4::kPieceWarps * q4::kStep;
+  if (max_seq_len <= 2 * kShort || items >= kWarpSlots) return 1;
+  const long long room = kWarpSlots / q4::kShortWarps / items, share = (max_seq_len + kShort - 1) / kShort;
+  long long cluster = share < room ? share : room;
+  if (cluster > q4::kMaxCluster) cluster = q4::kMaxCluster;
+  if (cluster >= 2 && max_seq_len <= cluster * q4::kClusterShare) return static_cast<int>(cluster);
+  if (room < 2 && max_seq_len <= 8 * kShort) return 1;  // the rows alone fill the GPU, and a merge would not pay
+  long long n = kWarpSlots / q4::kPieceWarps / items;
+  const long long most = (max_seq_len + kPiece - 1) / kPiece;
+  n = n < 1 ? 1 : n > most ? most : n;
   return static_cast<int>(n > 1023 ? 1024 : n + 1);
 }
 

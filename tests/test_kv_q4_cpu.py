@@ -127,5 +127,5 @@ def test_cache_rows_round_trip_on_the_host():
 
 
 def test_launch_counts():
-    assert K.attention_q4_launches(1, 100000) == 1 and K.attention_q4_launches(8, 5120) == 1
-    assert K.attention_q4_launches(8, 5121) == 2 and K.attention_q4_launches(9, 100) == 2
+    assert K.attention_q4_launches(1, 100000) == 1 and K.attention_q4_launches(8, 10240) == 1
+    assert K.attention_q4_launches(8, 10241) == 2 and K.attention_q4_launches(9, 100) == 2
