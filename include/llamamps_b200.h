@@ -276,7 +276,8 @@ int lmps_sample_rows(const uint16_t* logits, int ld, int rows, int n, int top_k,
  *
  * head_dim 128, page_size a multiple of 16, at most 8 query heads per KV head
  * (else UNSUPPORTED), max_pages * page_size <= 2^29; pools, q, qkv, outputs
- * and workspace 16-byte aligned.  error (int32, may be NULL where not said
+ * and workspace 16-byte aligned; calls that may overlap on the GPU need
+ * workspaces of their own.  error (int32, may be NULL where not said
  * otherwise) collects LMPS_Q4_ERR_* bits: a page number outside [0, n_pages)
  * is neither read nor written (its positions count as absent), a position
  * outside the cache likewise.  Zero it before the first call and after
@@ -335,7 +336,8 @@ int lmps_gqa_decode_attention_rope_q4(const uint16_t* qkv, const int32_t* pos, c
  * i >= q_lens[b] of out stay as they were.  starts[b] + q_lens[b] <=
  * max_seq_len.  n_splits from lmps_prefill_q4_splits (few rows over a long
  * context are split over the context), workspace from
- * lmps_prefill_q4_workspace_size.  error must not be NULL. */
+ * lmps_prefill_q4_workspace_size.  out and workspace 32-byte aligned; error
+ * must not be NULL. */
 int lmps_prefill_q4_splits(int batch, int seq_len, int n_q_heads, int n_kv_heads, int max_seq_len);
 size_t lmps_prefill_q4_workspace_size(int batch, int seq_len, int n_q_heads, int head_dim, int n_splits);
 int lmps_prefill_attention_q4(const uint16_t* q, const uint8_t* k_pool, const uint8_t* v_pool, int n_pages,

@@ -111,20 +111,19 @@ __device__ __forceinline__ int entry_tiles(const Params& P, int e) {
 __device__ __forceinline__ int entry_pieces(int tiles, int cut) { return tiles < 0 ? 0 : max(1, (tiles + cut - 1) / cut); }
 
 // Tiles per piece: the fewest (in steps of a sixteenth) with which the pieces of all entries fit
-// n_splits per entry.  A warp computes it.
+// n_splits per entry.  A warp computes it; the tiles of the first 32 entries stay in its registers.
 __device__ __forceinline__ int piece_tiles(const Params& P) {
   const int entries = P.n_blocks * P.batch, lane = threadIdx.x & 31;
   const int room = P.n_splits * entries;
-  int total = 0;
-  for (int e = lane; e < entries; e += kWarp) total += max(0, entry_tiles(P, e));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const int own = lane < entries ? entry_tiles(P, lane) : -1;
+  int total = max(0, own);
+  for (int e = lane + kWarp; e < entries; e += kWarp) total += max(0, entry_tiles(P, e));
+  total = __reduce_add_sync(0xffffffffu, total);
   int cut = max(1, (total + room - 1) / room);
   for (;;) {  // ends: with `cut` at the longest entry every entry is one piece
-    int n = 0;
-    for (int e = lane; e < entries; e += kWarp) n += entry_pieces(entry_tiles(P, e), cut);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    int n = entry_pieces(own, cut);
+    for (int e = lane + kWarp; e < entries; e += kWarp) n += entry_pieces(entry_tiles(P, e), cut);
+    n = __reduce_add_sync(0xffffffffu, n);
     if (n <= room || cut > total) return cut;
     cut += max(1, cut >> 4);
   }
@@ -292,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   volatile int* abort_v = abort_flag;
   uint32_t* absent = tmem_slot + 2;    // [4][4]: keys of a tile whose page is not in the pool, ring of 4 tiles
   uint32_t* absent_raw = absent + 16;  // [4]: of the tile in the raw stage
+  volatile int* cut_slot = reinterpret_cast<int*>(absent_raw + 4);
 
   lmps_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -324,10 +324,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
   lmps_pdl_wait();
+  if (P.n_splits > 1) {  // (uniform) one warp looks the lengths over
+    if (warp == 14) {
+      const int c = piece_tiles(P);
+      if (lane == 0) *cut_slot = c;
+    }
+    __syncthreads();
+  }
 
   // Every role walks the same work units; stages, S halves and their barriers' phases run on over them.
   const int n_items = P.n_blocks * P.batch * P.n_splits * P.c.n_kv;
-  const int cut = P.n_splits > 1 ? piece_tiles(P) : 0;
+  const int cut = P.n_splits > 1 ? *cut_slot : 0;
   // the CTA's units: every gridDim.x-th, odd rounds in reverse (units are ordered by size)
   auto nth = [&](int turn) {
     return turn * static_cast<int>(gridDim.x) +
@@ -730,9 +737,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                              : "memory");
               }
             } else {
-              float4* dst = reinterpret_cast<float4*>(P.part_o + part * kDim + cc + 8 * g);
-              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+              asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(P.part_o + part * kDim + cc + 8 * g),
+                           "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                           : "memory");
             }
           }
         }
@@ -791,7 +798,7 @@ extern "C" int lmps_prefill_attention_q4(const uint16_t* q, const uint8_t* k_poo
                                      n_splits);
   if (st != LMPS_OK) return st;
   LMPS_CHECK_ARG(lmps_aligned(q, 16) && lmps_aligned(k_pool, 16) && lmps_aligned(v_pool, 16) &&
-                 lmps_aligned(out, 32) && lmps_aligned(workspace, 16));
+                 lmps_aligned(out, 32) && lmps_aligned(workspace, 32));
   const int G = n_q_heads / n_kv_heads;
   const long long rows = static_cast<long long>(batch) * seq_len, blocks = blocks_of(seq_len, G);
   const long long items = blocks * n_kv_heads * batch;

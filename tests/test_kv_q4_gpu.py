@@ -389,6 +389,34 @@ def test_prefill_long_context_rows(cuda):
                 R.close(got[b, i], *R.attend(q[b, i], *c.rows[b], starts[b] + i + 1), f"{b}, {i}, {n_splits}")
 
 
+def test_prefill_many_pieces(cuda):
+    """One long context beside two short ones is cut into more pieces than the lanes of a warp; pieces whose pages
+    are all bad, the first one of the row among them, weigh nothing."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(14)
+    starts, seq, hq, hkv, page, n_splits = [9000, 0, 5], 8, 12, 2, 64, 33
+    c = R.Cache(rng, [s + seq for s in starts], hkv, page)
+    q = rng.normal(0, 2, (3, seq, hq, D)).astype(np.float16)
+    seen = np.ones(9008, bool)
+    for bad in (0, 1, 70, 71, 72, 73):  # positions 0..127 and 4480..4735
+        c.bt[0, bad] = -1
+        seen[bad * page:(bad + 1) * page] = False
+    e = _err()
+    buf, out = _guarded(3 * seq, hq * D)
+    K.prefill_attention_q4(_cu(q.reshape(3 * seq, -1)), c.k, c.v, c.bt, out, 3, seq, page, hq, hkv, D, c.max_seq_len,
+                           starts=torch.tensor(starts, dtype=torch.int32, device="cuda"),
+                           workspace=_ws(K.prefill_q4_workspace_size(3, seq, hq, D, n_splits)), n_splits=n_splits,
+                           error=e)
+    assert e.item() == K.Q4_ERR_PAGE and _guards_ok(buf)
+    got = out.cpu().numpy().reshape(3, seq, hq, D)
+    for b in range(3):
+        for i in range(seq):
+            n = starts[b] + i + 1
+            keep = seen[:n] if b == 0 else np.ones(n, bool)
+            k, v = c.rows[b]
+            R.close(got[b, i], *R.attend(q[b, i], k[:n][keep], v[:n][keep], int(keep.sum())), f"{b}, {i}")
+
+
 # -- the calls around the kernels ---------------------------------------------------
 def _all_calls(rng, c, lens, hq, hkv, page, out=None):
     """One call of each entry point on cache c, as functions of replaced arguments."""
