@@ -582,10 +582,53 @@ __global__ void __launch_bounds__(kWarps * kWarp, kWarpsPerSm / kWarps) attn_q4_
   }
 }
 
-// Log-sum-exp merge of the pieces of one (row, query head) of a decode call.  A warp takes every
-// 8th piece, 4 dims a lane; the partials of the first 64 pieces are on their
-// way before the weights are known.
 constexpr int kMergeWarps = 8, kMergeLoads = 8;
+// Log-sum-exp merge of the n pieces first + s * step of a (row, query head) by a warp, 4 dims a lane.  Lane j
+// holds the weight of piece j of a chunk of 32; eight partials are on their way at a time.
+__device__ __forceinline__ void merge_row(const Partials& P, size_t first, size_t step, int pieces, __half* out) {
+  const int lane = threadIdx.x & 31;
+  const float2* ml = P.ml + first;
+  const float4* o = reinterpret_cast<const float4*>(P.o + first * kDim) + lane;
+  const size_t stride = step * (kDim / 4);
+  float M = -INFINITY, den = 0.0f;  // den: of this lane's pieces
+  float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s0 = 0; s0 < pieces; s0 += kWarp) {
+    const float2 m = s0 + lane < pieces ? ml[(s0 + lane) * step] : make_float2(-INFINITY, 0.0f);
+    const int n = min(kWarp, pieces - s0);
+    float f = 0.0f;
+    for (int j0 = 0; j0 < n; j0 += kMergeLoads) {
+      float4 v[kMergeLoads];
+#pragma unroll
+      for (int j = 0; j < kMergeLoads; ++j)
+        v[j] = j0 + j < n ? o[(s0 + j0 + j) * stride] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (j0 == 0) {  // the weights, while the first partials travel
+        const float top = fmaxf(M, warp_max(m.x));
+        const float keep = M == -INFINITY ? 1.0f : ex2(M - top);
+        // a piece without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
+        f = m.x == -INFINITY ? 1.0f : ex2(m.x - top);
+        M = top;
+        den = fmaf(den, keep, m.y * f);
+        num.x *= keep, num.y *= keep, num.z *= keep, num.w *= keep;
+      }
+#pragma unroll
+      for (int j = 0; j < kMergeLoads; ++j) {
+        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+        num.x = fmaf(v[j].x, w, num.x);
+        num.y = fmaf(v[j].y, w, num.y);
+        num.z = fmaf(v[j].z, w, num.z);
+        num.w = fmaf(v[j].w, w, num.w);
+      }
+    }
+  }
+  den = warp_sum(den);
+  store_row4(out + 4 * lane, num, den);
+}
+
+// The merge of one (row, query head) of a decode call.  A warp takes every 8th
+// piece, 4 dims a lane; the partials of the first 64 pieces are on their way
+// before the weights are known.  Of a row of eight pieces or fewer every eighth
+// CTA merges eight heads, a warp each, and the others are done (64 rows of
+// 4100..8200: 37.3 -> 35.6 us; 4 of 32768, 37 pieces each, with a warp per head: 17.8 -> 20.8).
 __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(const Partials P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
@@ -594,6 +637,11 @@ __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(co
   const int h = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int2 pc = P.pieces[row];
   const size_t step = P.n_q, first = pc.x * step + h;  // piece s at first + s * step
+  if (pc.y <= kMergeLoads) {
+    if (h % kMergeWarps == 0 && h + warp < P.n_q)
+      merge_row(P, first + warp, step, pc.y, P.out + (static_cast<size_t>(row) * P.n_q + h + warp) * kDim);
+    return;
+  }
   const float2* ml = P.ml + first;
   const float4* o = reinterpret_cast<const float4*>(P.o + first * kDim) + lane;
   const size_t stride = step * (kDim / 4);
@@ -640,56 +688,21 @@ __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_kernel(co
   P.out[(static_cast<size_t>(row) * P.n_q + h) * kDim + tid] = __float2half_rn(d == 0.0f ? 0.0f : n / d);
 }
 
-// The same for many queries a sequence: thousands of rows of a few pieces, a warp each, 4 dims a lane.
-// Lane j holds the weight of piece j of a chunk of 32; eight partials are on their way at a time.
+// The same for many queries a sequence: thousands of rows, a warp each.
 // (4 x 256 queries behind 1..30000 positions, 18 MB of partials: a CTA per row 104 us the call, this one 80.)
 __global__ void __launch_bounds__(kMergeWarps * kWarp) attn_q4_combine_rows_kernel(const Partials P, int n_rows) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
-  const int lane = threadIdx.x & 31, item = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  const int item = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   const int row = item / P.n_q, h = item - row * P.n_q;
   if (row >= n_rows) return;
   const int b = row / P.seq, i = row - b * P.seq;
   if (P.q_lens && i >= P.q_lens[b]) return;
   const int G = P.n_q / P.n_kv, kvh = h / G, r = i * G + (h - kvh * G), blk = r / P.rows_item;
   const int2 pc = P.pieces[(P.n_blocks - 1 - blk) * P.batch + b];
-  const size_t step = static_cast<size_t>(P.n_kv) * P.rows_item;  // piece s at first + s * step
+  const size_t step = static_cast<size_t>(P.n_kv) * P.rows_item;
   const size_t first = pc.x * step + static_cast<size_t>(kvh) * P.rows_item + (r - blk * P.rows_item);
-  const float2* ml = P.ml + first;
-  const float4* o = reinterpret_cast<const float4*>(P.o + first * kDim) + lane;
-  const size_t stride = step * (kDim / 4);
-  float M = -INFINITY, den = 0.0f;  // den: of this lane's pieces
-  float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s0 = 0; s0 < pc.y; s0 += kWarp) {
-    const float2 m = s0 + lane < pc.y ? ml[(s0 + lane) * step] : make_float2(-INFINITY, 0.0f);
-    const int n = min(kWarp, pc.y - s0);
-    float f = 0.0f;
-    for (int j0 = 0; j0 < n; j0 += kMergeLoads) {
-      float4 v[kMergeLoads];
-#pragma unroll
-      for (int j = 0; j < kMergeLoads; ++j)
-        v[j] = j0 + j < n ? o[(s0 + j0 + j) * stride] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (j0 == 0) {  // the weights, while the first partials travel
-        const float top = fmaxf(M, warp_max(m.x));
-        const float keep = M == -INFINITY ? 1.0f : ex2(M - top);
-        // a piece without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
-        f = m.x == -INFINITY ? 1.0f : ex2(m.x - top);
-        M = top;
-        den = fmaf(den, keep, m.y * f);
-        num.x *= keep, num.y *= keep, num.z *= keep, num.w *= keep;
-      }
-#pragma unroll
-      for (int j = 0; j < kMergeLoads; ++j) {
-        const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-        num.x = fmaf(v[j].x, w, num.x);
-        num.y = fmaf(v[j].y, w, num.y);
-        num.z = fmaf(v[j].z, w, num.z);
-        num.w = fmaf(v[j].w, w, num.w);
-      }
-    }
-  }
-  den = warp_sum(den);
-  store_row4(P.out + (static_cast<size_t>(row) * P.n_q + h) * kDim + 4 * lane, num, den);
+  merge_row(P, first, step, pc.y, P.out + (static_cast<size_t>(row) * P.n_q + h) * kDim);
 }
 
 int combine_launch(const Partials& p, int rows, cudaStream_t stream) {
