@@ -24,13 +24,14 @@
 //     m-tile 2g + m: rows r < 8 are dims 32g + 4r + 2m, rows r >= 8 the dims
 //     32g + 4(r - 8) + 2m + 1; a lane ends with 4 consecutive dims per group.
 //
-// One piece of a sequence and a KV head per CTA of 4 warps.  The n_splits *
-// rows pieces that a call has room for are shared out by the sequences' lengths
-// (in the kernel: lengths are on the device), so that ragged batches finish
-// together.  A warp walks its own 32-position steps (every 4th) through its own ring of
-// cp.async stages; no CTA-wide barrier until the warps' states meet.  16-byte
-// chunk c of a staged row r is stored at c ^ ((r >> 1) & 3): both fragment
-// reads are then free of bank conflicts.
+// A CTA has one KV head of a row, of a share of a row that it merges with the
+// other CTAs of its cluster, or (long or many rows) of an equal share of all
+// rows laid end to end, merged by a second kernel; the lengths are on the
+// device, so the shares are found there.  A warp walks its own 32-position
+// steps through its own ring of cp.async stages; no CTA-wide barrier until the
+// warps' states meet.  16-byte chunk c of a staged row r is stored at
+// c ^ ((r >> 1) & 3): both fragment reads are then free of bank conflicts.
+#include <algorithm>
 #include <cmath>
 
 #include "attention_q4.cuh"
@@ -39,13 +40,15 @@
 namespace lmps {
 namespace q4 {
 
-// Warps per CTA.  A step takes a lone warp 1.4 us, so short rows want many warps at once (1 x 131: 8 warps
-// 4.0 us, 4 warps 4.6); long ones are cut into pieces, which fill the SMs better in units of 128 positions
-// (64 x 4100..8200: 4 warps 37 us, 8 warps 41).  16 warps run per SM either way (128 registers).
+// Warps per CTA.  A step takes a lone warp 1.4 us, so short rows want many warps at once: 8, one CTA to an SM
+// (1 x 131: 4.0 us, with 4 warps 4.6).  Pieces, and rows of which there are more than SMs, have 4, three CTAs to
+// an SM.  The 12 warps may have 168 registers each; 16 of 128 take 1 .. 2 us more (64 x 1..1000 in one CTA a row:
+// 12.6 us against 9.3; 4 x 32768 16.9 us with either).
 constexpr int kShortWarps = 8, kPieceWarps = 4;
-constexpr int kWarpsPerSm = 16;
+constexpr int kSms = 148, kPieceCtas = 3;
 constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
+constexpr int kHead = 3, kShortShare = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kClusterShare = 1280;  // positions of a CTA up to which a row is shared by a cluster
 constexpr int kOffV = kStep * kCodeBytes;
@@ -119,6 +122,13 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// Of the units of all rows, heads included: first one of the current row, the CTA's share from .. last - 1; their
+// number and that of the shares.
+struct Share {
+  unsigned long long before, from, last, total, ctas;
+  int row, head;
+};
+
 template <int kWarps>
 struct __align__(16) Smem {
   union {
@@ -131,6 +141,7 @@ struct __align__(16) Smem {
   float2 csf[kDim / 2];
   float wm[kWarps][kMaxHeads], wl[kWarps][kMaxHeads], wf[kWarps][kMaxHeads];
   float cm[kMaxHeads], cl[kMaxHeads];
+  Share share;
   __align__(16) float co[kMaxHeads][kDim];  // the CTA's, for the other CTAs of a cluster
 };
 
@@ -268,66 +279,14 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
   }
 }
 
+// Attends to positions start .. end - 1 of a row of T.  `slot`: where its partials go (pieces).
 template <int kWarps>
-__global__ void __launch_bounds__(kWarps * kWarp, kWarpsPerSm / kWarps) attn_q4_kernel(const AttnParams P) {
+__device__ __forceinline__ void attend(const AttnParams& P, Smem<kWarps>& S, int row, int T, int start, int end,
+                                       size_t slot) {
   constexpr int kThreads = kWarps * kWarp;
-  lmps_pdl_trigger();
-  lmps_pdl_wait();
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  Smem<kWarps>& S = *reinterpret_cast<Smem<kWarps>*>(smem_raw);
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const int G = P.n_q / P.c.n_kv;
-  int row = blockIdx.x, T, start = 0, end;
-  if (P.n_splits == 1) {
-    T = P.length(row);
-    end = T;
-  } else if (P.cluster) {  // equal shares of the row
-    row = blockIdx.x / P.cluster;
-    T = P.length(row);
-    const int share = ((T + P.cluster - 1) / P.cluster + kStep - 1) / kStep * kStep;
-    start = min(T, static_cast<int>(blockIdx.x - row * P.cluster) * share);
-    end = min(T, start + share);
-  } else {
-    // Pieces of equal size: blockIdx.x counts them over the rows in order, every warp finds the
-    // row of its own (`cut` is at least total / ((n_splits - 1) rows), so with a last, shorter piece
-    // per row there are at most n_splits * rows).
-    unsigned long long total = 0ull;
-    for (int r = lane; r < P.rows; r += kWarp) total += P.length(r);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const unsigned long long share = static_cast<unsigned long long>(P.n_splits - 1) * P.rows;
-    constexpr int kPiece = kWarps * kStep;
-    const int cut = max(1, static_cast<int>((total + share * kPiece - 1) / (share * kPiece))) * kPiece;
-    int before = 0, n = 0;
-    bool found = false;
-    for (int r0 = 0; r0 < P.rows && !found; r0 += kWarp) {
-      const int r = r0 + lane;
-      const int len = r < P.rows ? P.length(r) : 0;
-      const int mine = r < P.rows ? max(1, (len + cut - 1) / cut) : 0;
-      int sum = mine;  // inclusive prefix
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, static_cast<int>(blockIdx.x) < before + sum);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        row = r0 + l;
-        T = __shfl_sync(0xffffffffu, len, l);
-        n = __shfl_sync(0xffffffffu, mine, l);
-        before += __shfl_sync(0xffffffffu, sum - mine, l);
-        found = true;
-      } else {
-        before += __shfl_sync(0xffffffffu, sum, 31);
-      }
-    }
-    if (!found) return;  // (uniform) fewer pieces than the grid has room for
-    start = (static_cast<int>(blockIdx.x) - before) * cut;
-    end = min(T, start + cut);
-    if (start == 0 && kvh == 0 && tid == 0) P.pieces[row] = make_int2(before, n);
-  }
   if (tid == 0 && kvh == 0 && start == 0) {
     const int given = P.seq_lens[row];
     if (given < 0 || given > P.max_seq_len) raise_error(P.c.error, kErrPosition);
@@ -545,7 +504,7 @@ __global__ void __launch_bounds__(kWarps * kWarp, kWarpsPerSm / kWarps) attn_q4_
     } else if (P.cluster) {
       *reinterpret_cast<float4*>(&S.co[h][d]) = o;
     } else {
-      const size_t at = static_cast<size_t>(blockIdx.x) * P.n_q + kvh * G + h;
+      const size_t at = slot * P.n_q + kvh * G + h;
       *reinterpret_cast<float4*>(P.part_o + at * kDim + d) = o;
       if (d == 0) P.part_ml[at] = make_float2(S.cm[h], S.cl[h]);
     }
@@ -579,6 +538,85 @@ __global__ void __launch_bounds__(kWarps * kWarp, kWarpsPerSm / kWarps) attn_q4_
       store_row4(out + h * kDim + d, num, den);
     }
     cluster_sync();  // nobody's shared memory goes while it is read
+  }
+}
+
+// A row a CTA, or a share of one a CTA of a cluster.
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * kWarp, kWarps == kShortWarps ? 1 : kPieceCtas) attn_q4_kernel(const AttnParams P) {
+  lmps_pdl_trigger();
+  lmps_pdl_wait();
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int parts = P.cluster ? P.cluster : 1, row = blockIdx.x / parts, T = P.length(row);
+  const int share = ((T + parts - 1) / parts + kStep - 1) / kStep * kStep;
+  const int start = min(T, static_cast<int>(blockIdx.x - row * parts) * share);
+  attend(P, *reinterpret_cast<Smem<kWarps>*>(smem_raw), row, T, start, min(T, start + share), 0);
+}
+
+// Equal shares of the rows laid end to end, in units of a step of every warp (a row without positions has one):
+// a share may take in the end of a row and the start of the next, a segment each.  kHead units in front of each
+// row stand for what another segment costs; where a share is no longer than kShortShare, one more than a share
+// does, so that none takes in two rows.  Segment (CTA i, row r) has slot i + r.
+__global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_pieces_kernel(const AttnParams P) {
+  lmps_pdl_trigger();
+  lmps_pdl_wait();
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Smem<kPieceWarps>& S = *reinterpret_cast<Smem<kPieceWarps>*>(smem_raw);
+  constexpr int kUnit = kPieceWarps * kStep;
+  const int lane = threadIdx.x & 31;
+  auto units = [](int len) { return max(1, (len + kUnit - 1) / kUnit); };
+  {
+    unsigned long long total = 0ull, before = 0ull;  // before: units of the rows in front
+    for (int r = lane; r < P.rows; r += kWarp) total += units(P.length(r));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int head = total <= static_cast<unsigned long long>(kShortShare) * gridDim.x ? static_cast<int>(total / gridDim.x) + 1 : kHead;
+    total += static_cast<unsigned long long>(head) * P.rows;
+    const unsigned long long ctas = min(static_cast<unsigned long long>(gridDim.x), total);
+    if (blockIdx.x >= ctas) return;
+    const unsigned long long from = blockIdx.x * total / ctas;
+    int row = 0, r0 = 0;
+    for (;; r0 += kWarp) {  // ends: `from` is below the total
+      const int r = r0 + lane, mine = r < P.rows ? head + units(P.length(r)) : 0;
+      int sum = mine;  // inclusive prefix
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, from < before + sum);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        row = r0 + l;
+        before += __shfl_sync(0xffffffffu, sum - mine, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) S.share = Share{before, from, (blockIdx.x + 1) * total / ctas, total, ctas, row, head};
+  }
+  for (;;) {
+    __syncthreads();
+    const Share sh = S.share;
+    const int T = P.length(sh.row), n = sh.head + units(T);
+    const unsigned long long next = sh.before + n;
+    const int first = max(0, static_cast<int>(max(sh.from, sh.before) - sh.before) - sh.head);
+    const int stop = static_cast<int>(min(next, sh.last) - sh.before) - sh.head;
+    if (stop > first) {  // (uniform) else only the head of the row
+      // The owner of the row's first positions tells the merge from where to where: unit u is in share
+      // ((u + 1) * ctas - 1) / total.
+      if (first == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+        P.pieces[sh.row] = make_int2(static_cast<int>(blockIdx.x) + sh.row,
+                                     static_cast<int>((next * sh.ctas - 1) / sh.total) - static_cast<int>(blockIdx.x) + 1);
+      attend(P, S, sh.row, T, first * kUnit, min(T, stop * kUnit), static_cast<size_t>(blockIdx.x) + sh.row);
+    }
+    __syncthreads();  // the segment's states and the share are read
+    if (S.share.before + n >= S.share.last) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      S.share.before += n;
+      ++S.share.row;
+    }
   }
 }
 
@@ -724,9 +762,9 @@ int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, in
   return LMPS_OK;
 }
 
-template <int kWarps>
+template <void (*kKernel)(const AttnParams), int kWarps>
 static int attn_launch(dim3 grid, cudaStream_t stream, const AttnParams& P) {
-  const int st = lmps_max_dyn_smem<attn_q4_kernel<kWarps>>(static_cast<int>(sizeof(Smem<kWarps>)));
+  const int st = lmps_max_dyn_smem<kKernel>(static_cast<int>(sizeof(Smem<kWarps>)));
   if (st != LMPS_OK) return st;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -741,7 +779,7 @@ static int attn_launch(dim3 grid, cudaStream_t stream, const AttnParams& P) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = P.cluster ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q4_kernel<kWarps>, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kKernel, P);
   return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
 }
 
@@ -777,9 +815,17 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one
   // launch (1 x 2049: 8.8 -> 8.3 us, 64 x 500..2100 on 6 heads 13.9 -> 11.9).  Longer ones are cut into pieces by their lengths, merged by a kernel.
   P.cluster = n_splits > 1 && lmps_attention_q4_launches(n_splits, max_seq_len) == 1 ? n_splits : 0;
-  const dim3 grid(static_cast<unsigned>(rows) * n_splits, n_kv_heads);
-  const int status = n_splits == 1 || P.cluster ? attn_launch<kShortWarps>(grid, s, P) : attn_launch<kPieceWarps>(grid, s, P);
-  if (status || n_splits == 1 || P.cluster) return status;
+  if (n_splits == 1 || P.cluster) {  // with one CTA to an SM at most it has 8 warps, else 4
+    const dim3 grid(static_cast<unsigned>(rows) * n_splits, n_kv_heads);
+    const bool alone = static_cast<long long>(rows) * n_splits * n_kv_heads <= kSms;
+    return alone ? attn_launch<attn_q4_kernel<kShortWarps>, kShortWarps>(grid, s, P)
+                 : attn_launch<attn_q4_kernel<kPieceWarps>, kPieceWarps>(grid, s, P);
+  }
+  // No more shares than run at once; with the rows' borders they make at most rows * n_splits segments.
+  const unsigned slots = n_kv_heads >= kSms * kPieceCtas ? 1u : kSms * kPieceCtas / n_kv_heads;
+  const dim3 grid(std::min(slots, (n_splits - 1u) * rows), n_kv_heads);
+  const int status = attn_launch<attn_q4_pieces_kernel, kPieceWarps>(grid, s, P);
+  if (status) return status;
   return combine_launch(parts, rows, s);
 }
 
@@ -790,21 +836,24 @@ using namespace lmps;
 
 extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_len) {
   if (batch <= 0 || n_kv_heads <= 0 || max_seq_len <= 0) return 1;
-  // Short caches and batches that fill the GPU several times over are not split.  Else a cluster per row
-  // where that leaves few positions to a CTA, and beyond as many pieces as run at once, none below 128
-  // positions.  Sweeps, us per call (graph replay): 64 x 1..1000 1 12.6 / cluster 2 10.3; 1 x 2049 with the
-  // append 1 16.0 / 4 8.8 / 8 7.7; pieces: 64 x 4100..8200 4 44.5 / 5 37.2 / 6 41.7 / 10 40.3;
-  // 4 x 32768 37 24.4 / 75 17.2 / 112 22.8.
   const long long items = static_cast<long long>(batch) * n_kv_heads;
-  constexpr long long kWarpSlots = 148 * q4::kWarpsPerSm;
   constexpr int kShort = q4::kShortWarps * q4::kStep, kPiece = q4::kPieceWarps * q4::kStep;
-  if (max_seq_len <= 2 * kShort || items >= kWarpSlots) return 1;
-  const long long room = kWarpSlots / q4::kShortWarps / items, share = (max_seq_len + kShort - 1) / kShort;
-  long long cluster = share < room ? share : room;
-  if (cluster > q4::kMaxCluster) cluster = q4::kMaxCluster;
+  if (max_seq_len <= 2 * kShort || items >= q4::kSms * q4::kPieceCtas) return 1;
+  // Clusters of CTAs of 8 warps (one to an SM) or of 4, whichever gives a row more warps.  `room`: CTAs that
+  // still run at once as clusters; an SM group takes few large ones, and pairs fit everywhere.
+  auto fit = [max_seq_len, items](int room, int slots, int unit) {
+    long long n = room / items;
+    if (n > 6 && items > 12) n = unit == kShort ? 6 : n;
+    if (n < 2 && slots >= 2 * items) n = 2;
+    return std::min(std::min(n, static_cast<long long>(q4::kMaxCluster)), static_cast<long long>((max_seq_len + unit - 1) / unit));
+  };
+  const long long wide = fit(120, q4::kSms, kShort), many = fit(384, q4::kSms * q4::kPieceCtas, kPiece);
+  const long long warps = std::max(wide * q4::kShortWarps, many * q4::kPieceWarps);
+  if (items <= q4::kSms && warps < 2 * q4::kShortWarps && max_seq_len <= 4 * kShort) return 1;
+  const long long cluster = wide * q4::kShortWarps >= warps ? wide : many;
   if (cluster >= 2 && max_seq_len <= cluster * q4::kClusterShare) return static_cast<int>(cluster);
-  if (room < 2 && max_seq_len <= 8 * kShort) return 1;  // the rows alone fill the GPU, and a merge would not pay
-  long long n = kWarpSlots / q4::kPieceWarps / items;
+  if (cluster < 2 && max_seq_len <= 8 * kShort) return 1;  // the rows alone fill the GPU, and a merge would not pay
+  long long n = (q4::kSms * q4::kPieceCtas + items - 1) / items;
   const long long most = (max_seq_len + kPiece - 1) / kPiece;
   n = n < 1 ? 1 : n > most ? most : n;
   return static_cast<int>(n > 1023 ? 1024 : n + 1);

@@ -171,6 +171,31 @@ def test_decode_attention(cuda, lens, hq, hkv, page):
             assert (got[lens.index(0)] == 0).all()
 
 
+@pytest.mark.parametrize("lens,hq,hkv,page,n_splits,max_len", [
+    ([20000, 0, 9000], 12, 2, 64, 9, 20032),                                       # long shares across the rows
+    ([0, 1, 127, 128, 129, 255, 256, 257, 640, 2000, 0, 5], 8, 4, 16, 11, 2016),   # shorter than a share
+    ([(37 * i) % 300 for i in range(250)], 2, 2, 16, 9, 304),                      # more rows than shares
+    ([9000], 16, 2, 64, 1024, 9024), ([3] * 40, 6, 1, 16, 10, 16),                 # fewer units than shares
+])
+def test_decode_shares_of_ragged_rows(cuda, lens, hq, hkv, page, n_splits, max_len):
+    """Rows laid end to end and cut into equal shares: borders inside shares, rows shorter than one, empty ones."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(len(lens) + hq)
+    c = R.Cache(rng, lens, hkv, page, max_len=max_len)
+    B = len(lens)
+    assert K.attention_q4_launches(n_splits, c.max_seq_len) == 2
+    q = rng.normal(0, 1, (B, hq, D)).astype(np.float16)
+    buf, out = _guarded(B, hq * D)
+    e = _err()
+    K.gqa_decode_attention_q4(_cu(q.reshape(B, -1)), c.k, c.v, c.bt, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                              out, _ws(K.attention_q4_workspace_size(B, hq, D, n_splits)), page, hq, hkv, D,
+                              c.max_seq_len, n_splits, error=e)
+    assert e.item() == 0 and _guards_ok(buf)
+    got = out.cpu().numpy().reshape(B, hq, D)
+    for b in range(B):
+        R.close(got[b], *R.attend(q[b], *c.rows[b], lens[b]), f"length {lens[b]}")
+
+
 def test_decode_large_scores_and_long_flat_softmax(cuda):
     """Scores that differ by hundreds (one position takes all) and equal scores (the mean of V)."""
     from llamamps_b200 import kernels as K
