@@ -31,6 +31,17 @@
 // steps through its own ring of cp.async stages; no CTA-wide barrier until the
 // warps' states meet.  16-byte chunk c of a staged row r is stored at
 // c ^ ((r >> 1) & 3): both fragment reads are then free of bank conflicts.
+//
+// What bounds it.  A step of 32 positions is 4.6 KB and some 750 instructions a
+// warp (unpacking, scales, the softmax): with 12 warps an SM goes through its
+// steps at 5.3 TB/s over the GPU, 0.8 of the measured copy rate, issue slots
+// and memory latency about even.  What is left is around them: 4 us of an empty call
+// (launch, page table, first loads, meeting of the warps) and 3 us of the second
+// kernel.  Measured (12 query, 2 KV heads): 1 x 131 4.0 us; 64 x 1..1000 9.4;
+// 4 x 32768 17.0 (2.2 TB/s); 64 x 4100..8200 33.8 (3.3 TB/s); with RoPE and
+// append 1 x 2049 7.4.  Tried without gain: a third stage, 16 warps of 128
+// registers, codes left as fp16 subnormals (a third fewer unpacking
+// instructions, but the offset then goes into the sums in fp32).
 #include <algorithm>
 #include <cmath>
 
@@ -556,7 +567,8 @@ __global__ void __launch_bounds__(kWarps * kWarp, kWarps == kShortWarps ? 1 : kP
 // Equal shares of the rows laid end to end, in units of a step of every warp (a row without positions has one):
 // a share may take in the end of a row and the start of the next, a segment each.  kHead units in front of each
 // row stand for what another segment costs; where a share is no longer than kShortShare, one more than a share
-// does, so that none takes in two rows.  Segment (CTA i, row r) has slot i + r.
+// does, so that none takes in two rows (16 x 1..32000: 23.3 us, kHead alone 24.3; 4 x 32768: 17.0 and 19.0;
+// 64 x 4100..8200, kHead 0 / 2 / 3 / 4: 34.3 / 33.2 / 33.4 / 33.7).  Segment (CTA i, row r) has slot i + r.
 __global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_pieces_kernel(const AttnParams P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
@@ -812,8 +824,9 @@ static int attention_launch(AttnParams P, const uint8_t* k_pool, const uint8_t* 
   parts.out = P.out;
   parts.n_q = n_q_heads;
   cudaStream_t s = lmps_stream(stream);
-  // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one
-  // launch (1 x 2049: 8.8 -> 8.3 us, 64 x 500..2100 on 6 heads 13.9 -> 11.9).  Longer ones are cut into pieces by their lengths, merged by a kernel.
+  // Rows of medium length go to a cluster each, whose CTAs merge through distributed shared memory: one launch
+  // (with RoPE and append: 1 x 2049 7.4 us against 8.6 in pieces, 64 x 500..2100 on 6 heads 10.7 against 12.6).
+  // Longer ones are cut into pieces, merged by a second kernel.
   P.cluster = n_splits > 1 && lmps_attention_q4_launches(n_splits, max_seq_len) == 1 ? n_splits : 0;
   if (n_splits == 1 || P.cluster) {  // with one CTA to an SM at most it has 8 warps, else 4
     const dim3 grid(static_cast<unsigned>(rows) * n_splits, n_kv_heads);
@@ -840,7 +853,9 @@ extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_l
   constexpr int kShort = q4::kShortWarps * q4::kStep, kPiece = q4::kPieceWarps * q4::kStep;
   if (max_seq_len <= 2 * kShort || items >= q4::kSms * q4::kPieceCtas) return 1;
   // Clusters of CTAs of 8 warps (one to an SM) or of 4, whichever gives a row more warps.  `room`: CTAs that
-  // still run at once as clusters; an SM group takes few large ones, and pairs fit everywhere.
+  // still run at once as clusters; an SM group takes few large ones, and pairs fit everywhere (us per call,
+  // 12 query heads: 8 x 3000..6000 in clusters of 5 / 6 / 7 / 8 11.1 / 9.7 / 16.3 / 15.5, 6 x 3000..6000 in 8 8.8;
+  // 12 x 3000..6000 in 5 / 6 11.2 / 17.0; 27 x 500..2000 of 4 warps in 7 / 8 9.8 / 14.0).
   auto fit = [max_seq_len, items](int room, int slots, int unit) {
     long long n = room / items;
     if (n > 6 && items > 12) n = unit == kShort ? 6 : n;
@@ -849,6 +864,7 @@ extern "C" int lmps_attention_q4_splits(int batch, int n_kv_heads, int max_seq_l
   };
   const long long wide = fit(120, q4::kSms, kShort), many = fit(384, q4::kSms * q4::kPieceCtas, kPiece);
   const long long warps = std::max(wide * q4::kShortWarps, many * q4::kPieceWarps);
+  // (64 x 1..1000: one CTA a row 9.4, a cluster of 3 10.1; 32 x 1..1000: 9.5 and, of 6, 8.0)
   if (items <= q4::kSms && warps < 2 * q4::kShortWarps && max_seq_len <= 4 * kShort) return 1;
   const long long cluster = wide * q4::kShortWarps >= warps ? wide : many;
   if (cluster >= 2 && max_seq_len <= cluster * q4::kClusterShare) return static_cast<int>(cluster);

@@ -3,7 +3,14 @@
 //
 // A CTA takes one token row, or four of a long call (so that all threads have
 // a cosine to compute): the rows' 64 (cos, sin) pairs once in fp64, q in units
-// of 16 bytes a thread, then a warp per K or V row (4 elements a lane).
+// of 16 bytes a thread, then a warp per two K or V rows (8 elements a lane).
+//
+// One row is launch and latency (3.5 us, as are 64).  A prompt of 8 x 2048 rows
+// (12 query, 2 KV heads: 139 MB) takes 33 us = 4.2 TB/s, 0.64 of the measured
+// copy rate, at 65 % of the issue slots: the fp64 rotation of K and the
+// quantiser (a maximum over 8 lanes, an exact division by 7 rounded up, 128
+// roundings) are its instructions.  K is rotated in fp64 so that the rounding
+// to fp16, and with it every code, is that of the exact formula.
 #include "kv_q4.cuh"
 
 namespace lmps {
@@ -70,9 +77,9 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv_append_q4_kernel(const
       if (kUnit == 16) b[k] = *reinterpret_cast<const uint4*>(src + at(u) + kDim / 2);
     }
   }
-  const int r0 = l >> 5;
-  uint2 kv = make_uint2(0u, 0u);
-  if (r0 < 2 * n_kv) kv = *reinterpret_cast<const uint2*>(src + (P.n_q + r0) * kDim + 4 * lane);
+  const int sub = lane >> 4, l16 = lane & 15, r0 = 2 * (l >> 5);  // K and V: 16 lanes a row, 8 elements a lane
+  uint4 kv = make_uint4(0u, 0u, 0u, 0u);
+  if (r0 < 2 * n_kv) kv = *reinterpret_cast<const uint4*>(src + (P.n_q + r0 + sub) * kDim + 8 * l16);
 
   const int p = used ? P.pos[row] : -1;
   int page = -1, off = 0;
@@ -120,31 +127,37 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv_append_q4_kernel(const
     const uint4 x = *reinterpret_cast<const uint4*>(src + at(u));
     rotate(u, x, kUnit == 16 ? *reinterpret_cast<const uint4*>(src + at(u) + kDim / 2) : x);
   }
-  // K and V: a warp per row of 128, the next row's load ahead
-  for (int r = r0; r < 2 * n_kv; r += kPer / kWarp) {
+  // K and V (their 2 n_kv rows): a warp per two rows of 128, the next rows' load ahead
+  constexpr int kStride = 2 * (kPer / kWarp);
+  for (int r = r0; r < 2 * n_kv; r += kStride) {
     union {
-      uint2 u;
-      __half x[4];
-    } e;
+      uint4 u;
+      __half x[8];
+    } e, rot;
     e.u = kv;
-    if (r + kPer / kWarp < 2 * n_kv)
-      kv = *reinterpret_cast<const uint2*>(src + (P.n_q + r + kPer / kWarp) * kDim + 4 * lane);
-    const bool is_v = r >= n_kv;
-    const int kvh = r - (is_v ? n_kv : 0);
-    if (!is_v) rotate_head(e.x, csd[t], kStyle, lane);
-    const float x[4] = {__half2float(e.x[0]), __half2float(e.x[1]), __half2float(e.x[2]), __half2float(e.x[3])};
+    if (r + kStride < 2 * n_kv)
+      kv = *reinterpret_cast<const uint4*>(src + (P.n_q + r + kStride + sub) * kDim + 8 * l16);
+    const bool is_v = r + sub >= n_kv;
+    const int kvh = r + sub - (is_v ? n_kv : 0);
+    if (r < n_kv) {  // (uniform) one K row at least
+      rot.u = e.u;
+      rotate_head(rot.x, csd[t], kStyle, lane);
+      if (!is_v) e.u = rot.u;
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __half2float(e.x[i]);
     float scale;
     const uint32_t w = quantise_row(x, scale);
     uint8_t* block = (is_v ? P.v_pool : P.k_pool) + P.c.block(page, kvh);
-    *reinterpret_cast<uint16_t*>(block + off * kCodeBytes + 2 * lane) = static_cast<uint16_t>(w);
-    if ((lane & 7) == 0)
-      *reinterpret_cast<__half*>(block + P.c.page_size * kCodeBytes + off * 8 + (lane >> 3) * 2) = __float2half_rn(scale);
+    *reinterpret_cast<uint32_t*>(block + off * kCodeBytes + 4 * l16) = w;
+    if ((lane & 3) == 0)
+      *reinterpret_cast<__half*>(block + P.c.page_size * kCodeBytes + off * 8 + (l16 >> 2) * 2) = __float2half_rn(scale);
     __half* copy = is_v ? P.v_out : P.k_out;
     if (copy) {
-      const __half2 lo = __floats2half2_rn(nib_code(w, 0) * scale, nib_code(w, 1) * scale);
-      const __half2 hi = __floats2half2_rn(nib_code(w, 2) * scale, nib_code(w, 3) * scale);
-      *reinterpret_cast<uint2*>(copy + (static_cast<size_t>(row) * n_kv + kvh) * kDim + 4 * lane) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e.x[i] = __float2half_rn(nib_code(w, i) * scale);
+      *reinterpret_cast<uint4*>(copy + (static_cast<size_t>(row) * n_kv + kvh) * kDim + 8 * l16) = e.u;
     }
   }
 }

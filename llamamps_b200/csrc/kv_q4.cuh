@@ -70,22 +70,24 @@ __device__ __forceinline__ float group_scale(float a) {
   return fminf(s, 9344.0f);
 }
 
-// A warp quantises one row: lane l holds elements 4l .. 4l+3 (exact fp16
-// values).  Returns the lane's four nibbles (element 4l lowest: bytes 2l and
-// 2l + 1 of the row); `scale` is the scale of its group l / 8.
-__device__ __forceinline__ uint32_t quantise_row(const float (&x)[4], float& scale) {
+// 128 / N lanes of a warp quantise one row each: lane l of them holds elements
+// N l .. N l + N - 1 (exact fp16 values).  Returns the lane's N nibbles (element
+// N l lowest); `scale` is the scale of its group N l / 32.  All lanes take part.
+template <int N>
+__device__ __forceinline__ uint32_t quantise_row(const float (&x)[N], float& scale) {
+  constexpr int kLanes = kDim / N;
   float a = 0.0f;
-  bool finite = true;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a = fmaxf(a, fabsf(x[i]));
-    finite = finite && fabsf(x[i]) <= 65504.0f;
-  }
+  for (int i = 0; i < N; ++i) a = fmaxf(a, fabsf(x[i]));
+  bool finite = a <= 65504.0f;  // (the maximum takes the number where the other is NaN)
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if (!__all_sync(0xffffffffu, finite)) {
+  for (int i = 0; i < N; ++i) finite = finite && x[i] == x[i];
+#pragma unroll
+  for (int o = 1; o < kLanes / kGroups; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const uint32_t row = (kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1));
+  if ((__ballot_sync(0xffffffffu, finite) & row) != row) {
     scale = __int_as_float(0x7FC00000);
-    return 0x8888u;
+    return 0x88888888u >> (32 - 4 * N);
   }
   scale = group_scale(a);
   // x / s by a reciprocal and one residual step (Markstein): exact where the
@@ -96,7 +98,7 @@ __device__ __forceinline__ uint32_t quantise_row(const float (&x)[4], float& sca
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
   uint32_t w = 0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     const float q = x[i] * r;
     const float c = fmaf(fmaf(-q, scale, x[i]), r, q) + 12582920.0f;
     w |= (__float_as_uint(c) & 0xFu) << (4 * i);
@@ -159,21 +161,32 @@ __device__ __forceinline__ void rope_rotate_by(__half& a, __half& b, const float
   a = __float2half_rn(y1);
   b = __float2half_rn(y2);
 }
-// A warp rotates one head's row in place: lane l holds elements 4l .. 4l+3;
+// One of the two: the first (x = x1, other = x2) or the second (x = x2, other = x1), the same operations.
+__device__ __forceinline__ __half rope_rotate_one(__half x, __half other, bool first, const double2& t) {
+  const double o = static_cast<double>(__half2float(x)), p = static_cast<double>(__half2float(other));
+  const double m = __dmul_rn(first ? p : o, first ? t.y : t.x);
+  return __float2half_rn(static_cast<float>(__fma_rn(first ? o : p, first ? t.x : t.y, first ? -m : m)));
+}
+__device__ __forceinline__ __half rope_rotate_one(__half x, __half other, bool first, const float2& t) {
+  const float o = __half2float(x), p = __half2float(other);
+  const float m = __fmul_rn(first ? p : o, first ? t.y : t.x);
+  return __float2half_rn(__fmaf_rn(first ? o : p, first ? t.x : t.y, first ? -m : m));
+}
+// 128 / N lanes of a warp rotate one head's row each in place: lane l of them holds elements N l .. N l + N - 1;
 // cs: 64 (cos, sin), fp64 for K and fp32 for q.
-template <class Pair>
-__device__ __forceinline__ void rotate_head(__half (&x)[4], const Pair* cs, int style, int lane) {
+template <int N, class Pair>
+__device__ __forceinline__ void rotate_head(__half (&x)[N], const Pair* cs, int style, int lane) {
+  constexpr int kHalf = kDim / 2 / N;  // lanes of half a row
   if (style == LMPS_ROPE_INTERLEAVED) {
-    rope_rotate_by(x[0], x[1], cs[2 * lane]);
-    rope_rotate_by(x[2], x[3], cs[2 * lane + 1]);
-  } else {  // element j pairs with j + 64: the partner lane is 16 away
+    const int l = lane & (2 * kHalf - 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned other = __shfl_xor_sync(0xffffffffu, static_cast<unsigned>(__half_as_ushort(x[i])), 16);
-      const __half p = __ushort_as_half(static_cast<unsigned short>(other));
-      __half a = lane < 16 ? x[i] : p, b = lane < 16 ? p : x[i];
-      rope_rotate_by(a, b, cs[4 * (lane & 15) + i]);
-      x[i] = lane < 16 ? a : b;
+    for (int i = 0; i < N / 2; ++i) rope_rotate_by(x[2 * i], x[2 * i + 1], cs[N / 2 * l + i]);
+  } else {  // element j pairs with j + 64: the partner lane is half a row away
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned other = __shfl_xor_sync(0xffffffffu, static_cast<unsigned>(__half_as_ushort(x[i])), kHalf);
+      x[i] = rope_rotate_one(x[i], __ushort_as_half(static_cast<unsigned short>(other)), (lane & kHalf) == 0,
+                             cs[N * (lane & (kHalf - 1)) + i]);
     }
   }
 }

@@ -9,12 +9,11 @@
 // (two M = 128 tiles, t = 0, 1) of one KV head and sequence and walks its
 // 128-key tiles:
 //   * warp 14 brings a tile's cached rows to shared memory (bulk copies);
-//   * warps 8-11 write its K and V as
-//     fp16 code * scale -- exact, see kv_q4.cuh -- into two 128-byte-swizzled
-//     stages each (K read K-major, V MN-major);
-//   * warps 12, 13 (row tile 0, 1) issue S_t = Q_t K^T and O_t += P_t V in half tiles of 64 keys:
-//     S has two halves per row tile, so the softmax finds the next one ready
-//     while the products behind the last run;
+//   * warps 8-11 write its K and V as fp16 code * scale -- exact, see kv_q4.cuh
+//     -- into two 128-byte-swizzled stages each (K read K-major, V MN-major);
+//   * warps 12, 13 (row tile 0, 1) issue S_t = Q_t K^T and O_t += P_t V in half
+//     tiles of 64 keys: S has two halves per row tile, so the softmax finds the
+//     next one ready while the products behind the last run;
 //   * warps 0-3 / 4-7 (thread = row, its TMEM lane) take the softmax of row
 //     tile 0 / 1: row max, P = 2^(s - m) as fp16 packed over S's own columns
 //     (A operand from tensor memory), sums in fp32, and O rescaled in place
@@ -22,9 +21,20 @@
 // The dims inside a group of 8 stay in the order in which masking the nibbles
 // yields them (0 4 1 5 2 6 3 7): Q is staged in that order, and the epilogue
 // undoes it for O by naming registers.
-// Few rows over a long context are split over the context (grid.y): fp32
-// partials, merged by the decode attention's combine kernel.
+// Few rows over a long context are cut into pieces of equal length along it:
+// fp32 partials, merged by a second kernel.  Units of work go to 148 persistent
+// CTAs, from the longest rows to the shortest, forwards and backwards in turn.
 // Every mbarrier wait is bounded (error bit, no hang).
+//
+// What bounds it: not the tensor core.  A 256 x 128 tile has 2048 cycles of
+// products and takes about 4100: the softmax of 64 keys is a chain of one TMEM
+// load, 64 exponentials a thread, conversions and a TMEM store, and the four
+// dequantising warps share its schedulers.  Measured (12 query, 2 KV heads):
+// 8 x 2048 causal 150 us = 690 TFLOP/s, 0.41 of the bf16 peak measured by a
+// library product; 4 x 256 queries behind 1..30000 positions 80 us; one
+// prompt of 37 tokens 8 us.  Tried without gain: exponentials by polynomial on
+// the FMA units for a part of a row, the two softmax groups held half a step
+// apart, the next unit's queries fetched during the epilogue (64 registers, spilled).
 #include <cmath>
 
 #include "attention_q4.cuh"
