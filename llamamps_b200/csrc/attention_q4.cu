@@ -59,7 +59,7 @@ constexpr int kShortWarps = 8, kPieceWarps = 4;
 constexpr int kSms = 148, kPieceCtas = 3;
 constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
-constexpr int kHead = 3, kShortShare = 8;
+constexpr int kHead = 8, kManyShares = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kClusterShare = 1280;  // positions of a CTA up to which a row is shared by a cluster
 constexpr int kOffV = kStep * kCodeBytes;
@@ -564,17 +564,25 @@ __global__ void __launch_bounds__(kWarps * kWarp, kWarps == kShortWarps ? 1 : kP
   attend(P, *reinterpret_cast<Smem<kWarps>*>(smem_raw), row, T, start, min(T, start + share), 0);
 }
 
-// Equal shares of the rows laid end to end, in units of a step of every warp (a row without positions has one):
-// a share may take in the end of a row and the start of the next, a segment each.  kHead units in front of each
-// row stand for what another segment costs; where a share is no longer than kShortShare, one more than a share
-// does, so that none takes in two rows (16 x 1..32000: 23.3 us, kHead alone 24.3; 4 x 32768: 17.0 and 19.0;
-// 64 x 4100..8200, kHead 0 / 2 / 3 / 4: 34.3 / 33.2 / 33.4 / 33.7).  Segment (CTA i, row r) has slot i + r.
+// a * b / c; in 32 bits where the product fits (a 64-bit division is some 100 instructions in a row).
+__device__ __forceinline__ unsigned long long mul_div(unsigned long long a, unsigned long long b, unsigned long long c) {
+  const unsigned long long ab = a * b;
+  if (ab <= 0xFFFFFFFFull && c <= 0xFFFFFFFFull) return static_cast<uint32_t>(ab) / static_cast<uint32_t>(c);
+  return ab / c;
+}
+
+// Equal shares of the rows laid end to end, in units of a warp's step (a row without positions has one): a share
+// may take in the end of a row and the start of the next, a segment each.  `head` units in front of each row
+// stand for what starting another segment costs: under load a chain of three memory accesses, which other shares
+// hide only where every SM has many of them to do.  So with kManyShares shares or more to a row a head is one
+// unit longer than a share, and none takes in two rows (fresh caches: 8 x 20000..30000 24.5 us, 29 with short
+// heads; 32 x 1..16000 25.6 and 24.2).  Segment (CTA i, row r) has slot i + r.
 __global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_pieces_kernel(const AttnParams P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem<kPieceWarps>& S = *reinterpret_cast<Smem<kPieceWarps>*>(smem_raw);
-  constexpr int kUnit = kPieceWarps * kStep;
+  constexpr int kUnit = kStep;
   const int lane = threadIdx.x & 31;
   auto units = [](int len) { return max(1, (len + kUnit - 1) / kUnit); };
   {
@@ -582,11 +590,11 @@ __global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_piece
     for (int r = lane; r < P.rows; r += kWarp) total += units(P.length(r));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int head = total <= static_cast<unsigned long long>(kShortShare) * gridDim.x ? static_cast<int>(total / gridDim.x) + 1 : kHead;
+    const int head = gridDim.x >= static_cast<unsigned>(kManyShares) * P.rows ? static_cast<int>(total / gridDim.x) + 1 : kHead;
     total += static_cast<unsigned long long>(head) * P.rows;
     const unsigned long long ctas = min(static_cast<unsigned long long>(gridDim.x), total);
     if (blockIdx.x >= ctas) return;
-    const unsigned long long from = blockIdx.x * total / ctas;
+    const unsigned long long from = mul_div(blockIdx.x, total, ctas);
     int row = 0, r0 = 0;
     for (;; r0 += kWarp) {  // ends: `from` is below the total
       const int r = r0 + lane, mine = r < P.rows ? head + units(P.length(r)) : 0;
@@ -605,7 +613,7 @@ __global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_piece
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (threadIdx.x == 0) S.share = Share{before, from, (blockIdx.x + 1) * total / ctas, total, ctas, row, head};
+    if (threadIdx.x == 0) S.share = Share{before, from, mul_div(blockIdx.x + 1, total, ctas), total, ctas, row, head};
   }
   for (;;) {
     __syncthreads();
