@@ -5,12 +5,12 @@
 // a cosine to compute): the rows' 64 (cos, sin) pairs once in fp64, q in units
 // of 16 bytes a thread, then a warp per two K or V rows (8 elements a lane).
 //
-// One row is launch and latency (3.5 us, as are 64).  A prompt of 8 x 2048 rows
-// (12 query, 2 KV heads: 139 MB) takes 33 us = 4.2 TB/s, 0.64 of the measured
-// copy rate, at 65 % of the issue slots: the fp64 rotation of K and the
-// quantiser (a maximum over 8 lanes, an exact division by 7 rounded up, 128
-// roundings) are its instructions.  K is rotated in fp64 so that the rounding
-// to fp16, and with it every code, is that of the exact formula.
+// One row is launch and latency (3.4 us, as are 64).  A prompt of 8 x 2048 rows
+// (12 query, 2 KV heads: 139 MB) takes 28.7 us = 4.8 TB/s, 0.74 of the measured
+// copy rate; its instructions are the rotations and the quantiser, whose
+// maximum and scale a row's 16 lanes share (32 lanes of 4 elements: 32.6 us).
+// K is rotated in fp64 so that the rounding to fp16, and with it every code, is
+// that of the exact formula.
 #include "kv_q4.cuh"
 
 namespace lmps {
