@@ -30,7 +30,7 @@
 // products and takes about 4100: the softmax of 64 keys is a chain of one TMEM
 // load, 64 exponentials a thread, conversions and a TMEM store, and the four
 // dequantising warps share its schedulers.  Measured (12 query, 2 KV heads):
-// 8 x 2048 causal 150 us = 690 TFLOP/s, 0.41 of the bf16 peak measured by a
+// 8 x 2048 causal 151 us = 682 TFLOP/s, 0.41 of the bf16 peak measured by a
 // library product; 4 x 256 queries behind 1..30000 positions 80 us; one
 // prompt of 37 tokens 8 us.  Tried without gain: exponentials by polynomial on
 // the FMA units for a part of a row, the two softmax groups held half a step
