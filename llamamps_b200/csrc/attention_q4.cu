@@ -34,8 +34,8 @@
 //
 // What bounds it.  A step of 32 positions is 4.6 KB and some 750 instructions a
 // warp (unpacking, scales, the softmax): with 12 warps an SM goes through its
-// steps at 5.3 TB/s over the GPU, 0.8 of the measured copy rate, issue slots
-// and memory latency about even.  What is left is around them: 4 us of an empty
+// steps at 4.5 TB/s over the GPU, 0.7 of the measured copy rate, issue slots
+// (54 % used) and memory latency about even.  What is left is around them: 4 us of an empty
 // call (launch, page table, first loads, meeting of the warps) and 3 us of the
 // second kernel.  Measured (12 query, 2 KV heads, caches not in L2): 1 x 131
 // 3.9 us; 64 x 1..1000 11.0; 4 x 32768 18.9 (2.0 TB/s); 64 x 4100..8200 35.8

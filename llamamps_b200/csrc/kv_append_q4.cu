@@ -6,9 +6,9 @@
 // of 16 bytes a thread, then a warp per two K or V rows (8 elements a lane).
 //
 // One row is launch and latency (3.4 us, as are 64).  A prompt of 8 x 2048 rows
-// (12 query, 2 KV heads: 139 MB) takes 28.7 us = 4.8 TB/s, 0.74 of the measured
+// (12 query, 2 KV heads: 139 MB) takes 29.6 us = 4.7 TB/s, 0.72 of the measured
 // copy rate; its instructions are the rotations and the quantiser, whose
-// maximum and scale a row's 16 lanes share (32 lanes of 4 elements: 32.6 us).
+// maximum and scale a row's 16 lanes share (32 lanes of 4 elements: 33.0 us).
 // K is rotated in fp64 so that the rounding to fp16, and with it every code, is
 // that of the exact formula.
 #include "kv_q4.cuh"
