@@ -196,6 +196,40 @@ def test_decode_shares_of_ragged_rows(cuda, lens, hq, hkv, page, n_splits, max_l
         R.close(got[b], *R.attend(q[b], *c.rows[b], lens[b]), f"length {lens[b]}")
 
 
+def test_decode_shares_follow_the_lengths_in_a_graph(cuda):
+    """The shares are cut from the lengths that the device holds when the call runs: a captured call replayed with
+    other lengths gives the bits of an eager call, whatever the replay before it left in the workspace."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(31)
+    B, hq, hkv, page, n_splits, longest = 40, 6, 1, 32, 9, 700
+    c = R.Cache(rng, [longest] * B, hkv, page)
+    q = _cu(rng.normal(0, 1, (B, hq * D)).astype(np.float16))
+    seq = torch.full((B,), longest, dtype=torch.int32, device="cuda")
+    ws, out = _ws(K.attention_q4_workspace_size(B, hq, D, n_splits)), torch.empty(B, hq * D, dtype=torch.float16, device="cuda")
+
+    def call(o, w):
+        K.gqa_decode_attention_q4(q, c.k, c.v, c.bt, seq, o, w, page, hq, hkv, D, 20000, n_splits)
+
+    c.bt = torch.nn.functional.pad(c.bt, (0, 625 - c.bt.shape[1]), value=0)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        call(out, ws)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(out, ws)
+    for lens in ([longest] * B, [0] * B, [(61 * i) % longest for i in range(B)], [longest] + [1] * (B - 1), [0] * (B - 1) + [33]):
+        seq.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.empty_like(out)
+        call(eager, torch.zeros_like(ws))
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+        for b in (0, 1, B - 1):
+            R.close(out[b].cpu().numpy(), *R.attend(q[b].cpu().numpy().reshape(hq, D), *c.rows[b], lens[b]), f"{b}, {lens[b]}")
+
+
 def test_decode_large_scores_and_long_flat_softmax(cuda):
     """Scores that differ by hundreds (one position takes all) and equal scores (the mean of V)."""
     from llamamps_b200 import kernels as K
