@@ -2,12 +2,16 @@
 //
 // For the query heads h of one KV head and one sequence of n positions:
 //   s_i = 0.088388 q_h . k_i,  p = softmax(s),  o_h = sum_i p_i v_i,
-// with k_i = c s (codes times the scale of their 32-element group).  The
-// codes go to the tensor cores as exact fp16 integers and the scales are
-// applied in fp32 around them, so neither K nor V is rounded:
-//   S   = sum_g ks[i, g] (sum_{d in g} c_k[i, d] q[d])   4 accumulators a block
-//   O_g = sum_i (p_i vs[i, g]) c_v[i, d],  d in g        P scaled per group
-// (P times a V scale is rounded to fp16 once, as P alone would be.)
+// with k_i = c s (codes times the scale of their 32-element group).  K's codes
+// go to the tensor cores as exact fp16 integers and their scales are applied in
+// fp32 around them; V's go there times their scales, which is exact in fp16
+// (kv_q4.cuh).  So neither K nor V is rounded:
+//   S = sum_g ks[i, g] (sum_{d in g} c_k[i, d] q[d])   4 accumulators a block
+//   O = sum_i p_i (c_v[i, d] vs[i, g])
+// P is rounded to fp16 once, held times 2^15: under a running maximum p is at
+// most 1, so it keeps 11 bits down to 2^-29 of the maximum whatever V's size.
+// (P times V's scale instead, over codes, lost the weights behind a strong
+// position where V is small: 2500 positions of size 0.01, 7e-3 of the result.)
 //
 // mma.sync m16n8k16: M = 16 positions (S) or 16 dims (O), N = 8 heads.
 // tcgen05 has M = 128 rows: with at most 8 query heads a KV head it would
@@ -62,6 +66,7 @@ constexpr int kStep = 32;  // positions per warp step: two runs of 16
 constexpr int kStages = 2;
 constexpr int kHead = 8, kManyShares = 8;
 constexpr int kMaxCluster = 8;
+constexpr float kPBias = 15.0f;  // P is held times 2^15
 constexpr int kClusterShare = 1280;  // positions of a CTA up to which a row is shared by a cluster
 constexpr int kOffV = kStep * kCodeBytes;
 constexpr int kOffKs = 2 * kOffV;
@@ -130,6 +135,18 @@ __device__ __forceinline__ void load_scales(const unsigned char* p, float (&s)[4
   s[2] = hi.x;
   s[3] = hi.y;
 }
+// The scales of the two rows at p (16-byte aligned) as pairs, one per group, with `keep` cleared bits zero.
+__device__ __forceinline__ void load_scale_pairs(const unsigned char* p, uint32_t keep, uint32_t (&s)[4]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  s[0] = __byte_perm(v.x, v.z, 0x5410) & keep;
+  s[1] = __byte_perm(v.x, v.z, 0x7632) & keep;
+  s[2] = __byte_perm(v.y, v.w, 0x5410) & keep;
+  s[3] = __byte_perm(v.y, v.w, 0x7632) & keep;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -193,7 +210,8 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A warp's running state: per lane heads 2t, 2t + 1; l is the lane's own part of the sum.
+// A warp's running state: per lane heads 2t, 2t + 1; m is the largest score q . k, l the lane's own part of the
+// sum; l and O times 2^kPBias.
 struct State {
   float o[8][4];
   float m0, m1, l0, l1;
@@ -208,12 +226,8 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
   // this lane's row address for ldmatrix: row lane & 7, chunk lane >> 3, stored at chunk ^ ((row >> 1) & 3)
   const uint32_t lm = smem_u32(st) + (lane & 7) * kCodeBytes + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
   float s[2][4];
-  bool v0[2], v1[2];  // rows g8 / g8 + 8 of each run count
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const bool run = (ok >> x) & 1u;
-    v0[x] = kFull || (run && p0 + 16 * x + g8 < end);
-    v1[x] = kFull || (run && p0 + 16 * x + g8 + 8 < end);
     uint32_t w0[4], w1[4];  // word 4g + t of rows g8 and g8 + 8
     ldmatrix4(lm + 16 * x * kCodeBytes, w0);
     ldmatrix4(lm + (16 * x + 8) * kCodeBytes, w1);
@@ -232,13 +246,14 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
         s[x][i] = g == 0 ? ks * a[i] : fmaf(ks, a[i], s[x][i]);
       }
     }
-    if (!kFull) {
+    if (!kFull) {  // rows g8, g8 + 8 of the run that do not count
+      const int left = ((ok >> x) & 1u) ? end - p0 - 16 * x - g8 : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[x][i] = (i < 2 ? v0[x] : v1[x]) ? s[x][i] : -INFINITY;
+      for (int i = 0; i < 4; ++i) s[x][i] = (i < 2 ? left > 0 : left > 8) ? s[x][i] : -INFINITY;
     }
   }
-  float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * kScaleLog2;
-  float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * kScaleLog2;
+  float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+  float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
@@ -247,7 +262,8 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
   if (__any_sync(0xffffffffu, mx0 > S.m0 || mx1 > S.m1)) {  // some head's max grew
     const float n0 = fmaxf(S.m0, mx0), n1 = fmaxf(S.m1, mx1);
     // a head without a position yet keeps max -inf; its sums are zero
-    const float a0 = n0 == -INFINITY ? 1.0f : ex2(S.m0 - n0), a1 = n1 == -INFINITY ? 1.0f : ex2(S.m1 - n1);
+    const float a0 = n0 == -INFINITY ? 1.0f : ex2((S.m0 - n0) * kScaleLog2);
+    const float a1 = n1 == -INFINITY ? 1.0f : ex2((S.m1 - n1) * kScaleLog2);
     S.l0 *= a0;
     S.l1 *= a1;
 #pragma unroll
@@ -260,33 +276,35 @@ __device__ __forceinline__ void fold_step(const unsigned char* st, int p0, int e
     S.m0 = n0;
     S.m1 = n1;
   }
-  const float r0 = S.m0 == -INFINITY ? 0.0f : -S.m0, r1 = S.m1 == -INFINITY ? 0.0f : -S.m1;
+  // differences to the maximum before the scale: exactly 0 at the maximum, so that P stays below 2^15 for scores of
+  // any size
+  const float m0 = S.m0 == -INFINITY ? 0.0f : S.m0, m1 = S.m1 == -INFINITY ? 0.0f : S.m1;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const float e0 = ex2(fmaf(s[x][0], kScaleLog2, r0)), e1 = ex2(fmaf(s[x][1], kScaleLog2, r1));
-    const float e2 = ex2(fmaf(s[x][2], kScaleLog2, r0)), e3 = ex2(fmaf(s[x][3], kScaleLog2, r1));
+    const float e0 = ex2(fmaf(s[x][0] - m0, kScaleLog2, kPBias)), e1 = ex2(fmaf(s[x][1] - m1, kScaleLog2, kPBias));
+    const float e2 = ex2(fmaf(s[x][2] - m0, kScaleLog2, kPBias)), e3 = ex2(fmaf(s[x][3] - m1, kScaleLog2, kPBias));
     S.l0 += e0 + e2;
     S.l1 += e1 + e3;
     uint32_t u0[4], u1[4];  // halfword g8 of chunk g: positions 2t, 2t + 1 and 2t + 8, 2t + 9
     ldmatrix4_trans(lm + kOffV + 16 * x * kCodeBytes, u0);
     ldmatrix4_trans(lm + kOffV + (16 * x + 8) * kCodeBytes, u1);
-    float vs0[4], vs1[4];
-    load_scales(st + kOffVs + (16 * x + g8) * 8, vs0);
-    load_scales(st + kOffVs + (16 * x + g8 + 8) * 8, vs1);
-    if (!kFull) {  // rows that do not count: whatever lies there as a scale, zero
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        vs0[g] = v0[x] ? vs0[g] : 0.0f;
-        vs1[g] = v1[x] ? vs1[g] : 0.0f;
-      }
+    uint32_t vs0[4], vs1[4];  // their scales; of positions that do not count zero, whatever lies there
+    uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
+    if (!kFull) {
+      const int left = ((ok >> x) & 1u) ? end - p0 - 16 * x - 2 * (lane & 3) : 0;
+      keep0 = left > 1 ? 0xFFFFFFFFu : left == 1 ? 0x0000FFFFu : 0u;
+      keep1 = left > 9 ? 0xFFFFFFFFu : left == 9 ? 0x0000FFFFu : 0u;
     }
+    load_scale_pairs(st + kOffVs + (16 * x + 2 * (lane & 3)) * 8, keep0, vs0);
+    load_scale_pairs(st + kOffVs + (16 * x + 2 * (lane & 3) + 8) * 8, keep1, vs1);
+    const uint32_t b0 = transpose(fd::pack_half2(e0, e1)), b1 = transpose(fd::pack_half2(e2, e3));
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const uint32_t u = u0[g], w = u1[g];
-      const uint32_t b0 = transpose(fd::pack_half2(e0 * vs0[g], e1 * vs0[g]));
-      const uint32_t b1 = transpose(fd::pack_half2(e2 * vs1[g], e3 * vs1[g]));
-      mma(S.o[2 * g], codes_lo(u), codes_hi(u), codes_lo(w), codes_hi(w), b0, b1);
-      mma(S.o[2 * g + 1], codes_lo(u >> 8), codes_hi(u >> 8), codes_lo(w >> 8), codes_hi(w >> 8), b0, b1);
+      mma(S.o[2 * g], mul2(codes_lo(u), vs0[g]), mul2(codes_hi(u), vs0[g]), mul2(codes_lo(w), vs1[g]),
+          mul2(codes_hi(w), vs1[g]), b0, b1);
+      mma(S.o[2 * g + 1], mul2(codes_lo(u >> 8), vs0[g]), mul2(codes_hi(u >> 8), vs0[g]),
+          mul2(codes_lo(w >> 8), vs1[g]), mul2(codes_hi(w >> 8), vs1[g]), b0, b1);
     }
   }
 }
@@ -497,7 +515,7 @@ __device__ __forceinline__ void attend(const AttnParams& P, Smem<kWarps>& S, int
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       // a warp without positions has max -inf and sums 0; a NaN score leaves NaN in its sums
-      const float f = S.wm[i][tid] == -INFINITY ? 1.0f : ex2(S.wm[i][tid] - M);
+      const float f = S.wm[i][tid] == -INFINITY ? 1.0f : ex2((S.wm[i][tid] - M) * kScaleLog2);
       l = fmaf(S.wl[i][tid], f, l);
       S.wf[i][tid] = f;
     }
@@ -518,7 +536,7 @@ __device__ __forceinline__ void attend(const AttnParams& P, Smem<kWarps>& S, int
     } else {
       const size_t at = slot * P.n_q + kvh * G + h;
       *reinterpret_cast<float4*>(P.part_o + at * kDim + d) = o;
-      if (d == 0) P.part_ml[at] = make_float2(S.cm[h], S.cl[h]);
+      if (d == 0) P.part_ml[at] = make_float2(S.cm[h] * kScaleLog2, S.cl[h]);
     }
   }
   if (P.cluster) {  // the CTAs' states meet: each writes its part of the row
@@ -543,7 +561,7 @@ __device__ __forceinline__ void attend(const AttnParams& P, Smem<kWarps>& S, int
 #pragma unroll
       for (int i = 0; i < kMaxCluster; ++i)
         if (i < P.cluster) {
-          const float f = m[i] == -INFINITY ? 1.0f : ex2(m[i] - M);
+          const float f = m[i] == -INFINITY ? 1.0f : ex2((m[i] - M) * kScaleLog2);
           fma4(num, o[i], f);
           den = fmaf(l[i], f, den);
         }
