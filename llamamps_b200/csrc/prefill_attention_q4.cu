@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
       const int r = W.r0 + rl, qi = quotient(r, P.by_G);
       const int lim = r < W.n_rows ? limit(P, W.first, qi) : W.kv_end;
       const int lim_min = limit(P, W.first, quotient(W.r0 + kRows * t, P.by_G));
-      float m_used = -INFINITY, l = 0.0f;  // running max (scaled, base 2) and sum
+      float m_used = -INFINITY, l = 0.0f;  // running max (of q . k) and sum
       for (int i = 0; ok && i < W.nh; ++i) {
         const int u = i & 1, k0 = W.tile0 * kKeys + i * kHalf;
         const uint32_t ts = tl + kColS + kHalf * (2 * t + u);
@@ -653,11 +653,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < kHalf; c += 2)
           mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(sc[c]), __uint_as_float(sc[c + 1]));
-        const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * kScaleLog2;
-        const float mnew = fmaxf(m_used, mt);
-        const bool grow = mnew > m_used + kRescaleLog2;  // (always on a row's first positions)
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        const float more = (top - m_used) * kScaleLog2;
+        const bool grow = more > kRescaleLog2;  // (always on a row's first positions)
         if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = grow ? ex2(m_used - mnew) : 1.0f;
+          const float alpha = grow ? ex2(-more) : 1.0f;
           if (i > 0) {  // warp-wide read-modify-write of O_t, once the P V of the step before is done
             ok = wait_warp(&o_done[2 * t + (u ^ 1)], (~used >> (u ^ 1)) & 1u, err, abort_v);
             if (!ok) break;
@@ -672,16 +672,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             }
           }
           l *= alpha;
-          if (grow) m_used = mnew;
+          if (grow) m_used = top;
         }
-        const float nm = m_used == -INFINITY ? 0.0f : kPBias - m_used;
-        const uint64_t nm2 = pair(nm, nm), scale2 = pair(kScaleLog2, kScaleLog2);
+        // differences to the maximum before the scale: exactly 0 at the maximum, so that P stays below 2^15 for scores
+        // of any size (score times scale less a rounded product, one operation in place of two, is off by up to 2^3 at
+        // scores of 10^9; 8 x 2048 155.0 us, with it 151.4)
+        const float nm = m_used == -INFINITY ? 0.0f : -m_used;
+        const uint64_t nm2 = pair(nm, nm), bias2 = pair(kPBias, kPBias), scale2 = pair(kScaleLog2, kScaleLog2);
         uint64_t sm[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           float a0, a1;
-          unpair(fma2(pair(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), scale2, nm2), a0, a1);
+          unpair(fma2(add2(pair(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), nm2), scale2, bias2), a0, a1);
           a0 = ex2(a0);
           a1 = ex2(a1);
           sm[e & 3] = add2(sm[e & 3], pair(a0, a1));
@@ -715,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
       const size_t head = (static_cast<size_t>(D.b) * P.seq + qi) * P.n_q + D.kvh * P.G + (r - qi * P.G);
       const size_t part = (static_cast<size_t>(D.piece) * P.c.n_kv + D.kvh) * P.rows_item + rl;
       const bool there = r < D.n_rows;
-      if (P.n_splits > 1 && there) P.part_ml[part] = make_float2(m_used, l);
+      if (P.n_splits > 1 && there) P.part_ml[part] = make_float2(m_used * kScaleLog2, l);
 #pragma unroll 1
       for (int cc = 0; cc < kDim; cc += 32) {
         uint32_t o[32];

@@ -53,3 +53,42 @@ def test_decode_behind_a_sink(cuda, gain, lens, hq, hkv, page, n_splits, max_len
     for b in sorted({0, 1 % B, B - 1}):
         T.close(out[b].cpu().numpy(), *T.attend(q[b], *c.rows[b], lens[b]), f"decode, length {lens[b]}")
         T.close(other[b].cpu().numpy(), *T.attend(q[b], *c.rows[b], lens[b], 2.0 ** -32, 16), f"prefill, length {lens[b]}")
+
+
+@pytest.mark.parametrize("size", [40.0, 2000.0, 60000.0])
+def test_scores_of_any_size(cuda, size):
+    """Scores from some 10^7 to 4 * 10^10, positive and negative: where they differ, they differ by thousands, so
+    the result is V of the largest (or the mean over equal ones), off by the roundings of P (2^-11) and of the
+    result (2^-11) at most; sums and factors in fp32 are within the rest of 2^-9."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(int(size))
+    n, hq, hkv, page = 700, 6, 1, 16
+    u = rng.choice([-1.0, 1.0], D)
+    c = R.Cache(rng, [0], hkv, page, max_len=n)
+    k = (rng.choice([-1.0, 1.0], (n, 1, 1)) * rng.uniform(20000, 60000, (n, 1, 1)) * u).astype(np.float16)
+    k[0] = -u * 50000  # the first position sees a negative score alone
+    rows = c._write(c.k_np, 0, 0, k), c._write(c.v_np, 0, 0, rng.normal(0, 1, (n, hkv, D)).astype(np.float16))
+    c.k, c.v = _cu(c.k_np), _cu(c.v_np)
+    q = np.repeat((u * size).astype(np.float16)[None], hq, 0)
+    seq = torch.tensor([n], dtype=torch.int32, device="cuda")
+
+    def check(got, length, what):
+        want, _ = R.attend(q, *rows, length)
+        got = got.cpu().numpy().reshape(hq, D).astype(np.float64)
+        assert np.isfinite(got).all(), f"{what}: not finite"
+        assert (np.abs(got - want) <= 2.0 ** -9 * np.abs(rows[1][:length]).max(0)).all(), what
+
+    qd = _cu(q.reshape(1, -1))
+    for n_splits, max_len in ((1, n), (3, n), (9, c.max_seq_len)):
+        out = torch.empty(1, hq * D, dtype=torch.float16, device="cuda")
+        K.gqa_decode_attention_q4(qd, c.k, c.v, c.bt, seq, out, _ws(K.attention_q4_workspace_size(1, hq, D, n_splits)),
+                                  page, hq, hkv, D, max_len, n_splits)
+        check(out, n, f"decode, {n_splits} splits")
+    for n_splits in (1, 3):
+        e, out = _err(), torch.empty(n, hq * D, dtype=torch.float16, device="cuda")
+        K.prefill_attention_q4(qd.repeat(n, 1), c.k, c.v, c.bt, out, 1, n, page, hq, hkv, D, c.max_seq_len,
+                               workspace=_ws(K.prefill_q4_workspace_size(1, n, hq, D, n_splits)), n_splits=n_splits,
+                               error=e)
+        assert e.item() == 0
+        for i in [0, 1, 2, 5, 31, 63, 64, 65, 127, 128, 300, n - 1]:
+            check(out[i], i + 1, f"prefill, {n_splits} splits, query {i}")
