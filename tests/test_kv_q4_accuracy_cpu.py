@@ -54,3 +54,23 @@ def test_weights_survive_small_values(n, warps, gain):
     assert not T.outside(got[0], want, tol)
     if gain <= 0.02:
         assert T.outside(got[1], want, tol)
+
+
+@pytest.mark.parametrize("n", [300, 2000, 20000])
+def test_lost_and_doubled_steps_stand_out(n):
+    """A step of 32 positions left out, counted twice, or read from its neighbour, anywhere in a row, leaves the
+    tolerance; so does one position too many or too few in a short row."""
+    rng = np.random.default_rng(n)
+    q = rng.normal(0, 1, (2, D)).astype(np.float16)
+    k, v = (_values(rng.normal(0, 1, (n + 32, 1, D)).astype(np.float16))[0] for _ in range(2))
+    want, tol = T.attend(q, k, v, n)
+    every = np.arange(n)
+    for p in (0, 32, n // 2 // 32 * 32, (n - 1) // 32 * 32 - 32, n - 32):
+        lost, doubled = np.delete(every, every[p:p + 32]), np.append(every, every[p:p + 32])
+        swapped = every.copy()
+        swapped[p:p + 32] += 32 if p + 64 <= n else -32
+        for rows in (lost, doubled, swapped):
+            assert T.outside(R.attend(q, k[rows], v[rows], len(rows))[0], want, tol), p
+    if n == 300:
+        for m in (n - 1, n + 1):
+            assert T.outside(R.attend(q, k, v, m)[0], want, tol)

@@ -92,3 +92,67 @@ def test_scores_of_any_size(cuda, size):
         assert e.item() == 0
         for i in [0, 1, 2, 5, 31, 63, 64, 65, 127, 128, 300, n - 1]:
             check(out[i], i + 1, f"prefill, {n_splits} splits, query {i}")
+
+
+@pytest.mark.parametrize("lens,hq,hkv,page,n_splits,max_len", [
+    # one CTA a row: of 8 warps, of 4
+    ([1, 31, 33, 300], 12, 2, 16, 1, 300), ([(29 * i) % 700 for i in range(160)], 2, 1, 48, 1, 700),
+    # clusters of 2, 3, 8
+    ([513, 64, 65], 12, 2, 64, 2, 2560), ([700, 95, 0, 96], 8, 8, 32, 3, 3840), ([1000, 257], 7, 1, 16, 8, 1008),
+    # pieces: long shares across the rows, rows shorter than a share, fewer units than shares, one row
+    ([20000, 0, 9000], 12, 2, 64, 9, 20032), ([0, 1, 127, 128, 129, 255, 256, 257, 640, 2000, 0, 5], 8, 4, 16, 11, 2016),
+    ([(37 * i) % 300 for i in range(250)], 2, 2, 16, 9, 304), ([9000], 16, 2, 64, 1024, 9024),
+    ([3] * 40, 6, 1, 16, 10, 16),
+    # many shares to a row, and borders inside some of them
+    ([3000, 2000, 2500], 8, 4, 32, 100, 3008), ([4000, 3000, 3500, 2500], 6, 1, 64, 30, 4032),
+])
+def test_decode_loses_and_doubles_no_step(cuda, lens, hq, hkv, page, n_splits, max_len):
+    """Every way of sharing rows out, under a tolerance that a step of 32 positions lost, doubled or read from its
+    neighbour leaves (test_kv_q4_accuracy_cpu.py)."""
+    from llamamps_b200 import kernels as K
+    rng = np.random.default_rng(len(lens) + hq)
+    c = R.Cache(rng, lens, hkv, page)
+    B, max_pages = len(lens), -(-max_len // page)
+    c.bt = torch.nn.functional.pad(c.bt, (0, max(0, max_pages - c.bt.shape[1])))
+    q = rng.normal(0, 1, (B, hq, D)).astype(np.float16)
+    assert K.attention_q4_launches(n_splits, max_len) == (1 if n_splits <= 8 else 2)
+    buf, out = _guarded(B, hq * D)
+    e = _err()
+    K.gqa_decode_attention_q4(_cu(q.reshape(B, -1)), c.k, c.v, c.bt, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                              out, _ws(K.attention_q4_workspace_size(B, hq, D, n_splits)), page, hq, hkv, D,
+                              max(max_len, max(lens)), n_splits, error=e)
+    assert e.item() == 0 and _guards_ok(buf)
+    got = out.cpu().numpy().reshape(B, hq, D)
+    for b in range(B):
+        T.close(got[b], *T.attend(q[b], *c.rows[b], lens[b]), f"row {b}, length {lens[b]}")
+        if lens[b] == 0:
+            assert (got[b] == 0).all()
+
+
+def test_step_loses_no_position(cuda):
+    """The decode step's own position and all before it, in one CTA a row, a cluster and pieces."""
+    from llamamps_b200 import kernels as K
+    from tests.test_kv_q4_gpu import _inv
+    rng = np.random.default_rng(41)
+    lens, hq, hkv, page = [1, 33, 1000, 640], 12, 2, 32
+    for n_splits, max_len in ((1, 1024), (4, 1024), (9, 1024)):
+        c = R.Cache(rng, [n - 1 for n in lens], hkv, page, max_len=max_len)
+        qkv = rng.normal(0, 1, (4, hq + 2 * hkv, D)).astype(np.float16)
+        seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        buf, out = _guarded(4, hq * D)
+        e = _err()
+        K.gqa_decode_attention_rope_q4(_cu(qkv.reshape(4, -1)), seq - 1, _cu(_inv()), c.k, c.v, c.bt, seq, out,
+                                       _ws(K.attention_q4_workspace_size(4, hq, D, n_splits)), page, hq, hkv, D,
+                                       max_len, n_splits, error=e)
+        assert e.item() == 0 and _guards_ok(buf)
+        # the rotated q as the append gives it (the step's attention has the same bits)
+        q = torch.empty_like(out)
+        K.rope_kv_append_q4(_cu(qkv.reshape(4, -1)), seq - 1, _cu(_inv()), q, c.k.clone(), c.v.clone(), c.bt, page, hq,
+                            hkv, D)
+        q = q.cpu().numpy().reshape(4, hq, D)
+        rot = R.rotate(qkv[:, hq:hq + hkv], np.array(lens) - 1, _inv(), 0)
+        got = out.cpu().numpy().reshape(4, hq, D)
+        for b in range(4):
+            k, v = (np.concatenate([old, R.values(*R.quantise(new))[None]])
+                    for old, new in zip(c.rows[b], (rot[b], qkv[b, hq + hkv:])))
+            T.close(got[b], *T.attend(q[b], k, v, lens[b]), f"length {lens[b]}, {n_splits} splits")
