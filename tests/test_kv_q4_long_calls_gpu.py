@@ -1,10 +1,12 @@
-"""Calls of the 4-bit cache's kernels that fill the GPU: appends of more than 1024 rows (four tokens a CTA)."""
+"""Calls of the 4-bit cache's kernels that fill the GPU: appends of more than 1024 rows (four tokens a CTA), and
+prefill attention with several units of work a CTA."""
 import numpy as np
 import pytest
 import torch
 
 from tests import _kv_q4 as R
-from tests.test_kv_q4_gpu import _cu, _err, _guarded, _guards_ok, _inv
+from tests import _kv_q4_tight as T
+from tests.test_kv_q4_gpu import _cu, _err, _guarded, _guards_ok, _inv, _ws
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +59,43 @@ def test_append_of_many_rows(cuda, style, rows, hq, hkv, page):
     assert (off <= np.abs(exact) * 2.0 ** -11 + size * 3 * 2.0 ** -24 * (1 + 2.0 ** -11) + 2.0 ** -25).all()
     rest = np.append(gone, skip)
     assert all((x[rest] == 7).all() for x in (q, k, v))
+
+
+@pytest.mark.parametrize("starts,q_lens,seq,hq,hkv,page,splits", [
+    # units of work: 204 and 400 (148 CTAs); ragged, so that some row blocks have one row tile and some none
+    ([0, 500, 7, 129, 64, 1000], [700, 3, 0, 301, 699, 43], 700, 12, 2, 64, (1, 2)),
+    ([(211 * i) % 900 for i in range(25)], [(97 * i + 40) % 513 for i in range(25)], 512, 8, 2, 16, (1, 3)),
+    # one position a sequence beside one long context: more sequences than CTAs, pieces of all lengths
+    ([4000] + [(13 * i) % 90 for i in range(159)], None, 1, 6, 1, 32, (1, 2)),
+    # whole prompts, 3 units a CTA and a last round that few CTAs have
+    (None, None, 600, 7, 1, 48, (1,)),
+])
+def test_prefill_with_several_units_a_cta(cuda, starts, q_lens, seq, hq, hkv, page, splits):
+    from llamamps_b200 import kernels as K
+    B = len(starts) if starts else 30
+    s_np, n_np = starts or [0] * B, q_lens or [seq] * B
+    units = -(-seq * (hq // hkv) // 256) * hkv * B
+    assert units > 148
+    rng = np.random.default_rng(B + seq)
+    c = R.Cache(rng, [s + n for s, n in zip(s_np, n_np)], hkv, page, max_len=max(s_np) + seq)
+    q = rng.normal(0, 1, (B, seq, hq, D)).astype(np.float16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for n_splits in splits:
+        buf, out = _guarded(B * seq, hq * D)
+        e = _err()
+        K.prefill_attention_q4(_cu(q.reshape(B * seq, -1)), c.k, c.v, c.bt, out, B, seq, page, hq, hkv, D,
+                               c.max_seq_len, starts=torch.tensor(s_np, **i32) if starts else None,
+                               q_lens=torch.tensor(n_np, **i32) if q_lens else None,
+                               workspace=_ws(K.prefill_q4_workspace_size(B, seq, hq, D, n_splits)),
+                               n_splits=n_splits, error=e)
+        assert e.item() == 0 and _guards_ok(buf)
+        got = out.cpu().numpy().reshape(B, seq, hq, D)
+        for b in range(B):
+            n = n_np[b]
+            assert (got[b, n:] == 7).all(), "a row behind the sequence was written"
+            assert np.isfinite(got[b, :n]).all()
+            # the borders of row tiles and blocks, and some between
+            at = {0, 1, n - 1, n // 2, *(x // (hq // hkv) + d for x in (127, 255, 511, 1023, 2047) for d in (0, 1))}
+            for i in sorted(x for x in at if 0 <= x < n)[:: 1 if B < 10 else 3]:
+                T.close(got[b, i], *T.attend(q[b, i], *c.rows[b], s_np[b] + i + 1, 2.0 ** -32, 16),
+                        f"sequence {b}, query {i}, {n_splits} splits")
