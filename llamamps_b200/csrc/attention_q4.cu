@@ -797,7 +797,8 @@ int check_attention(int n_pages, int max_pages, int page_size, int n_q_heads, in
   LMPS_CHECK_ARG(max_seq_len <= static_cast<long long>(max_pages) * page_size);
   LMPS_CHECK_ARG(n_kv_heads >= 1 && n_q_heads >= 1 && n_q_heads % n_kv_heads == 0 && n_q_heads <= 65535);
   LMPS_CHECK_ARG(n_splits >= 1 && n_splits <= 1024);
-  if (head_dim != kDim || page_size % kRun != 0 || n_q_heads / n_kv_heads > kMaxHeads) return LMPS_ERR_UNSUPPORTED;
+  if (head_dim != kDim || page_size % kRun != 0 || page_size > kMaxPage || n_q_heads / n_kv_heads > kMaxHeads)
+    return LMPS_ERR_UNSUPPORTED;
   return LMPS_OK;
 }
 

@@ -176,7 +176,7 @@ extern "C" int lmps_rope_kv_append_q4(const uint16_t* qkv, const int32_t* pos, c
   LMPS_CHECK_ARG(rows >= 1 && n_pages >= 1 && max_pages >= 1 && page_size >= 1 && n_q_heads >= 1 && n_kv_heads >= 1);
   LMPS_CHECK_ARG(static_cast<long long>(max_pages) * page_size <= 1LL << 29);
   LMPS_CHECK_ARG(style == LMPS_ROPE_INTERLEAVED || style == LMPS_ROPE_NEOX);
-  if (head_dim != q4::kDim || page_size % q4::kRun != 0) return LMPS_ERR_UNSUPPORTED;
+  if (head_dim != q4::kDim || page_size % q4::kRun != 0 || page_size > q4::kMaxPage) return LMPS_ERR_UNSUPPORTED;
   LMPS_CHECK_ARG(lmps_aligned(qkv, 16) && lmps_aligned(q_out, 16) && lmps_aligned(k_out, 16) &&
                  lmps_aligned(v_out, 16) && lmps_aligned(k_pool, 16) && lmps_aligned(v_pool, 16));
   q4::AppendParams P{};

@@ -28,6 +28,7 @@ constexpr int kGroups = 4;      // scales per row
 constexpr int kCodeBytes = 64;  // code bytes per row
 constexpr int kRowBytes = 72;   // code bytes + 4 fp16 scales
 constexpr int kRun = 16;        // positions per contiguous run (page_size is a multiple)
+constexpr int kMaxPage = 1 << 24;  // offsets inside a (page, head) block are 32 bits: 72 * 2^24 < 2^31
 
 // Bits of the int32 error word that the 4-bit cache's kernels raise.
 constexpr int kErrTimeout = LMPS_Q4_ERR_TIMEOUT;
