@@ -642,10 +642,7 @@ class QwenEngine:
         bits = int(self.kv_err.item())
         if bits:
             self.kv_err.zero_()
-            names = [n for b, n in ((K.Q4_ERR_TIMEOUT, "a wait for the tensor core timed out"),
-                                    (K.Q4_ERR_PAGE, "a block table entry outside the pool"),
-                                    (K.Q4_ERR_POSITION, "a position outside the cache")) if bits & b]
-            raise RuntimeError("4-bit KV cache: " + ", ".join(names))
+            K.raise_q4_error(bits)
 
     def generate(self, token_ids: Sequence[int], max_new_tokens: int, temperature: float = 0.0, top_k: int = 0,
                  seed: int = 0) -> List[int]:

@@ -307,6 +307,15 @@ Q4_ERR_TIMEOUT, Q4_ERR_PAGE, Q4_ERR_POSITION = 1, 2, 4
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 
 
+def raise_q4_error(bits: int) -> None:
+    """RuntimeError for the Q4_ERR_* bits of a 4-bit cache kernel's error word (none: no error)."""
+    if bits:
+        names = [n for b, n in ((Q4_ERR_TIMEOUT, "a wait for the tensor core timed out"),
+                                (Q4_ERR_PAGE, "a block table entry outside the pool"),
+                                (Q4_ERR_POSITION, "a position outside the cache")) if bits & b]
+        raise RuntimeError("4-bit KV cache: " + ", ".join(names))
+
+
 def _q4_explain(dev: int, named) -> None:
     """Raises for the first of (name, tensor, dtype, elements) that is not on
     device ``dev`` (the first argument's), of this type, contiguous and of
@@ -476,9 +485,18 @@ def prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch: int, seq_le
     b * seq_len + i of ``q`` is the query at position ``starts[b] + i`` (0 + i
     without ``starts``) for i < ``q_lens[b]`` (seq_len without); other rows of
     ``out`` stay as they were.  The K and V of all these positions are already
-    in the cache; starts + q_lens <= ``max_seq_len``."""
+    in the cache; starts + q_lens <= ``max_seq_len``.  Without ``error`` the
+    call waits for the kernel and raises what it reports (so a graph capture
+    needs one)."""
     if error is None and q.is_cuda:
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("error: a captured prefill_attention_q4 needs an int32 error word")
         error = torch.zeros(1, dtype=_I32, device=q.device)
+        prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch, seq_len, page_size, n_q_heads, n_kv_heads,
+                             head_dim, max_seq_len, starts=starts, q_lens=q_lens, workspace=workspace,
+                             n_splits=n_splits, error=error)
+        raise_q4_error(int(error.item()))
+        return out
     if _q4_done(binding().prefill(q, k_pool, v_pool, block_table, out, batch, seq_len, page_size, n_q_heads, n_kv_heads,
                                   head_dim, max_seq_len, starts, q_lens, workspace, n_splits, error),
                 "lmps_prefill_attention_q4"):
