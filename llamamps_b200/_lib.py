@@ -116,21 +116,43 @@ def lib() -> ctypes.CDLL:
 _BIND = None
 
 
+class _Unbound:
+    """In the extension's place: leaves every call to the ctypes path."""
+
+    @staticmethod
+    def _leave(*args):
+        return None
+
+    append = decode = step = prefill = _leave
+
+
 def binding():
     """The Python extension of the 4-bit KV cache's eager calls (csrc/bind_q4.cpp), over the entry points of
-    :func:`lib`."""
+    :func:`lib`.  It reads tensors of the torch that it was built against; with another one, or if it does not
+    load, a warning says so once and the calls go through ctypes."""
     global _BIND
     if _BIND is None:
         import importlib.machinery
         import importlib.util
+        import warnings
 
-        import torch  # noqa: F401  (its libraries resolve the extension's symbols)
+        import torch  # (its libraries resolve the extension's symbols)
         if not os.path.exists(BIND_PATH):
             raise RuntimeError(f"{BIND_PATH} is missing: build it with `python -m llamamps_b200.build`")
         loader = importlib.machinery.ExtensionFileLoader("bind_q4", BIND_PATH)
-        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("bind_q4", loader))
-        loader.exec_module(mod)
+        try:
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("bind_q4", loader))
+            loader.exec_module(mod)
+            built = getattr(mod, "torch_version", "of some other version")
+            why = None if built == torch.__version__ else f"it was built against torch {built}"
+        except ImportError as e:
+            why = str(e)
         L = lib()
+        if why is not None:
+            warnings.warn(f"{BIND_PATH} is left out ({why}): 4-bit cache calls take some 6 us longer on the host; "
+                          "rebuild it with `python -m llamamps_b200.build`", RuntimeWarning, stacklevel=3)
+            _BIND = _Unbound
+            return _BIND
         mod.bind(*(ctypes.cast(getattr(L, n), c_vp).value for n in (
             "lmps_rope_kv_append_q4", "lmps_gqa_decode_attention_q4", "lmps_gqa_decode_attention_rope_q4",
             "lmps_prefill_attention_q4")))

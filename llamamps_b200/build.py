@@ -80,7 +80,8 @@ def build_binding(force: bool = False) -> str:
     from torch.utils.cpp_extension import include_paths
     src = os.path.join(CSRC, "bind_q4.cpp")
     flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             f'-DLMPS_TORCH_VERSION="{torch.__version__}"']
     stamp = os.path.join(LIBDIR, ".bind_stamp")
     digest = _digest([src, os.path.join(INCLUDE, "llamamps_b200.h")],
                      " ".join(flags) + torch.__version__ + sys.version)

@@ -238,4 +238,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "bind_q4", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_bind_q4() { return PyModule_Create(&module); }
+// torch_version: the torch it was built against, whose tensors alone it can read.
+PyMODINIT_FUNC PyInit_bind_q4() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", LMPS_TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
