@@ -594,8 +594,9 @@ __device__ __forceinline__ unsigned long long mul_div(unsigned long long a, unsi
 // may take in the end of a row and the start of the next, a segment each.  `head` units in front of each row
 // stand for what starting another segment costs: under load a chain of three memory accesses, which other shares
 // hide only where every SM has many of them to do.  So with kManyShares shares or more to a row a head is one
-// unit longer than a share, and none takes in two rows (fresh caches: 8 x 20000..30000 24.5 us, 29 with short
-// heads; 32 x 1..16000 25.6 and 24.2).  Segment (CTA i, row r) has slot i + r.
+// unit longer than a share of the rows without heads.  The heads make a share longer by `head` times the rows to a
+// share, an eighth at most, so few shares take in two rows: of 54 x 8000..16000 on one KV head 1 of 444 (fresh
+// caches: 8 x 20000..30000 24.5 us, 29 with short heads; 32 x 1..16000 25.6 and 24.2).  Segment (CTA i, row r) has slot i + r.
 __global__ void __launch_bounds__(kPieceWarps * kWarp, kPieceCtas) attn_q4_pieces_kernel(const AttnParams P) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
