@@ -275,9 +275,9 @@ int lmps_sample_rows(const uint16_t* logits, int ld, int rows, int n, int top_k,
  * NaN to the queries that attend to its position, and to no others.
  *
  * head_dim 128, page_size a multiple of 16 and at most 2^24, at most 8 query
- * heads per KV head (else UNSUPPORTED), max_pages * page_size <= 2^29; pools, q, qkv, outputs
- * and workspace 16-byte aligned; calls that may overlap on the GPU need
- * workspaces of their own.  error (int32, may be NULL where not said
+ * heads per KV head (else UNSUPPORTED), max_pages * page_size <= 2^29; pools,
+ * q, qkv, outputs and workspace 16-byte aligned; calls that may overlap on the
+ * GPU need workspaces of their own.  error (int32, may be NULL where not said
  * otherwise) collects LMPS_Q4_ERR_* bits: a page number outside [0, n_pages)
  * is neither read nor written (its positions count as absent), a position
  * outside the cache likewise.  Zero it before the first call and after

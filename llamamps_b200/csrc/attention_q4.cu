@@ -36,15 +36,15 @@
 // warps' states meet.  16-byte chunk c of a staged row r is stored at
 // c ^ ((r >> 1) & 3): both fragment reads are then free of bank conflicts.
 //
-// What bounds it.  A step of 32 positions is 4.6 KB and some 750 instructions a
+// What bounds it.  A step of 32 positions is 4.6 KB and some 740 instructions a
 // warp (unpacking, scales, the softmax): with 12 warps an SM goes through its
-// steps at 4.5 TB/s over the GPU, 0.7 of the measured copy rate, issue slots
-// (54 % used) and memory latency about even.  What is left is around them: 4 us of an empty
+// steps at 4.4 TB/s over the GPU, 0.7 of the measured copy rate, issue slots
+// (55 % used) and memory latency about even.  What is left is around them: 4 us of an empty
 // call (launch, page table, first loads, meeting of the warps) and 3 us of the
-// second kernel.  Measured (12 query, 2 KV heads, caches not in L2): 1 x 131
-// 3.9 us; 64 x 1..1000 11.0; 4 x 32768 18.9 (2.0 TB/s); 64 x 4100..8200 35.8
-// (3.1 TB/s); with RoPE and append 1 x 2049 7.3, 64 x 500..2100 on 6 heads
-// 12.1.  Tried without gain: a third stage, 16 warps of 128 registers, codes
+// second kernel.  Measured (12 query, 2 KV heads, a stream of calls on a few
+// caches): 1 x 131 4.2 us; 64 x 1..1000 9.8; 4 x 32768 19.1 (2.0 TB/s);
+// 64 x 4100..8200 35.4 (3.1 TB/s; on caches that are never in L2 36.2); with
+// RoPE and append 1 x 2049 8.0, 64 x 500..2100 on 6 heads 11.5.  Tried without gain: a third stage, 16 warps of 128 registers, codes
 // left as fp16 subnormals (a third fewer unpacking instructions, but the offset
 // then goes into the sums in fp32).
 #include <algorithm>
@@ -57,7 +57,7 @@ namespace lmps {
 namespace q4 {
 
 // Warps per CTA.  A step takes a lone warp 1.4 us, so short rows want many warps at once: 8, one CTA to an SM
-// (1 x 131: 4.0 us, with 4 warps 4.6).  Pieces, and rows of which there are more than SMs, have 4, three CTAs to
+// (1 x 131: with 4 warps 0.6 us longer).  Pieces, and rows of which there are more than SMs, have 4, three CTAs to
 // an SM.  The 12 warps may have 168 registers each; 16 of 128 take longer (64 x 1..1000 in one CTA a row: 12.6 us
 // against 9.3).
 constexpr int kShortWarps = 8, kPieceWarps = 4;

@@ -5,8 +5,8 @@
 // a cosine to compute): the rows' 64 (cos, sin) pairs once in fp64, q in units
 // of 16 bytes a thread, then a warp per two K or V rows (8 elements a lane).
 //
-// One row is launch and latency (3.4 us, as are 64).  A prompt of 8 x 2048 rows
-// (12 query, 2 KV heads: 139 MB) takes 29.6 us = 4.7 TB/s, 0.72 of the measured
+// One row is launch and latency (3.3 us, as are 64).  A prompt of 8 x 2048 rows
+// (12 query, 2 KV heads: 139 MB) takes 29.9 us = 4.6 TB/s, 0.71 of the measured
 // copy rate; its instructions are the rotations and the quantiser, whose
 // maximum and scale a row's 16 lanes share (32 lanes of 4 elements: 33.0 us).
 // K is rotated in fp64 so that the rounding to fp16, and with it every code, is

@@ -27,11 +27,11 @@
 // Every mbarrier wait is bounded (error bit, no hang).
 //
 // What bounds it: not the tensor core.  A 256 x 128 tile has 2048 cycles of
-// products and takes about 4100: the softmax of 64 keys is a chain of one TMEM
+// products and takes about 4200: the softmax of 64 keys is a chain of one TMEM
 // load, 64 exponentials a thread, conversions and a TMEM store, and the four
 // dequantising warps share its schedulers.  Measured (12 query, 2 KV heads):
-// 8 x 2048 causal 151 us = 682 TFLOP/s, 0.41 of the bf16 peak measured by a
-// library product; 4 x 256 queries behind 1..30000 positions 80 us; one
+// 8 x 2048 causal 155 us = 665 TFLOP/s, 0.40 of the bf16 peak measured by a
+// library product; 4 x 256 queries behind 1..30000 positions 81 us; one
 // prompt of 37 tokens 8 us.  Tried without gain: exponentials by polynomial on
 // the FMA units for a part of a row, the two softmax groups held half a step
 // apart, the next unit's queries fetched during the epilogue (64 registers, spilled).
