@@ -410,6 +410,38 @@ int lmps_tp2_argmax_exchange(const uint16_t* logits, int ld, const int32_t* loca
                              int32_t* ids, void* comm, void* peer_comm, uint32_t* seen, int site, int n_sites,
                              int max_n, int32_t* error, unsigned long long wait_ns, void* stream);
 
+/* ---- 8-bit linear layers -------------------------------------------------
+ * A row of k fp16 elements in 8 bits: k int8 codes in [-127, 127] and one fp32
+ * scale, codes = rint(127 v / max|v|) of the exact elements v, scale = max|v| /
+ * 127.  A zero row has codes and scale 0; a row with a NaN or an infinity has
+ * codes 0 and scale NaN, so that what is computed from it is NaN.  All
+ * matrices have a row stride in elements (ldx, ldc, ...) of at least their
+ * row's length; elements between rows are neither read nor written. */
+
+/* Quantise rows of x [rows, k].  values (fp16, or NULL) receives code * scale. */
+int lmps_quantise_rows_q8(const uint16_t* x, int ldx, int8_t* codes, int ldc, float* scales, uint16_t* values,
+                          int ldv, int rows, int k, void* stream);
+
+/* RMSNorm (kernels/rms_norm.metal:20-39, over the full vector) of x, or with
+ * residual of fp16(residual + x), written to sum (both or neither; sum may be
+ * residual or x with the same stride), times gamma, quantised as above without
+ * a rounding to fp16 in between. */
+int lmps_rms_norm_q8(const uint16_t* x, int ldx, const uint16_t* residual, int ldr, uint16_t* sum, int lds,
+                     const uint16_t* gamma, float eps, int8_t* codes, int ldc, float* scales, uint16_t* values,
+                     int ldv, int rows, int k, void* stream);
+
+/* y[t][c] = fp16(x_scales[t] w_scales[c] sum_k x[t][k] w[c][k] + bias[c] +
+ * residual[t][c]), x [m, k] and w [n, k] int8 (any codes, -128 too), the sum
+ * exact in 32 bits, the rest fp32 and rounded once; bias and residual may be
+ * NULL, y may be residual with the same stride.  swiglu = 1: w and w_scales
+ * have 2n rows, gate row c and up row n + c, and y[t][c] = fp16(silu(gate) *
+ * up) of the scaled sums (no bias or residual).  x and w start at, and their
+ * strides are, multiples of 16 bytes; k <= 131071.  error is set to 1 when a
+ * bounded wait on the device gave up (then y is not complete). */
+int lmps_w8a8_gemm(const int8_t* x, int ldx, const float* x_scales, const int8_t* w, int ldw,
+                   const float* w_scales, const uint16_t* bias, const uint16_t* residual, int ldr, uint16_t* y,
+                   int ldy, int m, int n, int k, int swiglu, int32_t* error, void* stream);
+
 /* ---- weight format ---------------------------------------------------- */
 
 /* Device Q4 packer, bit-exact with utils/pack_weights.py:18-46

@@ -14,7 +14,7 @@ import os
 import re
 from typing import List
 
-from .build import BIND_PATH, INCLUDE, LIB_PATH
+from .build import BIND_PATH, BIND_Q8_PATH, INCLUDE, LIB_PATH
 
 c_int, c_float, c_ll, c_size = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_size_t
 c_vp = ctypes.c_void_p
@@ -81,6 +81,11 @@ _SIGS = {
     "lmps_prefill_q4_workspace_size": (c_size, [c_int] * 5),
     "lmps_prefill_attention_q4": (c_int, [c_vp] * 3 + [c_int] + [c_vp] * 5 + [c_size] + [c_int] * 9
                                   + [c_vp, c_vp]),
+    "lmps_quantise_rows_q8": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_int, c_int, c_int, c_vp]),
+    "lmps_rms_norm_q8": (c_int, [c_vp, c_int, c_vp, c_int, c_vp, c_int, c_vp, c_float, c_vp, c_int, c_vp, c_vp,
+                                 c_int, c_int, c_int, c_vp]),
+    "lmps_w8a8_gemm": (c_int, [c_vp, c_int, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int,
+                               c_int, c_int, c_vp, c_vp]),
     "lmps_w4a16_gemm_workspace_size": (c_size, [c_int, c_int]),
     "lmps_w4a16_gemm": (c_int, [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_int,
                                 c_int, c_vp, c_vp, c_size, c_vp]),
@@ -114,6 +119,7 @@ def lib() -> ctypes.CDLL:
 
 
 _BIND = None
+_BIND_Q8 = None
 
 
 class _Unbound:
@@ -123,41 +129,54 @@ class _Unbound:
     def _leave(*args):
         return None
 
-    append = decode = step = prefill = _leave
+    append = decode = step = prefill = quantise = norm = gemm = _leave
+
+
+def _extension(path: str, name: str, calls: str, entries):
+    """The Python extension at ``path``, bound to these entry points of :func:`lib`.  It reads tensors of the
+    torch that it was built against; with another one, or if it does not load, a warning says so and
+    :class:`_Unbound` takes its place."""
+    import importlib.machinery
+    import importlib.util
+    import warnings
+
+    import torch  # (its libraries resolve the extension's symbols)
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python -m llamamps_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    try:
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+        loader.exec_module(mod)
+        built = getattr(mod, "torch_version", "of some other version")
+        why = None if built == torch.__version__ else f"it was built against torch {built}"
+    except ImportError as e:
+        why = str(e)
+    L = lib()
+    if why is not None:
+        warnings.warn(f"{path} is left out ({why}): {calls} calls take some 6 us longer on the host; "
+                      "rebuild it with `python -m llamamps_b200.build`", RuntimeWarning, stacklevel=4)
+        return _Unbound
+    mod.bind(*(ctypes.cast(getattr(L, n), c_vp).value for n in entries))
+    return mod
 
 
 def binding():
-    """The Python extension of the 4-bit KV cache's eager calls (csrc/bind_q4.cpp), over the entry points of
-    :func:`lib`.  It reads tensors of the torch that it was built against; with another one, or if it does not
-    load, a warning says so once and the calls go through ctypes."""
+    """The extension of the 4-bit KV cache's eager calls (csrc/bind_q4.cpp)."""
     global _BIND
     if _BIND is None:
-        import importlib.machinery
-        import importlib.util
-        import warnings
-
-        import torch  # (its libraries resolve the extension's symbols)
-        if not os.path.exists(BIND_PATH):
-            raise RuntimeError(f"{BIND_PATH} is missing: build it with `python -m llamamps_b200.build`")
-        loader = importlib.machinery.ExtensionFileLoader("bind_q4", BIND_PATH)
-        try:
-            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("bind_q4", loader))
-            loader.exec_module(mod)
-            built = getattr(mod, "torch_version", "of some other version")
-            why = None if built == torch.__version__ else f"it was built against torch {built}"
-        except ImportError as e:
-            why = str(e)
-        L = lib()
-        if why is not None:
-            warnings.warn(f"{BIND_PATH} is left out ({why}): 4-bit cache calls take some 6 us longer on the host; "
-                          "rebuild it with `python -m llamamps_b200.build`", RuntimeWarning, stacklevel=3)
-            _BIND = _Unbound
-            return _BIND
-        mod.bind(*(ctypes.cast(getattr(L, n), c_vp).value for n in (
+        _BIND = _extension(BIND_PATH, "bind_q4", "4-bit cache", (
             "lmps_rope_kv_append_q4", "lmps_gqa_decode_attention_q4", "lmps_gqa_decode_attention_rope_q4",
-            "lmps_prefill_attention_q4")))
-        _BIND = mod
+            "lmps_prefill_attention_q4"))
     return _BIND
+
+
+def binding_q8():
+    """The extension of the 8-bit linear layers' eager calls (csrc/bind_q8.cpp)."""
+    global _BIND_Q8
+    if _BIND_Q8 is None:
+        _BIND_Q8 = _extension(BIND_Q8_PATH, "bind_q8", "8-bit linear layer", (
+            "lmps_quantise_rows_q8", "lmps_rms_norm_q8", "lmps_w8a8_gemm"))
+    return _BIND_Q8
 
 
 def status_string(status: int) -> str:

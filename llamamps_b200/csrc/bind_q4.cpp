@@ -8,13 +8,7 @@
 // argument that is not a tensor -- which kernels.py then diagnoses.
 //
 // bind(addresses) takes the entry points' addresses in the order of Entry.
-#define PY_SSIZE_T_CLEAN
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAStream.h>
-
-#include "../../include/llamamps_b200.h"
+#include "bind_args.h"
 
 namespace {
 
@@ -24,57 +18,6 @@ struct Entry {
   decltype(&lmps_gqa_decode_attention_rope_q4) step;
   decltype(&lmps_prefill_attention_q4) prefill;
 } entry;
-
-constexpr auto kHalf = at::kHalf, kFloat = at::kFloat, kInt = at::kInt, kByte = at::kByte;
-
-// The arguments of one call; ok turns false at the first that does not fit.
-struct Args {
-  PyObject* const* a;
-  bool ok;
-  int dev = -1;
-
-  Args(PyObject* const* args, Py_ssize_t n, Py_ssize_t want) : a(args), ok(n == want) {}
-
-  const at::Tensor* tensor(int i) {
-    if (!ok || !THPVariable_Check(a[i])) {
-      ok = false;
-      return nullptr;
-    }
-    return &THPVariable_Unpack(a[i]);
-  }
-  // Address of argument i: this type, on the call's device (the first one sets it: the current one),
-  // contiguous, exactly n elements (at least -n for n < 0).
-  void* data(int i, at::ScalarType type, int64_t n) {
-    const at::Tensor* t = tensor(i);
-    if (!t) return nullptr;
-    const int64_t m = t->numel();
-    ok = t->scalar_type() == type && t->is_cuda() && t->is_contiguous() && (n >= 0 ? m == n : m >= -n);
-    if (!ok) return nullptr;
-    if (dev < 0) dev = t->get_device();
-    ok = t->get_device() == dev;
-    return ok ? t->data_ptr() : nullptr;
-  }
-  void* optional(int i, at::ScalarType type, int64_t n) { return ok && a[i] == Py_None ? nullptr : data(i, type, n); }
-  int number(int i) {
-    if (!ok) return 0;
-    int overflow = 0;
-    const long long v = PyLong_Check(a[i]) ? PyLong_AsLongLongAndOverflow(a[i], &overflow) : (ok = false, 0);
-    if (overflow || v != static_cast<int>(v)) ok = false;
-    return static_cast<int>(v);
-  }
-  int64_t rows(int i) {
-    const at::Tensor* t = tensor(i);
-    if (!t || t->dim() < 1 || t->size(0) > 0x7FFFFFFF) {
-      ok = false;
-      return 0;
-    }
-    return t->size(0);
-  }
-  // Element counts stay in 64 bits with these (others are refused by the entry points, through ctypes).
-  void heads(int n_q, int n_kv, int head_dim) {
-    ok = ok && n_q >= 1 && n_q <= 65535 && n_kv >= 1 && n_kv <= 65535 && head_dim == 128;
-  }
-};
 
 // One layer's pools at arguments i, i + 1 and the block table at i + 2.
 struct Pools {
@@ -108,30 +51,6 @@ struct Workspace {
     n = static_cast<size_t>(t->numel());
   }
 };
-
-uint16_t* half(void* p) { return static_cast<uint16_t*>(p); }
-
-// Calls on the current stream where the tensors are on the current device.
-template <class Call>
-PyObject* run(Args& A, Call call) {
-  if (!A.ok || A.dev != c10::cuda::current_device()) Py_RETURN_NONE;
-  void* stream = c10::cuda::getCurrentCUDAStream(A.dev).stream();
-  int status;
-  Py_BEGIN_ALLOW_THREADS;
-  status = call(stream);
-  Py_END_ALLOW_THREADS;
-  return PyLong_FromLong(status);
-}
-
-template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
-PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  try {
-    return F(args, n);
-  } catch (...) {  // (a tensor without storage, and the like)
-    PyErr_Clear();
-    Py_RETURN_NONE;
-  }
-}
 
 // qkv, pos, inv_freq, q_out, k_pool, v_pool, block_table, page_size, n_q, n_kv, head_dim, style, k_out, v_out, error
 PyObject* append(PyObject* const* args, Py_ssize_t n) {
@@ -224,11 +143,6 @@ PyObject* bind(PyObject*, PyObject* args) {
   entry.step = reinterpret_cast<decltype(entry.step)>(c);
   entry.prefill = reinterpret_cast<decltype(entry.prefill)>(d);
   Py_RETURN_NONE;
-}
-
-template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
-PyMethodDef method(const char* name) {
-  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<F>)), METH_FASTCALL, nullptr};
 }
 
 PyMethodDef methods[] = {method<append>("append"),   method<decode>("decode"), method<step>("step"),

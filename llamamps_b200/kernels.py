@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import binding, call, check, lib
+from ._lib import binding, binding_q8, call, check, lib
 
 FP16 = torch.float16
 
@@ -511,6 +511,154 @@ def prefill_attention_q4(q, k_pool, v_pool, block_table, out, batch: int, seq_le
              _q4_arg(q_lens, "q_lens", _I32, dev, -batch) if q_lens is not None else None,
              _q4_arg(out, "out", FP16, dev, n), ws, ws_bytes, max_pages, page_size, n_q_heads, n_kv_heads,
              head_dim, batch, seq_len, max_seq_len, n_splits, _q4_arg(error, "error", _I32, dev, -1))
+    return out
+
+
+# -- 8-bit linear layers -------------------------------------------------------
+_I8 = torch.int8
+
+
+def _q8_arg(t: torch.Tensor, name: str, dtype, dev: int, rows: int, k: int):
+    """Address and row stride of ``t`` as ``rows`` rows of ``k`` elements, or the error that says why it is none."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (the decode path has no CPU fallback)")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on another device than the call's other tensors")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != (rows, k) and not (rows == 1 and tuple(t.shape) == (k,)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{rows}, {k}]")
+    if k > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be side by side")
+    ld = t.stride(0) if rows > 1 else -(-k // 16) * 16
+    if ld < k:
+        raise ValueError(f"{name}: rows must not overlap (stride {ld} for {k} elements)")
+    return t.data_ptr(), ld
+
+
+def _q8_vector(t: torch.Tensor, name: str, dtype, dev: int, n: int) -> int:
+    if isinstance(t, torch.Tensor) and (t.numel() != n or not t.is_contiguous()):
+        raise ValueError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}")
+    return _q8_arg(t.reshape(-1) if isinstance(t, torch.Tensor) else t, name, dtype, dev, 1, n)[0]
+
+
+def _q8_shape(t: torch.Tensor, name: str):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if t.dim() not in (1, 2) or t.shape[-1] == 0:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [rows, k] or [k]")
+    return (1 if t.dim() == 1 else t.shape[0]), t.shape[-1]
+
+
+def _q8_codes(x: torch.Tensor, codes, scales):
+    """Codes (rows start at multiples of 16 bytes) and scales for x's rows where they are not given."""
+    rows, k = _q8_shape(x, "x")
+    if codes is None:
+        codes = torch.empty(rows, -(-k // 16) * 16, dtype=_I8, device=x.device)[:, :k]
+        codes = codes if x.dim() == 2 else codes[0]
+    if scales is None:
+        scales = torch.empty(rows, dtype=_F32, device=x.device)
+    return rows, k, codes, scales
+
+
+def quantise_rows_q8(x, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
+                     values: Optional[torch.Tensor] = None):
+    """Rows of fp16 ``x`` ([rows, k], or [k]; any row stride) as int8 codes in
+    [-127, 127] and one fp32 scale each, max|row| / 127: (codes, scales).  A
+    zero row has scale 0, a row with a NaN or an infinity scale NaN.  Without
+    ``codes``, the result's rows start at multiples of 16 bytes, as
+    :func:`w8a8_gemm` needs them.  ``values`` (fp16) receives code * scale."""
+    rows, k, codes, scales = _q8_codes(x, codes, scales)
+    if _q4_done(binding_q8().quantise(x, codes, scales, values), "lmps_quantise_rows_q8"):
+        return codes, scales
+    dev = x.get_device()
+    a_x, ldx = _q8_arg(x, "x", FP16, dev, rows, k)
+    a_c, ldc = _q8_arg(codes, "codes", _I8, dev, rows, k)
+    a_v, ldv = _q8_arg(values, "values", FP16, dev, rows, k) if values is not None else (None, 0)
+    a_s = _q8_vector(scales, "scales", _F32, dev, rows)
+    if rows:
+        _q4_call("lmps_quantise_rows_q8", dev, a_x, ldx, a_c, ldc, a_s, a_v, ldv, rows, k)
+    return codes, scales
+
+
+def rms_norm_q8(x, gamma, eps: float = 1e-6, *, residual: Optional[torch.Tensor] = None,
+                sum_out: Optional[torch.Tensor] = None, codes: Optional[torch.Tensor] = None,
+                scales: Optional[torch.Tensor] = None, values: Optional[torch.Tensor] = None):
+    """:func:`rms_norm` with its output in 8 bits, as :func:`quantise_rows_q8`
+    gives it (of the unrounded norm): (codes, scales).  With ``residual`` the
+    norm is of s = fp16(residual + x), which ``sum_out`` receives: (codes,
+    scales, sum).  ``sum_out`` may be ``residual`` or ``x`` itself."""
+    rows, k, codes, scales = _q8_codes(x, codes, scales)
+    eps = float(eps)
+    if residual is None and sum_out is not None:
+        raise ValueError("sum_out: only with a residual")
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    done = (codes, scales) if residual is None else (codes, scales, sum_out)
+    if _q4_done(binding_q8().norm(x, gamma, eps, residual, sum_out, codes, scales, values), "lmps_rms_norm_q8"):
+        return done
+    dev = x.get_device()
+    a_x, ldx = _q8_arg(x, "x", FP16, dev, rows, k)
+    a_g = _q8_vector(gamma, "gamma", FP16, dev, k)
+    a_r, ldr = _q8_arg(residual, "residual", FP16, dev, rows, k) if residual is not None else (None, 0)
+    a_o, lds = _q8_arg(sum_out, "sum_out", FP16, dev, rows, k) if residual is not None else (None, 0)
+    a_c, ldc = _q8_arg(codes, "codes", _I8, dev, rows, k)
+    a_v, ldv = _q8_arg(values, "values", FP16, dev, rows, k) if values is not None else (None, 0)
+    a_s = _q8_vector(scales, "scales", _F32, dev, rows)
+    if rows:
+        _q4_call("lmps_rms_norm_q8", dev, a_x, ldx, a_r, ldr, a_o, lds, a_g, eps, a_c, ldc, a_s, a_v, ldv, rows, k)
+    return done
+
+
+def w8a8_gemm(codes, scales, w_codes, w_scales, *, bias: Optional[torch.Tensor] = None,
+              residual: Optional[torch.Tensor] = None, swiglu: bool = False, out: Optional[torch.Tensor] = None,
+              error: Optional[torch.Tensor] = None):
+    """out[t] = scales[t] * w_scales * (w_codes . codes[t]) (+ bias) (+ residual[t]),
+    rounded to fp16 once: int8 rows ([m, k], or [k]) with a scale for each
+    token, weights [n, k] with a scale for each channel (both as
+    :func:`quantise_rows_q8` makes them: rows at multiples of 16 bytes, k up to
+    131071).  ``swiglu``: the n gate rows of ``w_codes`` are followed by n up
+    rows, out[t] = silu(gate) * up, without bias or residual.  ``out`` may be
+    ``residual``.  ``error`` (int32 [1]) is set to 1 if a wait on the device ran
+    out; without it the call waits for the kernel and raises that (so a graph
+    capture needs one)."""
+    gated = 1 if swiglu else 0
+    m, k = _q8_shape(codes, "codes")
+    w_rows, _ = _q8_shape(w_codes, "w_codes")
+    if gated and w_rows % 2:
+        raise ValueError(f"w_codes: {w_rows} rows, expected as many gate rows as up rows")
+    if gated and (bias is not None or residual is not None):
+        raise ValueError("the SwiGLU epilogue takes no bias or residual")
+    n = w_rows // 2 if gated else w_rows
+    if out is None:
+        out = torch.empty((m, n) if codes.dim() == 2 else (n,), dtype=FP16, device=codes.device)
+    if error is None and codes.is_cuda:
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("error: a captured w8a8_gemm needs an int32 error word")
+        error = torch.zeros(1, dtype=_I32, device=codes.device)
+        w8a8_gemm(codes, scales, w_codes, w_scales, bias=bias, residual=residual, swiglu=swiglu, out=out, error=error)
+        if int(error.item()):
+            raise RuntimeError("w8a8_gemm: a wait for the tensor core timed out")
+        return out
+    if _q4_done(binding_q8().gemm(codes, scales, w_codes, w_scales, bias, residual, gated, out, error),
+                "lmps_w8a8_gemm"):
+        return out
+    dev = codes.get_device()
+    a_x, ldx = _q8_arg(codes, "codes", _I8, dev, m, k)
+    a_w, ldw = _q8_arg(w_codes, "w_codes", _I8, dev, w_rows, k)
+    a_xs = _q8_vector(scales, "scales", _F32, dev, m)
+    a_ws = _q8_vector(w_scales, "w_scales", _F32, dev, w_rows)
+    a_b = _q8_vector(bias, "bias", FP16, dev, n) if bias is not None else None
+    a_r, ldr = _q8_arg(residual, "residual", FP16, dev, m, n) if residual is not None else (None, 0)
+    a_y, ldy = _q8_arg(out, "out", FP16, dev, m, n)
+    a_e = _q8_vector(error, "error", _I32, dev, error.numel() if isinstance(error, torch.Tensor) else 1)
+    for name, at, ld in (("codes", a_x, ldx), ("w_codes", a_w, ldw)):
+        if at % 16 or ld % 16:
+            raise ValueError(f"{name}: rows must start at multiples of 16 bytes")
+    if m and n:
+        _q4_call("lmps_w8a8_gemm", dev, a_x, ldx, a_xs, a_w, ldw, a_ws, a_b, a_r, ldr, a_y, ldy, m, n, k, gated, a_e)
     return out
 
 
