@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kCta) rows_vec_kernel(const RowArgs A) {
       unpack8(s[i], f);
       if (gamma) {
         float g[8];
-        unpack8(__ldg(gamma + t + T * i), g);
+        unpack8(gamma[t + T * i], g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           ss = fmaf(f[e], f[e], ss);
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kCta) rows_vec_kernel(const RowArgs A) {
       unpack8(s[i], f);
       if (gamma) {
         float g[8];
-        unpack8(__ldg(gamma + t + T * i), g);
+        unpack8(gamma[t + T * i], g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= g[e];
       }

@@ -6,7 +6,7 @@
 //
 // The sum of up to 131071 products of codes fits 32 bits; everything after it
 // is fp32 and rounded once.  Three kernels, by the number of tokens:
-//   * gemv_kernel: dp4a, a warp per channel; the weights' bytes are all there is;
+//   * few_kernel: mma.sync on weights straight from global memory; their bytes are all there is;
 //   * split_kernel: tcgen05 with 128 weight rows as the MMA's M and the tokens
 //     as its N, K shared out over a thread-block cluster that adds the integer
 //     sums through distributed shared memory (any order gives the same);
@@ -33,64 +33,135 @@ struct Args {
   size_t ldr;
   __half* y;
   size_t ldy;
-  int m, n, k, swiglu;
+  int m, n, k;
 };
 
 // y[t][c] from the integer sum(s) and the scales.
 __device__ __forceinline__ float linear_value(int acc, float xs, float ws) { return static_cast<float>(acc) * xs * ws; }
 
-// A warp per output channel and four tokens, lanes over K, four products a
-// dp4a: for single tokens, where the weights' bytes are all there is.
-constexpr int kTokens = 4;
-constexpr int kGemvWarps = 4;
-
-template <bool GATED>
-__global__ void __launch_bounds__(kGemvWarps* kWarp) gemv_kernel(const Args A) {
-  lmps_pdl_trigger();
-  lmps_pdl_wait();
-  const int c = blockIdx.x * kGemvWarps + static_cast<int>(threadIdx.x / kWarp), lane = threadIdx.x % kWarp;
-  const int t0 = blockIdx.y * kTokens;
-  if (c >= A.n) return;
-  const int8_t* w0 = A.w + static_cast<size_t>(c) * A.ldw;
-  const int8_t* w1 = w0 + static_cast<size_t>(A.n) * A.ldw;
-  const int whole = A.k / 16;
-  int acc[2][kTokens] = {};
-  for (int j = lane; j < whole; j += kWarp) {
-    const int4 a = *reinterpret_cast<const int4*>(w0 + 16 * j);
-    const int4 b = GATED ? *reinterpret_cast<const int4*>(w1 + 16 * j) : make_int4(0, 0, 0, 0);
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      if (t0 + t >= A.m) break;
-      const int4 v = *reinterpret_cast<const int4*>(A.x + static_cast<size_t>(t0 + t) * A.ldx + 16 * j);
-      acc[0][t] = __dp4a(a.x, v.x, __dp4a(a.y, v.y, __dp4a(a.z, v.z, __dp4a(a.w, v.w, acc[0][t]))));
-      if (GATED) acc[1][t] = __dp4a(b.x, v.x, __dp4a(b.y, v.y, __dp4a(b.z, v.z, __dp4a(b.w, v.w, acc[1][t]))));
-    }
-  }
-  if (16 * whole + lane < A.k) {  // the last k % 16 elements
-    const int i = 16 * whole + lane;
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      if (t0 + t >= A.m) break;
-      const int v = A.x[static_cast<size_t>(t0 + t) * A.ldx + i];
-      acc[0][t] += w0[i] * v;
-      if (GATED) acc[1][t] += w1[i] * v;
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) {
-    if (t0 + t >= A.m) break;
-    const int a = __reduce_add_sync(0xffffffffu, acc[0][t]);
-    const int b = GATED ? __reduce_add_sync(0xffffffffu, acc[1][t]) : 0;
-    if (lane != 0) continue;
-    const size_t row = static_cast<size_t>(t0 + t);
-    float v = linear_value(a, A.xs[row], A.ws[c]);
-    if (GATED) v = silu_mul(v, linear_value(b, A.xs[row], A.ws[A.n + c]));
-    if (A.bias) v += __half2float(A.bias[c]);
-    if (A.residual) v += __half2float(A.residual[row * A.ldr + c]);
-    A.y[row * A.ldy + c] = __float2half_rn(v);
-  }
+__device__ __forceinline__ float silu_product(float g, float u) {
+  // e^-g past 2^126 makes the quotient 0, which fp16 makes of it anyway
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
+// --- few_kernel -----------------------------------------------------------------
+// A CTA per 16 channels (gated: 16 gate rows and their up rows) and all of up
+// to 8 NT tokens; its warps share K out in chunks of 64 codes and add their
+// sums through shared memory.  mma.sync with the weights as the 16 rows: the
+// order of k within a product is free as long as both operands have the same,
+// so lane l holds codes 16 (l % 4) .. of the chunk of its rows, 16 bytes of
+// global memory each, as they come; nothing is staged.
+__device__ __forceinline__ uint4 load_codes(const int8_t* p, int left) {  // 16 codes, those from `left` on zero
+  if (left >= 16) return *reinterpret_cast<const uint4*>(p);
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (left > 0) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+      if (i < left) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[i])) << (8 * (i % 4));
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+template <int NT, bool GATED, int WARPS>
+__global__ void __launch_bounds__(WARPS* kWarp) few_kernel(const Args A) {
+  constexpr int kRows = 16, kToks = 8 * NT, kW = GATED ? 2 : 1;
+  // chunks a warp has on their way: the more warps an SM holds the fewer (64 x 8960 gated rows, 8 warps a CTA: 7.1 us
+  // with one, 9.1 with two; 1536 x 8960, 32 warps: 5.3 with three, 6.6 with one)
+  constexpr int kAhead = WARPS == 32 ? (NT * kW == 1 ? 3 : 1) : 2 / kW;
+  constexpr int kPitch = kRows + 4;                                // (the four token pairs of a row: other banks)
+  __shared__ int red[WARPS][kW][kToks][kPitch];
+  lmps_pdl_trigger();
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  const int r = lane / 4, at = 16 * (lane % 4);
+  const int c0 = blockIdx.x * kRows, chunks = (A.k + 63) / 64;
+  const int8_t* w[kW][2];  // this lane's two weight rows (gated: and their up rows)
+  bool in[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = c0 + r + 8 * h;
+    in[h] = c < A.n;
+#pragma unroll
+    for (int z = 0; z < kW; ++z)
+      w[z][h] = A.w + static_cast<size_t>(z * A.n + (in[h] ? c : 0)) * A.ldw + at;
+  }
+  for (int i = warp; i < chunks; i += WARPS)  // the weights come nearer while the kernel before ends
+    if (64 * i + at < A.k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int z = 0; z < kW; ++z)
+          if (in[h]) prefetch_l2(w[z][h] + 64 * i);
+  lmps_pdl_wait();
+  int acc[kW][NT][4] = {};
+  for (int i0 = warp; i0 < chunks; i0 += kAhead * WARPS) {
+    uint4 wv[kAhead][kW][2], xv[kAhead][NT];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k0 = 64 * (i0 + j * WARPS), left = A.k - k0 - at;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int z = 0; z < kW; ++z) wv[j][z][h] = load_codes(w[z][h] + k0, in[h] ? left : 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        xv[j][t] = load_codes(A.x + static_cast<size_t>(8 * t + r) * A.ldx + at + k0, 8 * t + r < A.m ? left : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int z = 0; z < kW; ++z) {
+          const uint4 &lo = wv[j][z][0], &hi = wv[j][z][1], &x = xv[j][t];
+          mma_s8(acc[z][t], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+          mma_s8(acc[z][t], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+        }
+  }
+  // what the sums meet, on its way before they do: output o = 16 token + channel
+  constexpr int kOuts = kRows * kToks, kMine = (kOuts + WARPS * kWarp - 1) / (WARPS * kWarp);
+  float ws[kMine], wu[kMine], xs[kMine], add[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int o = static_cast<int>(threadIdx.x) + i * WARPS * kWarp, t = o / kRows, c = c0 + o % kRows;
+    const bool live = o < kOuts && t < A.m && c < A.n;
+    ws[i] = live ? A.ws[c] : 0.0f;
+    wu[i] = GATED && live ? A.ws[A.n + c] : 0.0f;
+    xs[i] = live ? A.xs[t] : 0.0f;
+    add[i] = live && A.bias ? __half2float(A.bias[c]) : 0.0f;
+    if (live && A.residual) add[i] += __half2float(A.residual[static_cast<size_t>(t) * A.ldr + c]);
+  }
+#pragma unroll
+  for (int z = 0; z < kW; ++z)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][z][8 * t + 2 * (lane % 4) + (e & 1)][r + 8 * (e >> 1)] = acc[z][t][e];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int o = static_cast<int>(threadIdx.x) + i * WARPS * kWarp, t = o / kRows, row = o % kRows;
+    if (o >= kOuts || t >= A.m || c0 + row >= A.n) continue;
+    int g = 0, u = 0;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      g += red[v][0][t][row];
+      if (GATED) u += red[v][kW - 1][t][row];
+    }
+    float v = linear_value(g, xs[i], ws[i]);
+    if (GATED) v = silu_product(v, linear_value(u, xs[i], wu[i]));
+    A.y[static_cast<size_t>(t) * A.ldy + c0 + row] = __float2half_rn(v + add[i]);
+  }
+}
 
 // ---------------------------------------------------------------------------
 // tcgen05: kind::i8, signed operands, 32-bit integer accumulators
@@ -149,6 +220,12 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -156,23 +233,42 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
                : "memory");
 }
 
+// 32 accumulator columns of this thread's TMEM lane on their way; tmem_arrived ends the wait for all such loads.
+__device__ __forceinline__ void tmem_start32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {  // (the operands keep uses behind the wait)
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 struct __align__(64) Params {
   CUtensorMap tx;  // codes [m, k], box 128 x (tokens of a CTA)
   CUtensorMap tw;  // weight codes [n or 2n, k], box 128 x (weight rows of a CTA's load)
-  CUtensorMap ty;  // y [m, n] fp16, box 64 x 32, 128-byte swizzle (pair_kernel, aligned y)
+  CUtensorMap ty;  // pair_kernel, aligned rows: y [m, n] fp16, box (64 or 32) x 32, swizzled by its row length
+  CUtensorMap tr;  // residual, the same
   Args a;
-  int tma_y;    // y goes out by TMA (ty is set)
+  int tma_y;    // y goes out, and the residual comes in, by TMA (ty and tr are set)
   int xrows;    // split_kernel: tokens of a tile
   int stages;   // split_kernel: K steps in flight
   int ksteps;   // split_kernel: K steps of each CTA of a cluster
   int tiles_n, tiles;  // pair_kernel: tiles along n, all tiles
   int* error;
 };
-
-__device__ __forceinline__ float silu_product(float g, float u) {
-  // e^-g past 2^126 makes the quotient 0, which fp16 makes of it anyway
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
-}
 
 // Shared-memory ring position (slot and the parity of its fill).
 struct Ring {
@@ -186,204 +282,7 @@ struct Ring {
   }
 };
 
-// --- split_kernel -------------------------------------------------------------
-// One tile of 128 weight rows (gated: 64 gate and their 64 up rows) and xrows
-// tokens a cluster; CTA z of the cluster multiplies K steps z * ksteps .. .
-//   warp 0 lane 0: TMA loads; warp 1 lane 0: MMAs; warps 2-5: sums out of TMEM.
-// The int32 partial sums go to the CTA that finishes their channels, [split]
-// [rows of the CTA][xrows + 4] in the (by then idle) ring.
-constexpr int kSplitThreads = 192;
-constexpr int kSplitStages = 8;  // at most
-constexpr int kWBytes = 128 * kBK;
-
-template <bool GATED>
-__global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_constant__ Params P) {
-  extern __shared__ unsigned char smem_raw[];
-  const Args& A = P.a;
-  const int S = P.stages, xbytes = P.xrows * kBK;
-  unsigned char* base = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char* wt = base;
-  unsigned char* xt = base + static_cast<size_t>(S) * kWBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(xt + static_cast<size_t>(S) * xbytes);
-  uint64_t* empty = full + kSplitStages;
-  uint64_t* done = empty + kSplitStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile int* abort_v = abort_flag;
-  constexpr int kOut = GATED ? 64 : 128;  // channels of a tile
-
-  lmps_pdl_trigger();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c0 = blockIdx.x * kOut, t0 = blockIdx.y * P.xrows;
-  const int splits = gridDim.z;
-  const int all = (A.k + kBK - 1) / kBK, kbeg = blockIdx.z * P.ksteps;
-  const int ksteps = max(0, min(P.ksteps, all - kbeg));
-  const uint32_t tcols = P.xrows <= 32 ? 32u : P.xrows <= 64 ? 64u : P.xrows <= 128 ? 128u : 256u;
-
-  if (tid == 0) {
-    for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    mbar_init(done, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(tcols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;
-
-  if (tid == 0) {
-    lmps_pdl_wait();  // both operands may be the previous kernel's output
-    Ring r;
-    int issued = 0;
-    for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
-      if (kt >= S && !mbar_wait(&empty[r.slot], r.phase ^ 1u, P.error, abort_v)) break;
-      mbar_expect_tx(&full[r.slot], static_cast<uint32_t>(kWBytes + xbytes));
-      unsigned char* w = wt + static_cast<size_t>(r.slot) * kWBytes;
-      const int kx = (kbeg + kt) * kBK;
-      if (GATED) {
-        tma_load_2d(w, &P.tw, kx, c0, &full[r.slot]);
-        tma_load_2d(w + kWBytes / 2, &P.tw, kx, A.n + c0, &full[r.slot]);
-      } else {
-        tma_load_2d(w, &P.tw, kx, c0, &full[r.slot]);
-      }
-      tma_load_2d(xt + static_cast<size_t>(r.slot) * xbytes, &P.tx, kx, t0, &full[r.slot]);
-      issued = kt + 1;
-    }
-    for (int kt = max(0, issued - S); kt < issued; ++kt) {  // every issued copy lands before the ring is reused
-      const uint64_t since = globaltimer();
-      while (!mbar_try(&full[kt % S], (kt / S) & 1))
-        if (globaltimer() - since > kTimeoutNs) break;
-    }
-  } else if (warp == 1 && lane == 0) {
-    lmps_pdl_wait();  // (bounded waits begin when the work does)
-    const uint32_t idesc = idesc_i8(128, P.xrows);
-    Ring r;
-    for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
-      if (!mbar_wait(&full[r.slot], r.phase, P.error, abort_v)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t wd = sw128_desc(smem_u32(wt + static_cast<size_t>(r.slot) * kWBytes));
-      const uint64_t xd = sw128_desc(smem_u32(xt + static_cast<size_t>(r.slot) * xbytes));
-#pragma unroll
-      for (int j = 0; j < kBK / 32; ++j)  // K = 32 a MMA: 32 bytes further into the swizzle row
-        mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u);
-      mma_commit(&empty[r.slot]);
-    }
-    mma_commit(done);
-    const uint64_t since = globaltimer();  // the tensor memory and the ring are free once these finish
-    while (!mbar_try(done, 0u))
-      if (globaltimer() - since > kTimeoutNs) break;
-  }
-  __syncwarp();
-  lmps_pdl_wait();  // before any read of scales and residual, or write of y
-  const bool epi = warp >= 2;
-  bool ok = false;
-  if (epi) {
-    ok = mbar_wait(done, 0, P.error, abort_v) && ksteps > 0 && *abort_v == 0;
-    ok = __all_sync(0xffffffffu, ok);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  }
-  // Every CTA of the cluster is past its products: the rings may receive sums.
-  __syncthreads();
-  if (splits > 1) cluster_sync();
-  int* red = reinterpret_cast<int*>(base);
-  const int rs = P.xrows + 4, rows = 128 / splits, outs = kOut / splits;  // sums and channels a CTA finishes
-  const uint32_t rank = splits > 1 ? cluster_rank() : 0u;
-  if (epi) {
-    const int q = warp & 3, row = 32 * q + lane;  // TMEM lane = row of the tile
-    const int half = GATED ? row / 64 : 0, c = row % kOut;
-    const int slot = static_cast<int>(rank) * rows + half * outs + c % outs;
-    const uint32_t to = cluster_addr(red + static_cast<size_t>(slot) * rs, static_cast<uint32_t>(c / outs));
-    const uint32_t tl = tmem + (static_cast<uint32_t>(32 * q) << 16);
-    for (int j0 = 0; j0 < P.xrows; j0 += 32) {
-      uint32_t v[32];
-      if (ok) {
-        tmem_ld32(tl + j0, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0u;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; j += 4)
-        if (j0 + j < P.xrows)
-          asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (j0 + j) * 4), "r"(v[j]),
-                       "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3])
-                       : "memory");
-    }
-  }
-  if (splits > 1) cluster_sync();
-  __syncthreads();
-  const int tok = min(P.xrows, A.m - t0), tok4 = (tok + 3) / 4;
-  const int cbase = c0 + static_cast<int>(rank) * outs;
-  for (int i = tid; i < outs * tok4; i += kSplitThreads) {
-    const int lc = i % outs, j = 4 * (i / outs), c = cbase + lc;
-    if (c >= A.n) continue;
-    int g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-    for (int z = 0; z < splits; ++z) {
-      const int4 v = *reinterpret_cast<const int4*>(red + static_cast<size_t>(z * rows + lc) * rs + j);
-      g[0] += v.x, g[1] += v.y, g[2] += v.z, g[3] += v.w;
-      if (GATED) {
-        const int4 b = *reinterpret_cast<const int4*>(red + static_cast<size_t>(z * rows + outs + lc) * rs + j);
-        u[0] += b.x, u[1] += b.y, u[2] += b.z, u[3] += b.w;
-      }
-    }
-    const float ws = A.ws[c], wu = GATED ? A.ws[A.n + c] : 0.0f, bias = A.bias ? __half2float(A.bias[c]) : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (j + e >= tok) break;
-      const size_t row = static_cast<size_t>(t0 + j + e);
-      const float xs = A.xs[row];
-      float v = linear_value(g[e], xs, ws);
-      if (GATED) v = silu_product(v, linear_value(u[e], xs, wu));
-      v += bias;
-      if (A.residual) v += __half2float(A.residual[row * A.ldr + c]);
-      A.y[row * A.ldy + c] = __float2half_rn(v);
-    }
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tcols) : "memory");
-}
-
-static size_t split_smem(int stages, int xrows) {
-  return static_cast<size_t>(stages) * (kWBytes + xrows * kBK) + 1024 + (2 * kSplitStages + 1) * sizeof(uint64_t) + 16;
-}
-
-// --- pair_kernel ----------------------------------------------------------------
-// A tile: 256 tokens (128 for each CTA of the pair) x BN weight rows (each CTA
-// loads BN / 2 of them; gated: the first CTA gate rows, the second their up
-// rows, so that a CTA's accumulator holds a token's gates in columns 0 .. and
-// their up values BN / 2 further).  One elected thread of the first CTA issues
-// the MMAs of both.  Each pair walks tiles pair, + pairs, ..; two accumulators
-// in tensor memory.
-//   warp 0 lane 0: TMA loads of this CTA's half of both operands
-//   warp 1 lane 0 of the first CTA: MMAs
-//   warps 2-9: epilogue (TMEM lanes 32 (w % 4) .., half of the columns each)
-constexpr int kPairThreads = 320;
-constexpr int kEpiWarps = 8;
-constexpr int kPairStages = 5;
-
-template <int BN>
-struct PairShape {
-  static constexpr int kX = 128 * kBK, kW = BN / 2 * kBK;
-  static constexpr int kStage = kX + kW;
-  static constexpr int kStore = kEpiWarps * 32 * 128;  // 32 rows x 64 fp16 a warp
-  static constexpr int kCols = kEpiWarps * BN * 4;  // a warp's BN / 2 scales and biases (gated: BN / 4 gate and up scales)
-  static constexpr size_t kSmem = static_cast<size_t>(kPairStages) * kStage + kStore + kCols + 1024 +
-                                  (2 * kPairStages + 5) * sizeof(uint64_t) + 16;
-};
-
-// Bounded wait for a barrier that threads of both CTAs arrive at.
+// Bounded wait for a barrier that other CTAs of the cluster report to.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
   const uint64_t t0 = globaltimer();
   while (true) {
@@ -407,11 +306,248 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// --- split_kernel -------------------------------------------------------------
+// One tile of 128 weight rows (gated: 64 gate and their 64 up rows) and xrows
+// tokens a cluster; CTA z of the cluster multiplies K steps z * ksteps .. .
+//   warp 0 lane 0: TMA loads; warp 1 lane 0: MMAs; warps 2-17: sums out of
+//   TMEM, 32 tokens of 32 rows each; all warps: finish the CTA's rows.
+// Each CTA finishes 128 / splits of the tile's rows: all CTAs store their sums
+// of these rows into its shared memory ([tokens / 4][split][row][4], so that a
+// warp's stores and loads are contiguous), counted in bytes by its barrier.
+constexpr int kSplitThreads = 64 + 512;
+constexpr int kSplitStages = 8;   // at most
+constexpr int kSplitTokens = 128;  // of a tile at most
+constexpr int kWBytes = 128 * kBK;
+
+// 16 bytes into the shared memory of a CTA of the cluster, reported to a barrier there.
+__device__ __forceinline__ void store_cluster(uint32_t to, const uint32_t* v, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+      : "memory");
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_constant__ Params P) {
+  extern __shared__ unsigned char smem_raw[];
+  const Args& A = P.a;
+  const int S = P.stages, xbytes = P.xrows * kBK;
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* wt = base;
+  unsigned char* xt = base + static_cast<size_t>(S) * kWBytes;
+  int4* red = reinterpret_cast<int4*>(xt + static_cast<size_t>(S) * xbytes);
+  float* xs = reinterpret_cast<float*>(red + 32 * P.xrows);  // [kSplitTokens] token scales
+  float* cs = xs + kSplitTokens;                             // [3][128] channel scales, up scales, biases
+  uint64_t* full = reinterpret_cast<uint64_t*>(cs + 3 * 128);
+  uint64_t* empty = full + kSplitStages;
+  uint64_t* done = empty + kSplitStages;
+  uint64_t* sums = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abort_v = abort_flag;
+  constexpr int kOut = GATED ? 64 : 128;  // channels of a tile
+
+  lmps_pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c0 = blockIdx.x * kOut, t0 = blockIdx.y * P.xrows;
+  const int splits = gridDim.z;
+  const int all = (A.k + kBK - 1) / kBK, kbeg = blockIdx.z * P.ksteps;
+  const int ksteps = max(0, min(P.ksteps, all - kbeg));
+  const uint32_t tcols = P.xrows <= 32 ? 32u : P.xrows <= 64 ? 64u : 128u;
+  const uint32_t rank = cluster_rank();  // = blockIdx.z
+
+  if (warp == 0) {  // a lane per barrier
+    if (lane < S) {
+      mbar_init(&full[lane], 1);
+      mbar_init(&empty[lane], 1);
+    } else if (lane == 30) {
+      mbar_init(done, 1);
+      *abort_flag = 0;
+    } else if (lane == 31) {
+      mbar_init(sums, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (lane == 31) mbar_expect_tx(sums, static_cast<uint32_t>(128 * P.xrows * 4));
+    __syncwarp();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(tcols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (the barriers exist; waited for before the sums go out)
+  const uint32_t tmem = *tmem_slot;
+  const int rows = 128 / splits, outs = kOut / splits;  // sums and channels that this CTA finishes
+  const int cbase = c0 + static_cast<int>(rank) * outs;
+  const int log_outs = __ffs(outs) - 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      lmps_pdl_wait();  // both operands may be the previous kernel's output
+      Ring r;
+      int issued = 0;
+      for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
+        if (kt >= S && !mbar_wait(&empty[r.slot], r.phase ^ 1u, P.error, abort_v)) break;
+        mbar_expect_tx(&full[r.slot], static_cast<uint32_t>(kWBytes + xbytes));
+        unsigned char* w = wt + static_cast<size_t>(r.slot) * kWBytes;
+        const int kx = (kbeg + kt) * kBK;
+        tma_load_2d(w, &P.tw, kx, c0, &full[r.slot]);
+        if (GATED) tma_load_2d(w + kWBytes / 2, &P.tw, kx, A.n + c0, &full[r.slot]);
+        tma_load_2d(xt + static_cast<size_t>(r.slot) * xbytes, &P.tx, kx, t0, &full[r.slot]);
+        issued = kt + 1;
+      }
+      for (int kt = max(0, issued - S); kt < issued; ++kt) {  // every issued copy lands before the CTA leaves
+        const uint64_t since = globaltimer();
+        while (!mbar_try(&full[kt % S], (kt / S) & 1))
+          if (globaltimer() - since > kTimeoutNs) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      lmps_pdl_wait();  // (bounded waits begin when the work does)
+      const uint32_t idesc = idesc_i8(128, P.xrows);
+      Ring r;
+      for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
+        if (!mbar_wait(&full[r.slot], r.phase, P.error, abort_v)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t wd = sw128_desc(smem_u32(wt + static_cast<size_t>(r.slot) * kWBytes));
+        const uint64_t xd = sw128_desc(smem_u32(xt + static_cast<size_t>(r.slot) * xbytes));
+#pragma unroll
+        for (int j = 0; j < kBK / 32; ++j)  // K = 32 a MMA: 32 bytes further into the swizzle row
+          mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u);
+        mma_commit(&empty[r.slot]);
+      }
+      mma_commit(done);
+      const uint64_t since = globaltimer();  // every MMA is finished before the tensor memory is freed
+      while (!mbar_try(done, 0u))
+        if (globaltimer() - since > kTimeoutNs) break;
+    }
+  } else {
+    if (warp == 2)
+      for (int kt = lane; kt < ksteps; kt += 32) {  // the weights come nearer while the kernel before ends
+        prefetch_2d(&P.tw, (kbeg + kt) * kBK, c0);
+        if (GATED) prefetch_2d(&P.tw, (kbeg + kt) * kBK, A.n + c0);
+      }
+    lmps_pdl_wait();  // before any read of scales and residual, or write of y
+    // what the sums meet, on its way before they do
+    if (const int i = tid - 64 - 128; i >= 0 && i < P.xrows) xs[i] = t0 + i < A.m ? A.xs[t0 + i] : 0.0f;
+    if (const int i = tid - 64 - 256; i >= 0 && i < outs) {
+      const bool in = cbase + i < A.n;
+      cs[i] = in ? A.ws[cbase + i] : 0.0f;
+      if (GATED) cs[128 + i] = in ? A.ws[A.n + cbase + i] : 0.0f;
+      cs[256 + i] = in && A.bias ? __half2float(A.bias[cbase + i]) : 0.0f;
+    }
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp >= 2) {
+    // (a wait that ran out leaves the sums without meaning; they still go out, so that no CTA waits for them)
+    bool ok = ksteps > 0;
+    if (lane == 0) ok = mbar_wait(done, 0, P.error, abort_v) && ok;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const int q = warp & 3, row = 32 * q + lane;  // TMEM lane = row of the tile
+    const int c = row % kOut, owner = c >> log_outs, local = (GATED ? row / 64 * outs : 0) + (c & (outs - 1));
+    if (const int j0 = 32 * ((warp - 2) / 4); j0 < P.xrows) {
+      uint32_t v[32];
+      if (ok) {
+        tmem_ld32(tmem + (static_cast<uint32_t>(32 * q) << 16) + j0, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0u;
+      }
+      const uint32_t bar = cluster_addr(sums, static_cast<uint32_t>(owner));
+      const uint32_t to = cluster_addr(red + j0 / 4 * 128 + static_cast<int>(rank) * rows + local, static_cast<uint32_t>(owner));
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        if (j0 + j < P.xrows) store_cluster(to + j / 4 * 128 * 16, v + j, bar);
+    }
+  }
+  lmps_pdl_wait();
+  const int tok = min(P.xrows, A.m - t0), tok4 = (tok + 3) / 4;
+  const bool here = __syncthreads_and(tid != 0 || mbar_wait_cluster(sums, 0u, P.error, abort_v));
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  for (int i = tid; here && i < outs * tok4; i += kSplitThreads) {
+    const int lc = i & (outs - 1), j = 4 * (i >> log_outs), c = cbase + lc;
+    if (c >= A.n) continue;
+    float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      res[e] = !GATED && A.residual && j + e < tok ? __half2float(A.residual[static_cast<size_t>(t0 + j + e) * A.ldr + c]) : 0.0f;
+    int g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
+    const int4* at = red + j / 4 * 128 + lc;
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z, at += rows) {
+      const int4 v = at[0];
+      g[0] += v.x, g[1] += v.y, g[2] += v.z, g[3] += v.w;
+      if (GATED) {
+        const int4 b = at[outs];
+        u[0] += b.x, u[1] += b.y, u[2] += b.z, u[3] += b.w;
+      }
+    }
+    const float ws = cs[lc], bias = GATED ? 0.0f : cs[256 + lc], wu = GATED ? cs[128 + lc] : 0.0f;
+    const float4 x4 = *reinterpret_cast<const float4*>(xs + j);
+    const float xv[4] = {x4.x, x4.y, x4.z, x4.w};
+    __half* y = A.y + static_cast<size_t>(t0 + j) * A.ldy + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e, y += A.ldy) {
+      float v = linear_value(g[e], xv[e], ws);
+      if (GATED) v = silu_product(v, linear_value(u[e], xv[e], wu));
+      else v += bias + res[e];
+      if (j + e < tok) *y = __float2half_rn(v);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // no CTA leaves while another waits for sums
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tcols) : "memory");
+}
+
+static size_t split_smem(int stages, int xrows) {
+  return static_cast<size_t>(stages) * (kWBytes + xrows * kBK) + static_cast<size_t>(xrows) * 512 +
+         (kSplitTokens + 3 * 128) * sizeof(float) + 1024 + (2 * kSplitStages + 2) * sizeof(uint64_t) + 16;
+}
+
+// --- pair_kernel ----------------------------------------------------------------
+// A tile: 256 tokens (128 for each CTA of the pair) x BN weight rows (each CTA
+// loads BN / 2 of them; gated: the first CTA gate rows, the second their up
+// rows, so that a CTA's accumulator holds a token's gates in columns 0 .. and
+// their up values BN / 2 further).  One elected thread of the first CTA issues
+// the MMAs of both.  Each pair walks tiles pair, + pairs, ..; two accumulators
+// in tensor memory.
+//   warp 0 lane 0: TMA loads of this CTA's half of both operands
+//   warp 1 lane 0 of the first CTA: MMAs
+//   warps 2 ..: epilogue, four warps (TMEM lanes 32 (w % 4) ..) for each 64 or 32 channels of the tile
+constexpr int kPairStages = 4;
+
 template <int BN, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pair_kernel(const __grid_constant__ Params P) {
-  using Sh = PairShape<BN>;
-  constexpr int S = kPairStages;
-  constexpr int kOut = GATED ? BN / 2 : BN;  // channels of a tile
+struct PairShape {
+  static constexpr int kX = 128 * kBK, kW = BN / 2 * kBK;
+  static constexpr int kStage = kX + kW;
+  static constexpr int kOut = GATED ? BN / 2 : BN;     // channels of a tile
+  static constexpr int kParts = kOut >= 128 ? 4 : 2;   // epilogue warps side by side
+  static constexpr int kWarps = 4 * kParts;
+  static constexpr int kThreads = 64 + kWarps * kWarp;
+  static constexpr int kMine = kOut / kParts;          // channels of an epilogue warp: a store of 32 rows
+  static constexpr int kBoxBytes = 32 * kMine * 2;
+  static constexpr int kStore = kWarps * kBoxBytes;
+  static constexpr int kCols = kWarps * 2 * kMine * 4;  // a warp's scales and biases (gated: gate and up scales)
+  static constexpr int kBars = 2 * kPairStages + 5 + kWarps;
+  static constexpr size_t kSmem =
+      static_cast<size_t>(kPairStages) * kStage + kStore + kCols + 1024 + kBars * sizeof(uint64_t) + 16;
+};
+
+template <int BN, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>::kThreads, 1)
+    pair_kernel(const __grid_constant__ Params P) {
+  using Sh = PairShape<BN, GATED>;
+  constexpr int S = kPairStages, kOut = Sh::kOut;
   constexpr uint32_t kTmem = BN > 128 ? 512u : 256u;
   constexpr uint32_t kAcc = kTmem / 2;  // columns from one accumulator to the other
   extern __shared__ unsigned char smem_raw[];
@@ -426,7 +562,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pai
   uint64_t* tfull = empty + S;   // [2] accumulator complete
   uint64_t* tempty = tfull + 2;  // [2] accumulator read by both CTAs' epilogues (the first CTA's counts)
   uint64_t* done = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* rfull = done + 1;  // [epilogue warps] residual box arrived
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + Sh::kWarps);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
 
@@ -442,9 +579,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pai
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 2 * kEpiWarps);
+      mbar_init(&tempty[i], 2 * Sh::kWarps);
     }
     mbar_init(done, 1);
+    for (int i = 0; i < Sh::kWarps; ++i) mbar_init(&rfull[i], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -523,108 +661,150 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) pai
     }
   } else {
     lmps_pdl_wait();  // before any read of scales and residual, or write of y
-    const int e = warp - 2, q = warp & 3, part = e / 4;  // part: which half of the columns
-    unsigned char* mine = store + e * (32 * 128);
-    float* ws = cols + e * BN;  // this warp's scales and biases (gated: gate and up scales)
-    float* bs = ws + BN / 2;
-    uint32_t uses[2] = {0u, 0u};
+    constexpr int kMine = Sh::kMine, kChunks = kMine / 32;
+    const int e = warp - 2, q = warp & 3, first = e / 4 * kMine;  // TMEM lanes 32 q .., channels first ..
+    unsigned char* box = store + e * Sh::kBoxBytes;  // [32 rows][kMine] fp16, swizzled as the TMA unit does
+    float* ws = cols + e * (2 * kMine);
+    float* bs = ws + kMine;
+    // byte of the box at which the 16-byte piece i of row r lies
+    auto piece = [&](int r, int i) { return r * (kMine * 2) + ((kMine == 64 ? i ^ (r & 7) : i ^ ((r >> 1) & 3)) << 4); };
+    // scales (and biases) of this warp's channels and this lane's token, on their way for the next tile
+    float nxs = 0.0f, nws[kChunks], nus[kChunks];
+    __half nbs[kChunks];
+    auto fetch = [&](int tile) {
+      const int c0 = (tile % P.tiles_n) * kOut + first;
+      const int row = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128 + 32 * q + lane;
+      nxs = row < A.m ? A.xs[row] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = c0 + 32 * i + lane;
+        const bool in = c < A.n;
+        nws[i] = in ? A.ws[c] : 0.0f;
+        if (GATED) nus[i] = in ? A.ws[A.n + c] : 0.0f;
+        else nbs[i] = in && A.bias ? A.bias[c] : __half(0.0f);
+      }
+    };
+    if (pair < P.tiles) fetch(pair);
+    const bool add = !GATED && A.residual != nullptr;
+    uint32_t uses[2] = {0u, 0u}, rphase = 0u;
+    bool awaited = false;  // a residual is on its way
     int buf = 0;
     for (int tile = pair; tile < P.tiles; tile += pairs, buf ^= 1) {
-      const int c0 = (tile % P.tiles_n) * kOut, t0 = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128;
-      constexpr int kMine = kOut / 2;  // channels of this warp's half, from first on
-      const int first = part * kMine;
+      const int c0 = (tile % P.tiles_n) * kOut + first;
+      const int t0 = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128 + 32 * q;
+      const float xs = nxs;
       __syncwarp();
-      for (int i = lane; i < kMine; i += 32) {
-        const int c = c0 + first + i;
-        const bool in = c < A.n;
-        ws[i] = in ? A.ws[c] : 0.0f;
-        bs[i] = GATED ? (in ? A.ws[A.n + c] : 0.0f) : (in && A.bias ? __half2float(A.bias[c]) : 0.0f);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        ws[32 * i + lane] = nws[i];
+        bs[32 * i + lane] = GATED ? nus[i] : __half2float(nbs[i]);
       }
-      const int row = t0 + 32 * q + lane;
-      const bool live = row < A.m;
-      const float xs = live ? A.xs[row] : 0.0f;
+      if (tile + pairs < P.tiles) fetch(tile + pairs);
+      // the box is free once the last tile's store has read it; the residual comes in where the sums go out
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (add && P.tma_y) {
+          mbar_expect_tx(&rfull[e], Sh::kBoxBytes);
+          tma_load_2d(box, &P.tr, c0, t0, &rfull[e]);
+        }
+      }
       __syncwarp();
+      if (add && P.tma_y) {
+        awaited = true;
+      } else if (add) {  // rows of any alignment: a row a time
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r)
+          if (t0 + r < A.m)
+#pragma unroll
+            for (int j = lane; j < kMine; j += 32)
+              if (c0 + j < A.n)
+                *reinterpret_cast<__half*>(box + piece(r, j / 8) + (j % 8) * 2) =
+                    A.residual[static_cast<size_t>(t0 + r) * A.ldr + c0 + j];
+        __syncwarp();
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], uses[buf] & 1u, P.error, abort_v))) break;
       ++uses[buf];
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t tl = tmem + static_cast<uint32_t>(buf) * kAcc + (static_cast<uint32_t>(32 * q) << 16);
-#pragma unroll 1
-      for (int o = first; o < first + kMine; o += 32) {  // 32 channels a time, half a store box
-        uint32_t packed[16];
-        if (GATED) {
-          uint32_t g[32], u[32];
-          tmem_ld32(tl + o, g);
-          tmem_ld32(tl + kOut + o, u);
+      const uint32_t tl = tmem + static_cast<uint32_t>(buf) * kAcc + (static_cast<uint32_t>(32 * q) << 16) + first;
+      uint32_t g[kChunks][32], u[kChunks][32];  // (u: gated)
+      tmem_start32(tl, g[0]);
+      if (GATED) tmem_start32(tl + kOut, u[0]);
+      if (awaited) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&rfull[e], rphase, P.error, abort_v))) break;
+        rphase ^= 1u;
+        awaited = false;
+      }
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float a = silu_product(linear_value(static_cast<int>(g[j]), xs, ws[o - first + j]),
-                                         linear_value(static_cast<int>(u[j]), xs, bs[o - first + j]));
-            const float b = silu_product(linear_value(static_cast<int>(g[j + 1]), xs, ws[o - first + j + 1]),
-                                         linear_value(static_cast<int>(u[j + 1]), xs, bs[o - first + j + 1]));
-            const __half2 h = __floats2half2_rn(a, b);
-            packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        } else {
-          uint32_t g[32];
-          tmem_ld32(tl + o, g);
-          float res[32];
-          if (A.residual) {
-            const __half* rr = A.residual + static_cast<size_t>(row) * A.ldr + c0 + o;
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (P.tma_y && live && c0 + o + j + 8 <= A.n) {  // (then residual rows are 16-byte aligned)
-                const uint4 v = *reinterpret_cast<const uint4*>(rr + j);
-                const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 f = __half22float2(h[i]);
-                  res[j + 2 * i] = f.x, res[j + 2 * i + 1] = f.y;
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) res[j + i] = live && c0 + o + j + i < A.n ? __half2float(rr[j + i]) : 0.0f;
-              }
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float a = linear_value(static_cast<int>(g[j]), xs, ws[o - first + j]) + bs[o - first + j];
-            float b = linear_value(static_cast<int>(g[j + 1]), xs, ws[o - first + j + 1]) + bs[o - first + j + 1];
-            if (A.residual) a += res[j], b += res[j + 1];
-            const __half2 h = __floats2half2_rn(a, b);
-            packed[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
-          }
+      for (int i = 0; i < kChunks; ++i) {  // 32 channels; the next ones are on their way meanwhile
+        tmem_arrived(g[i]);
+        if (GATED) tmem_arrived(u[i]);
+        if (i + 1 < kChunks) {
+          tmem_start32(tl + 32 * (i + 1), g[i + 1]);
+          if (GATED) tmem_start32(tl + kOut + 32 * (i + 1), u[i + 1]);
+        } else {  // the accumulator is read
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], 0));
         }
-        if (P.tma_y) {
-          const int box = o & 32;  // first or second half of a 64-column box
-          if (box == 0) {          // the box's last store has left the buffer
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-          }
+        const float4* w4 = reinterpret_cast<const float4*>(ws + 32 * i);
+        const float4* b4 = reinterpret_cast<const float4*>(bs + 32 * i);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(mine + lane * 128 + (((box / 8 + j) ^ (lane & 7)) << 4)) =
-                make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
-          if (box != 0) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0 && c0 + o - 32 < A.n && t0 + 32 * q < A.m) {
-              tma_store_2d(&P.ty, c0 + o - 32, t0 + 32 * q, mine);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        for (int j = 0; j < 32; j += 8) {
+          float v[8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 w = w4[j / 4 + h], o = b4[j / 4 + h];
+            const float wv[4] = {w.x, w.y, w.z, w.w}, ov[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+              const int k = j + 4 * h + l;
+              const float lin = linear_value(static_cast<int>(g[i][k]), xs, wv[l]);
+              v[4 * h + l] = GATED ? silu_product(lin, linear_value(static_cast<int>(u[i][k]), xs, ov[l])) : lin + ov[l];
             }
           }
-        } else if (live) {
-          __half* y = A.y + static_cast<size_t>(row) * A.ldy + c0 + o;
+          uint4* to = reinterpret_cast<uint4*>(box + piece(lane, (32 * i + j) / 8));
+          if (add) {
+            const uint4 rv = *to;
+            const __half2* r2 = reinterpret_cast<const __half2*>(&rv);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + o + j < A.n) y[j] = reinterpret_cast<const __half*>(packed)[j];
+            for (int l = 0; l < 4; ++l) {
+              const float2 f = __half22float2(r2[l]);
+              v[2 * l] += f.x, v[2 * l + 1] += f.y;
+            }
+          }
+          uint4 packed;
+          __half2* h2 = reinterpret_cast<__half2*>(&packed);
+#pragma unroll
+          for (int l = 0; l < 4; ++l) h2[l] = __floats2half2_rn(v[2 * l], v[2 * l + 1]);
+          *to = packed;
         }
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], 0));
+      if (P.tma_y) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && c0 < A.n && t0 < A.m) {
+          tma_store_2d(&P.ty, c0, t0, box);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else {
+        __syncwarp();
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r)
+          if (t0 + r < A.m)
+#pragma unroll
+            for (int j = lane; j < kMine; j += 32)
+              if (c0 + j < A.n)
+                A.y[static_cast<size_t>(t0 + r) * A.ldy + c0 + j] =
+                    *reinterpret_cast<const __half*>(box + piece(r, j / 8) + (j % 8) * 2);
+      }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) {
+      // (after a wait that ran out: a residual on its way lands before the CTA leaves)
+      const uint64_t since = globaltimer();
+      while (awaited && !mbar_try(&rfull[e], rphase))
+        if (globaltimer() - since > kTimeoutNs) break;
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -655,35 +835,45 @@ static bool encode_codes(CUtensorMap* map, const int8_t* p, int k, size_t rows, 
                    static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static int launch_gemv(const Args& A, cudaStream_t st) {
-  const dim3 grid((A.n + kGemvWarps - 1) / kGemvWarps, (A.m + kTokens - 1) / kTokens);
-  return lmps_launch_pdl(A.swiglu ? gemv_kernel<true> : gemv_kernel<false>, grid, dim3(kGemvWarps * kWarp), 0, st, A);
+template <int NT, bool GATED, int WARPS>
+static int launch_few_warps(const Args& A, int tiles, cudaStream_t st) {
+  return lmps_launch_pdl(few_kernel<NT, GATED, WARPS>, dim3(tiles), dim3(WARPS * kWarp), 0, st, A);
+}
+// The fewer tiles there are for an SM, the more warps share one out (as their sums fit 48 KB of shared memory).
+template <int NT, bool GATED>
+static int launch_few(const Args& A, int sms, cudaStream_t st) {
+  constexpr int kFit = 64 / (NT * (GATED ? 2 : 1));
+  const int tiles = (A.n + 15) / 16;
+  if constexpr (kFit >= 32)
+    if (tiles <= sms) return launch_few_warps<NT, GATED, 32>(A, tiles, st);
+  if constexpr (kFit >= 16)
+    if (tiles <= 2 * sms) return launch_few_warps<NT, GATED, 16>(A, tiles, st);
+  return launch_few_warps<NT, GATED, 8>(A, tiles, st);
 }
 
-static int launch_split(const Args& A, int* error, cudaStream_t st) {
+template <bool GATED>
+static int launch_split(const Args& A, int* error, int sms, cudaStream_t st) {
   Params P{};
   P.a = A;
   P.error = error;
-  P.xrows = A.m >= 128 ? 128 : (A.m + 15) / 16 * 16;
-  const int out = A.swiglu ? 64 : 128;
+  P.xrows = A.m >= kSplitTokens ? kSplitTokens : (A.m + 15) / 16 * 16;
+  const int out = GATED ? 64 : 128;
   const int tiles = (A.n + out - 1) / out, ty = (A.m + P.xrows - 1) / P.xrows, steps = (A.k + kBK - 1) / kBK;
-  int sms = 148;
-  if (const int e = device_sms(&sms)) return e;
-  int splits = 1;  // about two CTAs an SM, at least two K steps each
-  while (2 * splits <= 8 && 2 * splits * tiles * ty <= 2 * sms && 4 * splits <= steps) splits *= 2;
+  // at most two CTAs an SM, at least three K steps each (64 x 2048 x 1536: 5.6 us with 4 splits, 5.9 with 8, 7.5 with 2)
+  int splits = 1;
+  while (splits < 8 && 2 * splits * tiles * ty <= 2 * sms && 6 * splits <= steps) splits *= 2;
   P.ksteps = (steps + splits - 1) / splits;
-  int stages = P.ksteps < 6 ? P.ksteps : 6;
-  while (stages > 2 && split_smem(stages, P.xrows) > 113 * 1024) --stages;
-  // the ring also holds the sums: 128 rows of xrows + 4
-  while (static_cast<size_t>(stages) * (kWBytes + P.xrows * kBK) < static_cast<size_t>(128) * (P.xrows + 4) * 4) ++stages;
+  // two CTAs an SM where there are so many, else the whole SM's shared memory
+  const size_t room = tiles * ty * splits > sms ? 113 * 1024 : 226 * 1024;
+  int stages = P.ksteps < 2 ? 2 : P.ksteps < kSplitStages ? P.ksteps : kSplitStages;  // (the ring also holds the CTA's sums)
+  while (stages > 2 && split_smem(stages, P.xrows) > room) --stages;
   P.stages = stages;
-  const size_t w_rows = static_cast<size_t>(A.n) * (A.swiglu ? 2 : 1);
+  const size_t w_rows = static_cast<size_t>(A.n) * (GATED ? 2 : 1);
   if (!encode_codes(&P.tx, A.x, A.k, static_cast<size_t>(A.m), A.ldx, P.xrows) ||
       !encode_codes(&P.tw, A.w, A.k, w_rows, A.ldw, out))
     return LMPS_ERR_INVALID_ARGUMENT;
   const size_t smem = split_smem(stages, P.xrows);
-  const int attr = A.swiglu ? lmps_max_dyn_smem<split_kernel<true>>(static_cast<int>(smem))
-                            : lmps_max_dyn_smem<split_kernel<false>>(static_cast<int>(smem));
+  const int attr = lmps_max_dyn_smem<split_kernel<GATED>>(static_cast<int>(smem));
   if (attr != LMPS_OK) return attr;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles, ty, splits);
@@ -699,16 +889,16 @@ static int launch_split(const Args& A, int* error, cudaStream_t st) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, A.swiglu ? split_kernel<true> : split_kernel<false>, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, split_kernel<GATED>, P);
   return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
 }
 
 template <int BN, bool GATED>
-static int launch_pair(const Args& A, int* error, cudaStream_t st) {
+static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
   Params P{};
   P.a = A;
   P.error = error;
-  constexpr int kOut = GATED ? BN / 2 : BN;
+  constexpr int kOut = PairShape<BN, GATED>::kOut;
   P.tiles_n = (A.n + kOut - 1) / kOut;
   const long long tiles = static_cast<long long>(P.tiles_n) * ((A.m + 255) / 256);
   if (tiles > (1ll << 30)) return LMPS_ERR_UNSUPPORTED;
@@ -717,18 +907,44 @@ static int launch_pair(const Args& A, int* error, cudaStream_t st) {
   if (!encode_codes(&P.tx, A.x, A.k, static_cast<size_t>(A.m), A.ldx, 128) ||
       !encode_codes(&P.tw, A.w, A.k, w_rows, A.ldw, BN / 2))
     return LMPS_ERR_INVALID_ARGUMENT;
+  using Sh = PairShape<BN, GATED>;
   P.tma_y = A.ldy % 8 == 0 && lmps_aligned(A.y, 16) &&
             (!A.residual || (A.ldr % 8 == 0 && lmps_aligned(A.residual, 16)));
-  if (P.tma_y && !encode_2d(&P.ty, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, A.y, static_cast<uint64_t>(A.n),
-                            static_cast<uint64_t>(A.m), A.ldy * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+  const CUtensorMapSwizzle swz = Sh::kMine == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (P.tma_y && (!encode_2d(&P.ty, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, A.y, static_cast<uint64_t>(A.n),
+                             static_cast<uint64_t>(A.m), A.ldy * 2, Sh::kMine, 32, swz) ||
+                  (A.residual && !encode_2d(&P.tr, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, A.residual,
+                                            static_cast<uint64_t>(A.n), static_cast<uint64_t>(A.m), A.ldr * 2, Sh::kMine,
+                                            32, swz))))
     return LMPS_ERR_INVALID_ARGUMENT;
-  constexpr int kBytes = static_cast<int>(PairShape<BN>::kSmem);
+  constexpr int kBytes = static_cast<int>(Sh::kSmem);
   const int attr = lmps_max_dyn_smem<pair_kernel<BN, GATED>>(kBytes);
   if (attr != LMPS_OK) return attr;
-  int sms = 148;
-  if (const int e = device_sms(&sms)) return e;
   const int pairs = P.tiles < sms / 2 ? P.tiles : sms / 2;
-  return lmps_launch_pdl(pair_kernel<BN, GATED>, dim3(2 * pairs), dim3(kPairThreads), kBytes, st, P);
+  return lmps_launch_pdl(pair_kernel<BN, GATED>, dim3(2 * pairs), dim3(Sh::kThreads), kBytes, st, P);
+}
+
+static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+template <bool GATED>
+static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
+  const long long codes = static_cast<long long>(A.n) * A.k * (GATED ? 2 : 1);  // weight bytes
+  // Weights straight into mma.sync: up to 8 tokens always (8 x 8960 x 1536 gated 7.1 us, split_kernel 9.0), up to 16
+  // with at most a tile an SM (16 x 1536 x 8960 6.9, 7.7; not 16 x 8192 x 1536: 6.8, 5.4), up to 32 with small
+  // weights (32 x 2048 x 1536 2.9, 4.3; not 32 x 1536 x 8960: 8.7, 8.0).
+  if (A.m <= 8) return launch_few<1, GATED>(A, sms, st);
+  if (A.m <= 16 && ceil_div(A.n, 16) <= sms) return launch_few<2, GATED>(A, sms, st);
+  if (A.m <= 32 && codes <= (4 << 20)) return launch_few<4, GATED>(A, sms, st);
+  // CTA pairs with 128 or 256 weight rows a tile, by the waves they take: a tile of 128 takes 0.78 of the time of one
+  // of 256 (16384 x 8960 x 1536 gated: 495, 318 us), so it is for equal waves (1024 x 2048 x 1536: 9.5, 11.0 us).
+  const int pairs = sms / 2;
+  const long long rows = ceil_div(A.m, 256), t128 = rows * ceil_div(A.n, GATED ? 64 : 128),
+                  t256 = rows * ceil_div(A.n, GATED ? 128 : 256);
+  // Up to 64 tokens, and up to 256 where pairs would leave two thirds of the GPU idle, K is split (256 x 2048 x 1536
+  // 7.3 us, pairs 8.2; 256 x 1536 x 8960 21, 28; not 128 x 8192 x 1536: 10.7, 10.0).
+  if (A.m <= 64 || (A.m <= 256 && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
+  if (100 * ceil_div(t256, pairs) > 78 * ceil_div(t128, pairs)) return launch_pair<128, GATED>(A, error, sms, st);
+  return launch_pair<256, GATED>(A, error, sms, st);
 }
 
 }  // namespace w8
@@ -762,9 +978,8 @@ extern "C" int lmps_w8a8_gemm(const int8_t* x, int ldx, const float* x_scales, c
   A.m = m;
   A.n = n;
   A.k = k;
-  A.swiglu = swiglu;
   cudaStream_t st = lmps_stream(stream);
-  if (m <= w8::kTokens) return w8::launch_gemv(A, st);
-  if (m <= 256) return w8::launch_split(A, error, st);
-  return swiglu ? w8::launch_pair<256, true>(A, error, st) : w8::launch_pair<256, false>(A, error, st);
+  int sms = 0;
+  if (const int e = w8::device_sms(&sms)) return e;
+  return swiglu ? w8::launch<true>(A, error, sms, st) : w8::launch<false>(A, error, sms, st);
 }
