@@ -55,7 +55,7 @@ PyObject* gemm(PyObject* const* args, Py_ssize_t n) {
   A.shape(0, m, k);
   A.shape(2, w_rows, w_k);
   const int gated = A.number(6);
-  A.ok = A.ok && w_k == k && (gated == 0 || (gated == 1 && w_rows % 2 == 0));
+  A.ok = A.ok && w_k == k && (gated == 0 || (gated == 1 && w_rows % 2 == 0 && args[4] == Py_None && args[5] == Py_None));
   const int64_t cols = gated ? w_rows / 2 : w_rows;
   int ldx = 0, ldw = 0, ldr = 0, ldy = 0;
   auto* x = static_cast<int8_t*>(A.matrix(0, kChar, m, k, ldx));

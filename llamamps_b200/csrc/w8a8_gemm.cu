@@ -36,8 +36,11 @@ struct Args {
   int m, n, k;
 };
 
-// y[t][c] from the integer sum(s) and the scales.
-__device__ __forceinline__ float linear_value(int acc, float xs, float ws) { return static_cast<float>(acc) * xs * ws; }
+// The scaled sum, and the bias in the rounding of the second product.  Every kernel goes through the same roundings
+// (this, then the residual), so a token's result does not depend on the other tokens of its call.
+__device__ __forceinline__ float linear_value(int acc, float xs, float ws, float bias = 0.0f) {
+  return fmaf(__fmul_rn(static_cast<float>(acc), xs), ws, bias);
+}
 
 __device__ __forceinline__ float silu_product(float g, float u) {
   // e^-g past 2^126 makes the quotient 0, which fp16 makes of it anyway
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(WARPS* kWarp) few_kernel(const Args A) {
   }
   // what the sums meet, on its way before they do: output o = 16 token + channel
   constexpr int kOuts = kRows * kToks, kMine = (kOuts + WARPS * kWarp - 1) / (WARPS * kWarp);
-  float ws[kMine], wu[kMine], xs[kMine], add[kMine];
+  float ws[kMine], wu[kMine], xs[kMine], bias[kMine], res[kMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int o = static_cast<int>(threadIdx.x) + i * WARPS * kWarp, t = o / kRows, c = c0 + o % kRows;
@@ -137,8 +140,8 @@ __global__ void __launch_bounds__(WARPS* kWarp) few_kernel(const Args A) {
     ws[i] = live ? A.ws[c] : 0.0f;
     wu[i] = GATED && live ? A.ws[A.n + c] : 0.0f;
     xs[i] = live ? A.xs[t] : 0.0f;
-    add[i] = live && A.bias ? __half2float(A.bias[c]) : 0.0f;
-    if (live && A.residual) add[i] += __half2float(A.residual[static_cast<size_t>(t) * A.ldr + c]);
+    bias[i] = live && A.bias ? __half2float(A.bias[c]) : 0.0f;
+    res[i] = live && A.residual ? __half2float(A.residual[static_cast<size_t>(t) * A.ldr + c]) : 0.0f;
   }
 #pragma unroll
   for (int z = 0; z < kW; ++z)
@@ -157,9 +160,9 @@ __global__ void __launch_bounds__(WARPS* kWarp) few_kernel(const Args A) {
       g += red[v][0][t][row];
       if (GATED) u += red[v][kW - 1][t][row];
     }
-    float v = linear_value(g, xs[i], ws[i]);
+    float v = linear_value(g, xs[i], ws[i], bias[i]);
     if (GATED) v = silu_product(v, linear_value(u, xs[i], wu[i]));
-    A.y[static_cast<size_t>(t) * A.ldy + c0 + row] = __float2half_rn(v + add[i]);
+    A.y[static_cast<size_t>(t) * A.ldy + c0 + row] = __float2half_rn(v + res[i]);
   }
 }
 
@@ -496,10 +499,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     __half* y = A.y + static_cast<size_t>(t0 + j) * A.ldy + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e, y += A.ldy) {
-      float v = linear_value(g[e], xv[e], ws);
+      float v = linear_value(g[e], xv[e], ws, bias);
       if (GATED) v = silu_product(v, linear_value(u[e], xv[e], wu));
-      else v += bias + res[e];
-      if (j + e < tok) *y = __float2half_rn(v);
+      if (j + e < tok) *y = __float2half_rn(v + res[e]);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -758,8 +760,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
 #pragma unroll
             for (int l = 0; l < 4; ++l) {
               const int k = j + 4 * h + l;
-              const float lin = linear_value(static_cast<int>(g[i][k]), xs, wv[l]);
-              v[4 * h + l] = GATED ? silu_product(lin, linear_value(static_cast<int>(u[i][k]), xs, ov[l])) : lin + ov[l];
+              const int sum = static_cast<int>(g[i][k]);
+              v[4 * h + l] = GATED ? silu_product(linear_value(sum, xs, wv[l]),
+                                                  linear_value(static_cast<int>(u[i][k]), xs, ov[l]))
+                                   : linear_value(sum, xs, wv[l], ov[l]);
             }
           }
           uint4* to = reinterpret_cast<uint4*>(box + piece(lane, (32 * i + j) / 8));

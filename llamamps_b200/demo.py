@@ -72,6 +72,7 @@ def main(argv: Optional[Sequence[str]] = None, config: ModelConfig = QWEN2_5_1_5
     ap.add_argument("--ids", required=True, help="comma-separated prompt token ids")
     ap.add_argument("--new", type=int, default=16, help="tokens to generate")
     ap.add_argument("--kv-bits", type=int, choices=(4, 16), default=16, help="bits of the KV cache's elements")
+    ap.add_argument("--w8a8", action="store_true", help="8-bit projections in dense prefill and larger batches")
     a = ap.parse_args(argv)
     import torch
     from .engine import QwenEngine
@@ -80,10 +81,10 @@ def main(argv: Optional[Sequence[str]] = None, config: ModelConfig = QWEN2_5_1_5
     if a.synthetic:
         from .weights import synth_model
         engine = QwenEngine(weights=synth_model(config, seed=a.seed, device="cuda"), max_seq_len=max_seq,
-                            kv_bits=a.kv_bits)
+                            kv_bits=a.kv_bits, w8a8=a.w8a8)
         embed_row = engine.weights.embed[ids[0]].cpu().numpy()
     elif a.weights:
-        engine = QwenEngine(a.weights, config=config, max_seq_len=max_seq, kv_bits=a.kv_bits)
+        engine = QwenEngine(a.weights, config=config, max_seq_len=max_seq, kv_bits=a.kv_bits, w8a8=a.w8a8)
         embed_row, _ = get_input_vector(ids, os.path.join(a.weights, "global", "embed_tokens.bin"),
                                         hidden=config.hidden)
     else:

@@ -35,7 +35,7 @@ from . import kernels as K
 from ._lib import lib
 from .config import QWEN2_5_1_5B, ModelConfig
 from .kv_cache import PagedKVCache, PagedKVCacheQ4
-from .weights import ModelWeights, load_reference_layout
+from .weights import ModelWeights, add_q8, load_reference_layout
 
 
 # The CUDA-core GEMV serves up to 4 sequences; larger batches use the
@@ -89,7 +89,8 @@ class QwenEngine:
                  weights: Optional[ModelWeights] = None, config: ModelConfig = QWEN2_5_1_5B,
                  max_batch: int = 1, max_seq_len: int = 2048, page_size: int = 64,
                  use_graphs: bool = True, page_order: Optional[List[int]] = None,
-                 decoder: Optional[str] = None, gemv_max_batch: int = GEMV_MAX_BATCH, kv_bits: int = 16):
+                 decoder: Optional[str] = None, gemv_max_batch: int = GEMV_MAX_BATCH, kv_bits: int = 16,
+                 w8a8: bool = False):
         if kv_bits not in (4, 16):
             raise ValueError(f"kv_bits is 16 (fp16 cache) or 4, not {kv_bits}")
         if kv_bits == 4:  # the one-launch decoders read fp16 pools
@@ -113,6 +114,12 @@ class QwenEngine:
         self.max_batch = max_batch
         # batches above this run the projections and LM head on the tensor-core GEMM
         self.gemv_max_batch = gemv_max_batch
+        # w8a8: where the projections run on the tensor-core GEMM (dense prefill, steps of larger batches), their
+        # weights and activations are in 8 bits with a scale for each channel and token; smaller batches and the LM
+        # head keep the Q4 weights
+        self.w8a8 = w8a8
+        if w8a8:
+            add_q8(weights)
         self.use_graphs = use_graphs
         # kv_bits=4: keys and values in the 4-bit paged cache (72 bytes a row of 128 instead of 256); up to four
         # sequences it is slower than the persistent decoder that it goes without (1 x 2048: 1.75 ms a step, not 0.96)
@@ -162,6 +169,7 @@ class QwenEngine:
         # fused gate|up GEMM output (batched path): [B, 2 * intermediate]
         self.buf_up = torch.zeros(B if B > self.gemv_max_batch else 1, 2 * c.intermediate, dtype=h, device=dev)
         self.gemm_err = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.q8_rows = self._q8_buffer(B) if self.w8a8 and B > self.gemv_max_batch else None
         # split-K partial tiles of the small-m GEMMs (zero between calls)
         ws = K.w4a16_gemm_workspace_size(B, c.intermediate) if B > self.gemv_max_batch else 0
         self.gemm_ws = torch.zeros(ws + 256, dtype=torch.uint8, device=dev)
@@ -208,6 +216,12 @@ class QwenEngine:
         self.step_counter.zero_()
         self.host_pos = start_pos
 
+    def _q8_buffer(self, rows: int):
+        """Codes and scales of one projection's input at a time, for up to ``rows`` tokens."""
+        c = self.cfg
+        return (torch.empty(rows * max(c.hidden, c.q_dim, c.intermediate), dtype=torch.int8, device=self.device),
+                torch.empty(rows, dtype=torch.float32, device=self.device))
+
     # -- one forward over the current tokens/pos ----------------------------
     def _layers(self, B: int) -> None:
         c, w = self.cfg, self.weights
@@ -219,11 +233,10 @@ class QwenEngine:
         gemm = B > self.gemv_max_batch   # dense contraction: tcgen05 W4A16 GEMM
         for li, lw in enumerate(w.layers):
             kp, vp = self.cache.layer(li)
-            K.rms_norm(x, lw.in_norm, c.eps, out=xn)
             if gemm:
-                K.w4a16_gemm(xn, lw.qkv_packed, lw.qkv_scales, c.qkv_rows, c.hidden, bias=lw.qkv_bias,
-                             out=self.buf_qkv[:B], error=self.gemm_err, workspace=self.gemm_ws)
+                self._qkv_proj(lw, x, xn, self.buf_qkv[:B], q8=self.q8_rows)
             else:
+                K.rms_norm(x, lw.in_norm, c.eps, out=xn)
                 K.gemv_q4_bias(lw.qkv_packed, lw.qkv_scales, lw.qkv_bias, xn, c.qkv_rows, c.hidden,
                                out=self.buf_qkv[:B])
             # RoPE + KV append + attention in one launch (rope_kv_append's work
@@ -239,20 +252,47 @@ class QwenEngine:
                                             self.cache.block_table, self.seq_lens, self.buf_attn[:B],
                                             self.attn_ws, self.cache.page_size, c.n_q_heads, c.n_kv_heads,
                                             c.head_dim, self.max_seq_len, self.n_splits, c.rope_style_code)
-            self._o_proj(lw, self.buf_attn[:B], x, gemm)
-            K.rms_norm(x, lw.post_norm, c.eps, out=xn)
+            self._o_proj(lw, self.buf_attn[:B], x, gemm, q8=self.q8_rows)
             if gemm:
-                self._gate_up(lw, xn, self.buf_up[:B], self.buf_mlp[:B])
+                self._gate_up(lw, x, xn, self.buf_up[:B], self.buf_mlp[:B], q8=self.q8_rows)
             else:
+                K.rms_norm(x, lw.post_norm, c.eps, out=xn)
                 K.gemv_q4_swiglu(lw.gate_packed, lw.gate_scales, lw.up_packed, lw.up_scales, xn,
                                  c.intermediate, c.hidden, out=self.buf_mlp[:B])
-            self._down_proj(lw, self.buf_mlp[:B], x, gemm)
+            self._down_proj(lw, self.buf_mlp[:B], x, gemm, q8=self.q8_rows)
 
-    def _gate_up(self, lw, xn, gu, out, ws=None) -> None:
-        """a = SwiGLU(W_gate xn, W_up xn) on the GEMM path: one GEMM over the
+    def _w8a8(self, rows, weight, out, **epilogue) -> None:
+        """out = 8-bit rows (codes, scales) times an 8-bit weight of the layer."""
+        K.w8a8_gemm(*rows, *weight, out=out, error=self.gemm_err, **epilogue)
+
+    @staticmethod
+    def _q8_view(q8, x):
+        """The buffer of _q8_buffer as (codes, scales) for x's shape."""
+        return q8[0][:x.numel()].view(x.shape), q8[1][:x.shape[0]]
+
+    def _norm_q8(self, x, gamma, q8):
+        codes, scales = self._q8_view(q8, x)
+        return K.rms_norm_q8(x, gamma, self.cfg.eps, codes=codes, scales=scales)
+
+    def _qkv_proj(self, lw, x, xn, out, ws=None, q8=None) -> None:
+        """out = W_qkv norm(x) + bias on the GEMM path (xn: the norm's rows; q8: the 8-bit path's buffer)."""
+        c = self.cfg
+        if q8 is not None:
+            self._w8a8(self._norm_q8(x, lw.in_norm, q8), lw.q8.qkv, out, bias=lw.qkv_bias)
+            return
+        K.rms_norm(x, lw.in_norm, c.eps, out=xn)
+        K.w4a16_gemm(xn, lw.qkv_packed, lw.qkv_scales, c.qkv_rows, c.hidden, bias=lw.qkv_bias, out=out,
+                     error=self.gemm_err, workspace=self._ws(ws))
+
+    def _gate_up(self, lw, x, xn, gu, out, ws=None, q8=None) -> None:
+        """a = SwiGLU(W_gate xn, W_up xn) with xn = norm(x) on the GEMM path: one GEMM over the
         interleaved gate/up rows with the SwiGLU epilogue when the layer has
         them, else two GEMMs and the SwiGLU kernel."""
         c = self.cfg
+        if q8 is not None:
+            self._w8a8(self._norm_q8(x, lw.post_norm, q8), lw.q8.gate_up, out, swiglu=True)
+            return
+        K.rms_norm(x, lw.post_norm, c.eps, out=xn)
         if lw.gu_packed is not None:
             K.w4a16_gemm(xn, lw.gu_packed, lw.gu_scales, 2 * c.intermediate, c.hidden, swiglu=True, out=out,
                          error=self.gemm_err, workspace=self._ws(ws))
@@ -271,17 +311,21 @@ class QwenEngine:
         none (unsplit) for the token rows of a dense prefill (ws=False)."""
         return None if ws is False else (ws if ws is not None else self.gemm_ws)
 
-    def _o_proj(self, lw, att, x, gemm: bool, ws=None) -> None:
+    def _o_proj(self, lw, att, x, gemm: bool, ws=None, q8=None) -> None:
         c = self.cfg
-        if gemm:
+        if gemm and q8 is not None:
+            self._w8a8(K.quantise_rows_q8(att, *self._q8_view(q8, att)), lw.q8.o, x, residual=x)
+        elif gemm:
             K.w4a16_gemm(att, lw.o_packed, lw.o_scales, c.hidden, c.q_dim, residual=x, out=x,
                          error=self.gemm_err, workspace=self._ws(ws))
         else:
             K.gemv_q4_residual(lw.o_packed, lw.o_scales, att, x, c.hidden, c.q_dim, out=x)
 
-    def _down_proj(self, lw, a, x, gemm: bool, ws=None) -> None:
+    def _down_proj(self, lw, a, x, gemm: bool, ws=None, q8=None) -> None:
         c = self.cfg
-        if gemm:
+        if gemm and q8 is not None:
+            self._w8a8(K.quantise_rows_q8(a, *self._q8_view(q8, a)), lw.q8.down, x, residual=x)
+        elif gemm:
             K.w4a16_gemm(a, lw.down_packed, lw.down_scales, c.hidden, c.intermediate, residual=x, out=x,
                          error=self.gemm_err, workspace=self._ws(ws))
         else:
@@ -417,13 +461,14 @@ class QwenEngine:
             return 1 + 1 + 1 + 2 + 1
         # norm, q|k|v, RoPE + append + attention (+ split combine), o, norm,
         # gate/up (+ SwiGLU on the GEMM path), down; then embed, final norm, the
-        # LM head with its argmax (two launches on either path), advance
+        # LM head with its argmax (two launches on either path), advance; the 8-bit path has a quantiser before o and
+        # before down instead of the SwiGLU kernel
         gemm = self.batch > self.gemv_max_batch
         if self.kv_bits == 4:
             attn = K.attention_q4_launches(self.n_splits, self.max_seq_len)
         else:
             attn = 2 if self.n_splits > 1 else 1
-        per_layer = 6 + attn + (1 if gemm else 0)
+        per_layer = 6 + attn + ((2 if self.w8a8 else 1) if gemm else 0)
         return 1 + self.layers * per_layer + 1 + 2 + 1
 
     def step_tokens(self, token_ids) -> np.ndarray:
@@ -443,6 +488,7 @@ class QwenEngine:
         if self.bdec is not None:
             self.bdec.check_error()
         self.check_kv_error()
+        self.check_gemm_error()
         return self._pin_next.numpy()[:B].copy()
 
     def decode_step(self, record: bool = True) -> None:
@@ -511,7 +557,7 @@ class QwenEngine:
 
     def prefill_dense(self, prompts: torch.Tensor) -> None:
         """All B*P prompt tokens through every layer at once: the projections
-        are W4A16 tensor-core GEMMs over M = B*P token rows, RoPE and the KV
+        are tensor-core GEMMs (W4A16, or W8A8 with ``w8a8``) over M = B*P token rows, RoPE and the KV
         append run on every (sequence, position) row, and the causal
         attention of all rows is one flash-attention launch over the paged
         cache.  The LM head runs on each sequence's last row only.  With the
@@ -533,7 +579,8 @@ class QwenEngine:
         q = torch.empty(Mt, c.q_dim, dtype=h, device=dev)
         att = torch.empty(Mt, c.q_dim, dtype=h, device=dev)
         gate = torch.empty(Mt, c.intermediate, dtype=h, device=dev)
-        gu = torch.empty(Mt, 2 * c.intermediate, dtype=h, device=dev)
+        gu = None if self.w8a8 else torch.empty(Mt, 2 * c.intermediate, dtype=h, device=dev)
+        q8 = self._q8_buffer(Mt) if self.w8a8 else None
         err = self.gemm_err
         if q4:  # the prompt's queries attend to what is cached before them, too
             starts = torch.full((B,), start, dtype=i32, device=dev)
@@ -543,9 +590,7 @@ class QwenEngine:
         K.embed_gather(w.embed, ids, x, self.bad_ids)
         for li, lw in enumerate(w.layers):
             kp, vp = self.cache.layer(li)
-            K.rms_norm(x, lw.in_norm, c.eps, out=xn)
-            K.w4a16_gemm(xn, lw.qkv_packed, lw.qkv_scales, c.qkv_rows, c.hidden, bias=lw.qkv_bias,
-                         out=qkv, error=err)
+            self._qkv_proj(lw, x, xn, qkv, ws=False, q8=q8)
             if q4:
                 K.rope_kv_append_q4(qkv, rows_pos, self.inv_freq, q, kp, vp, rows_bt, self.cache.page_size,
                                     c.n_q_heads, c.n_kv_heads, c.head_dim, c.rope_style_code, error=self.kv_err)
@@ -557,10 +602,9 @@ class QwenEngine:
                                  c.n_q_heads, c.n_kv_heads, c.head_dim, c.rope_style_code)
                 K.prefill_attention(q, kp, vp, self.cache.block_table[:B], att, B, P, self.cache.page_size,
                                     c.n_q_heads, c.n_kv_heads, c.head_dim, error=err)
-            self._o_proj(lw, att, x, True, ws=False)
-            K.rms_norm(x, lw.post_norm, c.eps, out=xn)
-            self._gate_up(lw, xn, gu, gate, ws=False)
-            self._down_proj(lw, gate, x, True, ws=False)
+            self._o_proj(lw, att, x, True, ws=False, q8=q8)
+            self._gate_up(lw, x, xn, gu, gate, ws=False, q8=q8)
+            self._down_proj(lw, gate, x, True, ws=False, q8=q8)
         # last position of every sequence -> final norm, LM head, argmax
         self.buf_residual[:B].copy_(x.view(B, P, c.hidden)[:, P - 1])
         self._head(B, want_logits=False)
@@ -632,9 +676,16 @@ class QwenEngine:
             self.bad_ids.zero_()
             raise ValueError("token id outside the vocabulary")
         self.check_kv_error()
+        self.check_gemm_error()
         # decode_advance writes row-major [step, B] with the active batch as stride
         hist = self.history.reshape(-1)[: max_new_tokens * B].reshape(max_new_tokens, B)
         return hist.t().cpu().numpy()
+
+    def check_gemm_error(self) -> None:
+        """Raises if a W8A8 product's wait on the device ran out since the last check."""
+        if self.w8a8 and int(self.gemm_err.item()):
+            self.gemm_err.zero_()
+            raise RuntimeError("tensor-core GEMM: a wait on the device timed out")
 
     def check_kv_error(self) -> None:
         """Raises if a kernel of the 4-bit cache reported an error since the last check."""

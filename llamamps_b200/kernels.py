@@ -552,15 +552,13 @@ def _q8_shape(t: torch.Tensor, name: str):
     return (1 if t.dim() == 1 else t.shape[0]), t.shape[-1]
 
 
-def _q8_codes(x: torch.Tensor, codes, scales):
+def _q8_outputs(x: torch.Tensor, codes, scales):
     """Codes (rows start at multiples of 16 bytes) and scales for x's rows where they are not given."""
     rows, k = _q8_shape(x, "x")
     if codes is None:
         codes = torch.empty(rows, -(-k // 16) * 16, dtype=_I8, device=x.device)[:, :k]
         codes = codes if x.dim() == 2 else codes[0]
-    if scales is None:
-        scales = torch.empty(rows, dtype=_F32, device=x.device)
-    return rows, k, codes, scales
+    return codes, torch.empty(rows, dtype=_F32, device=x.device) if scales is None else scales
 
 
 def quantise_rows_q8(x, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
@@ -570,9 +568,11 @@ def quantise_rows_q8(x, codes: Optional[torch.Tensor] = None, scales: Optional[t
     zero row has scale 0, a row with a NaN or an infinity scale NaN.  Without
     ``codes``, the result's rows start at multiples of 16 bytes, as
     :func:`w8a8_gemm` needs them.  ``values`` (fp16) receives code * scale."""
-    rows, k, codes, scales = _q8_codes(x, codes, scales)
+    if codes is None or scales is None:
+        codes, scales = _q8_outputs(x, codes, scales)
     if _q4_done(binding_q8().quantise(x, codes, scales, values), "lmps_quantise_rows_q8"):
         return codes, scales
+    rows, k = _q8_shape(x, "x")
     dev = x.get_device()
     a_x, ldx = _q8_arg(x, "x", FP16, dev, rows, k)
     a_c, ldc = _q8_arg(codes, "codes", _I8, dev, rows, k)
@@ -590,15 +590,18 @@ def rms_norm_q8(x, gamma, eps: float = 1e-6, *, residual: Optional[torch.Tensor]
     gives it (of the unrounded norm): (codes, scales).  With ``residual`` the
     norm is of s = fp16(residual + x), which ``sum_out`` receives: (codes,
     scales, sum).  ``sum_out`` may be ``residual`` or ``x`` itself."""
-    rows, k, codes, scales = _q8_codes(x, codes, scales)
-    eps = float(eps)
-    if residual is None and sum_out is not None:
-        raise ValueError("sum_out: only with a residual")
-    if residual is not None and sum_out is None:
+    if codes is None or scales is None:
+        codes, scales = _q8_outputs(x, codes, scales)
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError("sum_out: only with a residual")
+    elif sum_out is None:
         sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    eps = float(eps)
     done = (codes, scales) if residual is None else (codes, scales, sum_out)
     if _q4_done(binding_q8().norm(x, gamma, eps, residual, sum_out, codes, scales, values), "lmps_rms_norm_q8"):
         return done
+    rows, k = _q8_shape(x, "x")
     dev = x.get_device()
     a_x, ldx = _q8_arg(x, "x", FP16, dev, rows, k)
     a_g = _q8_vector(gamma, "gamma", FP16, dev, k)
@@ -625,6 +628,9 @@ def w8a8_gemm(codes, scales, w_codes, w_scales, *, bias: Optional[torch.Tensor] 
     out; without it the call waits for the kernel and raises that (so a graph
     capture needs one)."""
     gated = 1 if swiglu else 0
+    if out is not None and error is not None and _q4_done(
+            binding_q8().gemm(codes, scales, w_codes, w_scales, bias, residual, gated, out, error), "lmps_w8a8_gemm"):
+        return out
     m, k = _q8_shape(codes, "codes")
     w_rows, _ = _q8_shape(w_codes, "w_codes")
     if gated and w_rows % 2:
@@ -641,9 +647,6 @@ def w8a8_gemm(codes, scales, w_codes, w_scales, *, bias: Optional[torch.Tensor] 
         w8a8_gemm(codes, scales, w_codes, w_scales, bias=bias, residual=residual, swiglu=swiglu, out=out, error=error)
         if int(error.item()):
             raise RuntimeError("w8a8_gemm: a wait for the tensor core timed out")
-        return out
-    if _q4_done(binding_q8().gemm(codes, scales, w_codes, w_scales, bias, residual, gated, out, error),
-                "lmps_w8a8_gemm"):
         return out
     dev = codes.get_device()
     a_x, ldx = _q8_arg(codes, "codes", _I8, dev, m, k)

@@ -38,6 +38,13 @@ def pack_q4(w: torch.Tensor):
     return pack_q4_host(w)
 
 
+def unpack_q4(packed: torch.Tensor, scales: torch.Tensor, rows: int, k: int) -> torch.Tensor:
+    """The fp16 [rows, k] values of a Q4 matrix (code * scale, rounded once)."""
+    p = packed.reshape(-1, GROUP // 2)
+    c = torch.stack([p & 15, p >> 4], dim=-1).flatten(-2).to(torch.float32) - 8.0
+    return (c * scales.reshape(-1, 1).to(torch.float32)).to(torch.float16).reshape(rows, k)
+
+
 # -- rows of the 4-bit KV cache (include/llamamps_b200.h, "4-bit KV cache") ----
 KV_ROW_BYTES = 72     # 64 code bytes and 4 fp16 scales for 128 elements
 

@@ -201,9 +201,11 @@ class TPEngine(QwenEngine):
         return self._part[:rows] if rows <= self._part.shape[0] else torch.empty(
             rows, self.cfg.hidden, dtype=torch.float16, device=self.device)
 
-    def _o_proj(self, lw, att, x, gemm: bool, ws=None) -> None:
+    def _o_proj(self, lw, att, x, gemm: bool, ws=None, q8=None) -> None:
         c, part = self.cfg, self._partial(x.shape[0])
-        if gemm:
+        if gemm and q8 is not None:
+            self._w8a8(K.quantise_rows_q8(att, *self._q8_view(q8, att)), lw.q8.o, part)
+        elif gemm:
             K.w4a16_gemm(att, lw.o_packed, lw.o_scales, c.hidden, c.q_dim, out=part, error=self.gemm_err,
                          workspace=self._ws(ws))
         elif self._fused(x):
@@ -214,9 +216,11 @@ class TPEngine(QwenEngine):
             K.gemv_q4(lw.o_packed, lw.o_scales, att, c.hidden, c.q_dim, out=part)
         self._reduce_add(part, x, self._site[id(lw)])
 
-    def _down_proj(self, lw, a, x, gemm: bool, ws=None) -> None:
+    def _down_proj(self, lw, a, x, gemm: bool, ws=None, q8=None) -> None:
         c, part = self.cfg, self._partial(x.shape[0])
-        if gemm:
+        if gemm and q8 is not None:
+            self._w8a8(K.quantise_rows_q8(a, *self._q8_view(q8, a)), lw.q8.down, part)
+        elif gemm:
             K.w4a16_gemm(a, lw.down_packed, lw.down_scales, c.hidden, c.intermediate, out=part,
                          error=self.gemm_err, workspace=self._ws(ws))
         elif self._fused(x):

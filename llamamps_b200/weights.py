@@ -29,9 +29,19 @@ import numpy as np
 import torch
 
 from .config import ModelConfig
-from .quant import pack_q4, pack_q4_host
+from .quant import pack_q4, pack_q4_host, unpack_q4
 
 _MATS = ("q", "k", "v", "o", "gate", "up", "down")
+
+
+@dataclasses.dataclass
+class LayerQ8:
+    """A layer's projections in 8 bits: (int8 codes [rows, k], fp32 scale of each row) as
+    :func:`kernels.quantise_rows_q8` makes them; ``gate_up`` holds the gate rows, then the up rows."""
+    qkv: tuple
+    o: tuple
+    gate_up: tuple
+    down: tuple
 
 
 @dataclasses.dataclass
@@ -54,6 +64,8 @@ class LayerWeights:
     # when absent (two GEMMs and a SwiGLU kernel instead).
     gu_packed: Optional[torch.Tensor] = None
     gu_scales: Optional[torch.Tensor] = None
+    # 8-bit copies for the W8A8 path (add_q8)
+    q8: Optional[LayerQ8] = None
 
     def q4_bytes(self) -> int:
         ts = [self.qkv_packed, self.qkv_scales, self.o_packed, self.o_scales, self.gate_packed,
@@ -86,6 +98,23 @@ def interleave_rows(a: torch.Tensor, b: torch.Tensor, rows: int) -> torch.Tensor
     is a's row t, row 2t + 1 is b's (the gate/up layout of the GEMM's SwiGLU
     epilogue)."""
     return torch.stack([a.reshape(rows, -1), b.reshape(rows, -1)], dim=1).reshape(-1).contiguous()
+
+
+def add_q8(mw: "ModelWeights") -> None:
+    """Gives every layer on the device its 8-bit copies: the values of the Q4 matrices with one scale a row
+    instead of one for each 32 elements (1.31 GB for the 1.5B model)."""
+    from .kernels import quantise_rows_q8
+    c = mw.cfg
+    for lw in mw.layers:
+        if lw.q8 is None:
+            qkv = unpack_q4(lw.qkv_packed, lw.qkv_scales, c.qkv_rows, c.hidden)
+            gate_up = torch.cat([unpack_q4(lw.gate_packed, lw.gate_scales, c.intermediate, c.hidden),
+                                 unpack_q4(lw.up_packed, lw.up_scales, c.intermediate, c.hidden)])
+            lw.q8 = LayerQ8(qkv=quantise_rows_q8(qkv), gate_up=quantise_rows_q8(gate_up),
+                            o=quantise_rows_q8(unpack_q4(lw.o_packed, lw.o_scales, c.hidden, c.q_dim)),
+                            down=quantise_rows_q8(unpack_q4(lw.down_packed, lw.down_scales, c.hidden,
+                                                            c.intermediate)))
+    torch.cuda.synchronize(mw.device)  # (they may be used on any stream)
 
 
 def layer_from_parts(cfg: ModelConfig, parts: Dict[str, torch.Tensor], device) -> LayerWeights:

@@ -224,6 +224,23 @@ def test_gate_values_of_any_size(cuda, m, n):
     R.check_gated(K.w8a8_gemm(x, xs, w, ws, swiglu=True), x, xs, w, ws)
 
 
+@pytest.mark.parametrize("n,k,form", [(320, 1536, "both"), (200, 4480, "bias"), (131, 257, "residual"), (192, 640, "gated"),
+                                      (1500, 768, "none")])
+def test_a_token_does_not_depend_on_its_call(cuda, n, k, form):
+    """Bit for bit: the rows of a call of 700 tokens, of calls of the first few, and each alone."""
+    m, gated = 700, form == "gated"
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g, x, xs, w, ws = _operands(m, 2 * n if gated else n, k, 5)
+    bias = torch.randn(n, generator=g, device="cuda").half() if form in ("bias", "both") else None
+    res = torch.randn(m, n, generator=g, device="cuda").half() if form in ("residual", "both") else None
+    y = K.w8a8_gemm(x, xs, w, ws, bias=bias, residual=res, swiglu=gated, error=err)
+    for a, b in ((0, 1), (3, 11), (5, 20), (0, 32), (7, 71), (100, 200), (0, 257), (699, 700)):
+        part = K.w8a8_gemm(x[a:b], xs[a:b], w, ws, bias=bias, residual=None if res is None else res[a:b], swiglu=gated,
+                           error=err)
+        assert torch.equal(part, y[a:b]), (a, b)
+    assert int(err) == 0
+
+
 # -- as they are used ----------------------------------------------------------------
 def _block(x, part, gamma, wq, err, out=None):
     """Residual and norm, the gated projections, the quantiser, the down projection onto the residual stream."""
