@@ -11,7 +11,7 @@
 // the sum of squares come from one reduction.  A zero row has codes and scale
 // 0, a row with a NaN or an infinity codes 0 and scale NaN.  127 v / m is one
 // rounding of 127 / m and one fused multiply-add that rounds to the integer;
-// where that quotient is within 2^-16 of a tie (an element that is half the
+// where that quotient is within rounding of a tie (an element that is half the
 // largest is one), the code comes from fp64, so every code is the formula's.
 //
 // What bounds it: bytes (a row in once, codes and sum out once).
@@ -37,31 +37,54 @@ struct RowArgs {
   float eps;
 };
 
-constexpr int kCta = 256;                    // threads of a CTA
-constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: adding it rounds to an integer, half to even
-constexpr float kNearTie = 0.5f - 1.0f / 65536.0f;
-
-// Over the T threads of a row: the sum of ss and the largest of the bits of m
-// (|v| as an unsigned number: a NaN is above infinity).
+constexpr int kCta = 256;  // threads of a CTA, but where a row has more
 template <int T>
-__device__ __forceinline__ void reduce_row(float& ss, uint32_t& m) {
+constexpr int kCtaOf = T > kCta ? T : kCta;
+constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even, in the low bits
+constexpr float kNearTie = 0.5f - 7.8e-6f;  // (127 / m is off by 2^-24 of itself, so a quotient by 127 x 2^-24 = 7.6e-6)
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // (a NaN stays)
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+// Two fp32 operations at once.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 both(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// Over the T threads of a row: the sum of ss and the largest m (|v|; a NaN stays) as its bits.
+template <int T>
+__device__ __forceinline__ void reduce_row(float& ss, float m, uint32_t& mbits) {
   ss = warp_sum(ss);
-  m = __reduce_max_sync(0xffffffffu, m);
+  mbits = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7FFFFFFFu);  // (a NaN's bits are above infinity's)
   if constexpr (T > kWarp) {
-    __shared__ float rs[T / kWarp];
-    __shared__ uint32_t rm[T / kWarp];
-    const int warp = threadIdx.x / kWarp;
+    __shared__ float rs[kCtaOf<T> / kWarp];
+    __shared__ uint32_t rm[kCtaOf<T> / kWarp];
+    const int warp = threadIdx.x / kWarp, first = warp / (T / kWarp) * (T / kWarp);
     if (threadIdx.x % kWarp == 0) {
       rs[warp] = ss;
-      rm[warp] = m;
+      rm[warp] = mbits;
     }
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + first / (T / kWarp)), "n"(T) : "memory");
     ss = 0.0f;
-    m = 0u;
+    mbits = 0u;
 #pragma unroll
     for (int w = 0; w < T / kWarp; ++w) {
-      ss += rs[w];
-      m = max(m, rm[w]);
+      ss += rs[first + w];
+      mbits = max(mbits, rm[first + w]);
     }
   }
 }
@@ -79,25 +102,27 @@ __device__ __forceinline__ void row_scale(const RowArgs& A, float ss, uint32_t m
   }
 }
 
-// The codes of N elements, as integers in fp32.
-template <int N>
-__device__ __forceinline__ void row_codes(const float (&v)[N], float inv, uint32_t mbits, float (&c)[N]) {
-  float far = 0.0f;  // the largest distance from an integer
+// The codes of eight elements, in the low bytes of t (and as t - kMagic).
+__device__ __forceinline__ void row_codes(const float (&v)[8], float inv, uint32_t mbits, float (&t)[8]) {
+  const uint64_t inv2 = pair2(inv, inv), magic2 = pair2(kMagic, kMagic), minus2 = pair2(-1.0f, -1.0f);
+  float far = 0.0f;  // the largest distance of a quotient from its code
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    c[i] = fmaf(v[i], inv, kMagic) - kMagic;
-    far = fmaxf(far, fabsf(fmaf(v[i], inv, -c[i])));
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t v2 = pair2(v[i], v[i + 1]), t2 = fma2(v2, inv2, magic2);
+    const float2 f = both(t2), d = both(fma2(v2, inv2, fma2(t2, minus2, magic2)));
+    t[i] = f.x, t[i + 1] = f.y;
+    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
   }
   if (far > kNearTie) {
     const double m = static_cast<double>(__uint_as_float(mbits));
 #pragma unroll
-    for (int i = 0; i < N; ++i) c[i] = static_cast<float>(rint(127.0 * static_cast<double>(v[i]) / m));
+    for (int i = 0; i < 8; ++i) t[i] = static_cast<float>(rint(127.0 * static_cast<double>(v[i]) / m)) + kMagic;
   }
 }
 
-__device__ __forceinline__ uint32_t pack4(const float* c) {
-  return (static_cast<uint32_t>(static_cast<int>(c[0])) & 0xFFu) | (static_cast<uint32_t>(static_cast<int>(c[1])) & 0xFFu) << 8 |
-         (static_cast<uint32_t>(static_cast<int>(c[2])) & 0xFFu) << 16 | static_cast<uint32_t>(static_cast<int>(c[3])) << 24;
+__device__ __forceinline__ uint32_t pack4(const float* t) {  // four low bytes
+  return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                     __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ void unpack8(const uint4& p, float (&f)[8]) {
@@ -116,14 +141,14 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return p;
 }
 
-// 16-byte pieces of eight elements, T threads a row (32: eight rows a CTA), at most E pieces a thread.
+// 16-byte pieces of eight elements, T threads a row, at most E pieces a thread.
 template <int T, int E>
-__global__ void __launch_bounds__(kCta) rows_vec_kernel(const RowArgs A) {
+__global__ void __launch_bounds__(kCtaOf<T>) rows_vec_kernel(const RowArgs A) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
   const int t = threadIdx.x % T;
-  const size_t row = static_cast<size_t>(blockIdx.x) * (kCta / T) + threadIdx.x / T;
-  if (row >= static_cast<size_t>(A.rows)) return;  // (whole warps, or none: T = 256 has a CTA per row)
+  const size_t row = static_cast<size_t>(blockIdx.x) * (kCtaOf<T> / T) + threadIdx.x / T;
+  if (row >= static_cast<size_t>(A.rows)) return;  // (all T threads of the row)
   const int pieces = A.k / 8;
   const uint4* x = reinterpret_cast<const uint4*>(A.x + row * A.ldx);
   const uint4* gamma = reinterpret_cast<const uint4*>(A.gamma);
@@ -150,153 +175,182 @@ __global__ void __launch_bounds__(kCta) rows_vec_kernel(const RowArgs A) {
         sum[t + T * i] = s[i];
       }
   }
-  float ss = 0.0f;
-  uint32_t m = 0u;
+  float ss = 0.0f, m = 0.0f;
+  if (gamma) {
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (t + T * i < pieces) {
-      float f[8];
-      unpack8(s[i], f);
-      if (gamma) {
-        float g[8];
+    for (int i = 0; i < E; ++i)
+      if (t + T * i < pieces) {
+        float f[8], g[8];
+        unpack8(s[i], f);
         unpack8(gamma[t + T * i], g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           ss = fmaf(f[e], f[e], ss);
-          m = max(m, __float_as_uint(f[e] * g[e]) & 0x7FFFFFFFu);
+          m = max_nan(m, fabsf(f[e] * g[e]));
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[e]) & 0x7FFFFFFFu);
       }
-    }
-  reduce_row<T>(ss, m);
+  } else {
+    __half2 m2 = __float2half2_rn(0.0f);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (t + T * i < pieces) {
+        const __half2* h = reinterpret_cast<const __half2*>(&s[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m2 = __hmax2_nan(m2, __habs2(h[e]));
+      }
+    m = max_nan(__low2float(m2), __high2float(m2));
+  }
+  uint32_t mbits;
+  reduce_row<T>(ss, m, mbits);
   float inv, scale;
-  row_scale(A, ss, m, inv, scale);
+  row_scale(A, ss, mbits, inv, scale);
   if (t == 0) A.scales[row] = scale;
-  const bool dead = m >= 0x7F800000u;
+  const bool dead = mbits >= 0x7F800000u;
   uint2* codes = reinterpret_cast<uint2*>(A.codes + row * A.ldc);
   uint4* values = A.values ? reinterpret_cast<uint4*>(A.values + row * A.ldv) : nullptr;
 #pragma unroll
   for (int i = 0; i < E; ++i)
     if (t + T * i < pieces) {
       float f[8], c[8];
+      if (dead) s[i] = make_uint4(0u, 0u, 0u, 0u);
       unpack8(s[i], f);
       if (gamma) {
         float g[8];
         unpack8(gamma[t + T * i], g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= g[e];
+        for (int e = 0; e < 8; ++e) f[e] = dead ? 0.0f : f[e] * g[e];
       }
-      if (dead)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-      row_codes(f, inv, m, c);
+      row_codes(f, inv, mbits, c);
       codes[t + T * i] = make_uint2(pack4(c), pack4(c + 4));
       if (values) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] *= scale;
+        for (int e = 0; e < 8; ++e) c[e] = (c[e] - kMagic) * scale;
         values[t + T * i] = pack8(c);
       }
     }
 }
 
-// Any length, stride and alignment: element t + T i of a row in thread t, the first E of a thread in registers,
-// later ones (rows past T E elements) read again, the sum from what this thread wrote.
+// Any length, stride and alignment: element t + T i of a row in thread t, the first 8 E of a thread in registers,
+// later ones (rows past 8 T E elements) read again, the sum from what this thread wrote.
 template <int T, int E>
-__global__ void __launch_bounds__(kCta) rows_any_kernel(const RowArgs A) {
+__global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
   const int t = threadIdx.x % T;
-  const size_t row = static_cast<size_t>(blockIdx.x) * (kCta / T) + threadIdx.x / T;
+  const size_t row = static_cast<size_t>(blockIdx.x) * (kCtaOf<T> / T) + threadIdx.x / T;
   if (row >= static_cast<size_t>(A.rows)) return;
   const __half* x = A.x + row * A.ldx;
   const __half* r = A.residual ? A.residual + row * A.ldr : nullptr;
   __half* sum = A.residual ? A.sum + row * A.lds : nullptr;
-  __half s[E];
+  const __half none = __ushort_as_half(0);
+  // elements base + T j for j < 8 (zero past the row); the sum is written on the way
+  auto load8 = [&](int base, __half (&s)[8]) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) s[i] = t + T * i < A.k ? x[t + T * i] : __half(0.0f);
-  if (r) {
-    __half b[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) b[i] = t + T * i < A.k ? r[t + T * i] : __half(0.0f);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      s[i] = __float2half_rn(__half2float(b[i]) + __half2float(s[i]));
-      if (t + T * i < A.k) sum[t + T * i] = s[i];
-    }
-  }
-  float ss = 0.0f;
-  uint32_t m = 0u;
-  auto take = [&](int i, float f) {
-    if (A.gamma) {
-      ss = fmaf(f, f, ss);
-      f *= __half2float(A.gamma[i]);
-    }
-    m = max(m, __float_as_uint(f) & 0x7FFFFFFFu);
-  };
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (t + T * i < A.k) take(t + T * i, __half2float(s[i]));
-  for (int i = t + T * E; i < A.k; i += T) {
-    __half v = x[i];
+    for (int j = 0; j < 8; ++j) s[j] = base + T * j < A.k ? x[base + T * j] : none;
     if (r) {
-      v = __float2half_rn(__half2float(r[i]) + __half2float(v));
-      sum[i] = v;
+      __half b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = base + T * j < A.k ? r[base + T * j] : none;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[j] = __float2half_rn(__half2float(b[j]) + __half2float(s[j]));
+        if (base + T * j < A.k) sum[base + T * j] = s[j];
+      }
     }
-    take(i, __half2float(v));
+  };
+  float ss = 0.0f, m = 0.0f;
+  auto stat8 = [&](int base, const __half (&s)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f = __half2float(s[j]);
+      if (A.gamma) {
+        ss = fmaf(f, f, ss);
+        f *= base + T * j < A.k ? __half2float(A.gamma[base + T * j]) : 0.0f;
+      }
+      m = max_nan(m, fabsf(f));
+    }
+  };
+  __half s[E][8];
+#pragma unroll
+  for (int i = 0; i < E; ++i) load8(t + 8 * T * i, s[i]);
+#pragma unroll
+  for (int i = 0; i < E; ++i) stat8(t + 8 * T * i, s[i]);
+  for (int base = t + 8 * T * E; base < A.k; base += 8 * T) {
+    __half v[8];
+    load8(base, v);
+    stat8(base, v);
   }
-  reduce_row<T>(ss, m);
+  uint32_t mbits;
+  reduce_row<T>(ss, m, mbits);
   float inv, scale;
-  row_scale(A, ss, m, inv, scale);
+  row_scale(A, ss, mbits, inv, scale);
   if (t == 0) A.scales[row] = scale;
-  const bool dead = m >= 0x7F800000u;
+  const bool dead = mbits >= 0x7F800000u;
   int8_t* codes = A.codes + row * A.ldc;
   __half* values = A.values ? A.values + row * A.ldv : nullptr;
-  auto give = [&](int i, float f) {
-    float v[1] = {A.gamma ? f * __half2float(A.gamma[i]) : f}, c[1];
-    if (dead) v[0] = 0.0f;
-    row_codes(v, inv, m, c);
-    codes[i] = static_cast<int8_t>(static_cast<int>(c[0]));
-    if (values) values[i] = __float2half_rn(c[0] * scale);
+  auto give8 = [&](int base, const __half (&s)[8]) {
+    float f[8], c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = __half2float(s[j]);
+      if (A.gamma) f[j] *= base + T * j < A.k ? __half2float(A.gamma[base + T * j]) : 0.0f;
+      if (dead) f[j] = 0.0f;
+    }
+    row_codes(f, inv, mbits, c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (base + T * j < A.k) {
+        codes[base + T * j] = static_cast<int8_t>(__float_as_uint(c[j]) & 0xFFu);
+        if (values) values[base + T * j] = __float2half_rn((c[j] - kMagic) * scale);
+      }
   };
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (t + T * i < A.k) give(t + T * i, __half2float(s[i]));
-  for (int i = t + T * E; i < A.k; i += T) give(i, __half2float(r ? sum[i] : x[i]));
+  for (int i = 0; i < E; ++i) give8(t + 8 * T * i, s[i]);
+  const __half* again = r ? sum : x;
+  for (int base = t + 8 * T * E; base < A.k; base += 8 * T) {
+    __half v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = base + T * j < A.k ? again[base + T * j] : none;
+    give8(base, v);
+  }
 }
 
 template <int T>
 static int launch(void (*kernel)(RowArgs), const RowArgs& A, cudaStream_t st) {
-  constexpr int per = kCta / T;
-  return lmps_launch_pdl(kernel, dim3((A.rows + per - 1) / per), dim3(kCta), 0, st, A);
+  constexpr int per = kCtaOf<T> / T;
+  return lmps_launch_pdl(kernel, dim3((A.rows + per - 1) / per), dim3(kCtaOf<T>), 0, st, A);
 }
 
-// A warp per row where there are rows enough to fill the GPU and a row fits a warp's registers.
-constexpr int kWarpRows = 592;
+// `pieces` of eight elements, T threads a row.
+template <int T>
+static int launch_threads(const RowArgs& A, bool vec, int pieces, cudaStream_t st) {
+  const int e = (pieces + T - 1) / T;
+  if (e <= 1) return launch<T>(vec ? rows_vec_kernel<T, 1> : rows_any_kernel<T, 1>, A, st);
+  if (e <= 2) return launch<T>(vec ? rows_vec_kernel<T, 2> : rows_any_kernel<T, 2>, A, st);
+  return launch<T>(vec ? rows_vec_kernel<T, 3> : rows_any_kernel<T, 3>, A, st);
+}
+
+// Threads a row: as few as hold it in three pieces each and still make half of the threads that fit 148 SMs (16384 x
+// 1536 with residual: 36 us with 64, 40 with 32, 44 with 128; 2048 x 1536: 6.8 us with 128, 7.8 with 256), else a CTA;
+// 1024 where there are few long rows (64 x 8960: 3.7 us, 4.2 with 256).
+constexpr long long kFill = 148ll * 1024;
 
 static int launch_rows(const RowArgs& A, cudaStream_t st) {
   const bool vec = A.k % 8 == 0 && A.ldx % 8 == 0 && A.ldc % 8 == 0 && A.ldr % 8 == 0 && A.lds % 8 == 0 &&
                    A.ldv % 8 == 0 && lmps_aligned(A.x, 16) && lmps_aligned(A.residual, 16) &&
                    lmps_aligned(A.sum, 16) && lmps_aligned(A.gamma, 16) && lmps_aligned(A.codes, 8) &&
-                   lmps_aligned(A.values, 16);
-  const int pieces = A.k / 8;
-  const bool many = A.rows >= kWarpRows;
-  if (vec && (many || pieces <= 32) && pieces <= 32 * 8) {
-    if (pieces <= 32 * 1) return launch<32>(rows_vec_kernel<32, 1>, A, st);
-    if (pieces <= 32 * 3) return launch<32>(rows_vec_kernel<32, 3>, A, st);
-    if (pieces <= 32 * 6) return launch<32>(rows_vec_kernel<32, 6>, A, st);
-    return launch<32>(rows_vec_kernel<32, 8>, A, st);
-  }
-  if (vec && pieces <= kCta * 8) {
-    if (pieces <= kCta * 1) return launch<kCta>(rows_vec_kernel<kCta, 1>, A, st);
-    if (pieces <= kCta * 3) return launch<kCta>(rows_vec_kernel<kCta, 3>, A, st);
-    if (pieces <= kCta * 5) return launch<kCta>(rows_vec_kernel<kCta, 5>, A, st);
-    return launch<kCta>(rows_vec_kernel<kCta, 8>, A, st);
-  }
-  if (A.k <= 32 * 16 && (many || A.k <= 64)) return launch<32>(rows_any_kernel<32, 16>, A, st);
-  if (A.k <= kCta * 8) return launch<kCta>(rows_any_kernel<kCta, 8>, A, st);
-  return launch<kCta>(rows_any_kernel<kCta, 36>, A, st);
+                   lmps_aligned(A.values, 16) && A.k <= kCta * 8 * 8;
+  const int pieces = (A.k + 7) / 8;
+  auto fits = [&](int t) { return pieces <= t || (pieces <= 3 * t && static_cast<long long>(A.rows) * t >= kFill); };
+  if (fits(32)) return launch_threads<32>(A, vec, pieces, st);
+  if (fits(64)) return launch_threads<64>(A, vec, pieces, st);
+  if (fits(128)) return launch_threads<128>(A, vec, pieces, st);
+  if (pieces <= 3 * kCta && (pieces <= kCta || A.rows * 1024ll > kFill))
+    return launch_threads<kCta>(A, vec, pieces, st);
+  if (pieces <= 1024 * 2 && A.rows * 1024ll <= kFill)
+    return launch<1024>(vec ? rows_vec_kernel<1024, 2> : rows_any_kernel<1024, 2>, A, st);
+  if (!vec) return launch<kCta>(rows_any_kernel<kCta, 5>, A, st);
+  return launch<kCta>(pieces <= 5 * kCta ? rows_vec_kernel<kCta, 5> : rows_vec_kernel<kCta, 8>, A, st);
 }
 
 }  // namespace q8
