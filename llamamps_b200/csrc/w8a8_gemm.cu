@@ -178,27 +178,31 @@ __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
+// Issued by the lane with `lead`, inside uniform code of the whole warp: descriptors then stay in uniform registers
+// (a branch to one lane moved each there, 16384 x 8960 x 1536 gated 324 us instead of 308).
 template <int GROUP>
-__device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc,
+                                       uint32_t lead) {
   if (GROUP == 2)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(
-            tmem),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
+        "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(
-            tmem),
-        "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
+        "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
 }
 // Completion of this thread's MMAs so far, to the barrier at this offset in both CTAs of the pair.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t lead) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}" ::"r"(
           smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(3)), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -216,11 +220,13 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 2-D TMA load into this CTA's shared memory that reports to a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar,
+                                              uint32_t lead) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
-      "%3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+      " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+      "{%2, %3}], [%4];\n}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
@@ -234,6 +240,32 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
                    reinterpret_cast<uint64_t>(map)),
                "r"(x), "r"(y), "r"(smem_u32(src))
                : "memory");
+}
+
+// Two fp32 operations at once.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 both(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// linear_value of two channels.
+__device__ __forceinline__ uint64_t linear2(uint32_t a0, uint32_t a1, uint64_t xs, uint64_t ws, uint64_t bias) {
+  return fma2(mul2(pair2(static_cast<float>(static_cast<int>(a0)), static_cast<float>(static_cast<int>(a1))), xs), ws, bias);
 }
 
 // 32 accumulator columns of this thread's TMEM lane on their way; tmem_arrived ends the wait for all such loads.
@@ -304,6 +336,10 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       return false;
     }
   }
+}
+// The wait of a whole warp (one that runs out does so for all of its lanes).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, abort_flag));
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -422,7 +458,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         const uint64_t xd = sw128_desc(smem_u32(xt + static_cast<size_t>(r.slot) * xbytes));
 #pragma unroll
         for (int j = 0; j < kBK / 32; ++j)  // K = 32 a MMA: 32 bytes further into the swizzle row
-          mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u);
+          mma_i8<1>(tmem, wd + 2 * j, xd + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u, 1u);
         mma_commit(&empty[r.slot]);
       }
       mma_commit(done);
@@ -450,9 +486,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp >= 2) {
     // (a wait that ran out leaves the sums without meaning; they still go out, so that no CTA waits for them)
-    bool ok = ksteps > 0;
-    if (lane == 0) ok = mbar_wait(done, 0, P.error, abort_v) && ok;
-    ok = __shfl_sync(0xffffffffu, ok, 0);
+    const bool ok = warp_wait(done, 0u, P.error, abort_v) && ksteps > 0;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const int q = warp & 3, row = 32 * q + lane;  // TMEM lane = row of the tile
     const int c = row % kOut, owner = c >> log_outs, local = (GATED ? row / 64 * outs : 0) + (c & (outs - 1));
@@ -601,65 +635,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      lmps_pdl_wait();  // both operands may be the previous kernel's output
-      Ring r;
-      int issued = 0;
-      bool ok = true;
-      for (int tile = pair; ok && tile < P.tiles; tile += pairs) {
-        const int c0 = (tile % P.tiles_n) * kOut, t0 = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128;
-        const int w0 = GATED ? static_cast<int>(rank) * A.n + c0 : c0 + static_cast<int>(rank) * (BN / 2);
-        for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
-          if (issued >= S && !mbar_wait(&empty[r.slot], r.phase ^ 1u, P.error, abort_v)) {
-            ok = false;
-            break;
-          }
-          // the first CTA's barrier counts the bytes of both
-          if (rank == 0) mbar_expect_tx(&full[r.slot], 2u * Sh::kStage);
-          const uint32_t bar = cluster_addr(&full[r.slot], 0);
-          unsigned char* x = stage + static_cast<size_t>(r.slot) * Sh::kStage;
-          tma_load_pair(x, &P.tx, kt * kBK, t0, bar);
-          tma_load_pair(x + Sh::kX, &P.tw, kt * kBK, w0, bar);
-          ++issued;
+    lmps_pdl_wait();  // both operands may be the previous kernel's output
+    const uint32_t lead = lane == 0 ? 1u : 0u, x0 = smem_u32(stage), bar0 = cluster_addr(full, 0);
+    Ring r;
+    int issued = 0;
+    bool ok = true;
+    for (int tile = pair; ok && tile < P.tiles; tile += pairs) {
+      const int c0 = (tile % P.tiles_n) * kOut, t0 = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128;
+      const int w0 = GATED ? static_cast<int>(rank) * A.n + c0 : c0 + static_cast<int>(rank) * (BN / 2);
+      for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
+        if (issued >= S && !warp_wait(&empty[r.slot], r.phase ^ 1u, P.error, abort_v)) {
+          ok = false;
+          break;
         }
-      }
-      // every copy has landed and every release of a stage has reached this CTA before it leaves
-      for (int g = max(0, issued - S); g < issued; ++g) {
-        const uint64_t since = globaltimer();
-        while (!mbar_try(&empty[g % S], (g / S) & 1))
-          if (globaltimer() - since > kTimeoutNs) break;
+        // the first CTA's barrier counts the bytes of both
+        if (rank == 0 && lane == 0) mbar_expect_tx(&full[r.slot], 2u * Sh::kStage);
+        const uint32_t x = x0 + static_cast<uint32_t>(r.slot) * Sh::kStage, bar = bar0 + 8u * static_cast<uint32_t>(r.slot);
+        tma_load_pair(x, &P.tx, kt * kBK, t0, bar, lead);
+        tma_load_pair(x + Sh::kX, &P.tw, kt * kBK, w0, bar, lead);
+        ++issued;
       }
     }
+    // every copy has landed and every release of a stage has reached this CTA before it leaves
+    for (int g = max(0, issued - S); lane == 0 && g < issued; ++g) {
+      const uint64_t since = globaltimer();
+      while (!mbar_try(&empty[g % S], (g / S) & 1))
+        if (globaltimer() - since > kTimeoutNs) break;
+    }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       lmps_pdl_wait();  // (bounded waits begin when the work does)
       constexpr uint32_t idesc = idesc_i8(256, BN);
+      const uint32_t lead = lane == 0 ? 1u : 0u;
+      const uint64_t xd0 = sw128_desc(smem_u32(stage)), wd0 = sw128_desc(smem_u32(stage) + Sh::kX);
       Ring r;
       uint32_t uses[2] = {0u, 0u};
       int buf = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < P.tiles; tile += pairs, buf ^= 1) {
-        if (!mbar_wait_cluster(&tempty[buf], (uses[buf] & 1u) ^ 1u, P.error, abort_v)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster(&tempty[buf], (uses[buf] & 1u) ^ 1u, P.error, abort_v))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + static_cast<uint32_t>(buf) * kAcc;
         for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
-          if (!mbar_wait(&full[r.slot], r.phase, P.error, abort_v)) {
+          if (!warp_wait(&full[r.slot], r.phase, P.error, abort_v)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t x = smem_u32(stage + static_cast<size_t>(r.slot) * Sh::kStage);
-          const uint64_t xd = sw128_desc(x), wd = sw128_desc(x + Sh::kX);
+          const uint64_t at = static_cast<uint64_t>(r.slot) * (Sh::kStage >> 4);
 #pragma unroll
           for (int j = 0; j < kBK / 32; ++j)
-            mma_i8<2>(acc, xd + 2 * j, wd + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u);
-          commit_pair(&empty[r.slot]);
+            mma_i8<2>(acc, xd0 + at + 2 * j, wd0 + at + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u, lead);
+          commit_pair(&empty[r.slot], lead);
         }
         if (!ok) break;
-        commit_pair(&tfull[buf]);
+        commit_pair(&tfull[buf], lead);
         ++uses[buf];
       }
-      commit_pair(done);
+      commit_pair(done, lead);
     }
   } else {
     lmps_pdl_wait();  // before any read of scales and residual, or write of y
@@ -694,7 +727,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
     for (int tile = pair; tile < P.tiles; tile += pairs, buf ^= 1) {
       const int c0 = (tile % P.tiles_n) * kOut + first;
       const int t0 = (tile / P.tiles_n) * 256 + static_cast<int>(rank) * 128 + 32 * q;
-      const float xs = nxs;
+      const uint64_t xs2 = pair2(nxs, nxs);
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -724,7 +757,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
                     A.residual[static_cast<size_t>(t0 + r) * A.ldr + c0 + j];
         __syncwarp();
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], uses[buf] & 1u, P.error, abort_v))) break;
+      if (!warp_wait(&tfull[buf], uses[buf] & 1u, P.error, abort_v)) break;
       ++uses[buf];
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t tl = tmem + static_cast<uint32_t>(buf) * kAcc + (static_cast<uint32_t>(32 * q) << 16) + first;
@@ -732,7 +765,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
       tmem_start32(tl, g[0]);
       if (GATED) tmem_start32(tl + kOut, u[0]);
       if (awaited) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&rfull[e], rphase, P.error, abort_v))) break;
+        if (!warp_wait(&rfull[e], rphase, P.error, abort_v)) break;
         rphase ^= 1u;
         awaited = false;
       }
@@ -748,22 +781,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
           __syncwarp();
           if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], 0));
         }
-        const float4* w4 = reinterpret_cast<const float4*>(ws + 32 * i);
-        const float4* b4 = reinterpret_cast<const float4*>(bs + 32 * i);
+        const uint64_t* w2 = reinterpret_cast<const uint64_t*>(ws + 32 * i);
+        const uint64_t* b2 = reinterpret_cast<const uint64_t*>(bs + 32 * i);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           float v[8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 w = w4[j / 4 + h], o = b4[j / 4 + h];
-            const float wv[4] = {w.x, w.y, w.z, w.w}, ov[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-            for (int l = 0; l < 4; ++l) {
-              const int k = j + 4 * h + l;
-              const int sum = static_cast<int>(g[i][k]);
-              v[4 * h + l] = GATED ? silu_product(linear_value(sum, xs, wv[l]),
-                                                  linear_value(static_cast<int>(u[i][k]), xs, ov[l]))
-                                   : linear_value(sum, xs, wv[l], ov[l]);
+          for (int h = 0; h < 4; ++h) {
+            const int k = j + 2 * h;
+            const float2 l = both(linear2(g[i][k], g[i][k + 1], xs2, w2[k / 2], GATED ? 0ull : b2[k / 2]));
+            v[2 * h] = l.x, v[2 * h + 1] = l.y;
+            if (GATED) {
+              const float2 up = both(linear2(u[i][k], u[i][k + 1], xs2, b2[k / 2], 0ull));
+              v[2 * h] = silu_product(l.x, up.x), v[2 * h + 1] = silu_product(l.y, up.y);
             }
           }
           uint4* to = reinterpret_cast<uint4*>(box + piece(lane, (32 * i + j) / 8));
