@@ -560,7 +560,6 @@ static size_t split_smem(int stages, int xrows) {
 //   warp 0 lane 0: TMA loads of this CTA's half of both operands
 //   warp 1 lane 0 of the first CTA: MMAs
 //   warps 2 ..: epilogue, four warps (TMEM lanes 32 (w % 4) ..) for each 64 or 32 channels of the tile
-constexpr int kPairStages = 4;
 
 template <int BN, bool GATED>
 struct PairShape {
@@ -574,16 +573,17 @@ struct PairShape {
   static constexpr int kBoxBytes = 32 * kMine * 2;
   static constexpr int kStore = kWarps * kBoxBytes;
   static constexpr int kCols = kWarps * 2 * kMine * 4;  // a warp's scales and biases (gated: gate and up scales)
-  static constexpr int kBars = 2 * kPairStages + 5 + kWarps;
+  static constexpr int kStages = (208 * 1024 - kStore - kCols) / kStage;  // 4 (gated 5) of 32 KB, 7 of 24 KB
+  static constexpr int kBars = 2 * kStages + 5 + kWarps;
   static constexpr size_t kSmem =
-      static_cast<size_t>(kPairStages) * kStage + kStore + kCols + 1024 + kBars * sizeof(uint64_t) + 16;
+      static_cast<size_t>(kStages) * kStage + kStore + kCols + 1024 + kBars * sizeof(uint64_t) + 16;
 };
 
 template <int BN, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>::kThreads, 1)
     pair_kernel(const __grid_constant__ Params P) {
   using Sh = PairShape<BN, GATED>;
-  constexpr int S = kPairStages, kOut = Sh::kOut;
+  constexpr int S = Sh::kStages, kOut = Sh::kOut;
   constexpr uint32_t kTmem = BN > 128 ? 512u : 256u;
   constexpr uint32_t kAcc = kTmem / 2;  // columns from one accumulator to the other
   extern __shared__ unsigned char smem_raw[];
@@ -703,6 +703,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
     float* bs = ws + kMine;
     // byte of the box at which the 16-byte piece i of row r lies
     auto piece = [&](int r, int i) { return r * (kMine * 2) + ((kMine == 64 ? i ^ (r & 7) : i ^ ((r >> 1) & 3)) << 4); };
+    auto element = [&](int r, int j) { return reinterpret_cast<__half*>(box + piece(r, j / 8) + (j % 8) * 2); };
+    // Rows of any alignment, between memory and the box: kBatch rows of elements a lane loads before it stores any.
+    constexpr int kLane = kMine / 32, kBatch = 16 / kLane;
+    auto rows_any = [&](int t0, int c0, auto&& load, auto&& put) {
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += kBatch) {
+        __half v[kBatch][kLane];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int l = 0; l < kLane; ++l) {
+            const int j = lane + 32 * l;
+            v[i][l] = t0 + r0 + i < A.m && c0 + j < A.n ? load(r0 + i, j) : __half(0.0f);
+          }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int l = 0; l < kLane; ++l) {
+            const int j = lane + 32 * l;
+            if (t0 + r0 + i < A.m && c0 + j < A.n) put(r0 + i, j, v[i][l]);
+          }
+      }
+    };
     // scales (and biases) of this warp's channels and this lane's token, on their way for the next tile
     float nxs = 0.0f, nws[kChunks], nus[kChunks];
     __half nbs[kChunks];
@@ -747,14 +770,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
       if (add && P.tma_y) {
         awaited = true;
       } else if (add) {  // rows of any alignment: a row a time
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r)
-          if (t0 + r < A.m)
-#pragma unroll
-            for (int j = lane; j < kMine; j += 32)
-              if (c0 + j < A.n)
-                *reinterpret_cast<__half*>(box + piece(r, j / 8) + (j % 8) * 2) =
-                    A.residual[static_cast<size_t>(t0 + r) * A.ldr + c0 + j];
+        const __half* p = A.residual + static_cast<size_t>(t0) * A.ldr + c0;
+        rows_any(t0, c0, [&](int r, int j) { return p[static_cast<size_t>(r) * A.ldr + j]; },
+                 [&](int r, int j, __half v) { *element(r, j) = v; });
         __syncwarp();
       }
       if (!warp_wait(&tfull[buf], uses[buf] & 1u, P.error, abort_v)) break;
@@ -822,14 +840,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
         }
       } else {
         __syncwarp();
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r)
-          if (t0 + r < A.m)
-#pragma unroll
-            for (int j = lane; j < kMine; j += 32)
-              if (c0 + j < A.n)
-                A.y[static_cast<size_t>(t0 + r) * A.ldy + c0 + j] =
-                    *reinterpret_cast<const __half*>(box + piece(r, j / 8) + (j % 8) * 2);
+        __half* p = A.y + static_cast<size_t>(t0) * A.ldy + c0;
+        rows_any(t0, c0, [&](int r, int j) { return *element(r, j); },
+                 [&](int r, int j, __half v) { p[static_cast<size_t>(r) * A.ldy + j] = v; });
       }
     }
     if (lane == 0) {
