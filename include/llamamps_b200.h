@@ -416,7 +416,7 @@ int lmps_tp2_argmax_exchange(const uint16_t* logits, int ld, const int32_t* loca
  * 127.  A zero row has codes and scale 0; a row with a NaN or an infinity has
  * codes 0 and scale NaN, so that what is computed from it is NaN.  All
  * matrices have a row stride in elements (ldx, ldc, ...) of at least their
- * row's length; elements between rows are neither read nor written. */
+ * row's length; elements between rows are not written. */
 
 /* Quantise rows of x [rows, k].  values (fp16, or NULL) receives code * scale. */
 int lmps_quantise_rows_q8(const uint16_t* x, int ldx, int8_t* codes, int ldc, float* scales, uint16_t* values,
@@ -436,7 +436,8 @@ int lmps_rms_norm_q8(const uint16_t* x, int ldx, const uint16_t* residual, int l
  * NULL, y may be residual with the same stride.  swiglu = 1: w and w_scales
  * have 2n rows, gate row c and up row n + c, and y[t][c] = fp16(silu(gate) *
  * up) of the scaled sums (no bias or residual).  x and w start at, and their
- * strides are, multiples of 16 bytes; k <= 131071.  error is set to 1 when a
+ * strides are, multiples of 16 bytes; k <= 131071, m and n <= 2^29.  A row of y
+ * does not depend on the other rows of x in the call.  error is set to 1 when a
  * bounded wait on the device gave up (then y is not complete). */
 int lmps_w8a8_gemm(const int8_t* x, int ldx, const float* x_scales, const int8_t* w, int ldw,
                    const float* w_scales, const uint16_t* bias, const uint16_t* residual, int ldr, uint16_t* y,

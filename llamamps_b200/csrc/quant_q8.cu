@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
 template <int T>
 static int launch(void (*kernel)(RowArgs), const RowArgs& A, cudaStream_t st) {
   constexpr int per = kCtaOf<T> / T;
-  return lmps_launch_pdl(kernel, dim3((A.rows + per - 1) / per), dim3(kCtaOf<T>), 0, st, A);
+  return lmps_launch_pdl(kernel, dim3((A.rows - 1) / per + 1), dim3(kCtaOf<T>), 0, st, A);
 }
 
 // `pieces` of eight elements, T threads a row.

@@ -10,8 +10,9 @@
 //   * split_kernel: tcgen05 with 128 weight rows as the MMA's M and the tokens
 //     as its N, K shared out over a thread-block cluster that adds the integer
 //     sums through distributed shared memory (any order gives the same);
-//   * pair_kernel: tcgen05 over CTA pairs, 256 tokens x 256 weight rows a
-//     tile, persistent, the epilogue of a tile under the products of the next.
+//   * pair_kernel: tcgen05 over CTA pairs, 256 tokens x 256 or 128 weight rows
+//     a tile, persistent, the epilogue of a tile under the products of the
+//     next; with few tiles, several pairs share a tile's K out.
 // Every wait on the device is bounded (error flag, no hang).
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -197,12 +198,12 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t ad, uint64_t bd, 
         : "memory");
 }
 // Completion of this thread's MMAs so far, to the barrier at this offset in both CTAs of the pair.
-__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t lead) {
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t first_cta, uint32_t lead) {
   asm volatile(
       "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
       " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}" ::"r"(
           smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3)), "r"(lead)
+      "h"(static_cast<uint16_t>(3u << first_cta)), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -298,7 +299,7 @@ struct __align__(64) Params {
   CUtensorMap tr;  // residual, the same
   Args a;
   int tma_y;    // y goes out, and the residual comes in, by TMA (ty and tr are set)
-  int xrows;    // split_kernel: tokens of a tile
+  int xrows;    // split_kernel: tokens, rounded up to 16
   int stages;   // split_kernel: K steps in flight
   int ksteps;   // split_kernel: K steps of each CTA of a cluster
   int tiles_n, tiles;  // pair_kernel: tiles along n, all tiles
@@ -346,8 +347,8 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 }
 
 // --- split_kernel -------------------------------------------------------------
-// One tile of 128 weight rows (gated: 64 gate and their 64 up rows) and xrows
-// tokens a cluster; CTA z of the cluster multiplies K steps z * ksteps .. .
+// One tile of 128 weight rows (gated: 64 gate and their 64 up rows) and all
+// tokens (up to 128, in 16s) a cluster; CTA z of the cluster multiplies K steps z * ksteps .. .
 //   warp 0 lane 0: TMA loads; warp 1 lane 0: MMAs; warps 2-17: sums out of
 //   TMEM, 32 tokens of 32 rows each; all warps: finish the CTA's rows.
 // Each CTA finishes 128 / splits of the tile's rows: all CTAs store their sums
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 
   lmps_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c0 = blockIdx.x * kOut, t0 = blockIdx.y * P.xrows;
+  const int c0 = blockIdx.x * kOut;
   const int splits = gridDim.z;
   const int all = (A.k + kBK - 1) / kBK, kbeg = blockIdx.z * P.ksteps;
   const int ksteps = max(0, min(P.ksteps, all - kbeg));
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
         const int kx = (kbeg + kt) * kBK;
         tma_load_2d(w, &P.tw, kx, c0, &full[r.slot]);
         if (GATED) tma_load_2d(w + kWBytes / 2, &P.tw, kx, A.n + c0, &full[r.slot]);
-        tma_load_2d(xt + static_cast<size_t>(r.slot) * xbytes, &P.tx, kx, t0, &full[r.slot]);
+        tma_load_2d(xt + static_cast<size_t>(r.slot) * xbytes, &P.tx, kx, 0, &full[r.slot]);
         issued = kt + 1;
       }
       for (int kt = max(0, issued - S); kt < issued; ++kt) {  // every issued copy lands before the CTA leaves
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
       }
     lmps_pdl_wait();  // before any read of scales and residual, or write of y
     // what the sums meet, on its way before they do
-    if (const int i = tid - 64 - 128; i >= 0 && i < P.xrows) xs[i] = t0 + i < A.m ? A.xs[t0 + i] : 0.0f;
+    if (const int i = tid - 64 - 128; i >= 0 && i < P.xrows) xs[i] = i < A.m ? A.xs[i] : 0.0f;
     if (const int i = tid - 64 - 256; i >= 0 && i < outs) {
       const bool in = cbase + i < A.n;
       cs[i] = in ? A.ws[cbase + i] : 0.0f;
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     }
   }
   lmps_pdl_wait();
-  const int tok = min(P.xrows, A.m - t0), tok4 = (tok + 3) / 4;
+  const int tok = A.m, tok4 = (tok + 3) / 4;
   const bool here = __syncthreads_and(tid != 0 || mbar_wait_cluster(sums, 0u, P.error, abort_v));
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   for (int i = tid; here && i < outs * tok4; i += kSplitThreads) {
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      res[e] = !GATED && A.residual && j + e < tok ? __half2float(A.residual[static_cast<size_t>(t0 + j + e) * A.ldr + c]) : 0.0f;
+      res[e] = !GATED && A.residual && j + e < tok ? __half2float(A.residual[static_cast<size_t>(j + e) * A.ldr + c]) : 0.0f;
     int g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
     const int4* at = red + j / 4 * 128 + lc;
 #pragma unroll 4
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
     const float ws = cs[lc], bias = GATED ? 0.0f : cs[256 + lc], wu = GATED ? cs[128 + lc] : 0.0f;
     const float4 x4 = *reinterpret_cast<const float4*>(xs + j);
     const float xv[4] = {x4.x, x4.y, x4.z, x4.w};
-    __half* y = A.y + static_cast<size_t>(t0 + j) * A.ldy + c;
+    __half* y = A.y + static_cast<size_t>(j) * A.ldy + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e, y += A.ldy) {
       float v = linear_value(g[e], xv[e], ws, bias);
@@ -561,7 +562,7 @@ static size_t split_smem(int stages, int xrows) {
 //   warp 1 lane 0 of the first CTA: MMAs
 //   warps 2 ..: epilogue, four warps (TMEM lanes 32 (w % 4) ..) for each 64 or 32 channels of the tile
 
-template <int BN, bool GATED>
+template <int BN, bool GATED, int SPLITS = 1>
 struct PairShape {
   static constexpr int kX = 128 * kBK, kW = BN / 2 * kBK;
   static constexpr int kStage = kX + kW;
@@ -573,16 +574,19 @@ struct PairShape {
   static constexpr int kBoxBytes = 32 * kMine * 2;
   static constexpr int kStore = kWarps * kBoxBytes;
   static constexpr int kCols = kWarps * 2 * kMine * 4;  // a warp's scales and biases (gated: gate and up scales)
-  static constexpr int kStages = (208 * 1024 - kStore - kCols) / kStage;  // 4 (gated 5) of 32 KB, 7 of 24 KB
-  static constexpr int kBars = 2 * kStages + 5 + kWarps;
+  // split K: sums from the other pairs, [pair][warp][tokens 32 x channels kMine]
+  static constexpr int kSums = (SPLITS - 1) * (kWarps / SPLITS) * 32 * kMine * 4;
+  static constexpr int kStages = (208 * 1024 - kStore - kCols - kSums) / kStage;  // 4 (gated 5) of 32 KB, 7 of 24 KB
+  static constexpr int kBars = 2 * kStages + 6 + kWarps;
   static constexpr size_t kSmem =
-      static_cast<size_t>(kStages) * kStage + kStore + kCols + 1024 + kBars * sizeof(uint64_t) + 16;
+      static_cast<size_t>(kStages) * kStage + kSums + kStore + kCols + 1024 + kBars * sizeof(uint64_t) + 16;
 };
 
-template <int BN, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>::kThreads, 1)
+template <int BN, bool GATED, int SPLITS>
+__global__ void __launch_bounds__(PairShape<BN, GATED, SPLITS>::kThreads, 1)
     pair_kernel(const __grid_constant__ Params P) {
-  using Sh = PairShape<BN, GATED>;
+  static_assert(SPLITS == 1 || !GATED, "a gated tile is not split");
+  using Sh = PairShape<BN, GATED, SPLITS>;
   constexpr int S = Sh::kStages, kOut = Sh::kOut;
   constexpr uint32_t kTmem = BN > 128 ? 512u : 256u;
   constexpr uint32_t kAcc = kTmem / 2;  // columns from one accumulator to the other
@@ -591,7 +595,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* stage = base;  // [S] codes tile, weight tile
-  unsigned char* store = base + static_cast<size_t>(S) * Sh::kStage;
+  int4* sums = reinterpret_cast<int4*>(base + static_cast<size_t>(S) * Sh::kStage);  // (SPLITS > 1)
+  unsigned char* store = base + static_cast<size_t>(S) * Sh::kStage + Sh::kSums;
   float* cols = reinterpret_cast<float*>(store + Sh::kStore);
   uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(cols) + Sh::kCols);
   uint64_t* empty = full + S;
@@ -599,15 +604,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
   uint64_t* tempty = tfull + 2;  // [2] accumulator read by both CTAs' epilogues (the first CTA's counts)
   uint64_t* done = tempty + 2;
   uint64_t* rfull = done + 1;  // [epilogue warps] residual box arrived
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + Sh::kWarps);
+  uint64_t* arrived = rfull + Sh::kWarps;  // the other pairs' sums
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(arrived + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* abort_v = abort_flag;
 
   lmps_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = cluster_rank();
-  const int ksteps = (A.k + kBK - 1) / kBK;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  // split K: pair `split` of a cluster of SPLITS multiplies its share of the K steps of the cluster's one tile
+  const uint32_t crank = cluster_rank(), rank = crank & 1u, first_cta = crank & ~1u;
+  const int split = static_cast<int>(crank >> 1), steps = (A.k + kBK - 1) / kBK;
+  const int kbeg = steps * split / SPLITS, ksteps = steps * (split + 1) / SPLITS - kbeg;
+  const int pair = static_cast<int>(blockIdx.x) / (2 * SPLITS), pairs = static_cast<int>(gridDim.x) / (2 * SPLITS);
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
@@ -619,8 +627,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
     }
     mbar_init(done, 1);
     for (int i = 0; i < Sh::kWarps; ++i) mbar_init(&rfull[i], 1);
+    mbar_init(arrived, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (SPLITS > 1) mbar_expect_tx(arrived, Sh::kSums);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -636,7 +646,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
 
   if (warp == 0) {
     lmps_pdl_wait();  // both operands may be the previous kernel's output
-    const uint32_t lead = lane == 0 ? 1u : 0u, x0 = smem_u32(stage), bar0 = cluster_addr(full, 0);
+    const uint32_t lead = lane == 0 ? 1u : 0u, x0 = smem_u32(stage), bar0 = cluster_addr(full, first_cta);
     Ring r;
     int issued = 0;
     bool ok = true;
@@ -651,8 +661,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
         // the first CTA's barrier counts the bytes of both
         if (rank == 0 && lane == 0) mbar_expect_tx(&full[r.slot], 2u * Sh::kStage);
         const uint32_t x = x0 + static_cast<uint32_t>(r.slot) * Sh::kStage, bar = bar0 + 8u * static_cast<uint32_t>(r.slot);
-        tma_load_pair(x, &P.tx, kt * kBK, t0, bar, lead);
-        tma_load_pair(x + Sh::kX, &P.tw, kt * kBK, w0, bar, lead);
+        tma_load_pair(x, &P.tx, (kbeg + kt) * kBK, t0, bar, lead);
+        tma_load_pair(x + Sh::kX, &P.tw, (kbeg + kt) * kBK, w0, bar, lead);
         ++issued;
       }
     }
@@ -686,13 +696,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
 #pragma unroll
           for (int j = 0; j < kBK / 32; ++j)
             mma_i8<2>(acc, xd0 + at + 2 * j, wd0 + at + 2 * j, idesc, (kt > 0 || j > 0) ? 1u : 0u, lead);
-          commit_pair(&empty[r.slot], lead);
+          commit_pair(&empty[r.slot], first_cta, lead);
         }
         if (!ok) break;
-        commit_pair(&tfull[buf], lead);
+        commit_pair(&tfull[buf], first_cta, lead);
         ++uses[buf];
       }
-      commit_pair(done, lead);
+      commit_pair(done, first_cta, lead);
     }
   } else {
     lmps_pdl_wait();  // before any read of scales and residual, or write of y
@@ -743,7 +753,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
       }
     };
     if (pair < P.tiles) fetch(pair);
-    const bool add = !GATED && A.residual != nullptr;
+    // split K: the pair that finishes this warp's channels, and its place among the warps there
+    const int owner = e / 4 * SPLITS / Sh::kParts, place = e - owner * (Sh::kWarps / SPLITS);
+    const bool add = !GATED && A.residual != nullptr && (SPLITS == 1 || owner == split);
     uint32_t uses[2] = {0u, 0u}, rphase = 0u;
     bool awaited = false;  // a residual is on its way
     int buf = 0;
@@ -782,6 +794,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
       uint32_t g[kChunks][32], u[kChunks][32];  // (u: gated)
       tmem_start32(tl, g[0]);
       if (GATED) tmem_start32(tl + kOut, u[0]);
+      if constexpr (SPLITS > 1) {
+        static_assert(kChunks == 1, "a warp's sums are 32 registers");
+        // [pair][warp][channel / 4][lane]: a warp's stores and loads are contiguous
+        const int at = place * 8 * 32 + lane, block = Sh::kWarps / SPLITS * 8 * 32;
+        tmem_arrived(g[0]);
+        if (owner != split) {
+          const uint32_t cta = 2u * static_cast<uint32_t>(owner) + rank;
+          const uint32_t to = cluster_addr(sums + (split < owner ? split : split - 1) * block + at, cta);
+          const uint32_t bar = cluster_addr(arrived, cta);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) store_cluster(to + static_cast<uint32_t>(j * 32 * 16), &g[0][4 * j], bar);
+          break;
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster(arrived, 0u, P.error, abort_v))) break;
+#pragma unroll
+        for (int z = 0; z < SPLITS - 1; ++z)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int4 v = sums[z * block + at + j * 32];
+            g[0][4 * j] += v.x, g[0][4 * j + 1] += v.y, g[0][4 * j + 2] += v.z, g[0][4 * j + 3] += v.w;
+          }
+      }
       if (awaited) {
         if (!warp_wait(&rfull[e], rphase, P.error, abort_v)) break;
         rphase ^= 1u;
@@ -797,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<BN, GATED>
         } else {  // the accumulator is read
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], 0));
+          if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], first_cta));
         }
         const uint64_t* w2 = reinterpret_cast<const uint64_t*>(ws + 32 * i);
         const uint64_t* b2 = reinterpret_cast<const uint64_t*>(bs + 32 * i);
@@ -877,6 +911,27 @@ static int device_sms(int* sms) {
   return static_cast<int>(e);
 }
 
+// A launch of clusters that may begin while its predecessor ends.
+static int launch_clusters(void (*kernel)(Params), dim3 grid, int threads, size_t smem, dim3 cluster, cudaStream_t st,
+                           const Params& P) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster.x;
+  at[0].val.clusterDim.y = cluster.y;
+  at[0].val.clusterDim.z = cluster.z;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P);
+  return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
+}
+
 static bool encode_codes(CUtensorMap* map, const int8_t* p, int k, size_t rows, size_t ld, int box_rows) {
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, static_cast<uint64_t>(k), rows, ld, kBK,
                    static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
@@ -903,15 +958,15 @@ static int launch_split(const Args& A, int* error, int sms, cudaStream_t st) {
   Params P{};
   P.a = A;
   P.error = error;
-  P.xrows = A.m >= kSplitTokens ? kSplitTokens : (A.m + 15) / 16 * 16;
+  P.xrows = (A.m + 15) / 16 * 16;
   const int out = GATED ? 64 : 128;
-  const int tiles = (A.n + out - 1) / out, ty = (A.m + P.xrows - 1) / P.xrows, steps = (A.k + kBK - 1) / kBK;
+  const int tiles = (A.n + out - 1) / out, steps = (A.k + kBK - 1) / kBK;
   // at most two CTAs an SM, at least three K steps each (64 x 2048 x 1536: 5.6 us with 4 splits, 5.9 with 8, 7.5 with 2)
   int splits = 1;
-  while (splits < 8 && 2 * splits * tiles * ty <= 2 * sms && 6 * splits <= steps) splits *= 2;
+  while (splits < 8 && 2 * splits * tiles <= 2 * sms && 6 * splits <= steps) splits *= 2;
   P.ksteps = (steps + splits - 1) / splits;
   // two CTAs an SM where there are so many, else the whole SM's shared memory
-  const size_t room = tiles * ty * splits > sms ? 113 * 1024 : 226 * 1024;
+  const size_t room = tiles * splits > sms ? 113 * 1024 : 226 * 1024;
   int stages = P.ksteps < 2 ? 2 : P.ksteps < kSplitStages ? P.ksteps : kSplitStages;  // (the ring also holds the CTA's sums)
   while (stages > 2 && split_smem(stages, P.xrows) > room) --stages;
   P.stages = stages;
@@ -922,25 +977,10 @@ static int launch_split(const Args& A, int* error, int sms, cudaStream_t st) {
   const size_t smem = split_smem(stages, P.xrows);
   const int attr = lmps_max_dyn_smem<split_kernel<GATED>>(static_cast<int>(smem));
   if (attr != LMPS_OK) return attr;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles, ty, splits);
-  cfg.blockDim = dim3(kSplitThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 1;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = static_cast<unsigned>(splits);
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, split_kernel<GATED>, P);
-  return e == cudaSuccess ? lmps_launch_status() : static_cast<int>(e);
+  return launch_clusters(split_kernel<GATED>, dim3(tiles, 1, splits), kSplitThreads, smem, dim3(1, 1, splits), st, P);
 }
 
-template <int BN, bool GATED>
+template <int BN, bool GATED, int SPLITS = 1>
 static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
   Params P{};
   P.a = A;
@@ -954,7 +994,7 @@ static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
   if (!encode_codes(&P.tx, A.x, A.k, static_cast<size_t>(A.m), A.ldx, 128) ||
       !encode_codes(&P.tw, A.w, A.k, w_rows, A.ldw, BN / 2))
     return LMPS_ERR_INVALID_ARGUMENT;
-  using Sh = PairShape<BN, GATED>;
+  using Sh = PairShape<BN, GATED, SPLITS>;
   P.tma_y = A.ldy % 8 == 0 && lmps_aligned(A.y, 16) &&
             (!A.residual || (A.ldr % 8 == 0 && lmps_aligned(A.residual, 16)));
   const CUtensorMapSwizzle swz = Sh::kMine == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -965,10 +1005,12 @@ static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
                                             32, swz))))
     return LMPS_ERR_INVALID_ARGUMENT;
   constexpr int kBytes = static_cast<int>(Sh::kSmem);
-  const int attr = lmps_max_dyn_smem<pair_kernel<BN, GATED>>(kBytes);
+  const int attr = lmps_max_dyn_smem<pair_kernel<BN, GATED, SPLITS>>(kBytes);
   if (attr != LMPS_OK) return attr;
-  const int pairs = P.tiles < sms / 2 ? P.tiles : sms / 2;
-  return lmps_launch_pdl(pair_kernel<BN, GATED>, dim3(2 * pairs), dim3(Sh::kThreads), kBytes, st, P);
+  // one tile a cluster where K is split, else a pair walks several
+  const int clusters = SPLITS > 1 || P.tiles < sms / 2 ? P.tiles : sms / 2;
+  return launch_clusters(pair_kernel<BN, GATED, SPLITS>, dim3(2 * SPLITS * clusters), Sh::kThreads, kBytes,
+                         dim3(2 * SPLITS), st, P);
 }
 
 static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -987,9 +1029,16 @@ static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
   const int pairs = sms / 2;
   const long long rows = ceil_div(A.m, 256), t128 = rows * ceil_div(A.n, GATED ? 64 : 128),
                   t256 = rows * ceil_div(A.n, GATED ? 128 : 256);
-  // Up to 64 tokens, and up to 256 where pairs would leave two thirds of the GPU idle, K is split (256 x 2048 x 1536
-  // 7.3 us, pairs 8.2; 256 x 1536 x 8960 21, 28; not 128 x 8192 x 1536: 10.7, 10.0).
-  if (A.m <= 64 || (A.m <= 256 && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
+  // Up to 64 tokens, and up to 128 where pairs would leave two thirds of the GPU idle, the weights are the MMA's 128
+  // rows (128 x 1536 x 8960 8.3 us, pairs 11.7; not 128 x 8192 x 1536: 10.7, 10.0).
+  if (A.m <= 64 || (A.m <= kSplitTokens && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
+  // Few tiles: two or four pairs share K out, six steps or more each, as far as their clusters of four or eight CTAs
+  // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two; 768 x 1536 x 8960 would be 31 instead of 24).
+  if constexpr (!GATED) {
+    const long long steps = ceil_div(A.k, kBK), room = pairs * 13 / 16;
+    if (4 * t128 <= room && steps >= 24) return launch_pair<128, false, 4>(A, error, sms, st);
+    if (2 * t128 <= room && steps >= 12) return launch_pair<128, false, 2>(A, error, sms, st);
+  }
   if (100 * ceil_div(t256, pairs) > 78 * ceil_div(t128, pairs)) return launch_pair<128, GATED>(A, error, sms, st);
   return launch_pair<256, GATED>(A, error, sms, st);
 }
@@ -1009,7 +1058,7 @@ extern "C" int lmps_w8a8_gemm(const int8_t* x, int ldx, const float* x_scales, c
   LMPS_CHECK_ARG(!swiglu || (!bias && !residual));
   LMPS_CHECK_ARG(lmps_aligned(x, 16) && lmps_aligned(w, 16) && lmps_aligned(x_scales, 4) && lmps_aligned(w_scales, 4));
   LMPS_CHECK_ARG(lmps_aligned(y, 2) && lmps_aligned(bias, 2) && lmps_aligned(residual, 2) && lmps_aligned(error, 4));
-  if (k > w8::kMaxK || n > (1 << 30)) return LMPS_ERR_UNSUPPORTED;
+  if (k > w8::kMaxK || m > (1 << 29) || n > (1 << 29)) return LMPS_ERR_UNSUPPORTED;  // (tile numbers and rows fit 32 bits)
   w8::Args A{};
   A.x = x;
   A.ldx = static_cast<size_t>(ldx);

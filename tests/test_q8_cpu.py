@@ -55,7 +55,8 @@ def test_norm_refusals(kw):
     (dict(ldy=31), INVALID), (dict(r=A, ldr=31), INVALID), (dict(x=A + 8), INVALID), (dict(w=A + 8), INVALID),
     (dict(xs=A + 2), INVALID), (dict(y=A + 1), INVALID), (dict(b=A + 1), INVALID), (dict(gated=2), INVALID),
     (dict(gated=1, b=A), INVALID), (dict(gated=1, r=A, ldr=32), INVALID),
-    (dict(k=131072, ldx=131072, ldw=131072), UNSUPPORTED),
+    (dict(k=131072, ldx=131072, ldw=131072), UNSUPPORTED), (dict(m=(1 << 29) + 1), UNSUPPORTED),
+    (dict(n=(1 << 29) + 1, ldy=(1 << 29) + 1), UNSUPPORTED),
 ])
 def test_gemm_refusals(kw, status):
     assert _gemm(**kw) == status

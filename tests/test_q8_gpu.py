@@ -179,6 +179,57 @@ def test_model_shapes(cuda, m, n, k, gated):
     R.check_linear(K.w8a8_gemm(x, xs, w, ws, bias=bias, residual=res), x, xs, w, ws, bias, res)
 
 
+@pytest.mark.parametrize("m,n,k", [(129, 64, 8000), (200, 1536, 8960), (300, 128, 3200), (300, 131, 3101), (512, 1536, 4480),
+                                   (600, 300, 1537), (700, 1000, 1601), (1000, 333, 2999), (2000, 256, 4000)])
+@pytest.mark.parametrize("form", ["none", "both"])
+def test_few_tiles_share_k_out(cuda, m, n, k, form):
+    """Long K behind few tiles: shares of one step more or less, ragged last steps, with and without bias and residual."""
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g, x, xs, w, ws = _operands(m, n, k, m + k)
+    bias, res = (torch.randn(s, generator=g, device="cuda").half() if form == "both" else None for s in ((n,), (m, n)))
+    for _ in range(3):
+        y = K.w8a8_gemm(x, xs, w, ws, bias=bias, residual=res, error=err)
+        R.check_linear(y, x, xs, w, ws, bias, res)
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("m,n,k,gated", [(5, 4000, 1000, 0), (14, 2500, 777, 1), (14, 300, 4000, 0), (30, 600, 500, 1),
+                                         (30, 2500, 1600, 0), (8, 9000, 300, 1), (16, 1000, 256, 1)])
+def test_few_tokens(cuda, m, n, k, gated):
+    """The forms for few tokens, by weight rows and K: 8, 16 and 32 warps a tile."""
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g, x, xs, w, ws = _operands(m, 2 * n if gated else n, k, 3, extra=1)
+    if gated:
+        R.check_gated(K.w8a8_gemm(x, xs, w, ws, swiglu=True, error=err), x, xs, w, ws)
+    else:
+        R.check_linear(K.w8a8_gemm(x, xs, w, ws, error=err), x, xs, w, ws)
+    assert int(err) == 0
+
+
+def test_two_streams_at_once(cuda):
+    """Calls of every kind on two streams that overlap, each with its own operands, again and again."""
+    shapes = [(3, 500, 640, False), (64, 640, 2048, False), (100, 512, 1024, True), (300, 512, 4096, False),
+              (600, 700, 512, True), (1500, 1024, 768, False)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    ops, want, got = {}, {}, {}
+    err = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for s in range(2):
+        for i, (m, n, k, gated) in enumerate(shapes):
+            _, x, xs, w, ws = ops[s, i] = _operands(m, 2 * n if gated else n, k, 100 * s + i)
+            want[s, i] = K.w8a8_gemm(x, xs, w, ws, swiglu=gated)
+            got[s, i] = [torch.empty_like(want[s, i]) for _ in range(4)]
+    torch.cuda.synchronize()
+    for rep in range(4):
+        for i, (m, n, k, gated) in enumerate(shapes):
+            for s in range(2):
+                with torch.cuda.stream(sides[s]):
+                    _, x, xs, w, ws = ops[s, (i + 3 * s) % len(shapes)]
+                    j = (i + 3 * s) % len(shapes)
+                    K.w8a8_gemm(x, xs, w, ws, swiglu=shapes[j][3], out=got[s, j][rep], error=err[s:s + 1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[key]) for key in got for g in got[key]) and not bool(err.any())
+
+
 @pytest.mark.parametrize("m", [1, 7, 40, 130, 300])
 def test_largest_sums_and_extreme_codes(cuda, m):
     """Sums at the edge of 32 bits (k = 131071, all codes -128), and codes of one sign."""
