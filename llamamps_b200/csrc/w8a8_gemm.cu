@@ -43,9 +43,21 @@ __device__ __forceinline__ float linear_value(int acc, float xs, float ws, float
   return fmaf(__fmul_rn(static_cast<float>(acc), xs), ws, bias);
 }
 
+// 2^x and 1 / x to some 2^-22, results below 2^-126 as zero: e^-g past 2^126 makes the quotient 0, which fp16 makes of
+// it anyway.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kMinusLog2e = -1.4426950408889634f;
 __device__ __forceinline__ float silu_product(float g, float u) {
-  // e^-g past 2^126 makes the quotient 0, which fp16 makes of it anyway
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
+  return __fmul_rn(__fmul_rn(g, rcp_fast(__fadd_rn(exp2_fast(__fmul_rn(g, kMinusLog2e)), 1.0f))), u);
 }
 
 // --- few_kernel -----------------------------------------------------------------
@@ -266,7 +278,17 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-// linear_value of two channels.
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// silu_product and linear_value of two channels.
+__device__ __forceinline__ uint64_t silu2(uint64_t g, uint64_t u) {
+  const float2 e = both(mul2(g, pair2(kMinusLog2e, kMinusLog2e)));
+  const float2 d = both(add2(pair2(exp2_fast(e.x), exp2_fast(e.y)), pair2(1.0f, 1.0f)));
+  return mul2(mul2(g, pair2(rcp_fast(d.x), rcp_fast(d.y))), u);
+}
 __device__ __forceinline__ uint64_t linear2(uint32_t a0, uint32_t a1, uint64_t xs, uint64_t ws, uint64_t bias) {
   return fma2(mul2(pair2(static_cast<float>(static_cast<int>(a0)), static_cast<float>(static_cast<int>(a1))), xs), ws, bias);
 }
@@ -758,6 +780,7 @@ __global__ void __launch_bounds__(PairShape<BN, GATED, SPLITS>::kThreads, 1)
     if (pair < P.tiles) fetch(pair);
     // split K: the pair that finishes this warp's channels, and its place among the warps there
     const int owner = e / 4 * SPLITS / Sh::kParts, place = e - owner * (Sh::kWarps / SPLITS);
+    const bool extra = GATED || A.bias != nullptr;  // (bs holds something)
     const bool add = !GATED && A.residual != nullptr && (SPLITS == 1 || owner == split);
     uint32_t uses[2] = {0u, 0u}, rphase = 0u;
     bool awaited = false;  // a residual is on its way
@@ -836,19 +859,22 @@ __global__ void __launch_bounds__(PairShape<BN, GATED, SPLITS>::kThreads, 1)
           __syncwarp();
           if (lane == 0) arrive_cluster(cluster_addr(&tempty[buf], first_cta));
         }
-        const uint64_t* w2 = reinterpret_cast<const uint64_t*>(ws + 32 * i);
-        const uint64_t* b2 = reinterpret_cast<const uint64_t*>(bs + 32 * i);
+        const ulonglong2* w4 = reinterpret_cast<const ulonglong2*>(ws + 32 * i);
+        const ulonglong2* b4 = reinterpret_cast<const ulonglong2*>(bs + 32 * i);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           float v[8];
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int k = j + 2 * h;
-            const float2 l = both(linear2(g[i][k], g[i][k + 1], xs2, w2[k / 2], GATED ? 0ull : b2[k / 2]));
-            v[2 * h] = l.x, v[2 * h + 1] = l.y;
-            if (GATED) {
-              const float2 up = both(linear2(u[i][k], u[i][k + 1], xs2, b2[k / 2], 0ull));
-              v[2 * h] = silu_product(l.x, up.x), v[2 * h + 1] = silu_product(l.y, up.y);
+          for (int h = 0; h < 2; ++h) {
+            const ulonglong2 w = w4[j / 4 + h], o = extra ? b4[j / 4 + h] : make_ulonglong2(0ull, 0ull);
+#pragma unroll
+            for (int l = 0; l < 2; ++l) {
+              const int k = j + 4 * h + 2 * l;
+              const uint64_t wl = l ? w.y : w.x, ol = l ? o.y : o.x;
+              uint64_t r = linear2(g[i][k], g[i][k + 1], xs2, wl, GATED ? 0ull : ol);
+              if (GATED) r = silu2(r, linear2(u[i][k], u[i][k + 1], xs2, ol, 0ull));
+              const float2 f = both(r);
+              v[4 * h + 2 * l] = f.x, v[4 * h + 2 * l + 1] = f.y;
             }
           }
           uint4* to = reinterpret_cast<uint4*>(box + piece(lane, (32 * i + j) / 8));
