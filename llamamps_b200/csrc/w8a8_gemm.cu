@@ -5,11 +5,12 @@
 //   gated:   y[t][c] = fp16(silu(g) u) with g from weight row c, u from row n + c
 //
 // The sum of up to 131071 products of codes fits 32 bits; everything after it
-// is fp32 and rounded once.  Three kernels, by the number of tokens:
+// is fp32 and rounded once.  Four kernels, by the number of tokens:
 //   * few_kernel: mma.sync on weights straight from global memory; their bytes are all there is;
 //   * split_kernel: tcgen05 with 128 weight rows as the MMA's M and the tokens
 //     as its N, K shared out over a thread-block cluster that adds the integer
 //     sums through distributed shared memory (any order gives the same);
+//   * whole_kernel: tcgen05 with the tokens as rows, for wide outputs;
 //   * pair_kernel: tcgen05 over CTA pairs, 256 tokens x 256 or 128 weight rows
 //     a tile, persistent, the epilogue of a tile under the products of the
 //     next; with few tiles, several pairs share a tile's K out.
@@ -305,6 +306,14 @@ __device__ __forceinline__ void tmem_start32(uint32_t taddr, uint32_t (&r)[32]) 
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_start16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {  // (the operands keep uses behind the wait)
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -569,6 +578,166 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // no CTA leaves while another waits for sums
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tcols) : "memory");
+}
+
+// --- whole_kernel -------------------------------------------------------------
+// Up to 64 tokens and tiles enough for the GPU (no residual): a CTA multiplies
+// the whole of K for 128 weight rows (gated: 64 gate and their 64 up rows).  The tokens are
+// the MMA's 128 rows (those past the last hold what the ring held before, and
+// their sums are not read), so a TMEM lane has a token's gates in columns 0 ..
+// and their up values 64 further: nothing is exchanged, and a lane writes its
+// token's 16 or 32 channels side by side.
+//   warp 0: TMA loads; warp 1: MMAs; warps 2-17: epilogue, four for each 32
+//   tokens (those without tokens rest).
+constexpr int kWholeThreads = 64 + 512;
+constexpr int kWholeStages = 6;  // at most
+constexpr int kXSlot = 128 * kBK;
+
+template <bool GATED>
+__global__ void __launch_bounds__(kWholeThreads) whole_kernel(const __grid_constant__ Params P) {
+  extern __shared__ unsigned char smem_raw[];
+  const Args& A = P.a;
+  const int S = P.stages;
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float* cs = reinterpret_cast<float*>(base + static_cast<size_t>(S) * (kWBytes + kXSlot));  // [128] scales, [128] biases
+  uint64_t* full = reinterpret_cast<uint64_t*>(cs + 2 * 128);
+  uint64_t* empty = full + kWholeStages;
+  uint64_t* done = empty + kWholeStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abort_v = abort_flag;
+  constexpr int kOut = GATED ? 64 : 128, kMine = kOut / 4;  // channels of a tile, of an epilogue warp
+
+  lmps_pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c0 = blockIdx.x * kOut, ksteps = (A.k + kBK - 1) / kBK;
+  if (warp == 0) {  // a lane per barrier
+    if (lane < S) {
+      mbar_init(&full[lane], 1);
+      mbar_init(&empty[lane], 1);
+    } else if (lane == 31) {
+      mbar_init(done, 1);
+      *abort_flag = 0;
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 128;" ::"r"(smem_u32(tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      lmps_pdl_wait();  // both operands may be the previous kernel's output
+      Ring r;
+      int issued = 0;
+      for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
+        if (kt >= S && !mbar_wait(&empty[r.slot], r.phase ^ 1u, P.error, abort_v)) break;
+        mbar_expect_tx(&full[r.slot], static_cast<uint32_t>(kWBytes + P.xrows * kBK));
+        unsigned char* w = base + static_cast<size_t>(r.slot) * (kWBytes + kXSlot);
+        tma_load_2d(w, &P.tw, kt * kBK, c0, &full[r.slot]);
+        if (GATED) tma_load_2d(w + kWBytes / 2, &P.tw, kt * kBK, A.n + c0, &full[r.slot]);
+        tma_load_2d(w + kWBytes, &P.tx, kt * kBK, 0, &full[r.slot]);
+        issued = kt + 1;
+      }
+      for (int kt = max(0, issued - S); kt < issued; ++kt) {  // every issued copy lands before the CTA leaves
+        const uint64_t since = globaltimer();
+        while (!mbar_try(&full[kt % S], (kt / S) & 1))
+          if (globaltimer() - since > kTimeoutNs) break;
+      }
+    }
+  } else if (warp == 1) {
+    lmps_pdl_wait();  // (bounded waits begin when the work does)
+    const uint32_t lead = lane == 0 ? 1u : 0u;
+    const uint64_t wd0 = sw128_desc(smem_u32(base)), xd0 = sw128_desc(smem_u32(base) + kWBytes);
+    Ring r;
+    for (int kt = 0; kt < ksteps; ++kt, r.next(S)) {
+      if (!warp_wait(&full[r.slot], r.phase, P.error, abort_v)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t at = static_cast<uint64_t>(r.slot) * ((kWBytes + kXSlot) >> 4);
+#pragma unroll
+      for (int j = 0; j < kBK / 32; ++j)
+        mma_i8<1>(tmem, xd0 + at + 2 * j, wd0 + at + 2 * j, idesc_i8(128, 128), (kt > 0 || j > 0) ? 1u : 0u, lead);
+      if (lane == 0) mma_commit(&empty[r.slot]);
+    }
+    if (lane == 0) {
+      mma_commit(done);
+      const uint64_t since = globaltimer();  // every MMA is finished before the tensor memory is freed
+      while (!mbar_try(done, 0u))
+        if (globaltimer() - since > kTimeoutNs) break;
+    }
+  } else {
+    if (warp == 17)
+      for (int kt = lane; kt < ksteps; kt += 32) {  // the weights come nearer while the kernel before ends
+        prefetch_2d(&P.tw, kt * kBK, c0);
+        if (GATED) prefetch_2d(&P.tw, kt * kBK, A.n + c0);
+      }
+    lmps_pdl_wait();  // before any read of scales, or write of y
+    const int q = warp & 3, first = (warp - 2) / 4 * kMine, token = 32 * q + lane;
+    const bool live = token < A.m;
+    if (const int i = tid - 64; i < kOut) {
+      const bool in = c0 + i < A.n;
+      cs[i] = in ? A.ws[c0 + i] : 0.0f;
+      cs[128 + i] = !in ? 0.0f : GATED ? A.ws[A.n + c0 + i] : A.bias ? __half2float(A.bias[c0 + i]) : 0.0f;
+    }
+    const float xs = live ? A.xs[token] : 0.0f;
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    if (32 * q < A.m && warp_wait(done, 0u, P.error, abort_v)) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t tl = tmem + (static_cast<uint32_t>(32 * q) << 16) + first;
+      uint32_t g[32];  // gated: 16 gates, 16 up values
+      if (GATED) {
+        tmem_start16(tl, g);
+        tmem_start16(tl + kOut, g + 16);
+      } else {
+        tmem_start32(tl, g);
+      }
+      tmem_arrived(g);
+      const uint64_t xs2 = pair2(xs, xs);
+      const uint64_t* w2 = reinterpret_cast<const uint64_t*>(cs + first);
+      const uint64_t* b2 = reinterpret_cast<const uint64_t*>(cs + 128 + first);
+      __half* y = A.y + static_cast<size_t>(token) * A.ldy + c0 + first;
+#pragma unroll
+      for (int j = 0; j < kMine; j += 8) {
+        float v[8];
+#pragma unroll
+        for (int l = 0; l < 8; l += 2) {
+          uint64_t r = linear2(g[j + l], g[j + l + 1], xs2, w2[(j + l) / 2], GATED ? 0ull : b2[(j + l) / 2]);
+          if (GATED) r = silu2(r, linear2(g[16 + j + l], g[16 + j + l + 1], xs2, b2[(j + l) / 2], 0ull));
+          const float2 f = both(r);
+          v[l] = f.x, v[l + 1] = f.y;
+        }
+        const int left = live ? A.n - (c0 + first + j) : 0;
+        if (left >= 8) {  // (rows of y start at multiples of 16 bytes)
+          uint4 packed;
+          __half2* h2 = reinterpret_cast<__half2*>(&packed);
+#pragma unroll
+          for (int l = 0; l < 4; ++l) h2[l] = __floats2half2_rn(v[2 * l], v[2 * l + 1]);
+          *reinterpret_cast<uint4*>(y + j) = packed;
+        } else {
+#pragma unroll
+          for (int l = 0; l < 8; ++l)
+            if (l < left) y[j + l] = __float2half_rn(v[l]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
+}
+
+static size_t whole_smem(int stages) {
+  return static_cast<size_t>(stages) * (kWBytes + kXSlot) + 2 * 128 * sizeof(float) + 1024 +
+         (2 * kWholeStages + 1) * sizeof(uint64_t) + 16;
 }
 
 static size_t split_smem(int stages, int xrows) {
@@ -940,6 +1109,9 @@ static int device_sms(int* sms) {
   return static_cast<int>(e);
 }
 
+// Whether rows of fp16 start at multiples of 16 bytes.
+static bool rows16(const __half* p, size_t ld) { return ld % 8 == 0 && lmps_aligned(p, 16); }
+
 // A launch of clusters that may begin while its predecessor ends.
 static int launch_clusters(void (*kernel)(Params), dim3 grid, int threads, size_t smem, dim3 cluster, cudaStream_t st,
                            const Params& P) {
@@ -1009,6 +1181,25 @@ static int launch_split(const Args& A, int* error, int sms, cudaStream_t st) {
   return launch_clusters(split_kernel<GATED>, dim3(tiles, 1, splits), kSplitThreads, smem, dim3(1, 1, splits), st, P);
 }
 
+template <bool GATED>
+static int launch_whole(const Args& A, int* error, int sms, cudaStream_t st) {
+  Params P{};
+  P.a = A;
+  P.error = error;
+  P.xrows = (A.m + 15) / 16 * 16;
+  constexpr int out = GATED ? 64 : 128;
+  const int tiles = (A.n + out - 1) / out, steps = (A.k + kBK - 1) / kBK;
+  const int most = tiles > sms ? 3 : kWholeStages;  // (two CTAs an SM, the loads of one under the epilogue of the other)
+  P.stages = steps < most ? steps : most;
+  if (!encode_codes(&P.tx, A.x, A.k, static_cast<size_t>(A.m), A.ldx, P.xrows) ||
+      !encode_codes(&P.tw, A.w, A.k, static_cast<size_t>(A.n) * (GATED ? 2 : 1), A.ldw, out))
+    return LMPS_ERR_INVALID_ARGUMENT;
+  const size_t smem = whole_smem(P.stages);
+  const int attr = lmps_max_dyn_smem<whole_kernel<GATED>>(static_cast<int>(smem));
+  if (attr != LMPS_OK) return attr;
+  return lmps_launch_pdl(whole_kernel<GATED>, dim3(tiles), dim3(kWholeThreads), smem, st, P);
+}
+
 template <int BN, bool GATED, int SPLITS = 1>
 static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
   Params P{};
@@ -1024,8 +1215,7 @@ static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
       !encode_codes(&P.tw, A.w, A.k, w_rows, A.ldw, BN / 2))
     return LMPS_ERR_INVALID_ARGUMENT;
   using Sh = PairShape<BN, GATED, SPLITS>;
-  P.tma_y = A.ldy % 8 == 0 && lmps_aligned(A.y, 16) &&
-            (!A.residual || (A.ldr % 8 == 0 && lmps_aligned(A.residual, 16)));
+  P.tma_y = rows16(A.y, A.ldy) && (!A.residual || rows16(A.residual, A.ldr));
   const CUtensorMapSwizzle swz = Sh::kMine == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (P.tma_y && (!encode_2d(&P.ty, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, A.y, static_cast<uint64_t>(A.n),
                              static_cast<uint64_t>(A.m), A.ldy * 2, Sh::kMine, 32, swz) ||
@@ -1060,6 +1250,11 @@ static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
                   t256 = rows * ceil_div(A.n, GATED ? 128 : 256);
   // Up to 64 tokens, and up to 128 where pairs would leave two thirds of the GPU idle, the weights are the MMA's 128
   // rows (128 x 1536 x 8960 8.3 us, pairs 11.7; not 128 x 8192 x 1536: 10.7, 10.0).
+  // Wide outputs for 33 to 64 tokens: K whole in a CTA, the tokens as the MMA's rows, nothing exchanged (64 x 8960 x 1536
+  // gated 7.8 -> 6.7 us; 16 x 8960 x 1536 would be 6.7 instead of 6.0).
+  // Not for rows of y at odd places (64 x 9500 x 1536: 14.8 us, 7.3 split).
+  if (A.m > 32 && A.m <= 64 && !A.residual && rows16(A.y, A.ldy) && 2 * ceil_div(A.n, GATED ? 64 : 128) >= sms)
+    return launch_whole<GATED>(A, error, sms, st);
   if (A.m <= 64 || (A.m <= kSplitTokens && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
   // Few tiles: two or four pairs share K out, six steps or more each, as far as their clusters of four or eight CTAs
   // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two; 768 x 1536 x 8960 would be 31 instead of 24).
