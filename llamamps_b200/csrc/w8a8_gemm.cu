@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 }
 
 // --- whole_kernel -------------------------------------------------------------
-// Up to 64 tokens and tiles enough for the GPU (no residual): a CTA multiplies
+// Up to 128 tokens and tiles enough for the GPU (no residual): a CTA multiplies
 // the whole of K for 128 weight rows (gated: 64 gate and their 64 up rows).  The tokens are
 // the MMA's 128 rows (those past the last hold what the ring held before, and
 // their sums are not read), so a TMEM lane has a token's gates in columns 0 ..
@@ -1250,10 +1250,12 @@ static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
                   t256 = rows * ceil_div(A.n, GATED ? 128 : 256);
   // Up to 64 tokens, and up to 128 where pairs would leave two thirds of the GPU idle, the weights are the MMA's 128
   // rows (128 x 1536 x 8960 8.3 us, pairs 11.7; not 128 x 8192 x 1536: 10.7, 10.0).
-  // Wide outputs for 33 to 64 tokens: K whole in a CTA, the tokens as the MMA's rows, nothing exchanged (64 x 8960 x 1536
-  // gated 7.8 -> 6.7 us; 16 x 8960 x 1536 would be 6.7 instead of 6.0).
-  // Not for rows of y at odd places (64 x 9500 x 1536: 14.8 us, 7.3 split).
-  if (A.m > 32 && A.m <= 64 && !A.residual && rows16(A.y, A.ldy) && 2 * ceil_div(A.n, GATED ? 64 : 128) >= sms)
+  // Wide outputs for 33 to 64 tokens, or 128 where there is no tile a second time: K whole in a CTA, the tokens as the
+  // MMA's rows, nothing exchanged (64 x 8960 x 1536 gated 7.8 -> 6.5 us, 128 x 8960 x 1536 9.0 -> 7.4; 16 x 8960 x 1536
+  // would be 6.7 instead of 6.0, 128 x 151936 x 1536 74 instead of 59).  Not for rows of y at odd places (64 x 9500 x
+  // 1536: 14.8 us, 7.3 split).
+  const long long whole = ceil_div(A.n, GATED ? 64 : 128);
+  if (A.m > 32 && A.m <= (whole <= sms ? 128 : 64) && !A.residual && rows16(A.y, A.ldy) && 2 * whole >= sms)
     return launch_whole<GATED>(A, error, sms, st);
   if (A.m <= 64 || (A.m <= kSplitTokens && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
   // Few tiles: two or four pairs share K out, six steps or more each, as far as their clusters of four or eight CTAs

@@ -206,14 +206,14 @@ def test_few_tokens(cuda, m, n, k, gated):
     assert int(err) == 0
 
 
-@pytest.mark.parametrize("m", [33, 47, 64])
-@pytest.mark.parametrize("n,k,gated", [(9500, 333, 0), (9473, 1536, 0), (4737, 700, 1), (20000, 128, 0), (10000, 1000, 1)])
+@pytest.mark.parametrize("m", [33, 47, 64, 65, 99, 128])
+@pytest.mark.parametrize("n,k,gated", [(9504, 333, 0), (9500, 333, 0), (9473, 1536, 0), (4737, 700, 1), (20000, 128, 0), (10000, 1000, 1)])
 def test_wide_outputs(cuda, m, n, k, gated):
     """Wide outputs of a batch: whole tiles and ragged ones, one CTA an SM and more, with and without bias."""
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     for bias in (False, True)[:1 if gated else 2]:
         g, x, xs, w, ws = _operands(m, 2 * n if gated else n, k, m)
-        off = 8 if m == 47 else 3  # (rows at 16 bytes, or not)
+        off = 8 if m in (47, 99) else 3  # (rows at 16 bytes, or not)
         buf = torch.full((m, -(-n // 8) * 8 + 16), 3.0, dtype=torch.float16, device="cuda")
         y, b = buf[:, off:off + n], torch.randn(n, generator=g, device="cuda").half() if bias else None
         K.w8a8_gemm(x, xs, w, ws, bias=b, swiglu=bool(gated), out=y, error=err)
