@@ -14,7 +14,9 @@
 // where that quotient is within rounding of a tie (an element that is half the
 // largest is one), the code comes from fp64, so every code is the formula's.
 //
-// What bounds it: bytes (a row in once, codes and sum out once).
+// Bound by bytes (a row in once, codes and sum out once) where there are many:
+// 16384 x 8960 92 us (4.8 TB/s; with the values 117, 6.3 TB/s), 16384 x 1536 with
+// residual 36 us (4.9 TB/s); a row's latency else, 64 x 1536 3.1 us.
 #include "common.cuh"
 
 namespace lmps {

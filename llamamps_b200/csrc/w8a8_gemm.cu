@@ -67,7 +67,9 @@ __device__ __forceinline__ float silu_product(float g, float u) {
 // sums through shared memory.  mma.sync with the weights as the 16 rows: the
 // order of k within a product is free as long as both operands have the same,
 // so lane l holds codes 16 (l % 4) .. of the chunk of its rows, 16 bytes of
-// global memory each, as they come; nothing is staged.
+// global memory each, as they come; nothing is staged.  Bound by the weights'
+// bytes behind a kernel's start: 1 x 8960 x 1536 gated 7.0 us out of DRAM (3.9
+// TB/s), 5.4 out of L2; 1 x 2048 x 1536 2.4 us.
 __device__ __forceinline__ uint4 load_codes(const int8_t* p, int left) {  // 16 codes, those from `left` on zero
   if (left >= 16) return *reinterpret_cast<const uint4*>(p);
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -388,6 +390,8 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 // Each CTA finishes 128 / splits of the tile's rows: all CTAs store their sums
 // of these rows into its shared memory ([tokens / 4][split][row][4], so that a
 // warp's stores and loads are contiguous), counted in bytes by its barrier.
+// Latency: 64 x 1536 x 8960 6.7 us, of it start and barriers 1, loads 2.5 (some
+// 50 B a clock and SM), the sums' exchange 1.2 (25 B a clock), the rest 1.
 constexpr int kSplitThreads = 64 + 512;
 constexpr int kSplitStages = 8;   // at most
 constexpr int kSplitTokens = 128;  // of a tile at most
@@ -589,6 +593,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
 // token's 16 or 32 channels side by side.
 //   warp 0: TMA loads; warp 1: MMAs; warps 2-17: epilogue, four for each 32
 //   tokens (those without tokens rest).
+// Bound by what an SM loads, some 50 B a clock: 64 x 8960 x 1536 gated 6.5 us
+// out of L2 (288 KB a CTA: 3.3 us), 9.4 out of DRAM.
 constexpr int kWholeThreads = 64 + 512;
 constexpr int kWholeStages = 6;  // at most
 constexpr int kXSlot = 128 * kBK;
@@ -755,6 +761,12 @@ static size_t split_smem(int stages, int xrows) {
 //   warp 0 lane 0: TMA loads of this CTA's half of both operands
 //   warp 1 lane 0 of the first CTA: MMAs
 //   warps 2 ..: epilogue, four warps (TMEM lanes 32 (w % 4) ..) for each 64 or 32 channels of the tile
+// Tiles of 256 x 256 because a pair then loads 64 KB for 512 cycles of products
+// of both SMs, near what they can load (10 TB/s over the GPU); of 128 where
+// there are few.  Bound by power: 16384 x 8960 x 1536 gated 350 us (2.6 POP/s at
+// some 1.4 GHz; 258 without the epilogue, 222 of zeros), 16384 x 1536 x 8960 183.
+// Split K (SPLITS > 1): the pairs of a cluster send their sums of a warp's
+// channels to the pair that finishes them.
 
 template <int BN, bool GATED, int SPLITS = 1>
 struct PairShape {
@@ -1149,9 +1161,13 @@ static int launch_few(const Args& A, int sms, cudaStream_t st) {
   const int tiles = (A.n + 15) / 16;
   if constexpr (kFit >= 32)
     if (tiles <= sms) return launch_few_warps<NT, GATED, 32>(A, tiles, st);
-  if constexpr (kFit >= 16)
-    if (tiles <= 2 * sms) return launch_few_warps<NT, GATED, 16>(A, tiles, st);
-  return launch_few_warps<NT, GATED, 8>(A, tiles, st);
+  if constexpr (NT != 2) {
+    if constexpr (kFit >= 16)
+      if (tiles <= 2 * sms) return launch_few_warps<NT, GATED, 16>(A, tiles, st);
+    return launch_few_warps<NT, GATED, 8>(A, tiles, st);
+  } else {  // (two token tiles: never more tiles than SMs)
+    return launch_few_warps<NT, GATED, GATED ? 16 : 32>(A, tiles, st);
+  }
 }
 
 template <bool GATED>

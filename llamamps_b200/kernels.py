@@ -638,14 +638,16 @@ def w8a8_gemm(codes, scales, w_codes, w_scales, *, bias: Optional[torch.Tensor] 
     if gated and (bias is not None or residual is not None):
         raise ValueError("the SwiGLU epilogue takes no bias or residual")
     n = w_rows // 2 if gated else w_rows
-    if out is None:
-        out = torch.empty((m, n) if codes.dim() == 2 else (n,), dtype=FP16, device=codes.device)
-    if error is None and codes.is_cuda:
-        if torch.cuda.is_current_stream_capturing():
-            raise ValueError("error: a captured w8a8_gemm needs an int32 error word")
-        error = torch.zeros(1, dtype=_I32, device=codes.device)
-        w8a8_gemm(codes, scales, w_codes, w_scales, bias=bias, residual=residual, swiglu=swiglu, out=out, error=error)
-        if int(error.item()):
+    if (out is None or error is None) and codes.is_cuda:
+        word = error
+        if out is None:
+            out = torch.empty((m, n) if codes.dim() == 2 else (n,), dtype=FP16, device=codes.device)
+        if error is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("error: a captured w8a8_gemm needs an int32 error word")
+            word = torch.zeros(1, dtype=_I32, device=codes.device)
+        w8a8_gemm(codes, scales, w_codes, w_scales, bias=bias, residual=residual, swiglu=swiglu, out=out, error=word)
+        if error is None and int(word.item()):
             raise RuntimeError("w8a8_gemm: a wait for the tensor core timed out")
         return out
     dev = codes.get_device()
