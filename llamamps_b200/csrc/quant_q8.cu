@@ -17,6 +17,8 @@
 // Bound by bytes (a row in once, codes and sum out once) where there are many:
 // 16384 x 8960 92 us (4.8 TB/s; with the values 117, 6.3 TB/s), 16384 x 1536 with
 // residual 36 us (4.9 TB/s); a row's latency else, 64 x 1536 3.1 us.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lmps {
@@ -245,42 +247,49 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
   const __half* r = A.residual ? A.residual + row * A.ldr : nullptr;
   __half* sum = A.residual ? A.sum + row * A.lds : nullptr;
   const __half none = __ushort_as_half(0);
+  // (eight elements that are all in the row go without the checks)
+  auto each = [&](int base, auto&& f) {
+    if (base + 7 * T < A.k) f(std::true_type{});
+    else if (base < A.k) f(std::false_type{});
+  };
   // elements base + T j for j < 8 (zero past the row); the sum is written on the way
-  auto load8 = [&](int base, __half (&s)[8]) {
+  auto load8 = [&](auto whole, int base, __half (&s)[8]) {
+    auto in = [&](int j) { return whole() || base + T * j < A.k; };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = base + T * j < A.k ? x[base + T * j] : none;
+    for (int j = 0; j < 8; ++j) s[j] = in(j) ? x[base + T * j] : none;
     if (r) {
       __half b[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = base + T * j < A.k ? r[base + T * j] : none;
+      for (int j = 0; j < 8; ++j) b[j] = in(j) ? r[base + T * j] : none;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         s[j] = __float2half_rn(__half2float(b[j]) + __half2float(s[j]));
-        if (base + T * j < A.k) sum[base + T * j] = s[j];
+        if (in(j)) sum[base + T * j] = s[j];
       }
     }
   };
   float ss = 0.0f, m = 0.0f;
-  auto stat8 = [&](int base, const __half (&s)[8]) {
+  auto stat8 = [&](auto whole, int base, const __half (&s)[8]) {
+    auto in = [&](int j) { return whole() || base + T * j < A.k; };
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float f = __half2float(s[j]);
       if (A.gamma) {
         ss = fmaf(f, f, ss);
-        f *= base + T * j < A.k ? __half2float(A.gamma[base + T * j]) : 0.0f;
+        f *= in(j) ? __half2float(A.gamma[base + T * j]) : 0.0f;
       }
       m = max_nan(m, fabsf(f));
     }
   };
   __half s[E][8];
 #pragma unroll
-  for (int i = 0; i < E; ++i) load8(t + 8 * T * i, s[i]);
+  for (int i = 0; i < E; ++i) each(t + 8 * T * i, [&](auto w) { load8(w, t + 8 * T * i, s[i]); });
 #pragma unroll
-  for (int i = 0; i < E; ++i) stat8(t + 8 * T * i, s[i]);
+  for (int i = 0; i < E; ++i) each(t + 8 * T * i, [&](auto w) { stat8(w, t + 8 * T * i, s[i]); });
   for (int base = t + 8 * T * E; base < A.k; base += 8 * T) {
     __half v[8];
-    load8(base, v);
-    stat8(base, v);
+    load8(std::false_type{}, base, v);
+    stat8(std::false_type{}, base, v);
   }
   uint32_t mbits;
   reduce_row<T>(ss, m, mbits);
@@ -290,30 +299,31 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
   const bool dead = mbits >= 0x7F800000u;
   int8_t* codes = A.codes + row * A.ldc;
   __half* values = A.values ? A.values + row * A.ldv : nullptr;
-  auto give8 = [&](int base, const __half (&s)[8]) {
+  auto give8 = [&](auto whole, int base, const __half (&s)[8]) {
+    auto in = [&](int j) { return whole() || base + T * j < A.k; };
     float f[8], c[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       f[j] = __half2float(s[j]);
-      if (A.gamma) f[j] *= base + T * j < A.k ? __half2float(A.gamma[base + T * j]) : 0.0f;
+      if (A.gamma) f[j] *= in(j) ? __half2float(A.gamma[base + T * j]) : 0.0f;
       if (dead) f[j] = 0.0f;
     }
     row_codes(f, inv, mbits, c);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (base + T * j < A.k) {
+      if (in(j)) {
         codes[base + T * j] = static_cast<int8_t>(__float_as_uint(c[j]) & 0xFFu);
         if (values) values[base + T * j] = __float2half_rn((c[j] - kMagic) * scale);
       }
   };
 #pragma unroll
-  for (int i = 0; i < E; ++i) give8(t + 8 * T * i, s[i]);
+  for (int i = 0; i < E; ++i) each(t + 8 * T * i, [&](auto w) { give8(w, t + 8 * T * i, s[i]); });
   const __half* again = r ? sum : x;
   for (int base = t + 8 * T * E; base < A.k; base += 8 * T) {
     __half v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = base + T * j < A.k ? again[base + T * j] : none;
-    give8(base, v);
+    give8(std::false_type{}, base, v);
   }
 }
 
