@@ -15,6 +15,8 @@
 //     a tile, persistent, the epilogue of a tile under the products of the
 //     next; with few tiles, several pairs share a tile's K out.
 // Every wait on the device is bounded (error flag, no hang).
+#include <type_traits>
+
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -922,24 +924,24 @@ __global__ void __launch_bounds__(PairShape<BN, GATED, SPLITS>::kThreads, 1)
     auto element = [&](int r, int j) { return reinterpret_cast<__half*>(box + piece(r, j / 8) + (j % 8) * 2); };
     // Rows of any alignment, between memory and the box: kBatch rows of elements a lane loads before it stores any.
     constexpr int kLane = kMine / 32, kBatch = 16 / kLane;
+    auto rows_batch = [&](auto whole, int r0, int t0, int c0, auto&& load, auto&& put) {
+      auto in = [&](int i, int l) { return whole() || (t0 + r0 + i < A.m && c0 + lane + 32 * l < A.n); };
+      __half v[kBatch][kLane];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int l = 0; l < kLane; ++l) v[i][l] = in(i, l) ? load(r0 + i, lane + 32 * l) : __half(0.0f);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int l = 0; l < kLane; ++l)
+          if (in(i, l)) put(r0 + i, lane + 32 * l, v[i][l]);
+    };
     auto rows_any = [&](int t0, int c0, auto&& load, auto&& put) {
 #pragma unroll 1
       for (int r0 = 0; r0 < 32; r0 += kBatch) {
-        __half v[kBatch][kLane];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-          for (int l = 0; l < kLane; ++l) {
-            const int j = lane + 32 * l;
-            v[i][l] = t0 + r0 + i < A.m && c0 + j < A.n ? load(r0 + i, j) : __half(0.0f);
-          }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-          for (int l = 0; l < kLane; ++l) {
-            const int j = lane + 32 * l;
-            if (t0 + r0 + i < A.m && c0 + j < A.n) put(r0 + i, j, v[i][l]);
-          }
+        if (t0 + 32 <= A.m && c0 + kMine <= A.n) rows_batch(std::true_type{}, r0, t0, c0, load, put);
+        else rows_batch(std::false_type{}, r0, t0, c0, load, put);
       }
     };
     // scales (and biases) of this warp's channels and this lane's token, on their way for the next tile
