@@ -1252,6 +1252,35 @@ static int launch_pair(const Args& A, int* error, int sms, cudaStream_t st) {
 
 static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
+// Clusters of SPLITS pairs that the current device holds at once (asked once a device; 0: an error, then K is not split).
+template <int SPLITS>
+static int resident_clusters() {
+  constexpr int kMaxDevices = 64;
+  static int known[kMaxDevices] = {};  // the number, plus one
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  if (const int n = __atomic_load_n(&known[dev], __ATOMIC_ACQUIRE)) return n - 1;
+  using Sh = PairShape<128, false, SPLITS>;
+  if (lmps_max_dyn_smem<pair_kernel<128, false, SPLITS>>(static_cast<int>(Sh::kSmem)) != LMPS_OK) return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * SPLITS);
+  cfg.blockDim = dim3(Sh::kThreads);
+  cfg.dynamicSmemBytes = Sh::kSmem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2 * SPLITS;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<128, false, SPLITS>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  __atomic_store_n(&known[dev], n + 1, __ATOMIC_RELEASE);
+  return n;
+}
+
 template <bool GATED>
 static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
   const long long codes = static_cast<long long>(A.n) * A.k * (GATED ? 2 : 1);  // weight bytes
@@ -1277,11 +1306,14 @@ static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
     return launch_whole<GATED>(A, error, sms, st);
   if (A.m <= 64 || (A.m <= kSplitTokens && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
   // Few tiles: two or four pairs share K out, six steps or more each, as far as their clusters of four or eight CTAs
-  // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two; 768 x 1536 x 8960 would be 31 instead of 24).
+  // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two, 700 x 1300 x
+  // 8960 25 -> 17; 768 x 1536 x 8960 would be 31 instead of 24).
   if constexpr (!GATED) {
-    const long long steps = ceil_div(A.k, kBK), room = pairs * 13 / 16;
-    if (4 * t128 <= room && steps >= 24) return launch_pair<128, false, 4>(A, error, sms, st);
-    if (2 * t128 <= room && steps >= 12) return launch_pair<128, false, 2>(A, error, sms, st);
+    const long long steps = ceil_div(A.k, kBK);
+    if (4 * t128 <= pairs && steps >= 24 && t128 <= resident_clusters<4>())
+      return launch_pair<128, false, 4>(A, error, sms, st);
+    if (2 * t128 <= pairs && steps >= 12 && t128 <= resident_clusters<2>())
+      return launch_pair<128, false, 2>(A, error, sms, st);
   }
   if (100 * ceil_div(t256, pairs) > 78 * ceil_div(t128, pairs)) return launch_pair<128, GATED>(A, error, sms, st);
   return launch_pair<256, GATED>(A, error, sms, st);

@@ -1,4 +1,8 @@
 """The 8-bit linear layers' operators against their formulas in 64 bits."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -191,6 +195,43 @@ def test_few_tiles_share_k_out(cuda, m, n, k, form):
         y = K.w8a8_gemm(x, xs, w, ws, bias=bias, residual=res, error=err)
         R.check_linear(y, x, xs, w, ws, bias, res)
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("m", [512, 768, 1024, 1100, 1280, 2048, 2100, 2560])
+def test_as_many_tiles_as_clusters_fit(cuda, m):
+    """K shared out by four pairs, by two, by none: the numbers of tiles around what a device holds at once."""
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g, x, xs, w, ws = _operands(m, 512, 3200, m)
+    res = torch.randn(m, 512, generator=g, device="cuda").half()
+    R.check_linear(K.w8a8_gemm(x, xs, w, ws, residual=res, error=err), x, xs, w, ws, None, res)
+    assert int(err) == 0
+
+
+FIRST_IN_A_GRAPH = """
+import torch
+from llamamps_b200 import kernels as K
+from tests import _q8 as R
+x, w = (R.padded(n, 3200, torch.int8, "cuda") for n in (300, 500))
+x.random_(-127, 128), w.random_(-127, 128)
+xs, ws = (torch.rand(n, device="cuda") * 2 ** -10 for n in (300, 500))
+y, err = torch.zeros(300, 500, dtype=torch.float16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    K.w8a8_gemm(x, xs, w, ws, out=y, error=err)
+for _ in range(2):
+    y.zero_()
+    graph.replay()
+    R.check_linear(y, x, xs, w, ws)
+assert int(err) == 0
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda):
+    """What a call asks of the device once is asked inside a capture, too."""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 @pytest.mark.parametrize("m,n,k,gated", [(5, 4000, 1000, 0), (14, 2500, 777, 1), (14, 300, 4000, 0), (30, 600, 500, 1),
