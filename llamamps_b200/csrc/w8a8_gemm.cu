@@ -1306,8 +1306,8 @@ static int launch(const Args& A, int* error, int sms, cudaStream_t st) {
     return launch_whole<GATED>(A, error, sms, st);
   if (A.m <= 64 || (A.m <= kSplitTokens && 3 * t128 < pairs)) return launch_split<GATED>(A, error, sms, st);
   // Few tiles: two or four pairs share K out, six steps or more each, as far as their clusters of four or eight CTAs
-  // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two, 700 x 1300 x
-  // 8960 25 -> 17; 768 x 1536 x 8960 would be 31 instead of 24).
+  // are all resident at once (512 x 1536 x 8960 24 -> 16 us with two, 700 x 1300 x 8960 25 -> 17; 768 x 1536 x 8960
+  // would be 31 instead of 24).
   if constexpr (!GATED) {
     const long long steps = ceil_div(A.k, kBK);
     if (4 * t128 <= pairs && steps >= 24 && t128 <= resident_clusters<4>())
