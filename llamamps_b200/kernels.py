@@ -535,6 +535,8 @@ def _q8_arg(t: torch.Tensor, name: str, dtype, dev: int, rows: int, k: int):
     ld = t.stride(0) if rows > 1 else -(-k // 16) * 16
     if ld < k:
         raise ValueError(f"{name}: rows must not overlap (stride {ld} for {k} elements)")
+    if max(ld, rows, k) > 0x7FFFFFFF:
+        raise ValueError(f"{name}: {rows} rows of {k} elements, {ld} apart: more than 32 bits")
     return t.data_ptr(), ld
 
 

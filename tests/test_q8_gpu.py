@@ -433,6 +433,45 @@ def test_products_right_behind_what_writes_their_operands(cuda):
     assert int(err) == 0
 
 
+@pytest.mark.parametrize("m,apart", [(3, 1 << 30), (40, 1 << 26), (140, 1 << 25)])
+@pytest.mark.parametrize("k,n", [(256, 192), (131, 77)])
+def test_rows_far_apart(cuda, m, apart, k, n):
+    """Rows whose offsets pass 32 bits: x, codes, residual, y and weights; the results of rows side by side."""
+    def far(rows, cols, dtype):
+        return torch.empty((rows - 1) * apart + cols, dtype=dtype, device="cuda").as_strided((rows, cols), (apart, 1))
+
+    h = torch.float16
+    x, w, gamma = _rows(m, k, 1), _rows(n, k, 2), _rows(1, k, 3)[0]
+    want, wq = K.rms_norm_q8(x, gamma, residual=x), K.quantise_rows_q8(w)
+    xf, codes, total = far(m, k, h).copy_(x), far(m, k, torch.int8), far(m, k, h)
+    _, scales, _ = K.rms_norm_q8(xf, gamma, residual=xf, sum_out=total, codes=codes)
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1]) and torch.equal(total, want[2])
+    del xf, total
+    res = _rows(m, n, 4)
+    gu = wq[0][:n // 2 * 2], wq[1][:n // 2 * 2]
+    plain, gated = K.w8a8_gemm(*want[:2], *wq, residual=res), K.w8a8_gemm(*want[:2], *gu, swiglu=True)
+    y = far(m, n, h).copy_(res)
+    assert torch.equal(K.w8a8_gemm(codes, scales, *wq, residual=y, out=y), plain)
+    few = min(n // 2 * 2, 4 if apart > 1 << 29 else 128)
+    wf = far(few, k, torch.int8).copy_(wq[0][:few])
+    near = K.w8a8_gemm(*want[:2], wq[0][:few], wq[1][:few])
+    assert torch.equal(K.w8a8_gemm(codes, scales, wf, wq[1][:few], out=y[:, :few]), near)
+    assert torch.equal(K.w8a8_gemm(codes, scales, *gu, swiglu=True, out=y[:, :n // 2]), gated)
+
+
+def test_strides_past_32_bits_are_refused(cuda):
+    """A distance of rows that does not fit the entry points' 32 bits must not arrive there as another one."""
+    apart, err = (1 << 32) + 64, torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.zeros(apart + 64, dtype=torch.int8, device="cuda").as_strided((2, 64), (apart, 1))
+    s, w = torch.ones(2, device="cuda"), torch.zeros(2, 64, dtype=torch.int8, device="cuda")
+    y = torch.zeros(2, 2, dtype=torch.float16, device="cuda")
+    for a, b in ((x, w), (w, x)):
+        with pytest.raises(ValueError, match="32 bits"):
+            K.w8a8_gemm(a, s, b, s, out=y, error=err)
+    with pytest.raises(ValueError, match="codes.*32 bits"):
+        K.quantise_rows_q8(torch.zeros(2, 64, dtype=torch.float16, device="cuda"), codes=x, scales=s)
+
+
 def test_argument_mistakes(cuda):
     g, x, xs, w, ws = _operands(4, 48, 64, 1)
     h = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
