@@ -47,10 +47,10 @@ constexpr int kCtaOf = T > kCta ? T : kCta;
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even, in the low bits
 constexpr float kNearTie = 0.5f - 7.8e-6f;  // (127 / m is off by 2^-24 of itself, so a quotient by 127 x 2^-24 = 7.6e-6)
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // (a NaN stays)
-  float c;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
+// The largest of m, |a| and |b| (a NaN stays).
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
+  return m;
 }
 // Two fp32 operations at once.
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
@@ -63,47 +63,55 @@ __device__ __forceinline__ float2 both(uint64_t p) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
   return f;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 
-// Over the T threads of a row: the sum of ss and the largest m (|v|; a NaN stays) as its bits.
-template <int T>
-__device__ __forceinline__ void reduce_row(float& ss, float m, uint32_t& mbits) {
-  ss = warp_sum(ss);
+// Over the T threads of a row: the largest m (|v|; a NaN stays) as its bits, and with SUM the sum of ss, which only
+// the threads get that `want` it (whole warps).
+template <int T, bool SUM>
+__device__ __forceinline__ void reduce_row(float& ss, float m, uint32_t& mbits, bool want) {
+  if constexpr (SUM) ss = warp_sum(ss);
   mbits = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7FFFFFFFu);  // (a NaN's bits are above infinity's)
   if constexpr (T > kWarp) {
+    constexpr int kWarps = T / kWarp;
     __shared__ float rs[kCtaOf<T> / kWarp];
     __shared__ uint32_t rm[kCtaOf<T> / kWarp];
-    const int warp = threadIdx.x / kWarp, first = warp / (T / kWarp) * (T / kWarp);
+    const int warp = threadIdx.x / kWarp, first = warp / kWarps * kWarps;
     if (threadIdx.x % kWarp == 0) {
-      rs[warp] = ss;
+      if constexpr (SUM) rs[warp] = ss;
       rm[warp] = mbits;
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + first / (T / kWarp)), "n"(T) : "memory");
-    ss = 0.0f;
-    mbits = 0u;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + first / kWarps), "n"(T) : "memory");
+    if constexpr (kWarps <= 4) {
 #pragma unroll
-    for (int w = 0; w < T / kWarp; ++w) {
-      ss += rs[first + w];
-      mbits = max(mbits, rm[first + w]);
+      for (int w = 0; w < kWarps; ++w) mbits = max(mbits, rm[first + w]);
+    } else {
+      mbits = __reduce_max_sync(0xffffffffu, rm[first + threadIdx.x % kWarps]);
+    }
+    if (SUM && want) {
+      ss = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) ss += rs[first + w];
     }
   }
 }
 
-// The factor of the codes and the scale of a row.
-__device__ __forceinline__ void row_scale(const RowArgs& A, float ss, uint32_t mbits, float& inv, float& scale) {
-  const float m = __uint_as_float(mbits);
+// The factor of the codes, and the scale of a row.
+__device__ __forceinline__ float row_factor(uint32_t mbits) {
+  return mbits == 0u || mbits >= 0x7F800000u ? 0.0f : 127.0f / __uint_as_float(mbits);
+}
+__device__ __forceinline__ float row_scale(const RowArgs& A, float ss, uint32_t mbits) {
   const float r = A.gamma ? 1.0f / sqrtf(ss / static_cast<float>(A.k) + A.eps) : 1.0f;
-  inv = 127.0f / m;
-  scale = m * r / 127.0f;
-  if (mbits == 0u) inv = scale = 0.0f;
-  if (mbits >= 0x7F800000u) {
-    inv = 0.0f;
-    scale = __uint_as_float(0x7FC00000u);
-  }
+  if (mbits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  return mbits == 0u ? 0.0f : __uint_as_float(mbits) * r / 127.0f;
 }
 
 // The codes of eight elements, in the low bytes of t (and as t - kMagic).
@@ -115,7 +123,7 @@ __device__ __forceinline__ void row_codes(const float (&v)[8], float inv, uint32
     const uint64_t v2 = pair2(v[i], v[i + 1]), t2 = fma2(v2, inv2, magic2);
     const float2 f = both(t2), d = both(fma2(v2, inv2, fma2(t2, minus2, magic2)));
     t[i] = f.x, t[i + 1] = f.y;
-    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    far = max_abs(far, d.x, d.y);
   }
   if (far > kNearTie) {
     const double m = static_cast<double>(__uint_as_float(mbits));
@@ -145,8 +153,9 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return p;
 }
 
-// 16-byte pieces of eight elements, T threads a row, at most E pieces a thread.
-template <int T, int E>
+// 16-byte pieces of eight elements, T threads a row, at most E pieces a thread.  GAMMA: the norm's rows.  Up to three
+// pieces a thread keeps their products with gamma, else it makes them again.
+template <int T, int E, bool GAMMA>
 __global__ void __launch_bounds__(kCtaOf<T>) rows_vec_kernel(const RowArgs A) {
   lmps_pdl_trigger();
   lmps_pdl_wait();
@@ -160,7 +169,7 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_vec_kernel(const RowArgs A) {
 #pragma unroll
   for (int i = 0; i < E; ++i)
     if (t + T * i < pieces) s[i] = x[t + T * i];
-  if (A.residual) {
+  if (GAMMA && A.residual) {
     const uint4* r = reinterpret_cast<const uint4*>(A.residual + row * A.ldr);
     uint4 rv[E];
 #pragma unroll
@@ -170,29 +179,41 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_vec_kernel(const RowArgs A) {
 #pragma unroll
     for (int i = 0; i < E; ++i)
       if (t + T * i < pieces) {
-        float a[8], b[8];
-        unpack8(s[i], a);
-        unpack8(rv[i], b);
+        __half2* a = reinterpret_cast<__half2*>(&s[i]);
+        const __half2* b = reinterpret_cast<const __half2*>(&rv[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] += b[e];
-        s[i] = pack8(a);
+        for (int e = 0; e < 4; ++e) a[e] = __hadd2_rn(a[e], b[e]);
         sum[t + T * i] = s[i];
       }
   }
+  constexpr bool kHold = GAMMA && E <= 3;
+  uint64_t held[kHold ? E : 1][4];  // two elements each
+  // the products of piece i with gamma
+  auto products = [&](int i, uint64_t (&v)[4], auto&& each) {
+    const __half2 *h = reinterpret_cast<const __half2*>(&s[i]);
+    const uint4 gp = gamma[t + T * i];
+    const __half2* g = reinterpret_cast<const __half2*>(&gp);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(h[e]), w = __half22float2(g[e]);
+      const uint64_t f2 = pair2(f.x, f.y);
+      v[e] = mul2(f2, pair2(w.x, w.y));
+      each(f2, v[e]);
+    }
+  };
   float ss = 0.0f, m = 0.0f;
-  if (gamma) {
+  if constexpr (GAMMA) {
+    uint64_t ss2 = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i)
-      if (t + T * i < pieces) {
-        float f[8], g[8];
-        unpack8(s[i], f);
-        unpack8(gamma[t + T * i], g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss = fmaf(f[e], f[e], ss);
-          m = max_nan(m, fabsf(f[e] * g[e]));
-        }
-      }
+      if (t + T * i < pieces)
+        products(i, held[kHold ? i : 0], [&](uint64_t f2, uint64_t v2) {
+          ss2 = fma2(f2, f2, ss2);
+          const float2 v = both(v2);
+          m = max_abs(m, v.x, v.y);
+        });
+    const float2 f = both(ss2);
+    ss = f.x + f.y;
   } else {
     __half2 m2 = __float2half2_rn(0.0f);
 #pragma unroll
@@ -202,27 +223,39 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_vec_kernel(const RowArgs A) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) m2 = __hmax2_nan(m2, __habs2(h[e]));
       }
-    m = max_nan(__low2float(m2), __high2float(m2));
+    m = max_abs(0.0f, __low2float(m2), __high2float(m2));
   }
+  const bool scaling = A.values || t < kWarp;
   uint32_t mbits;
-  reduce_row<T>(ss, m, mbits);
-  float inv, scale;
-  row_scale(A, ss, mbits, inv, scale);
+  reduce_row<T, GAMMA>(ss, m, mbits, scaling);
+  float scale = 0.0f;
+  if (scaling) scale = row_scale(A, ss, mbits);
   if (t == 0) A.scales[row] = scale;
-  const bool dead = mbits >= 0x7F800000u;
   uint2* codes = reinterpret_cast<uint2*>(A.codes + row * A.ldc);
   uint4* values = A.values ? reinterpret_cast<uint4*>(A.values + row * A.ldv) : nullptr;
+  if (mbits >= 0x7F800000u) {  // (codes 0, values NaN)
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (t + T * i < pieces) {
+        codes[t + T * i] = make_uint2(0u, 0u);
+        if (values) values[t + T * i] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+      }
+    return;
+  }
+  const float inv = row_factor(mbits);
 #pragma unroll
   for (int i = 0; i < E; ++i)
     if (t + T * i < pieces) {
       float f[8], c[8];
-      if (dead) s[i] = make_uint4(0u, 0u, 0u, 0u);
-      unpack8(s[i], f);
-      if (gamma) {
-        float g[8];
-        unpack8(gamma[t + T * i], g);
+      if constexpr (GAMMA) {
+        if constexpr (!kHold) products(i, held[0], [](uint64_t, uint64_t) {});
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = dead ? 0.0f : f[e] * g[e];
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = both(held[kHold ? i : 0][e]);
+          f[2 * e] = v.x, f[2 * e + 1] = v.y;
+        }
+      } else {
+        unpack8(s[i], f);
       }
       row_codes(f, inv, mbits, c);
       codes[t + T * i] = make_uint2(pack4(c), pack4(c + 4));
@@ -263,7 +296,7 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
       for (int j = 0; j < 8; ++j) b[j] = in(j) ? r[base + T * j] : none;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[j] = __float2half_rn(__half2float(b[j]) + __half2float(s[j]));
+        s[j] = __hadd_rn(b[j], s[j]);
         if (in(j)) sum[base + T * j] = s[j];
       }
     }
@@ -278,7 +311,7 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
         ss = fmaf(f, f, ss);
         f *= in(j) ? __half2float(A.gamma[base + T * j]) : 0.0f;
       }
-      m = max_nan(m, fabsf(f));
+      m = max_abs(m, f, 0.0f);
     }
   };
   __half s[E][8];
@@ -291,10 +324,10 @@ __global__ void __launch_bounds__(kCtaOf<T>) rows_any_kernel(const RowArgs A) {
     load8(std::false_type{}, base, v);
     stat8(std::false_type{}, base, v);
   }
+  const bool scaling = A.values || t < kWarp;
   uint32_t mbits;
-  reduce_row<T>(ss, m, mbits);
-  float inv, scale;
-  row_scale(A, ss, mbits, inv, scale);
+  reduce_row<T, true>(ss, m, mbits, scaling);
+  const float scale = scaling ? row_scale(A, ss, mbits) : 0.0f, inv = row_factor(mbits);
   if (t == 0) A.scales[row] = scale;
   const bool dead = mbits >= 0x7F800000u;
   int8_t* codes = A.codes + row * A.ldc;
@@ -334,12 +367,16 @@ static int launch(void (*kernel)(RowArgs), const RowArgs& A, cudaStream_t st) {
 }
 
 // `pieces` of eight elements, T threads a row.
+template <int T, int E>
+static int launch_pieces(const RowArgs& A, bool vec, cudaStream_t st) {
+  if (!vec) return launch<T>(rows_any_kernel<T, E>, A, st);
+  return launch<T>(A.gamma ? rows_vec_kernel<T, E, true> : rows_vec_kernel<T, E, false>, A, st);
+}
 template <int T>
 static int launch_threads(const RowArgs& A, bool vec, int pieces, cudaStream_t st) {
   const int e = (pieces + T - 1) / T;
-  if (e <= 1) return launch<T>(vec ? rows_vec_kernel<T, 1> : rows_any_kernel<T, 1>, A, st);
-  if (e <= 2) return launch<T>(vec ? rows_vec_kernel<T, 2> : rows_any_kernel<T, 2>, A, st);
-  return launch<T>(vec ? rows_vec_kernel<T, 3> : rows_any_kernel<T, 3>, A, st);
+  if (e <= 1) return launch_pieces<T, 1>(A, vec, st);
+  return e <= 2 ? launch_pieces<T, 2>(A, vec, st) : launch_pieces<T, 3>(A, vec, st);
 }
 
 // Threads a row: as few as hold it in three pieces each and still make half of the threads that fit 148 SMs (16384 x
@@ -359,10 +396,9 @@ static int launch_rows(const RowArgs& A, cudaStream_t st) {
   if (fits(128)) return launch_threads<128>(A, vec, pieces, st);
   if (pieces <= 3 * kCta && (pieces <= kCta || A.rows * 1024ll > kFill))
     return launch_threads<kCta>(A, vec, pieces, st);
-  if (pieces <= 1024 * 2 && A.rows * 1024ll <= kFill)
-    return launch<1024>(vec ? rows_vec_kernel<1024, 2> : rows_any_kernel<1024, 2>, A, st);
-  if (!vec) return launch<kCta>(rows_any_kernel<kCta, 5>, A, st);
-  return launch<kCta>(pieces <= 5 * kCta ? rows_vec_kernel<kCta, 5> : rows_vec_kernel<kCta, 8>, A, st);
+  if (pieces <= 1024 * 2 && A.rows * 1024ll <= kFill) return launch_pieces<1024, 2>(A, vec, st);
+  if (!vec || pieces <= 5 * kCta) return launch_pieces<kCta, 5>(A, vec, st);
+  return launch<kCta>(A.gamma ? rows_vec_kernel<kCta, 8, true> : rows_vec_kernel<kCta, 8, false>, A, st);
 }
 
 }  // namespace q8
