@@ -10,13 +10,14 @@
 // r cancels in the codes, so the row is read once and held in registers: m and
 // the sum of squares come from one reduction.  A zero row has codes and scale
 // 0, a row with a NaN or an infinity codes 0 and scale NaN.  127 v / m is one
-// rounding of 127 / m and one fused multiply-add that rounds to the integer;
-// where that quotient is within rounding of a tie (an element that is half the
-// largest is one), the code comes from fp64, so every code is the formula's.
+// division of two ulp and one fused multiply-add that rounds to the integer;
+// where that quotient is within rounding of a tie h (an element that is half
+// the largest is one), the sign of 127 v - h m decides, which two products and
+// what they lost give exactly, so every code is the formula's.
 //
 // Bound by bytes (a row in once, codes and sum out once) where there are many:
-// 16384 x 8960 92 us (4.8 TB/s; with the values 117, 6.3 TB/s), 16384 x 1536 with
-// residual 36 us (4.9 TB/s); a row's latency else, 64 x 1536 3.1 us.
+// 16384 x 8960 72 us (6.1 TB/s; with the values 108, 6.8 TB/s), 16384 x 1536 with
+// residual 31 us (5.8 TB/s); a row's latency else, 64 x 1536 2.4 us.
 #include <type_traits>
 
 #include "common.cuh"
@@ -45,7 +46,7 @@ constexpr int kCta = 256;  // threads of a CTA, but where a row has more
 template <int T>
 constexpr int kCtaOf = T > kCta ? T : kCta;
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even, in the low bits
-constexpr float kNearTie = 0.5f - 7.8e-6f;  // (127 / m is off by 2^-24 of itself, so a quotient by 127 x 2^-24 = 7.6e-6)
+constexpr float kNearTie = 0.5f - 3.2e-5f;  // (127 / m is off by 2^-22 of itself, so a quotient by 127 x 2^-22 = 3.1e-5)
 
 // The largest of m, |a| and |b| (a NaN stays).
 __device__ __forceinline__ float max_abs(float m, float a, float b) {
@@ -106,7 +107,7 @@ __device__ __forceinline__ void reduce_row(float& ss, float m, uint32_t& mbits, 
 
 // The factor of the codes, and the scale of a row.
 __device__ __forceinline__ float row_factor(uint32_t mbits) {
-  return mbits == 0u || mbits >= 0x7F800000u ? 0.0f : 127.0f / __uint_as_float(mbits);
+  return mbits == 0u || mbits >= 0x7F800000u ? 0.0f : __fdividef(127.0f, __uint_as_float(mbits));
 }
 __device__ __forceinline__ float row_scale(const RowArgs& A, float ss, uint32_t mbits) {
   const float r = A.gamma ? 1.0f / sqrtf(ss / static_cast<float>(A.k) + A.eps) : 1.0f;
@@ -126,9 +127,16 @@ __device__ __forceinline__ void row_codes(const float (&v)[8], float inv, uint32
     far = max_abs(far, d.x, d.y);
   }
   if (far > kNearTie) {
-    const double m = static_cast<double>(__uint_as_float(mbits));
+    const float m = __uint_as_float(mbits);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = static_cast<float>(rint(127.0 * static_cast<double>(v[i]) / m)) + kMagic;
+    for (int i = 0; i < 8; ++i) {
+      const float c = t[i] - kMagic, h = c + copysignf(0.5f, fmaf(v[i], inv, -c));
+      // With |127 v| < 2^e and v, m of 22 bits all four are multiples of 2^(e - 31).  Next to the tie p - q is exact, and
+      // lp - lq, at most 2^(e - 23), as well; away from it the sign is p - q's.
+      const float p = __fmul_rn(127.0f, v[i]), q = __fmul_rn(h, m), lp = fmaf(127.0f, v[i], -p), lq = fmaf(h, m, -q);
+      const float above = (p - q) + (lp - lq);
+      t[i] = (above == 0.0f ? h : above > 0.0f ? h + 0.5f : h - 0.5f) + kMagic;
+    }
   }
 }
 

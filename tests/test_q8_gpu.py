@@ -121,6 +121,32 @@ def test_rows_that_are_not_finite_and_extremes(cuda, m, k):
     assert bool(torch.isnan(K.rms_norm_q8(x, gamma, EPS)[1]).all())
 
 
+@pytest.mark.parametrize("k", [1536, 1535, 8960, 77])
+@pytest.mark.parametrize("norm", [False, True])
+def test_ties_and_their_neighbours(cuda, k, norm):
+    """Rows of elements at the ties h m / 127 and next to them: every code is the formula's, half to even (127 v and
+    h m have 31 bits at most, so their comparison in 64 bits is exact)."""
+    g, m = _gen(k), 64
+    gamma = (torch.rand(k, generator=g, device="cuda") + 0.5).half() if norm else torch.ones(k, device="cuda").half()
+    gamma[0] = 1.0
+    top = (torch.rand(m, 1, generator=g, device="cuda") * 3 + 0.5).half()
+    top[::4] = 254.0 * 2.0 ** torch.arange(-8, 8, device="cuda")[:m // 4, None].half()  # (odd multiples are ties)
+    h = torch.randint(-127, 127, (m, k), generator=g, device="cuda").double() + 0.5
+    s = (h * top.double() / 127 / gamma.double()).half()
+    s = (s.view(torch.int16) + torch.randint(-1, 2, (m, k), generator=g, device="cuda").short()).view(torch.float16)
+    s[:, :1] = top
+    v = s.double() * gamma.double()
+    most = v.abs().amax(dim=1, keepdim=True)
+    c = torch.floor(127 * v / most)
+    c = torch.where(127 * v - c * most < 0, c - 1, c)
+    c = torch.where(127 * v - (c + 1) * most >= 0, c + 1, c)
+    above = 127 * v - (c + 0.5) * most  # 0: a tie between c and c + 1
+    want = torch.where(above == 0, c + c.remainder(2), c + (above > 0))
+    assert norm or int((above == 0).sum()) > k // 4  # (few v = s gamma of 22 bits are ties)
+    got = K.rms_norm_q8(s, gamma)[0] if norm else K.quantise_rows_q8(s)[0]
+    assert torch.equal(got.double(), want)
+
+
 def test_vectors_and_no_rows(cuda):
     x = _rows(1, 1536, 1)[0]
     c, s = K.quantise_rows_q8(x)
