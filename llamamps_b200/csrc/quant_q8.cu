@@ -16,8 +16,8 @@
 // what they lost give exactly, so every code is the formula's.
 //
 // Bound by bytes (a row in once, codes and sum out once) where there are many:
-// 16384 x 8960 72 us (6.1 TB/s; with the values 108, 6.8 TB/s), 16384 x 1536 with
-// residual 31 us (5.8 TB/s); a row's latency else, 64 x 1536 2.4 us.
+// 16384 x 8960 64 us (6.8 TB/s; with the values 108, 6.8 TB/s), 16384 x 1536 with
+// residual 31 us (5.7 TB/s); a row's latency else, 64 x 1536 2.4 us.
 #include <type_traits>
 
 #include "common.cuh"
@@ -387,10 +387,21 @@ static int launch_threads(const RowArgs& A, bool vec, int pieces, cudaStream_t s
   return e <= 2 ? launch_pieces<T, 2>(A, vec, st) : launch_pieces<T, 3>(A, vec, st);
 }
 
-// Threads a row: as few as hold it in three pieces each and still make half of the threads that fit 148 SMs (16384 x
-// 1536 with residual: 36 us with 64, 40 with 32, 44 with 128; 2048 x 1536: 6.8 us with 128, 7.8 with 256), else a CTA;
-// 1024 where there are few long rows (64 x 8960: 3.7 us, 4.2 with 256).
-constexpr long long kFill = 148ll * 1024;
+// Four to nine pieces a thread (past six: neither gamma nor values).
+template <int T>
+static int launch_deep(const RowArgs& A, int pieces, cudaStream_t st) {
+  if (pieces > 6 * T) return launch<T>(rows_vec_kernel<T, 9, false>, A, st);
+  return launch<T>(A.gamma ? rows_vec_kernel<T, 6, true> : rows_vec_kernel<T, 6, false>, A, st);
+}
+
+// Threads a row (us at 16384 rows, else as said).  Where rows enough fill the SMs, as few as hold it in up to nine
+// pieces each, so that the reduction is of fewer warps (8960 64 with 128, 72 with 256; 2048 17 with 32, 25 with 128);
+// six with more to hold, gamma or the values (norm of 4096 48 with 128, 60 with 256), five with a residual (4096 72,
+// 78; but 1536 33 with 32 threads, 31 with 64).  Of fewer rows as few threads as hold it in three pieces and make a
+// quarter of what fits 148 SMs (with residual 600 x 1536: 3.4 with 128, 3.9 with 256; 2048 x 1536: 7.2 with 64, 8.0
+// with 128); else a CTA, of 1024 for long rows up to one an SM (128 x 8960: 2.6, 2.8 with 256).
+constexpr long long kFill = 148ll * 512, kFull = 148ll * 1536;
+constexpr int kFewRows = 148;
 
 static int launch_rows(const RowArgs& A, cudaStream_t st) {
   const bool vec = A.k % 8 == 0 && A.ldx % 8 == 0 && A.ldc % 8 == 0 && A.ldr % 8 == 0 && A.lds % 8 == 0 &&
@@ -398,13 +409,18 @@ static int launch_rows(const RowArgs& A, cudaStream_t st) {
                    lmps_aligned(A.sum, 16) && lmps_aligned(A.gamma, 16) && lmps_aligned(A.codes, 8) &&
                    lmps_aligned(A.values, 16) && A.k <= kCta * 8 * 8;
   const int pieces = (A.k + 7) / 8;
-  auto fits = [&](int t) { return pieces <= t || (pieces <= 3 * t && static_cast<long long>(A.rows) * t >= kFill); };
-  if (fits(32)) return launch_threads<32>(A, vec, pieces, st);
-  if (fits(64)) return launch_threads<64>(A, vec, pieces, st);
-  if (fits(128)) return launch_threads<128>(A, vec, pieces, st);
-  if (pieces <= 3 * kCta && (pieces <= kCta || A.rows * 1024ll > kFill))
-    return launch_threads<kCta>(A, vec, pieces, st);
-  if (pieces <= 1024 * 2 && A.rows * 1024ll <= kFill) return launch_pieces<1024, 2>(A, vec, st);
+  const int deep = A.residual ? 5 : A.gamma || A.values ? 6 : 9;
+  auto fits = [&](int t, int most, long long fill) { return pieces <= most * t && A.rows * static_cast<long long>(t) >= fill; };
+  if (vec && pieces > 3 * 32) {
+    if (fits(32, deep, kFull)) return launch_deep<32>(A, pieces, st);
+    if (fits(64, deep, kFull) && pieces > 3 * 64) return launch_deep<64>(A, pieces, st);
+    if (fits(128, deep, kFull) && pieces > 3 * 128) return launch_deep<128>(A, pieces, st);
+  }
+  if (pieces <= 32 || fits(32, 3, kFill)) return launch_threads<32>(A, vec, pieces, st);
+  if (pieces <= 64 || fits(64, 3, kFill)) return launch_threads<64>(A, vec, pieces, st);
+  if (pieces <= 128 || fits(128, 3, kFill)) return launch_threads<128>(A, vec, pieces, st);
+  if (pieces <= kCta || (pieces <= 3 * kCta && A.rows > kFewRows)) return launch_threads<kCta>(A, vec, pieces, st);
+  if (pieces <= 1024 * 2 && A.rows <= kFewRows) return launch_pieces<1024, 2>(A, vec, st);
   if (!vec || pieces <= 5 * kCta) return launch_pieces<kCta, 5>(A, vec, st);
   return launch<kCta>(A.gamma ? rows_vec_kernel<kCta, 8, true> : rows_vec_kernel<kCta, 8, false>, A, st);
 }

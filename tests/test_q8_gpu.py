@@ -64,6 +64,24 @@ def test_rms_norm(cuda, m, k, residual):
     R.check_rows(R.norm(s, gamma, EPS), codes, scales, values, k, additions=k / 32 + 13)
 
 
+@pytest.mark.parametrize("m,k", [(7200, 776), (7200, 1024), (7200, 1536), (3600, 2048), (3600, 2312), (1800, 3584), (1800, 4096),
+                                 (1800, 5120), (1800, 6152), (1800, 8960), (1800, 9216), (1800, 9224), (600, 1536), (300, 1032)])
+@pytest.mark.parametrize("form", ["quantise", "values", "norm", "residual", "norm values", "residual values"])
+def test_many_rows(cuda, m, k, form):
+    """Rows enough to fill the device: more pieces a thread, by what a thread has to hold; each form against 64 bits."""
+    x, gamma = _rows(m, k, m + k), 1 + _rows(1, k, 5)[0] / 4
+    res = _rows(m, k, 7) if "residual" in form else None
+    values = torch.empty(m, k, dtype=torch.float16, device="cuda") if "values" in form else None
+    if "norm" in form or "residual" in form:
+        out = K.rms_norm_q8(x, gamma, EPS, residual=res, values=values)
+        s = x if res is None else out[2]
+        assert res is None or torch.equal(s, x + res)
+        # (two running sums a thread of four pairs a piece, at most six pieces; 13 additions between threads)
+        R.check_rows(R.norm(s, gamma, EPS), out[0], out[1], values, k, additions=4 * 6 + 1 + 13)
+    else:
+        R.check_rows(x.double(), *K.quantise_rows_q8(x, values=values), values, k)
+
+
 @pytest.mark.parametrize("m,k", [(1, 1536), (64, 1536), (300, 1536), (300, 1535), (5, 8960), (3, 20000), (300, 100)])
 def test_strides_and_what_lies_between_rows(cuda, m, k):
     """Rows of larger buffers, odd strides and starts, sums in place; nothing outside the rows is written."""
