@@ -416,7 +416,8 @@ int lmps_tp2_argmax_exchange(const uint16_t* logits, int ld, const int32_t* loca
  * 127.  A zero row has codes and scale 0; a row with a NaN or an infinity has
  * codes 0 and scale NaN, so that what is computed from it is NaN.  All
  * matrices have a row stride in elements (ldx, ldc, ...) of at least their
- * row's length; elements between rows are not written. */
+ * row's length; elements between rows are not written.  Rows to be quantised
+ * have k <= 2^30 (LMPS_ERR_UNSUPPORTED past that). */
 
 /* Quantise rows of x [rows, k].  values (fp16, or NULL) receives code * scale. */
 int lmps_quantise_rows_q8(const uint16_t* x, int ldx, int8_t* codes, int ldc, float* scales, uint16_t* values,

@@ -42,6 +42,7 @@ struct RowArgs {
   float eps;
 };
 
+constexpr int kMaxK = 1 << 30;  // positions in a row, and the steps past its end, fit 32 bits
 constexpr int kCta = 256;  // threads of a CTA, but where a row has more
 template <int T>
 constexpr int kCtaOf = T > kCta ? T : kCta;
@@ -438,6 +439,7 @@ extern "C" int lmps_quantise_rows_q8(const uint16_t* x, int ldx, int8_t* codes, 
   LMPS_CHECK_ARG(x && codes && scales);
   LMPS_CHECK_ARG(rows >= 1 && k >= 1 && ldx >= k && ldc >= k && (!values || ldv >= k));
   LMPS_CHECK_ARG(lmps_aligned(x, 2) && lmps_aligned(scales, 4) && lmps_aligned(values, 2));
+  if (k > q8::kMaxK) return LMPS_ERR_UNSUPPORTED;
   q8::RowArgs A{};
   A.x = CH(x);
   A.ldx = static_cast<size_t>(ldx);
@@ -459,6 +461,7 @@ extern "C" int lmps_rms_norm_q8(const uint16_t* x, int ldx, const uint16_t* resi
   LMPS_CHECK_ARG(!residual == !sum && (!residual || (ldr >= k && lds >= k)));
   LMPS_CHECK_ARG(lmps_aligned(x, 2) && lmps_aligned(residual, 2) && lmps_aligned(sum, 2) && lmps_aligned(gamma, 2) &&
                  lmps_aligned(scales, 4) && lmps_aligned(values, 2));
+  if (k > q8::kMaxK) return LMPS_ERR_UNSUPPORTED;
   q8::RowArgs A{};
   A.x = CH(x);
   A.ldx = static_cast<size_t>(ldx);

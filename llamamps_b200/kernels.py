@@ -565,7 +565,7 @@ def _q8_outputs(x: torch.Tensor, codes, scales):
 
 def quantise_rows_q8(x, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
                      values: Optional[torch.Tensor] = None):
-    """Rows of fp16 ``x`` ([rows, k], or [k]; any row stride) as int8 codes in
+    """Rows of fp16 ``x`` ([rows, k], or [k]; any row stride, k up to 2^30) as int8 codes in
     [-127, 127] and one fp32 scale each, max|row| / 127: (codes, scales).  A
     zero row has scale 0, a row with a NaN or an infinity scale NaN.  Without
     ``codes``, the result's rows start at multiples of 16 bytes, as

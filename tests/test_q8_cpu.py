@@ -40,6 +40,15 @@ def test_row_refusals(call, kw):
     assert call(**kw) == INVALID
 
 
+@pytest.mark.parametrize("call", [_quantise, _norm])
+@pytest.mark.parametrize("k", [(1 << 30) + 1, (1 << 31) - 2049, (1 << 31) - 16, (1 << 31) - 1])
+def test_rows_whose_positions_pass_32_bits_are_refused(call, k):
+    """Positions are 32-bit numbers that step up to 2048 past the end of a row."""
+    far = (1 << 31) - 1
+    assert call(rows=1, k=k, ldx=far, ldc=far) == UNSUPPORTED
+    assert call(rows=1, k=k, ldx=far, ldc=far, values=A, ldv=far) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("kw", [
     dict(g=None), dict(g=A + 1), dict(eps=-1e-6), dict(eps=float("nan")), dict(r=A, ldr=64), dict(s=A, lds=64),
     dict(r=A, ldr=63, s=A, lds=64), dict(r=A, ldr=64, s=A, lds=63), dict(r=A + 1, ldr=64, s=A, lds=64),
