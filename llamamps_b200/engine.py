@@ -198,6 +198,8 @@ class QwenEngine:
         # run_inference's views, made once (it runs once per token)
         self._pin_vec_np, self._pin_logits_np, self._pin_err_np = (
             self._pin_vec.numpy(), self._pin_logits.numpy(), self._pin_err.numpy())
+        self._pin_gemm_err = torch.zeros(1, dtype=i32).pin_memory()
+        self._pin_gemm_err_np = self._pin_gemm_err.numpy()
         self._x_row0, self._x_rows1 = self.buf_residual[0], self.buf_residual[:1]
         self._lg_row0, self._lg_rows1 = self.buf_logits[0], self.buf_logits[:1]
         self._ri_warm = False  # run_inference has launched once eagerly (then it replays a graph)
@@ -382,13 +384,16 @@ class QwenEngine:
         if self.pdec is not None and self._pin_err_np[0] != 0:
             self.pdec.check_error()
         self.check_kv_error()
+        if self.w8a8 and self._pin_gemm_err_np[0] != 0:  # (the prompt's, if it was dense)
+            self.check_gemm_error()
         self.host_pos += 1
         return self._pin_logits_np.copy()
 
     def _persistent_token_ops(self) -> None:
         """run_inference's device work: pinned input row in, one decode step
         (persistent launch, graph replay or per-stage kernels), logits (and
-        the persistent kernel's error word) out to pinned memory."""
+        the error words of the persistent kernel and of 8-bit products) out to
+        pinned memory."""
         self._x_row0.copy_(self._pin_vec, non_blocking=True)
         if self.pdec is not None:
             self.pdec.run(1, self.tokens, self.pos, 1, x_in=self._x_rows1, logits=self._lg_rows1)
@@ -399,6 +404,8 @@ class QwenEngine:
         self._pin_logits.copy_(self._lg_row0, non_blocking=True)
         if self.pdec is not None:  # the device error word rides along with the logits
             self._pin_err.copy_(self.pdec.error, non_blocking=True)
+        if self.w8a8:
+            self._pin_gemm_err.copy_(self.gemm_err, non_blocking=True)
 
     def _persistent_token_graph(self):
         """The persistent per-token sequence captured once (after one eager

@@ -120,6 +120,35 @@ def test_a_reported_timeout_raises(cuda, model):
     assert np.array_equal(eng.generate_batch(prompts, 3), ids)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(use_graphs=False), dict(decoder="kernels"), dict(kv_bits=4)])
+def test_run_inference_raises_a_reported_timeout(cuda, model, kw):
+    """Logits behind a prompt whose products gave up are not handed out, eager (the first token) and replayed (later
+    ones), with a reset in between too; the error is raised once."""
+    cfg, mw = model
+    eng = _engine(mw, max_batch=1, max_seq_len=320, **kw)
+    prompt, vec = _prompts(cfg, 1, 300), mw.embed[17].cpu().numpy()
+    eng._ensure_history(4)
+
+    def logits(report=False, reset=False):
+        eng.reset(1)
+        eng.prefill(prompt, dense=True)
+        if report:
+            eng.gemm_err.fill_(1)
+        if reset:
+            eng.reset(1)
+        return eng.run_inference(vec)
+    want = None
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="timed out"):
+            logits(report=True)
+        got = logits()
+        assert np.isfinite(got).all() and (want is None or np.array_equal(got, want))
+        want = got
+    with pytest.raises(RuntimeError, match="timed out"):
+        logits(report=True, reset=True)
+    assert int(eng.gemm_err.item()) == 0
+
+
 def test_tensor_parallel_ranks(cuda, model):
     """Both ranks on one GPU, a thread a rank, the all-reduce a host rendezvous between steps: layer 0's cached rows
     of rank r are KV head r's of the whole engine, bit for bit, and both ranks name the same tokens."""
