@@ -41,7 +41,9 @@ struct Args {
 };
 
 // The scaled sum, and the bias in the rounding of the second product.  Every kernel goes through the same roundings
-// (this, then the residual), so a token's result does not depend on the other tokens of its call.
+// (this, then the residual), so a token's result does not depend on the other tokens of its call.  Where there is no
+// residual, nothing is added or kNone, which leaves a zero's sign as well.
+constexpr float kNone = -0.0f;
 __device__ __forceinline__ float linear_value(int acc, float xs, float ws, float bias = 0.0f) {
   return fmaf(__fmul_rn(static_cast<float>(acc), xs), ws, bias);
 }
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(WARPS* kWarp) few_kernel(const Args A) {
     wu[i] = GATED && live ? A.ws[A.n + c] : 0.0f;
     xs[i] = live ? A.xs[t] : 0.0f;
     bias[i] = live && A.bias ? __half2float(A.bias[c]) : 0.0f;
-    res[i] = live && A.residual ? __half2float(A.residual[static_cast<size_t>(t) * A.ldr + c]) : 0.0f;
+    res[i] = live && A.residual ? __half2float(A.residual[static_cast<size_t>(t) * A.ldr + c]) : kNone;
   }
 #pragma unroll
   for (int z = 0; z < kW; ++z)
@@ -553,10 +555,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_kernel(const __grid_co
   for (int i = tid; here && i < outs * tok4; i += kSplitThreads) {
     const int lc = i & (outs - 1), j = 4 * (i >> log_outs), c = cbase + lc;
     if (c >= A.n) continue;
-    float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float res[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      res[e] = !GATED && A.residual && j + e < tok ? __half2float(A.residual[static_cast<size_t>(j + e) * A.ldr + c]) : 0.0f;
+      res[e] = !GATED && A.residual && j + e < tok ? __half2float(A.residual[static_cast<size_t>(j + e) * A.ldr + c]) : kNone;
     int g[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
     const int4* at = red + j / 4 * 128 + lc;
 #pragma unroll 4

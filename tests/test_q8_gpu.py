@@ -398,6 +398,44 @@ def test_a_token_does_not_depend_on_its_call(cuda, n, k, form):
     assert int(err) == 0
 
 
+@pytest.mark.parametrize("n,k,form", [(200, 256, "gated"), (131, 77, "gated"), (4800, 96, "gated"), (200, 256, "none"),
+                                      (131, 77, "bias"), (9504, 96, "none"), (200, 256, "residual")])
+def test_the_sign_of_a_zero_does_not_depend_on_the_call(cuda, n, k, form):
+    """Gate sums of zero and far below zero against up values of both signs, zero sums and negative ones that vanish in
+    fp16: the bits of the rows of a call of 700 tokens, of few and of middling calls, and the formula's sign."""
+    m, gated = 700, form == "gated"
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g, x, xs, w, ws = _operands(m, 2 * n if gated else n, k, 6)
+    xs.fill_(1.0)
+    w[:n:3] = 0
+    if gated:
+        ws[:n] = 1000.0 / (k ** 0.5 * 73 * 73)  # (gates of some 1000: half of them vanish)
+        ws[n:] = 2.0 ** -10
+        if n > 16:
+            w[n:n + 16:2] = 0  # (up values of zero, both kinds of gates before them)
+    else:
+        ws.fill_(2.0 ** -46)
+    zero = torch.zeros(n, dtype=torch.float16, device="cuda")
+    bias = zero if form == "bias" else None
+    res = torch.where(torch.arange(n, device="cuda") % 2 == 0, zero, -zero).repeat(m, 1) if form == "residual" else None
+    y = K.w8a8_gemm(x, xs, w, ws, bias=bias, residual=res, swiglu=gated, error=err)
+    v = R.linear(x, xs, w, ws)
+    if gated:
+        v = v[:, :n] * torch.sigmoid(v[:, :n]) * v[:, n:]
+    elif bias is not None:
+        v = v + bias.double()
+    if res is not None:
+        v = v + res.double()
+    assert int((y == 0).sum()) > m * n // 4 and int(torch.signbit(y[y == 0]).sum()) > m * n // 64
+    # (a sum of zero times a scale is +0 here as there; an integer has no zero of its own sign)
+    assert torch.equal(torch.signbit(y), torch.signbit(v))
+    for a, b in ((0, 1), (3, 11), (5, 17), (5, 20), (0, 32), (7, 71), (100, 200), (0, 257)):
+        part = K.w8a8_gemm(x[a:b], xs[a:b], w, ws, bias=bias, residual=None if res is None else res[a:b], swiglu=gated,
+                           error=err)
+        assert torch.equal(part.view(torch.int16), y[a:b].view(torch.int16)), (a, b)
+    assert int(err) == 0
+
+
 # -- as they are used ----------------------------------------------------------------
 def _block(x, part, gamma, wq, err, out=None):
     """Residual and norm, the gated projections, the quantiser, the down projection onto the residual stream."""
