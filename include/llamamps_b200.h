@@ -426,7 +426,9 @@ int lmps_quantise_rows_q8(const uint16_t* x, int ldx, int8_t* codes, int ldc, fl
 /* RMSNorm (kernels/rms_norm.metal:20-39, over the full vector) of x, or with
  * residual of fp16(residual + x), written to sum (both or neither; sum may be
  * residual or x with the same stride), times gamma, quantised as above without
- * a rounding to fp16 in between. */
+ * a rounding to fp16 in between.  A row's codes do not depend on the other rows
+ * of the call; its scale does in the last bits (the squares are added in an
+ * order that goes by the number of rows). */
 int lmps_rms_norm_q8(const uint16_t* x, int ldx, const uint16_t* residual, int ldr, uint16_t* sum, int lds,
                      const uint16_t* gamma, float eps, int8_t* codes, int ldc, float* scales, uint16_t* values,
                      int ldv, int rows, int k, void* stream);

@@ -13,7 +13,9 @@
 // division of two ulp and one fused multiply-add that rounds to the integer;
 // where that quotient is within rounding of a tie h (an element that is half
 // the largest is one), the sign of 127 v - h m decides, which two products and
-// what they lost give exactly, so every code is the formula's.
+// what they lost give exactly, so every code is the formula's, whatever the
+// call.  The norm's scales differ in their last bits between calls of different
+// size: the squares are added in the order of the threads that a row has.
 //
 // Bound by bytes (a row in once, codes and sum out once) where there are many:
 // 16384 x 8960 64 us (6.8 TB/s; with the values 108, 6.8 TB/s), 16384 x 1536 with

@@ -591,7 +591,9 @@ def rms_norm_q8(x, gamma, eps: float = 1e-6, *, residual: Optional[torch.Tensor]
     """:func:`rms_norm` with its output in 8 bits, as :func:`quantise_rows_q8`
     gives it (of the unrounded norm): (codes, scales).  With ``residual`` the
     norm is of s = fp16(residual + x), which ``sum_out`` receives: (codes,
-    scales, sum).  ``sum_out`` may be ``residual`` or ``x`` itself."""
+    scales, sum).  ``sum_out`` may be ``residual`` or ``x`` itself.  A row's
+    scale may differ in its last bits between calls of different size (the
+    order of additions in its sum of squares), its codes do not."""
     if codes is None or scales is None:
         codes, scales = _q8_outputs(x, codes, scales)
     if residual is None:

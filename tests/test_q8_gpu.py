@@ -165,6 +165,25 @@ def test_ties_and_their_neighbours(cuda, k, norm):
     assert torch.equal(got.double(), want)
 
 
+@pytest.mark.parametrize("k", [1536, 2048, 8960, 1535])
+def test_rows_of_calls_of_any_size(cuda, k):
+    """Codes, the quantiser's scales and the sums are the same bits for 1 to 16384 rows.  The norm's scales are not:
+    two orders of the additions in a sum of squares are each off by a rounding for each addition that an element goes
+    through (k / 32 in a thread, 13 between threads), the scale by half of that and its other roundings."""
+    m = 16384
+    x, r, gamma = _rows(m, k, 3), _rows(m, k, 4), 1 + _rows(1, k, 5)[0] / 4
+    codes, scales = K.quantise_rows_q8(x)
+    ncodes, nscales, total = K.rms_norm_q8(x, gamma, EPS, residual=r)
+    rel = 2 * ((k / 32 + 13) / 2 + 6) * 2.0 ** -24
+    for a, b in ((0, 1), (5, 69), (100, 700), (7, 2007), (0, 5000), (m - 3, m)):
+        c, s = K.quantise_rows_q8(x[a:b])
+        assert torch.equal(c, codes[a:b]) and torch.equal(s, scales[a:b])
+        c, s, t = K.rms_norm_q8(x[a:b], gamma, EPS, residual=r[a:b])
+        assert torch.equal(c, ncodes[a:b]) and torch.equal(t, total[a:b])
+        want = nscales[a:b].double()
+        assert bool(((s.double() - want).abs() <= rel * want).all())
+
+
 def test_vectors_and_no_rows(cuda):
     x = _rows(1, 1536, 1)[0]
     c, s = K.quantise_rows_q8(x)
