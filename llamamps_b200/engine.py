@@ -115,8 +115,8 @@ class QwenEngine:
         # batches above this run the projections and LM head on the tensor-core GEMM
         self.gemv_max_batch = gemv_max_batch
         # w8a8: where the projections run on the tensor-core GEMM (dense prefill, steps of larger batches), their
-        # weights and activations are in 8 bits with a scale for each channel and token; smaller batches and the LM
-        # head keep the Q4 weights
+        # weights and activations are in 8 bits with a scale for each channel and token; smaller batches, the one-launch
+        # decoders (so decoder="batched" at any batch) and the LM head keep the Q4 weights
         self.w8a8 = w8a8
         if w8a8:
             add_q8(weights)

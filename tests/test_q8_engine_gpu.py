@@ -109,6 +109,28 @@ def test_small_batches_are_those_of_the_q4_engine(cuda, model):
     assert np.array_equal(_engine(mw, **kw).generate_batch(prompts, 8), _engine(mw, w8a8=False, **kw).generate_batch(prompts, 8))
 
 
+def test_the_batched_decoder_keeps_the_q4_weights(cuda, model):
+    """decoder="batched": a dense prompt is in 8 bits as with the per-stage kernels, steps are those without w8a8."""
+    cfg, mw = model
+    B, P = 8, 40
+    kw = dict(max_batch=B, max_seq_len=96, decoder="batched")
+    short = _prompts(cfg, B, 5).cpu().numpy()
+    eng = _engine(mw, **kw)
+    assert np.array_equal(eng.generate_batch(short, 8), _engine(mw, w8a8=False, **kw).generate_batch(short, 8))
+    stages = _engine(mw, max_batch=B, max_seq_len=96)
+    assert stages.decoder == "kernels"
+    for e in (eng, stages):
+        e.reset(B)
+        e._ensure_history(4)
+        e.prefill(_prompts(cfg, B, P), dense=True)
+        e.check_gemm_error()
+    for b in range(B):
+        for layer in range(2):
+            for x, y in zip(eng.cache.read_positions(b, layer, P), stages.cache.read_positions(b, layer, P)):
+                assert torch.equal(x, y)
+    assert torch.equal(eng.tokens, stages.tokens)
+
+
 def test_a_reported_timeout_raises(cuda, model):
     cfg, mw = model
     eng = _engine(mw, max_batch=8, max_seq_len=64)
