@@ -226,6 +226,42 @@ def test_tensor_parallel_ranks(cuda, model):
     assert float(off) < 0.08
 
 
+@pytest.mark.parametrize("B", [6, 40])
+def test_decode_steps_of_tensor_parallel_ranks(cuda, model, B):
+    """Steps of a batch on both ranks (one GPU, a thread a rank, host rendezvous): layer 0's cached rows of rank r are
+    KV head r's of the whole engine, bit for bit, both ranks name the same tokens, and the hidden rows are off the
+    whole engine's by what partial sums quantised apart take."""
+    from tests.test_kv_q4_tp_gpu import _both, _rank_engines
+    cfg, mw = model
+    P = 7
+    prompts = _prompts(cfg, B, P, seed=B)
+    kw = dict(max_batch=B, max_seq_len=64, kv_bits=4, w8a8=True)
+    whole = _engine(mw, **kw)
+    kw.pop("kv_bits")
+    ranks = _rank_engines(mw, **kw)
+
+    def feed(e):
+        e.reset(B)
+        for t in range(P):
+            e.tokens[:B].copy_(prompts[:, t])
+            e.decode_step(record=False)
+        torch.cuda.current_stream().synchronize()
+        e.check_gemm_error()
+        e.check_kv_error()
+    feed(whole)
+    _both(ranks, feed)
+    for e in ranks:
+        assert e.q8_rows is not None and e.pos[:B].tolist() == [P] * B
+        off = (e.buf_residual.double() - whole.buf_residual.double()).norm() / whole.buf_residual.double().norm()
+        assert float(off) < 0.08
+    for b in range(B):
+        full = whole.cache.read_positions(b, 0, P)
+        for r, e in enumerate(ranks):
+            for x, y in zip(full, e.cache.read_positions(b, 0, P)):
+                assert torch.equal(x[:, 128 * r:128 * (r + 1)], y)
+    assert torch.equal(ranks[0].tokens, ranks[1].tokens) and torch.equal(ranks[0].buf_residual, ranks[1].buf_residual)
+
+
 def test_demo_runs_with_8_bit_projections(cuda, capsys):
     from llamamps_b200 import demo
     from llamamps_b200.config import QWEN2_5_1_5B

@@ -355,6 +355,32 @@ def test_two_streams_at_once(cuda):
     assert all(torch.equal(g, want[key]) for key in got for g in got[key]) and not bool(err.any())
 
 
+def test_two_streams_of_wide_outputs_and_few_tokens(cuda):
+    """Two streams that overlap, with the calls whose tokens are the tensor core's rows and those of few tokens in two
+    and four tiles, pairs that share K out between them."""
+    shapes = [(48, 9504, 512, False), (12, 2000, 768, False), (64, 4800, 512, True), (24, 1000, 768, True),
+              (300, 512, 4096, False), (24, 2000, 333, False), (12, 1000, 512, True), (33, 9504, 3000, False)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    ops, want, got = {}, {}, {}
+    err = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for s in range(2):
+        for i, (m, n, k, gated) in enumerate(shapes):
+            _, x, xs, w, ws = ops[s, i] = _operands(m, 2 * n if gated else n, k, 100 * s + i)
+            want[s, i] = K.w8a8_gemm(x, xs, w, ws, swiglu=gated)
+            (R.check_gated if gated else R.check_linear)(want[s, i], x, xs, w, ws)
+            got[s, i] = [torch.full_like(want[s, i], 7.0) for _ in range(4)]
+    torch.cuda.synchronize()
+    for rep in range(4):
+        for i in range(len(shapes)):
+            for s in range(2):
+                j = (i + 3 * s) % len(shapes)
+                with torch.cuda.stream(sides[s]):
+                    _, x, xs, w, ws = ops[s, j]
+                    K.w8a8_gemm(x, xs, w, ws, swiglu=shapes[j][3], out=got[s, j][rep], error=err[s:s + 1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[key]) for key in got for g in got[key]) and not bool(err.any())
+
+
 @pytest.mark.parametrize("m", [1, 7, 40, 130, 300])
 def test_largest_sums_and_extreme_codes(cuda, m):
     """Sums at the edge of 32 bits (k = 131071, all codes -128), and codes of one sign."""
@@ -531,6 +557,33 @@ def test_products_right_behind_what_writes_their_operands(cuda):
         for j in range(40):
             a, b = K.quantise_rows_q8(xs_[j % 4]), K.quantise_rows_q8(ws_[(j // 2) % 4])
             R.check_linear(outs[j], a[0], a[1], b[0], b[1])
+    assert int(err) == 0
+
+
+@pytest.mark.parametrize("m,n,k,gated", [(48, 9504, 512, False), (64, 4800, 512, True), (12, 640, 512, False),
+                                         (24, 640, 512, True), (300, 512, 4096, False), (600, 384, 1600, False)])
+def test_every_product_right_behind_what_writes_its_operands(cuda, m, n, k, gated):
+    """The same for wide outputs, few tokens in several tiles, and pairs that share K out: each starts while the kernel
+    that writes its weights or rows still runs, and touches the weights before it may read them."""
+    g, rows = _gen(m + n), 2 * n if gated else n
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    wide = [(torch.randn(rows, k, generator=g, device="cuda") * (1 + j) / k ** 0.5).half() for j in range(3)]
+    toks = [torch.randn(m, k, generator=g, device="cuda").half() for _ in range(4)]
+    wc, wsc = K.quantise_rows_q8(wide[0])
+    xc, xsc = K.quantise_rows_q8(toks[0])
+    outs = [torch.full((m, n), 7.0, dtype=torch.float16, device="cuda") for _ in range(24)]
+    torch.cuda.synchronize()
+    for j in range(24):
+        if j % 2:  # the weights last, or the rows
+            K.quantise_rows_q8(toks[j % 4], xc, xsc)
+            K.quantise_rows_q8(wide[j % 3], wc, wsc)
+        else:
+            K.quantise_rows_q8(wide[j % 3], wc, wsc)
+            K.quantise_rows_q8(toks[j % 4], xc, xsc)
+        K.w8a8_gemm(xc, xsc, wc, wsc, swiglu=gated, out=outs[j], error=err)
+    for j in range(24):
+        a, b = K.quantise_rows_q8(toks[j % 4]), K.quantise_rows_q8(wide[j % 3])
+        (R.check_gated if gated else R.check_linear)(outs[j], a[0], a[1], b[0], b[1])
     assert int(err) == 0
 
 
