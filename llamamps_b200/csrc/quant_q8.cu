@@ -18,8 +18,10 @@
 // size: the squares are added in the order of the threads that a row has.
 //
 // Bound by bytes (a row in once, codes and sum out once) where there are many:
-// 16384 x 8960 64 us (6.8 TB/s; with the values 108, 6.8 TB/s), 16384 x 1536 with
-// residual 31 us (5.7 TB/s); a row's latency else, 64 x 1536 2.4 us.
+// 16384 x 8960 64 us (6.9 TB/s; with the values 107, 6.8 TB/s), norm of 16384 x
+// 1536 with residual 29 us (6.1 TB/s); by instructions without one, 18.3 us (4.1
+// TB/s: a thread's six products with gamma are made twice).  A row's latency else:
+// 64 x 8960 1.9 us, norm of 64 x 1536 with residual 2.0 (in a graph of 200 calls).
 #include <type_traits>
 
 #include "common.cuh"

@@ -48,8 +48,9 @@ __device__ __forceinline__ float linear_value(int acc, float xs, float ws, float
   return fmaf(__fmul_rn(static_cast<float>(acc), xs), ws, bias);
 }
 
-// 2^x and 1 / x to some 2^-22, results below 2^-126 as zero: e^-g past 2^126 makes the quotient 0, which fp16 makes of
-// it anyway.
+// 2^x and 1 / x to some 2^-22, results below 2^-126 as zero: e^-g past 2^126 makes silu(g) 0, and so the product with
+// any up value below some 2^94, which fp16 would round to 0.  (Codes and scales of fp16 rows give less than 2^64: a sum
+// of 2^31, scales below 2^10 and, behind a norm, 2^18.)
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -767,8 +768,10 @@ static size_t split_smem(int stages, int xrows) {
 //   warps 2 ..: epilogue, four warps (TMEM lanes 32 (w % 4) ..) for each 64 or 32 channels of the tile
 // Tiles of 256 x 256 because a pair then loads 64 KB for 512 cycles of products
 // of both SMs, near what they can load (10 TB/s over the GPU); of 128 where
-// there are few.  Bound by power: 16384 x 8960 x 1536 gated 350 us (2.6 POP/s at
-// some 1.4 GHz; 258 without the epilogue, 222 of zeros), 16384 x 1536 x 8960 183.
+// there are few.  Bound by power, so by the codes too: 16384 x 8960 x 1536 gated
+// 350 to 358 us of bell-shaped codes up to 127 (2.5 POP/s at some 1.4 GHz; 258
+// without the epilogue, 222 of zeros; 300 of even codes up to 34), 16384 x 1536 x
+// 8960 with residual 190 (166 of the latter).
 // Split K (SPLITS > 1): the pairs of a cluster send their sums of a warp's
 // channels to the pair that finishes them.
 
@@ -1182,11 +1185,14 @@ static int launch_split(const Args& A, int* error, int sms, cudaStream_t st) {
   P.xrows = (A.m + 15) / 16 * 16;
   const int out = GATED ? 64 : 128;
   const int tiles = (A.n + out - 1) / out, steps = (A.k + kBK - 1) / kBK;
-  // at most two CTAs an SM, at least three K steps each (64 x 2048 x 1536: 5.6 us with 4 splits, 5.9 with 8, 7.5 with 2)
+  // no more CTAs than two an SM, at least three K steps each (64 x 2048 x 1536: 5.6 us with 4 splits, 5.9 with 8, 7.5
+  // with 2).  This counts CTAs, not the clusters that fit: with an SM a CTA a device holds some 15 clusters of eight, so
+  // 16 to 18 tiles behind a long K take a second wave (64 x 2048 x 8192 16.7 us; 12 tiles, 64 x 1536 x 8960, 6.6).
   int splits = 1;
   while (splits < 8 && 2 * splits * tiles <= 2 * sms && 6 * splits <= steps) splits *= 2;
   P.ksteps = (steps + splits - 1) / splits;
-  // two CTAs an SM where there are so many, else the whole SM's shared memory
+  // half an SM's shared memory where there are more CTAs than SMs, else all of it.  Past 96 tokens two stages and the
+  // sums alone are more than half, so such CTAs run one an SM, in two waves (128 x 2560 x 9728 24.9 us).
   const size_t room = tiles * splits > sms ? 113 * 1024 : 226 * 1024;
   int stages = P.ksteps < 2 ? 2 : P.ksteps < kSplitStages ? P.ksteps : kSplitStages;  // (the ring also holds the CTA's sums)
   while (stages > 2 && split_smem(stages, P.xrows) > room) --stages;
